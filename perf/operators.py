@@ -245,7 +245,7 @@ def _prepare_tables(past, new, bs, rng):
     z = lambda n: torch.zeros(n, dtype=torch.int32, device=_DEV)  # noqa: E731
     return {"case": {"kind": "tables", "block": bs}, "S": S, "rows": rows, "max_blocks": mb,
             "past": _int32(past), "new": _int32(new), "tables": _int32(tables), "ring": _int32(ring),
-            "pool": _int32([head, len(free)]), "pool_out": z(2), "q_start": z(S), "q_len": z(S),
+            "pool": _int32([head, len(free), 0]), "pool_out": z(2), "q_start": z(S), "q_len": z(S),
             "ctx": z(S), "positions": z(rows), "slots": z(rows), "decode_token": z(rows),
             "decode_seq": z(rows), "prefill_seq": z(S), "counts": z(4)}
 
