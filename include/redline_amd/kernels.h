@@ -228,5 +228,49 @@ inline void gemv_w4a16_swiglu(const half* x, int m, const uint8_t* w, const half
                                       stream));
 }
 
+// ---- extensions without a counterpart in the reference: the block-scaled
+// 8-bit cache (one scale per block and kv head) and batch tables made on the GPU;
+// see rlk.h for their layouts and contracts.
+enum class KVBlockFormat { kINT8 = RLK_KV_BLOCK_INT8, kFP8 = RLK_KV_BLOCK_FP8 };
+using KVBlockView = rlk_kv_block_view;
+using BlockAttentionParams = rlk_block_attention_params;
+using BlockPool = rlk_block_pool;
+using BatchTables = rlk_batch_tables;
+
+// rope_and_write_kv into a block-scaled cache; qkv_bias may be null.
+inline void rope_and_write_kv_blocks(half* qkv, const int32_t* positions,
+                                     const int32_t* slot_mapping, int num_tokens, int num_heads,
+                                     const float* cos_table, const float* sin_table,
+                                     const KVBlockView& kv, const half* qkv_bias,
+                                     hipStream_t stream) {
+  detail::check(rlk_rope_and_write_kv_blocks(detail::bits(qkv), positions, slot_mapping, num_tokens,
+                                             num_heads, cos_table, sin_table, &kv,
+                                             detail::bits(qkv_bias), stream));
+}
+
+// Stored rows of a block-scaled cache as fp16 (either output may be null).
+inline void read_kv_blocks(const KVBlockView& kv, const int32_t* slots, int n, half* k_out,
+                           half* v_out, hipStream_t stream) {
+  detail::check(rlk_read_kv_blocks(&kv, slots, n, detail::bits(k_out), detail::bits(v_out), stream));
+}
+
+// Decode and prefill attention over a block-scaled cache.
+inline void paged_attention_decode_blocks(const BlockAttentionParams& p,
+                                          const DecodeAttentionWork& w, hipStream_t stream) {
+  detail::check(rlk_paged_attention_decode_blocks(
+      &p, reinterpret_cast<const rlk_decode_attention_work*>(&w), stream));
+}
+inline void paged_attention_prefill_blocks(const BlockAttentionParams& p,
+                                           const PrefillAttentionWork& w, hipStream_t stream) {
+  detail::check(rlk_paged_attention_prefill_blocks(
+      &p, reinterpret_cast<const rlk_prefill_attention_work*>(&w), stream));
+}
+
+// Positions, slots, work lists and block tables from request lengths.
+inline void build_batch_tables(const BlockPool& pool, const BatchTables& tables,
+                               hipStream_t stream) {
+  detail::check(rlk_build_batch_tables(&pool, &tables, stream));
+}
+
 }  // namespace kernels
 }  // namespace redline

@@ -318,6 +318,158 @@ int rlk_paged_attention_prefill_ex(const rlk_attention_params* params,
                                    const rlk_prefill_attention_work* work,
                                    const rlk_attention_options* options, hipStream_t stream);
 
+/* ------------------------------------------------- block-scaled 8-bit KV cache
+ *
+ * Extension, no counterpart in the reference: a paged cache in 8 bits with one
+ * scale per (block, kv head) for K and one for V, instead of one per (token,
+ * head).  A block holds block_size tokens (16 or 32) of one kv head, head_dim
+ * D = 16 E (64 or 128), as tiles of 16 tokens whose bytes stand in the order
+ * in which the matrix cores take them:
+ *   k  [num_blocks, num_kv_heads][block_size / 16 tiles][E pieces p][16 tokens]
+ *      [2 halves h][8 e]                 holds dim  h D/2 + 8 p + e
+ *   v  [num_blocks, num_kv_heads][block_size / 16 tiles][E/4 g][4 quads r][16 m]
+ *      [4 j][4 i]                        holds dim  E m + 4 g + j  of the tile's
+ *                                        token 4 r + i
+ *   k_scale, v_scale  fp32 [num_blocks, num_kv_heads]: 0 (every code is 0), or
+ *      a power of two from 2^-24 to 2^10; a stored value is code * scale, an
+ *      exact fp16 value.
+ * Codes are int8, or e4m3 (the finite-only form: largest value 448, no
+ * infinities).  Block ids read from block tables are held inside the pool: an
+ * id outside [0, num_blocks) is read as block 0. */
+#define RLK_KV_BLOCK_INT8 0
+#define RLK_KV_BLOCK_FP8 1
+
+typedef struct rlk_kv_block_view {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int num_blocks;
+  int block_size;
+  int num_kv_heads;
+  int head_dim;
+  int format; /* RLK_KV_BLOCK_INT8 | RLK_KV_BLOCK_FP8 */
+} rlk_kv_block_view;
+
+/* rlk_rope_and_write_kv into a block-scaled cache (same qkv, positions, slots
+ * and cos/sin tables; the bias as in rlk_rope_kv_options, NULL = none).
+ * Rows of one block come consecutively in the batch, each at the offset after
+ * the row before (a packed batch has them so); they form a run.  A run that
+ * starts at offset 0 starts the block: its scale s is the least power of two
+ * with amax / s <= 127 (INT8) or 448 (e4m3), from 2^-24 on, over the run's
+ * values of the head; 0 when all are 0.  A run that starts later continues the
+ * block: s = max(old scale, that power of two), and when s grew, the codes of
+ * the earlier offsets are requantised, code' = rne(code * old / s).  New codes
+ * are rne(x / s) of the fp16 value x, saturating at the largest code whose
+ * value is an fp16 number (INT8 127, 63 at s = 2^10; e4m3 448, 240 at 2^8);
+ * infinities saturate, NaN is stored as some finite value.  Bytes of offsets
+ * past the run are left as they were, and so are slots < 0 or past the pool.
+ * Two runs of one call must not share a block, except rows of graph padding
+ * that all write one scratch block, whose contents are then unspecified.
+ * num_tokens <= 0: no-op.  head_dim not in {64, 128} or block_size not in
+ * {16, 32}: RLK_EUNSUPPORTED.  qkv, bias, cos/sin tables, k and v 16-byte
+ * aligned, else RLK_EINVAL. */
+int rlk_rope_and_write_kv_blocks(uint16_t* qkv, const int32_t* positions,
+                                 const int32_t* slot_mapping, int num_tokens, int num_heads,
+                                 const float* cos_table, const float* sin_table,
+                                 const rlk_kv_block_view* kv, const uint16_t* qkv_bias,
+                                 hipStream_t stream);
+
+/* Stored rows back as fp16: k_out[i] / v_out[i] [n, num_kv_heads * head_dim] =
+ * code * scale of slot slots[i] (either output may be NULL).  A slot < 0 or
+ * past the pool leaves its rows as they were.  n <= 0: no-op.  Outputs 16-byte
+ * aligned, else RLK_EINVAL. */
+int rlk_read_kv_blocks(const rlk_kv_block_view* kv, const int32_t* slots, int n, uint16_t* k_out,
+                       uint16_t* v_out, hipStream_t stream);
+
+/* rlk_attention_params over a block-scaled cache. */
+typedef struct rlk_block_attention_params {
+  const uint16_t* q;
+  int q_stride;
+  uint16_t* out;
+  int num_heads;
+  float scale;
+  rlk_kv_block_view kv;
+  const int32_t* block_tables;
+  int max_blocks_per_seq;
+  const int32_t* positions;
+} rlk_block_attention_params;
+
+/* rlk_paged_attention_decode over a block-scaled cache (same work description,
+ * workspace and max_partitions contract).  An item whose token is negative is
+ * skipped (its rows of out are not known); an item whose position is negative
+ * attends to nothing and gets zeros.  Keys past the sequence's table row
+ * (max_blocks_per_seq * block_size) are not read. */
+int rlk_paged_attention_decode_blocks(const rlk_block_attention_params* params,
+                                      const rlk_decode_attention_work* work, hipStream_t stream);
+
+/* rlk_paged_attention_prefill over a block-scaled cache (same work
+ * description).  A negative sequence id is skipped; rows with nothing to
+ * attend to get zeros; keys past the sequence's table row are not read. */
+int rlk_paged_attention_prefill_blocks(const rlk_block_attention_params* params,
+                                       const rlk_prefill_attention_work* work,
+                                       hipStream_t stream);
+
+/* -------------------------------------------------- block tables on the GPU
+ *
+ * Extension: what the BatchBuilder writes on the host (positions, slots, work
+ * lists) made on the GPU from request lengths, with blocks taken from and
+ * given back to a ring of free blocks in device memory, so that a step needs
+ * no host round trip and can be captured whole.
+ *   ring       [capacity] block ids; the free ones are the `count` entries
+ *              from `head` on (modulo capacity)
+ *   state      {head, count, 0}: the third word belongs to the kernel and is
+ *              0 between calls
+ *   state_out  {head, count} after the call; NULL: written to state
+ * capacity is at least the number of blocks that can ever be free.  Calls on
+ * one pool must not overlap. */
+typedef struct rlk_block_pool {
+  int32_t* ring;
+  int capacity;
+  int32_t* state;
+  int32_t* state_out;
+} rlk_block_pool;
+
+typedef struct rlk_batch_tables {
+  const int32_t* past_len; /* [num_seqs] tokens that the cache holds */
+  const int32_t* new_len;  /* [num_seqs] tokens of this step; 0: idle; < 0: the
+                              sequence has ended, its blocks go back */
+  int num_seqs;
+  int num_rows;               /* token rows of the step, padding included */
+  int block_size;
+  int decode_query_threshold; /* as BatchBuilder's: at most so many new tokens
+                                 make decode items, more a prefill sequence */
+  int32_t* block_tables;      /* [num_seqs, max_blocks_per_seq], in and out */
+  int max_blocks_per_seq;
+  int32_t* q_start;      /* [num_seqs] first token row: the running sum of new_len */
+  int32_t* q_len;        /* [num_seqs] tokens accepted: new_len, or 0 */
+  int32_t* ctx_len;      /* [num_seqs] past + accepted; 0 for an ended sequence */
+  int32_t* positions;    /* [num_rows] */
+  int32_t* slot_mapping; /* [num_rows] block * block_size + offset */
+  int32_t* decode_token; /* [num_rows] the decode items; -1 behind the last */
+  int32_t* decode_seq;   /* [num_rows] 0 behind the last */
+  int32_t* prefill_seq;  /* [num_seqs] -1 behind the last */
+  int32_t* counts;       /* [4] rows asked for, decode items, prefill sequences,
+                            sequences refused */
+} rlk_batch_tables;
+
+/* Sequence s needs ceil((past + new) / block_size) - ceil(past / block_size)
+ * blocks; they are taken from the ring in the order of the sequences, and of
+ * the blocks within one, and entered into its table row.  A sequence is
+ * refused -- q_len 0, its table row as it was, its rows like padding -- when
+ * its needs with those of all sequences before it exceed the free blocks (one
+ * that needs none is not refused for that), when its tokens pass its table
+ * row or num_rows, or when past is negative.  Rows of refused sequences and
+ * rows behind the last get position 0 and slot -1 (the cache writes skip
+ * them).  The ceil(past / block_size) blocks of an ended sequence join the
+ * ring's tail in order and can be taken from the next call on; its table row
+ * is left as it was.  q_start and counts[0] saturate at 2^30.
+ * num_seqs > RLK_BATCH_TABLES_MAX_SEQS: RLK_EUNSUPPORTED; num_seqs and
+ * num_rows both 0: no-op. */
+#define RLK_BATCH_TABLES_MAX_SEQS 8192
+int rlk_build_batch_tables(const rlk_block_pool* pool, const rlk_batch_tables* tables,
+                           hipStream_t stream);
+
 /* ------------------------------------------------------ host-side helpers */
 
 /* IEEE fp16 <-> fp32 with round-to-nearest-even.

@@ -85,6 +85,45 @@ class PrefillAttentionWork(C.Structure):
                 ("ctx_len", C.c_void_p), ("num_seqs", C.c_int), ("max_q_tiles", C.c_int)]
 
 
+RLK_KV_BLOCK_INT8, RLK_KV_BLOCK_FP8 = 0, 1
+RLK_BATCH_TABLES_MAX_SEQS = 8192
+
+
+class KVBlockView(C.Structure):
+    """Mirror of rlk_kv_block_view (block-scaled 8-bit cache, an extension)."""
+
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p),
+                ("v_scale", C.c_void_p), ("num_blocks", C.c_int), ("block_size", C.c_int),
+                ("num_kv_heads", C.c_int), ("head_dim", C.c_int), ("format", C.c_int)]
+
+
+class BlockAttentionParams(C.Structure):
+    """Mirror of rlk_block_attention_params."""
+
+    _fields_ = [("q", C.c_void_p), ("q_stride", C.c_int), ("out", C.c_void_p),
+                ("num_heads", C.c_int), ("scale", C.c_float), ("kv", KVBlockView),
+                ("block_tables", C.c_void_p), ("max_blocks_per_seq", C.c_int),
+                ("positions", C.c_void_p)]
+
+
+class BlockPoolView(C.Structure):
+    """Mirror of rlk_block_pool."""
+
+    _fields_ = [("ring", C.c_void_p), ("capacity", C.c_int), ("state", C.c_void_p),
+                ("state_out", C.c_void_p)]
+
+
+class BatchTables(C.Structure):
+    """Mirror of rlk_batch_tables."""
+
+    _fields_ = [("past_len", C.c_void_p), ("new_len", C.c_void_p), ("num_seqs", C.c_int),
+                ("num_rows", C.c_int), ("block_size", C.c_int),
+                ("decode_query_threshold", C.c_int), ("block_tables", C.c_void_p),
+                ("max_blocks_per_seq", C.c_int)] + [(n, C.c_void_p) for n in (
+                    "q_start", "q_len", "ctx_len", "positions", "slot_mapping", "decode_token",
+                    "decode_seq", "prefill_seq", "counts")]
+
+
 class BatchShape(C.Structure):
     _fields_ = [(n, C.c_int) for n in (
         "num_tokens", "num_seqs", "num_logit_rows", "num_decode_items",
@@ -130,6 +169,14 @@ _SIGNATURES = {
     "rlk_paged_attention_prefill_ex": (_I, [C.POINTER(AttentionParams),
                                             C.POINTER(PrefillAttentionWork),
                                             C.POINTER(AttentionOptions), _P]),
+    "rlk_rope_and_write_kv_blocks": (_I, [_P, _P, _P, _I, _I, _P, _P, C.POINTER(KVBlockView), _P,
+                                          _P]),
+    "rlk_read_kv_blocks": (_I, [C.POINTER(KVBlockView), _P, _I, _P, _P, _P]),
+    "rlk_paged_attention_decode_blocks": (_I, [C.POINTER(BlockAttentionParams),
+                                               C.POINTER(DecodeAttentionWork), _P]),
+    "rlk_paged_attention_prefill_blocks": (_I, [C.POINTER(BlockAttentionParams),
+                                                C.POINTER(PrefillAttentionWork), _P]),
+    "rlk_build_batch_tables": (_I, [C.POINTER(BlockPoolView), C.POINTER(BatchTables), _P]),
     "rlk_gemv_w8a16": (_I, [_P, _I, _P, _P, _P, _I, _I, _P, _I, _P]),
     "rlk_gemv_w4a16": (_I, [_P, _I, _P, _P, _P, _I, _P, _I, _I, _P, _I, _P]),
     "rlk_gemv_w4a16_swiglu": (_I, [_P, _I, _P, _P, _P, _I, _I, _I, _P, _P]),

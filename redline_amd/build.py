@@ -21,6 +21,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 
 SOURCES = ["elementwise.hip", "rope_kv.hip", "attention.hip", "prefill.hip", "gemv_w4.hip", "gemv_stream.hip",
+           "kv_blocks.hip", "attention_blocks.hip", "prefill_blocks.hip", "batch_tables.hip",
            "host.cpp",
            "status.cpp"]
 

@@ -14,7 +14,7 @@ import ctypes as C
 import torch
 
 from . import _lib
-from ._lib import KVLayerView, check, lib
+from ._lib import KVBlockView, KVLayerView, check, lib
 
 __all__ = [
     "embedding_lookup", "embedding_rmsnorm", "fused_add_rmsnorm", "silu_and_mul", "silu_and_mul_interleaved",
@@ -23,7 +23,9 @@ __all__ = [
     "attention_params",
     "decode_work", "prefill_work", "paged_attention_prefill", "paged_attention_prefill_ex",
     "DecodeWorkspace", "kDecodePartitionSize", "gemv_w8a16", "gemv_w4a16", "gemv_w4a16_swiglu",
-    "kGemvW4MaxM",
+    "kGemvW4MaxM", "KVBlockFormat", "KVBlockCache", "kv_block_view", "rope_and_write_kv_blocks",
+    "read_kv_blocks", "block_attention_params", "paged_attention_decode_blocks",
+    "paged_attention_prefill_blocks", "BlockPool", "batch_tables", "build_batch_tables",
 ]
 
 kDecodePartitionSize = _lib.RLK_DECODE_PARTITION_SIZE
@@ -321,3 +323,155 @@ class KVCache:
     def tensors(self, i):
         """(k, v, k_scale, v_scale) torch views of layer i (scales None for FP16)."""
         return self._tensors[i]
+
+
+# ------------------------------------------------- block-scaled 8-bit KV cache
+
+class KVBlockFormat:
+    kINT8 = _lib.RLK_KV_BLOCK_INT8
+    kFP8 = _lib.RLK_KV_BLOCK_FP8  # e4m3, finite values only
+
+
+def kv_block_view(k, v, k_scale, v_scale, block_size, num_kv_heads, head_dim, fmt) -> KVBlockView:
+    """One layer of a block-scaled cache (extension): k, v [num_blocks, Hkv,
+    block_size * D] int8 (INT8) or uint8 (FP8) codes in the tile layout of rlk.h,
+    k_scale, v_scale fp32 [num_blocks, Hkv]."""
+    dt = torch.int8 if fmt == KVBlockFormat.kINT8 else torch.uint8
+    per = num_kv_heads * block_size * head_dim
+    if not isinstance(k, torch.Tensor) or per <= 0 or k.numel() % per != 0:
+        raise _lib.Error(_lib.RLK_EINVAL, "k must hold whole blocks")
+    nb = k.numel() // per
+    _need(v, nb * per, "v")
+    for t, w in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        _need(t, nb * num_kv_heads, w)
+    return KVBlockView(_ptr(k, dt, "k"), _ptr(v, dt, "v"), _ptr(k_scale, torch.float32, "k_scale"),
+                       _ptr(v_scale, torch.float32, "v_scale"), nb, block_size, num_kv_heads,
+                       head_dim, fmt)
+
+
+class KVBlockCache:
+    """Paged block-scaled cache (extension), zeroed: per layer K and V codes and
+    one fp32 scale per (block, kv head) of each.  Block 0 is the scratch block,
+    as in KVCache."""
+
+    def __init__(self, num_layers, num_blocks, num_kv_heads, head_dim, block_size=16,
+                 fmt=KVBlockFormat.kINT8, device="cuda"):
+        if num_blocks <= 1 or block_size <= 0 or num_layers <= 0:
+            raise _lib.Error(_lib.RLK_EINVAL, "bad KV cache config")
+        self.num_layers, self.num_blocks, self.block_size = num_layers, num_blocks, block_size
+        self.num_kv_heads, self.head_dim, self.fmt = num_kv_heads, head_dim, fmt
+        dt = torch.int8 if fmt == KVBlockFormat.kINT8 else torch.uint8
+        self._tensors = [tuple(torch.zeros((num_blocks, num_kv_heads, block_size * head_dim), dtype=dt,
+                                           device=device) for _ in range(2)) +
+                         tuple(torch.zeros((num_blocks, num_kv_heads), dtype=torch.float32, device=device)
+                               for _ in range(2)) for _ in range(num_layers)]
+        self._views = [kv_block_view(*t, block_size, num_kv_heads, head_dim, fmt) for t in self._tensors]
+
+    def layer(self, i) -> KVBlockView:
+        return self._views[i]
+
+    def tensors(self, i):
+        """(k, v, k_scale, v_scale) torch tensors of layer i (codes in the tile layout)."""
+        return self._tensors[i]
+
+
+def rope_and_write_kv_blocks(qkv, positions, slot_mapping, num_tokens, num_heads, cos_table, sin_table,
+                             kv: KVBlockView, qkv_bias=None, stream=None):
+    """Extension: RoPE on q/k heads (q in place) and the write of k/v into a
+    block-scaled cache; rows of a block come consecutively, at rising offsets."""
+    if num_tokens > 0:
+        _need(positions, num_tokens, "positions"); _need(slot_mapping, num_tokens, "slot_mapping")
+        cols = (num_heads + 2 * kv.num_kv_heads) * kv.head_dim
+        _need(qkv, num_tokens * cols, "qkv"); _need(qkv_bias, cols, "qkv_bias")
+    check(lib().rlk_rope_and_write_kv_blocks(
+        _ptr(qkv, torch.float16, "qkv"), _ptr(positions, torch.int32, "positions"),
+        _ptr(slot_mapping, torch.int32, "slot_mapping"), num_tokens, num_heads,
+        _ptr(cos_table, torch.float32, "cos_table"), _ptr(sin_table, torch.float32, "sin_table"),
+        C.byref(kv), _ptr(qkv_bias, torch.float16, "qkv_bias", True), _stream(stream)))
+
+
+def read_kv_blocks(kv: KVBlockView, slots, n, k_out=None, v_out=None, stream=None):
+    """Extension: the stored rows of `slots` as fp16 [n, Hkv * D] (code * scale);
+    a slot outside the pool leaves its rows as they were."""
+    if n > 0:
+        _need(slots, n, "slots")
+        for t, w in ((k_out, "k_out"), (v_out, "v_out")):
+            _need(t, n * kv.num_kv_heads * kv.head_dim, w)
+    check(lib().rlk_read_kv_blocks(C.byref(kv), _ptr(slots, torch.int32, "slots"), n,
+                                   _ptr(k_out, torch.float16, "k_out", True),
+                                   _ptr(v_out, torch.float16, "v_out", True), _stream(stream)))
+
+
+def block_attention_params(q, q_stride, out, num_heads, scale, kv: KVBlockView, block_tables,
+                           max_blocks_per_seq, positions) -> _lib.BlockAttentionParams:
+    """Parameters of the attention over a block-scaled cache (q may be a view
+    into qkv)."""
+    return _lib.BlockAttentionParams(
+        _ptr(q, torch.float16, "q"), q_stride, _ptr(out, torch.float16, "out"), num_heads,
+        float(scale), kv, _ptr(block_tables, torch.int32, "block_tables"), max_blocks_per_seq,
+        _ptr(positions, torch.int32, "positions"))
+
+
+def paged_attention_decode_blocks(params: _lib.BlockAttentionParams, work: _lib.DecodeAttentionWork,
+                                  stream=None):
+    """Extension: flash-decoding attention over a block-scaled cache; items with
+    a negative token are skipped."""
+    check(lib().rlk_paged_attention_decode_blocks(C.byref(params), C.byref(work), _stream(stream)))
+
+
+def paged_attention_prefill_blocks(params: _lib.BlockAttentionParams, work: _lib.PrefillAttentionWork,
+                                   stream=None):
+    """Extension: causal prefill attention over a block-scaled cache; negative
+    sequence ids are skipped."""
+    check(lib().rlk_paged_attention_prefill_blocks(C.byref(params), C.byref(work), _stream(stream)))
+
+
+# ------------------------------------------------------- block tables on the GPU
+
+class BlockPool:
+    """Free blocks of a paged cache in device memory (extension): `ring` int32
+    [capacity] block ids, `state` int32 [3] {head, count, 0} with the count free
+    ones from head on; with `state_out` int32 [2] a call leaves `state` as it was
+    and writes the new {head, count} there."""
+
+    def __init__(self, ring, state, state_out=None):
+        _need(state, 3, "state"); _need(state_out, 2, "state_out")
+        self.ring, self.state, self.state_out = ring, state, state_out
+        self.view = _lib.BlockPoolView(_ptr(ring, torch.int32, "ring"), ring.numel(),
+                                       _ptr(state, torch.int32, "state"),
+                                       _ptr(state_out, torch.int32, "state_out", True))
+
+    @classmethod
+    def of_blocks(cls, num_blocks, device="cuda"):
+        """All blocks of a cache of num_blocks but the scratch block 0, free."""
+        ring = torch.arange(1, num_blocks, dtype=torch.int32, device=device)
+        return cls(ring, torch.tensor([0, num_blocks - 1, 0], dtype=torch.int32, device=device))
+
+
+def batch_tables(pool: BlockPool, past_len, new_len, num_seqs, num_rows, block_size,
+                 decode_query_threshold, block_tables, max_blocks_per_seq, q_start, q_len, ctx_len,
+                 positions, slot_mapping, decode_token, decode_seq, prefill_seq, counts):
+    """What build_batch_tables reads and writes (rlk_batch_tables); all int32."""
+    for t, n, w in ((past_len, num_seqs, "past_len"), (new_len, num_seqs, "new_len"),
+                    (block_tables, num_seqs * max_blocks_per_seq, "block_tables"),
+                    (q_start, num_seqs, "q_start"), (q_len, num_seqs, "q_len"),
+                    (ctx_len, num_seqs, "ctx_len"), (prefill_seq, num_seqs, "prefill_seq"),
+                    (positions, num_rows, "positions"), (slot_mapping, num_rows, "slot_mapping"),
+                    (decode_token, num_rows, "decode_token"), (decode_seq, num_rows, "decode_seq"),
+                    (counts, 4, "counts")):
+        _need(t, n, w)
+    i = lambda t, w: _ptr(t, torch.int32, w)  # noqa: E731
+    work = _lib.BatchTables(
+        i(past_len, "past_len"), i(new_len, "new_len"), num_seqs, num_rows, block_size,
+        decode_query_threshold, i(block_tables, "block_tables"), max_blocks_per_seq,
+        i(q_start, "q_start"), i(q_len, "q_len"), i(ctx_len, "ctx_len"), i(positions, "positions"),
+        i(slot_mapping, "slot_mapping"), i(decode_token, "decode_token"),
+        i(decode_seq, "decode_seq"), i(prefill_seq, "prefill_seq"), i(counts, "counts"))
+    return pool, work
+
+
+def build_batch_tables(tables, stream=None):
+    """Extension: positions, slots, work lists and block tables of a step from
+    its request lengths, with blocks from the pool; `tables` from batch_tables()."""
+    pool, work = tables
+    check(lib().rlk_build_batch_tables(C.byref(pool.view), C.byref(work), _stream(stream)))
