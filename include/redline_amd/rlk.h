@@ -330,8 +330,8 @@ int rlk_paged_attention_prefill_ex(const rlk_attention_params* params,
  *   v  [num_blocks, num_kv_heads][block_size / 16 tiles][E/4 g][4 quads r][16 m]
  *      [4 j][4 i]                        holds dim  E m + 4 g + j  of the tile's
  *                                        token 4 r + i
- *   k_scale, v_scale  fp32 [num_blocks, num_kv_heads]: 0 (every code is 0), or
- *      a power of two from 2^-24 to 2^10; a stored value is code * scale, an
+ *   k_scale, v_scale  fp32 [num_blocks, num_kv_heads]: 0 (every code is a
+ *      zero), or a power of two from 2^-24 to 2^10; a stored value is code * scale, an
  *      exact fp16 value.
  * Codes are int8, or e4m3 (the finite-only form: largest value 448, no
  * infinities).  Block ids read from block tables are held inside the pool: an

@@ -104,10 +104,10 @@ __device__ __forceinline__ float join_scale(float old, float amax, float& ratio)
   return s;
 }
 
-// K of one head: lane p of LPT lanes per token.
+// K of one head: lane p of D / 16 lanes per token; pos: the run's positions.
 template <int D, int BS, bool kFp8>
-__device__ __forceinline__ void write_k(const WriteArgs& a, const Run& r, int pos_lane, int chunk0,
-                                        int kvh, int l16) {
+__device__ __forceinline__ void write_k(const WriteArgs& a, const Run& r, const int* pos, int kvh,
+                                        int l16) {
   constexpr int kLanes = D / 16, kTok = 16 / kLanes;  // lanes per token, tokens in flight
   constexpr int kIts = BS / kTok;
   const int p = l16 % kLanes, sub = l16 / kLanes;
@@ -124,7 +124,7 @@ __device__ __forceinline__ void write_k(const WriteArgs& a, const Run& r, int po
       const _Float16* row = a.qkv + static_cast<int64_t>(r.row0 + j) * heads * D;
       f32x8 x0 = load_biased(row, a.bias, col + 8 * p);
       f32x8 x1 = load_biased(row, a.bias, col + D / 2 + 8 * p);
-      rotate8<D>(a, __shfl(pos_lane, r.row0 + j - chunk0, kWave), 8 * p, x0, x1);
+      rotate8<D>(a, pos[j], 8 * p, x0, x1);
       amax = amax8(x1, amax8(x0, amax));
       x[it][0] = pack8(x0);
       x[it][1] = pack8(x1);
@@ -251,14 +251,18 @@ constexpr int kWriteThreads = 256;
 // The runs that start in rows chunk0 .. chunk0 + kRows - 1, for 4 of the
 // 2 * hkv (K heads, then V heads): head unit 4 * group + lane / 16.
 template <int D, int BS, bool kFp8, int kRows>
-__device__ __forceinline__ void write_chunk(const WriteArgs& a, int chunk0, int group, int lane) {
+__device__ __forceinline__ void write_chunk(const WriteArgs& a, int chunk0, int group, int lane,
+                                            int* pos) {
   static_assert(kRows + BS <= kWave, "a chunk's rows and the last run's rest fit one wave");
   const int hkv = a.kv.num_kv_heads;
   const int row = chunk0 + lane;
   const int slot = row < a.num_tokens ? a.slots[row] : -1;
   int before = __shfl_up(slot, 1, kWave);
   if (lane == 0) before = chunk0 > 0 ? a.slots[chunk0 - 1] : -1;
-  const int pos = row < a.num_tokens ? a.positions[row] : 0;
+  // positions of the rows, in LDS: the lanes of a K head need those of other
+  // rows, and lanes of the wave that do a V head are not there to hand them over
+  pos[lane] = row < a.num_tokens ? a.positions[row] : 0;
+  __builtin_amdgcn_wave_barrier();
   const bool valid = slot >= 0 && slot / BS < a.kv.num_blocks;
   // a row starts a run unless it continues the block of the row before
   const bool start = !valid || slot % BS == 0 || slot != before + 1;
@@ -273,7 +277,7 @@ __device__ __forceinline__ void write_chunk(const WriteArgs& a, int chunk0, int 
     const int sl = __builtin_amdgcn_readlane(slot, i);
     const Run r = {chunk0 + i, n, sl / BS, sl % BS};
     if (unit < hkv) {
-      write_k<D, BS, kFp8>(a, r, pos, chunk0, unit, lane % 16);
+      write_k<D, BS, kFp8>(a, r, pos + i, unit, lane % 16);
     } else if (unit < 2 * hkv) {
       write_v<D, BS, kFp8>(a, r, unit - hkv, lane % 16);
     }
@@ -282,12 +286,14 @@ __device__ __forceinline__ void write_chunk(const WriteArgs& a, int chunk0, int 
 
 template <int D, int BS, bool kFp8, int kRows>
 __global__ __launch_bounds__(kWriteThreads) void write_kv_blocks_kernel(WriteArgs a) {
+  __shared__ int pos[kWriteThreads / kWave][kWave];
   const int tid = threadIdx.x, lane = tid % kWave;
   if (static_cast<int>(blockIdx.x) < a.kv_groups) {
     const int w = blockIdx.x * (kWriteThreads / kWave) + tid / kWave;
     const int chunk = w / a.head_groups;
     if (chunk * kRows >= a.num_tokens) return;
-    write_chunk<D, BS, kFp8, kRows>(a, chunk * kRows, w - chunk * a.head_groups, lane);
+    write_chunk<D, BS, kFp8, kRows>(a, chunk * kRows, w - chunk * a.head_groups, lane,
+                                       pos[tid / kWave]);
     return;
   }
   // q heads: 8 rotation pairs per lane
