@@ -26,6 +26,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <cstdint>
+#include <type_traits>
 
 #include "kv_blocks.hpp"
 
@@ -35,13 +36,23 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kPart = RLK_DECODE_PARTITION_SIZE;
-constexpr int kStepTokens = 32;
+constexpr int kStep = 32;        // keys of a wave step
 constexpr int kMaxSlots = 4096;  // workspace slots that the merge joins
+constexpr int kMaxItemsLds = 1024;
+constexpr int kMinRange = 512 / kStep, kMaxRange = 1024 / kStep;  // steps of a wave's range
+// Steps in flight and ranges per CU of the range form.  Two waves of a SIMD with 3
+// steps of 8 KB each in flight; measured at 32 items to 8191 keys (8 kv heads of
+// 128, INT8) / 12 items to 40000 (4 kv heads, e4m3) / 32 items of 8000-8191, us:
+// 3 steps and 2 waves 48.4 / 60.4 / 91.6, 4 and 2 48.9 / 59.7 / 91.3, 2 and 3
+// 46.3 / 63.8 / 92.4, 2 and 4 (spills) 63.6 / 81.5 / 115.7; at D = 64 all within 5%.
+constexpr int kDepth = 3, kWavesPerCu = 8;
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct DecodeArgs {
   rlk_block_attention_params p;
   rlk_decode_attention_work w;
-  int wave_tokens;  // keys of a wave: a multiple of 64
+  int group_tokens;  // grid form: keys of a workgroup
+  int ranges;        // range form: ranges that the call is split into, at least
 };
 
 // Keys that an item attends to: its context, inside its table row and the
@@ -49,178 +60,247 @@ struct DecodeArgs {
 __device__ __forceinline__ int keys_of(const DecodeArgs& a, int token) {
   const int64_t most = min(static_cast<int64_t>(a.p.max_blocks_per_seq) * a.p.kv.block_size,
                            static_cast<int64_t>(a.w.max_partitions) * kPart);
-  return static_cast<int>(min(static_cast<int64_t>(a.p.positions[token]) + 1, most));
+  return static_cast<int>(max(min(static_cast<int64_t>(a.p.positions[token]) + 1, most), static_cast<int64_t>(0)));
 }
 
-// The codes of one wave step in flight: two tiles.
+// The codes of one wave step in flight: two tiles of K and of V.
 template <int D>
 struct StepCodes {
-  u32x4 r[2][D / 64];
+  u32x4 k[2][D / 64], v[2][D / 64];
 };
 
-template <int D>
-__device__ __forceinline__ void issue(StepCodes<D>& s, const uint8_t* t0, const uint8_t* t1, int lane) {
-  __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-  for (int x = 0; x < D / 64; ++x) {
-    s.r[0][x] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(t0 + x * 1024) + lane);
-    s.r[1][x] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(t1 + x * 1024) + lane);
-  }
-  __builtin_amdgcn_sched_barrier(0);
+__device__ __forceinline__ float lane_value(float v, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
 
-template <int D, int G>
-struct DecodeLds {
-  float o[kWaves][G][D];
-  float m[kWaves][G], l[kWaves][G];
+// What a wave has of its keys: column c = lane % 16 (head), rows 4 (lane / 16) + i
+// of output tile d; m and l per head, the same in the 4 row groups after finish().
+template <int D>
+struct WaveState {
+  f32x4 o[D / 16];
+  float m = -FLT_MAX, l = 0.f, vref = 0.f;  // o is relative to the V scale vref
+
+  __device__ __forceinline__ WaveState() {
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  __device__ __forceinline__ void finish() { l = rows_sum<true>(rows_sum<false>(l)); }
+  // element i of output tile d: dim
+  __device__ __forceinline__ static int dim(int d, int i) {
+    return (D / 16) * (4 * (static_cast<int>(threadIdx.x) % kWave / 16) + i) + d;
+  }
 };
 
-template <int D, int G, bool kFp8>
-__global__ __launch_bounds__(kThreads, 4) void decode_blocks_kernel(DecodeArgs a) {
-  constexpr int E = D / 16, kX = D / 64;
-  constexpr float kLog2e = 1.4426950408889634f;
-  __shared__ DecodeLds<D, G> s;
-  const rlk_block_attention_params& p = a.p;
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const int rho = lane / 16, c = lane % 16;
-  const int slot = blockIdx.x, kvh = blockIdx.y, item = blockIdx.z;
-  const int token = a.w.item_token[item];
-  if (token < 0) return;
-  const int n = keys_of(a, token);
-  const int group_tokens = kWaves * a.wave_tokens;
-  _Float16* out = reinterpret_cast<_Float16*>(p.out) + (static_cast<int64_t>(token) * p.num_heads + kvh * G) * D;
-  if (slot * group_tokens >= n) {
-    if (slot == 0)  // nothing to attend to
-      for (int i = tid; i < G * D; i += kThreads) out[i] = static_cast<_Float16>(0.f);
-    return;
-  }
-  const int seq = a.w.item_seq[item];
-  const int first = slot * group_tokens + wave * a.wave_tokens;
-  const int count = min(a.wave_tokens, n - first);  // <= 0: a wave without keys
+// Block of tile tile0 + lane in each lane; entries past the table row repeat its
+// last one.
+__device__ __forceinline__ int table_entries(const DecodeArgs& a, int seq, int tile0) {
+  const int t = tile0 + static_cast<int>(threadIdx.x) % kWave;
+  const int b = min(a.p.kv.block_size == 32 ? t / 2 : t, a.p.max_blocks_per_seq - 1);
+  return a.p.block_tables[static_cast<int64_t>(seq) * a.p.max_blocks_per_seq + b];
+}
 
-  f32x4 o[E];
+// One wave over `count` keys (at most 1024) from tile tile0 of one (item, kv
+// head); blk: table_entries(tile0).  kDepth steps are in flight: each step's
+// codes are requested kDepth steps ahead into the registers that it frees.
+template <int D, int G, bool kFp8, int kDepth>
+__device__ __forceinline__ void attend(const DecodeArgs& a, WaveState<D>& w, int token, int kvh, int tile0,
+                                       int count, int blk) {
+  constexpr int E = D / 16, kX = D / 64;
+  const rlk_block_attention_params& p = a.p;
+  const int lane = threadIdx.x % kWave, rho = lane / 16, c = lane % 16;
+  const int tiles = (count + kTileTokens - 1) / kTileTokens, steps = (tiles + 1) / 2;
+  const int tsh = p.kv.block_size == 32 ? 1 : 0;  // log2 tiles of a block
+  blk = static_cast<uint32_t>(blk) < static_cast<uint32_t>(p.kv.num_blocks) ? blk : 0;
+  const uint32_t cell = static_cast<uint32_t>(blk) * p.kv.num_kv_heads + kvh;
+  const uint32_t tile = (cell << tsh) + ((tile0 + lane) & tsh);  // layout tile of the pool
+  const uint8_t* kbase = static_cast<const uint8_t*>(p.kv.k);
+  const uint8_t* vbase = static_cast<const uint8_t*>(p.kv.v);
+  StepCodes<D> codes[kDepth];
+  // steps past the last repeat its last tile, so that every request is unconditional
+  auto issue = [&](StepCodes<D>& s, int st) {
+    __builtin_amdgcn_sched_barrier(0);
+    uint64_t at[2];
 #pragma unroll
-  for (int d = 0; d < E; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -FLT_MAX, l = 0.f, vref = 0.f;
-  if (count > 0) {
-    const int bs = p.kv.block_size, tpb = bs / kTileTokens, hkv = p.kv.num_kv_heads;
-    const int tiles = (count + kTileTokens - 1) / kTileTokens, tile0 = first / kTileTokens;
-    // lane t < tiles: the block of the wave's tile t (a wave has at most 64)
-    const int bt = (tile0 + min(lane, tiles - 1)) / tpb;
-    int blk = p.block_tables[static_cast<int64_t>(seq) * p.max_blocks_per_seq + bt];
-    blk = static_cast<uint32_t>(blk) < static_cast<uint32_t>(p.kv.num_blocks) ? blk : 0;
-    const uint8_t* kbase = static_cast<const uint8_t*>(p.kv.k);
-    const uint8_t* vbase = static_cast<const uint8_t*>(p.kv.v);
-    auto cell_of = [&](int t) {  // uniform; tiles past the last repeat it
-      return static_cast<int64_t>(__builtin_amdgcn_readlane(blk, min(t, tiles - 1))) * hkv + kvh;
-    };
-    auto tile_at = [&](const uint8_t* base, int t) {
-      return base + (cell_of(t) * tpb + (tile0 + min(t, tiles - 1)) % tpb) * (kTileTokens * D);
-    };
-    StepCodes<D> kc, vc;
-    issue<D>(kc, tile_at(kbase, 0), tile_at(kbase, 1), lane);
-    issue<D>(vc, tile_at(vbase, 0), tile_at(vbase, 1), lane);
-    // q: column c = head c, zero past the group
-    const _Float16* q = reinterpret_cast<const _Float16*>(p.q) + static_cast<int64_t>(token) * p.q_stride +
-                        (kvh * G + min(c, G - 1)) * D;
-    f16x8 qb[kX][2];
+    for (int t = 0; t < 2; ++t)
+      at[t] = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(
+                  static_cast<int>(tile), min(2 * st + t, tiles - 1)))) * (kTileTokens * D);
 #pragma unroll
-    for (int x = 0; x < kX; ++x)
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const u32x4 v = load16(q + h * (D / 2) + 8 * (4 * x + rho));
-        qb[x][h] = __builtin_bit_cast(f16x8, c < G ? v : u32x4{0, 0, 0, 0});
-      }
-    const float qscale = p.scale * kLog2e;
-    const int steps = (tiles + 1) / 2;
-    for (int st = 0; st < steps; ++st) {
-      const int64_t c0 = cell_of(2 * st), c1 = cell_of(2 * st + 1);
-      const float ks[2] = {p.kv.k_scale[c0] * qscale, p.kv.k_scale[c1] * qscale};
-      const float vs[2] = {p.kv.v_scale[c0], p.kv.v_scale[c1]};
-      f32x4 acc[2];
+      for (int x = 0; x < kX; ++x)
+        s.k[t][x] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kbase + at[t] + x * 1024) + lane);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int x = 0; x < kX; ++x)
+      for (int x = 0; x < kX; ++x)
+        s.v[t][x] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vbase + at[t] + x * 1024) + lane);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // lane t: the scales of tile t
+  float ksl = p.kv.k_scale[cell], vsl = p.kv.v_scale[cell];
+  // q: column c = head c, zero past the group
+  const _Float16* q = reinterpret_cast<const _Float16*>(p.q) + static_cast<int64_t>(token) * p.q_stride +
+                      (kvh * G + min(c, G - 1)) * D;
+  f16x8 qb[kX][2];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const f16x4 lo = codes_to_f16<kFp8>(kc.r[t][x][2 * h]), hi = codes_to_f16<kFp8>(kc.r[t][x][2 * h + 1]);
-            const f16x8 av = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, qb[x][h], acc[t], 0, 0, 0);
-          }
-      }
-      issue<D>(kc, tile_at(kbase, 2 * st + 2), tile_at(kbase, 2 * st + 3), lane);
-      // this lane: tokens 4 rho + i of both tiles, head c
-      const int left = count - st * kStepTokens;  // keys of this step (may pass 32)
-      float e[2][4];
+  for (int x = 0; x < kX; ++x)
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+    for (int h = 0; h < 2; ++h) qb[x][h] = __builtin_bit_cast(f16x8, load16(q + h * (D / 2) + 8 * (4 * x + rho)));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[t][i] = acc[t][i] * ks[t];
-      if (left < kStepTokens) {  // uniform: only a wave's last step
+  for (int b = 0; b < kDepth; ++b) issue(codes[b], b);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+  for (int x = 0; x < kX; ++x)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (16 * t + 4 * rho + i >= left) e[t][i] = -FLT_MAX;
-        // bytes of tokens past the context may be anything (an e4m3 NaN too)
+    for (int h = 0; h < 2; ++h)
+      if (c >= G) qb[x][h] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+  ksl *= p.scale * kLog2e;
+  float vmax = lane < tiles ? vsl : 0.f;
+  vmax = fmaxf(w.vref, rows_max<true>(rows_max<false>(group_max<16>(vmax))));
+  vsl *= inv_scale(vmax);
+  if (w.vref > 0.f && w.vref != vmax) {  // continued: o moves to the larger reference
+    const float f = w.vref * inv_scale(vmax);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int keep = min(max(left - 16 * t - 4 * rho, 0), 4);
-          const uint32_t mask = keep == 0 ? 0u : 0xffffffffu >> (32 - 8 * keep);
+    for (int d = 0; d < E; ++d) w.o[d] *= f;
+  }
+  w.vref = vmax;
+  auto step = [&](StepCodes<D>& s, int st, bool tail) {
+    f32x4 acc[2];
 #pragma unroll
-          for (int x = 0; x < kX; ++x) vc.r[t][x] &= u32x4{mask, mask, mask, mask};
-        }
-      }
-      float mx = fmaxf(fmaxf(fmaxf(e[0][0], e[0][1]), fmaxf(e[0][2], e[0][3])),
-                       fmaxf(fmaxf(e[1][0], e[1][1]), fmaxf(e[1][2], e[1][3])));
-      mx = rows_max<true>(rows_max<false>(mx));
-      const float mn = fmaxf(m, mx), vn = fmaxf(vref, fmaxf(vs[0], vs[1]));
-      if (__any(mn != m) || vn != vref) {  // the output so far moves to the new references
-        const float f = __builtin_amdgcn_exp2f(m - mn);
-        l *= f;
-        const float fo = f * vref * inv_scale(vn);
-#pragma unroll
-        for (int d = 0; d < E; ++d) o[d] *= fo;
-        m = mn;
-        vref = vn;
-      }
-      const float vi = inv_scale(vref);
-      const float w[2] = {vs[0] * vi, vs[1] * vi};
-      f16x8 b;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float pr = __builtin_amdgcn_exp2f(e[t][i] - m);
-          l += pr;
-          b[4 * t + i] = static_cast<_Float16>(pr * w[t]);
-        }
+    for (int t = 0; t < 2; ++t) {
+      acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int x = 0; x < kX; ++x)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const f16x4 lo = codes_to_f16<kFp8>(vc.r[0][x][j]), hi = codes_to_f16<kFp8>(vc.r[1][x][j]);
+        for (int h = 0; h < 2; ++h) {
+          const f16x4 lo = codes_to_f16<kFp8>(s.k[t][x][2 * h]), hi = codes_to_f16<kFp8>(s.k[t][x][2 * h + 1]);
           const f16x8 av = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-          o[4 * x + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, b, o[4 * x + j], 0, 0, 0);
+          acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, qb[x][h], acc[t], 0, 0, 0);
         }
-      issue<D>(vc, tile_at(vbase, 2 * st + 2), tile_at(vbase, 2 * st + 3), lane);
     }
-    l = rows_sum<true>(rows_sum<false>(l));
+    // this lane: tokens 4 rho + i of both tiles, head c
+    const int t1 = min(2 * st + 1, tiles - 1);
+    const float ks[2] = {lane_value(ksl, 2 * st), lane_value(ksl, t1)};
+    const float vs[2] = {lane_value(vsl, 2 * st), lane_value(vsl, t1)};
+    float e[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[t][i] = acc[t][i] * ks[t];
+    if (tail) {  // uniform
+      const int left = count - st * kStep;  // keys of this step
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (16 * t + 4 * rho + i >= left) e[t][i] = -FLT_MAX;
+        // bytes of tokens past the context may be anything (an e4m3 NaN too)
+        const int keep = min(max(left - 16 * t - 4 * rho, 0), 4);
+        const uint32_t mask = keep == 0 ? 0u : 0xffffffffu >> (32 - 8 * keep);
+#pragma unroll
+        for (int x = 0; x < kX; ++x) s.v[t][x] &= u32x4{mask, mask, mask, mask};
+      }
+    }
+    float mx = fmaxf(fmaxf(fmaxf(e[0][0], e[0][1]), fmaxf(e[0][2], e[0][3])),
+                     fmaxf(fmaxf(e[1][0], e[1][1]), fmaxf(e[1][2], e[1][3])));
+    mx = rows_max<true>(rows_max<false>(mx));
+    const float mn = fmaxf(w.m, mx);
+    if (__any(mn != w.m)) {  // the output so far moves to the new maximum
+      const float f = __builtin_amdgcn_exp2f(w.m - mn);
+      w.l *= f;
+#pragma unroll
+      for (int d = 0; d < E; ++d) w.o[d] *= f;
+      w.m = mn;
+    }
+    f16x8 b;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float pr = __builtin_amdgcn_exp2f(e[t][i] - w.m);
+        w.l += pr;
+        b[4 * t + i] = static_cast<_Float16>(pr * vs[t]);
+      }
+#pragma unroll
+    for (int x = 0; x < kX; ++x)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f16x4 lo = codes_to_f16<kFp8>(s.v[0][x][j]), hi = codes_to_f16<kFp8>(s.v[1][x][j]);
+        const f16x8 av = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        w.o[4 * x + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, b, w.o[4 * x + j], 0, 0, 0);
+      }
+  };
+  int st = 0;
+  for (; st + kDepth < steps; st += kDepth) {
+#pragma unroll
+    for (int b = 0; b < kDepth; ++b) {
+      step(codes[b], st + b, false);
+      issue(codes[b], st + b + kDepth);
+    }
   }
+#pragma unroll
+  for (int b = 0; b < kDepth; ++b)
+    if (st + b < steps) step(codes[b], st + b, (st + b + 1) * kStep > count);
+}
+
+// An item's output row of one head, or its partial in a slot of the workspace.
+// The last slot of an item is followed by the sum -1, which no sum of
+// exponentials takes; the rows of an item written whole have it in slot 0.
+__device__ __forceinline__ int64_t slot_row(const DecodeArgs& a, int item, int head) {
+  return (static_cast<int64_t>(item) * a.p.num_heads + head) * a.w.max_partitions;
+}
+__device__ __forceinline__ _Float16* out_row(const DecodeArgs& a, int token, int head, int D) {
+  return reinterpret_cast<_Float16*>(a.p.out) + (static_cast<int64_t>(token) * a.p.num_heads + head) * D;
+}
+__device__ __forceinline__ void mark_whole(const DecodeArgs& a, int item, int head) {
+  if (a.w.max_partitions > 1) a.w.ws_sum[slot_row(a, item, head)] = -1.f;
+}
+
+// The rows of an item that attends to nothing, for one kv head, by `threads`
+// threads.
+template <int D, int G>
+__device__ __forceinline__ void attend_nothing(const DecodeArgs& a, int item, int token, int kvh) {
+  for (int i = threadIdx.x; i < G * D; i += kThreads) {
+    out_row(a, token, kvh * G, D)[i] = static_cast<_Float16>(0.f);
+    if (i % D == 0) mark_whole(a, item, kvh * G + i / D);
+  }
+}
+
+// Grid form, for calls of few keys: one workgroup per (group_tokens keys, kv
+// head, item), whose waves split the keys and meet in LDS.
+template <int D, int G, bool kFp8>
+__global__ __launch_bounds__(kThreads, 2) void decode_blocks_grid_kernel(DecodeArgs a) {
+  struct Lds {
+    float o[kWaves][G][D];
+    float m[kWaves][G], l[kWaves][G];
+  };
+  __shared__ Lds s;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int slot = blockIdx.x, kvh = blockIdx.y, item = blockIdx.z;
+  const int token = a.w.item_token[item];
+  if (token < 0) return;
+  const int wave_tokens = a.group_tokens / kWaves, first = slot * a.group_tokens + wave * wave_tokens;
+  const int blk = table_entries(a, a.w.item_seq[item], first / kTileTokens);
+  const int n = keys_of(a, token);
+  if (slot * a.group_tokens >= n) {
+    if (slot == 0) attend_nothing<D, G>(a, item, token, kvh);
+    return;
+  }
+  WaveState<D> w;
+  if (first < n) attend<D, G, kFp8, 2>(a, w, token, kvh, first / kTileTokens, min(wave_tokens, n - first), blk);
+  w.finish();
+  const int c = lane % 16;
   if (c < G) {
 #pragma unroll
-    for (int d = 0; d < E; ++d)
+    for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s.o[wave][c][E * (4 * rho + i) + d] = o[d][i] * vref;
-    if (rho == 0) {
-      s.m[wave][c] = m;
-      s.l[wave][c] = l;
+      for (int i = 0; i < 4; ++i) s.o[wave][c][w.dim(d, i)] = w.o[d][i] * w.vref;
+    if (lane < 16) {
+      s.m[wave][c] = w.m;
+      s.l[wave][c] = w.l;
     }
   }
   __syncthreads();
-  const bool whole = n <= group_tokens;  // the item's only workgroup
+  const bool whole = n <= a.group_tokens, last = (slot + 1) * a.group_tokens >= n;
   for (int i = tid; i < G * D; i += kThreads) {
     const int g = i / D, d = i % D;
     float M = s.m[0][g];
@@ -234,46 +314,195 @@ __global__ __launch_bounds__(kThreads, 4) void decode_blocks_kernel(DecodeArgs a
       acc += f * s.o[v][g][d];
     }
     if (whole) {
-      out[i] = static_cast<_Float16>(acc / L);
+      out_row(a, token, kvh * G, D)[i] = static_cast<_Float16>(acc / L);
+      if (d == 0) mark_whole(a, item, kvh * G + g);
     } else {
-      const int64_t row = (static_cast<int64_t>(item) * p.num_heads + kvh * G + g) * a.w.max_partitions + slot;
+      const int64_t row = slot_row(a, item, kvh * G + g) + slot;
       a.w.ws_out[row * D + d] = acc;
       if (d == 0) {
         a.w.ws_max[row] = M;
         a.w.ws_sum[row] = L;
+        if (last && slot + 1 < a.w.max_partitions) a.w.ws_sum[row + 1] = -1.f;
       }
     }
   }
 }
 
-// Joins the partials of one (item, head): lane d takes dim d.
+// Range form: the steps of all (item, kv head) pairs in one row, cut into equal
+// ranges, one a wave, each with its own partial: no wave waits for another and
+// none has more to do, whatever the contexts are.  Every workgroup sums the
+// items' steps itself.
+template <int D, int G, bool kFp8>
+__global__ __launch_bounds__(kThreads, 2) void decode_blocks_range_kernel(DecodeArgs a) {
+  __shared__ int it_token[kMaxItemsLds], it_seq[kMaxItemsLds], it_keys[kMaxItemsLds];
+  __shared__ int it_before[kMaxItemsLds + 1];  // steps before item i, of one kv head
+  __shared__ int wave_tot[kWaves];
+  const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int items = a.w.num_items, hkv = a.p.kv.num_kv_heads;
+  const int per = (items + kThreads - 1) / kThreads;
+  const int i0 = min(tid * per, items), i1 = min(i0 + per, items);
+  int sum = 0;
+  for (int i = i0; i < i1; ++i) {
+    const int token = a.w.item_token[i];
+    it_seq[i] = a.w.item_seq[i];
+    const int n = token < 0 ? 0 : keys_of(a, token);
+    it_token[i] = token;
+    it_keys[i] = n;
+    sum += (n + kStep - 1) / kStep;
+  }
+  int incl = sum;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int v = __shfl_up(incl, o, kWave);
+    if (lane >= o) incl += v;
+  }
+  if (lane == kWave - 1) wave_tot[wave] = incl;
+  __syncthreads();
+  int before = incl - sum;
+  for (int v = 0; v < wave; ++v) before += wave_tot[v];
+  for (int i = i0; i < i1; ++i) {
+    it_before[i] = before;
+    before += (it_keys[i] + kStep - 1) / kStep;
+  }
+  if (tid == kThreads - 1) it_before[items] = before;
+  __syncthreads();
+  for (int i = blockIdx.x; i < items; i += gridDim.x) {  // (uniform: rarely anything to do)
+    if (it_keys[i] > 0) continue;
+    const int token = it_token[i];
+    if (token >= 0)
+      for (int h = 0; h < hkv; ++h) attend_nothing<D, G>(a, i, token, h);
+  }
+  // (steps fit 31 bits: the launch rule sees to that)
+  const int total = __builtin_amdgcn_readfirstlane(it_before[items]) * hkv;
+  const int range = min(max((total + a.ranges - 1) / a.ranges, kMinRange), kMaxRange);
+  const int r = blockIdx.x * kWaves + wave;
+  if (r > total / range) return;
+  int u = r * range;
+  const int end = min(u + range, total);
+  if (u >= end) return;
+  int lo = 0, hi = items - 1;  // the last item that starts at or before u (the others there are empty)
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (it_before[mid] * hkv <= u) lo = mid; else hi = mid - 1;
+  }
+  int item = __builtin_amdgcn_readfirstlane(lo);
+  while (u < end) {
+    const int n = __builtin_amdgcn_readfirstlane(it_keys[item]), steps = (n + kStep - 1) / kStep;
+    if (steps == 0) {
+      ++item;
+      continue;
+    }
+    const int item0 = __builtin_amdgcn_readfirstlane(it_before[item]) * hkv;
+    const int kvh = (u - item0) / steps;
+    const int seg = item0 + kvh * steps;  // where this (item, kv head) starts
+    const int at = u - seg, todo = min(end - u, steps - at);
+    const int token = __builtin_amdgcn_readfirstlane(it_token[item]), tile0 = 2 * at;
+    WaveState<D> w;
+    attend<D, G, kFp8, kDepth>(a, w, token, kvh, tile0, min(todo * kStep, n - at * kStep),
+                          table_entries(a, __builtin_amdgcn_readfirstlane(it_seq[item]), tile0));
+    w.finish();
+    const int c = lane % 16;
+    if (c < G) {
+      const int head = kvh * G + c;
+      if (todo == steps) {
+        const float inv = w.vref / w.l;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          _Float16* o = out_row(a, token, head, D) + w.dim(0, i);
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) o[d] = static_cast<_Float16>(w.o[d][i] * inv);
+        }
+        if (lane < 16) mark_whole(a, item, head);
+      } else {
+        const int slot = r - seg / range;
+        const int64_t row = slot_row(a, item, head) + slot;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float* o = a.w.ws_out + row * D + w.dim(0, i);
+#pragma unroll
+          for (int d = 0; d < D / 16; d += 4)
+            *reinterpret_cast<f32x4*>(o + d) = f32x4{w.o[d][i], w.o[d + 1][i], w.o[d + 2][i], w.o[d + 3][i]} * w.vref;
+        }
+        if (lane < 16) {
+          a.w.ws_max[row] = w.m;
+          a.w.ws_sum[row] = w.l;
+          if (at + todo == steps && slot + 1 < a.w.max_partitions) a.w.ws_sum[row + 1] = -1.f;
+        }
+      }
+    }
+    u += todo;
+    if (at + todo == steps && kvh == hkv - 1) ++item;
+  }
+}
+
+// Joins the partials of one (item, head): lane d of the workgroup takes dim d.
+// Each wave holds the weights of 64 slots, one a lane, and hands them to the
+// rows' sums.
 template <int D>
 __global__ __launch_bounds__(D) void merge_blocks_kernel(DecodeArgs a) {
-  const int item = blockIdx.x, h = blockIdx.y, d = threadIdx.x;
+  constexpr int kUnroll = 8;
+  const int item = blockIdx.x, h = blockIdx.y, d = threadIdx.x, lane = d % kWave;
+  const int mp = a.w.max_partitions;
+  const int64_t row = slot_row(a, item, h);
+  const float* src = a.w.ws_out + row * D + d;
   const int token = a.w.item_token[item];
-  if (token < 0) return;
-  const int n = keys_of(a, token), group_tokens = kWaves * a.wave_tokens;
-  if (n <= group_tokens) return;
-  const int slots = (n + group_tokens - 1) / group_tokens;
-  const int64_t row = (static_cast<int64_t>(item) * a.p.num_heads + h) * a.w.max_partitions;
   float M = -FLT_MAX, L = 0.f, o = 0.f;
-  for (int s = 0; s < slots; ++s) M = fmaxf(M, a.w.ws_max[row + s]);
-  for (int s = 0; s < slots; ++s) {
-    const float f = __builtin_amdgcn_exp2f(a.w.ws_max[row + s] - M);
-    L += f * a.w.ws_sum[row + s];
-    o += f * a.w.ws_out[(row + s) * D + d];
+  for (int s0 = 0; s0 < mp; s0 += kWave) {
+    const int at = min(s0 + lane, mp - 1);
+    const float ls = a.w.ws_sum[row + at], m0 = a.w.ws_max[row + at];
+    // the first rows are requested before the number of slots is known (slots
+    // that are not the item's hold anything and are not used)
+    float v[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) v[u] = src[static_cast<int64_t>(min(s0 + u, mp - 1)) * D];
+    // slots up to the one marked -1 (or all)
+    const uint64_t stop = __ballot(s0 + lane >= mp || ls < 0.f);
+    const int here = stop != 0 ? __builtin_ctzll(stop) : kWave;
+    if (token < 0 || (here == 0 && s0 == 0)) return;  // skipped, or written whole
+    if (here == 0) break;
+    const float ms = lane < here ? m0 : -FLT_MAX;
+    const float mn = fmaxf(M, rows_max<true>(rows_max<false>(group_max<16>(ms))));
+    const float f0 = __builtin_amdgcn_exp2f(M - mn), f = __builtin_amdgcn_exp2f(ms - mn);
+    L = L * f0 + wave_sum(lane < here ? f * ls : 0.f);
+    o *= f0;
+    M = mn;
+    for (int s = 0; s < here; s += kUnroll) {
+      float next[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        next[u] = src[static_cast<int64_t>(s0 + min(s + kUnroll + u, here - 1)) * D];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        if (s + u < here) o += lane_value(f, s + u) * v[u];
+        v[u] = next[u];
+      }
+    }
+    if (here < kWave) break;
   }
-  reinterpret_cast<_Float16*>(a.p.out)[(static_cast<int64_t>(token) * a.p.num_heads + h) * D + d] =
-      static_cast<_Float16>(o / L);
+  out_row(a, token, h, D)[d] = static_cast<_Float16>(o / L);
 }
 
 template <int D, int G, bool kFp8>
-void launch_g(const DecodeArgs& a, hipStream_t stream) {
-  const int group_tokens = kWaves * a.wave_tokens;
-  const int slots = (a.w.max_partitions * kPart + group_tokens - 1) / group_tokens;
-  const dim3 grid(slots, a.p.kv.num_kv_heads, a.w.num_items);
-  decode_blocks_kernel<D, G, kFp8><<<grid, kThreads, 0, stream>>>(a);
-  if (slots > 1) merge_blocks_kernel<D><<<dim3(a.w.num_items, a.p.num_heads), D, 0, stream>>>(a);
+void launch_g(DecodeArgs a, hipStream_t stream) {
+  const int mp = a.w.max_partitions;
+  const int64_t units = static_cast<int64_t>(a.w.num_items) * a.p.kv.num_kv_heads * mp;
+  const int cus = compute_units();
+  bool merge;
+  if (units > static_cast<int64_t>(cus) * 4 && a.w.num_items <= kMaxItemsLds && mp > 1 &&
+      units * (kPart / kStep) < (1 << 30)) {
+    a.ranges = kWavesPerCu * cus;
+    const int64_t most = std::max<int64_t>(a.ranges, (units * (kPart / kStep) + kMaxRange - 1) / kMaxRange);
+    decode_blocks_range_kernel<D, G, kFp8>
+        <<<static_cast<uint32_t>((most + kWaves - 1) / kWaves), kThreads, 0, stream>>>(a);
+    merge = true;
+  } else {
+    a.group_tokens = units > static_cast<int64_t>(cus) * 16 ? 1024 : 256;
+    const int slots = (mp * kPart + a.group_tokens - 1) / a.group_tokens;
+    const dim3 grid(slots, a.p.kv.num_kv_heads, a.w.num_items);
+    decode_blocks_grid_kernel<D, G, kFp8><<<grid, kThreads, 0, stream>>>(a);
+    merge = slots > 1;
+  }
+  if (merge) merge_blocks_kernel<D><<<dim3(a.w.num_items, a.p.num_heads), D, 0, stream>>>(a);
 }
 
 template <int D, bool kFp8>
@@ -333,9 +562,7 @@ extern "C" int rlk_paged_attention_decode_blocks(const rlk_block_attention_param
     return fail(RLK_EINVAL, "%s: null pointer argument", what);
   if (w->max_partitions > 1 && (w->ws_out == nullptr || w->ws_max == nullptr || w->ws_sum == nullptr))
     return fail(RLK_EINVAL, "%s: split-K workspace is required when max_partitions > 1", what);
-  DecodeArgs a = {*p, *w, 64};
-  const int64_t units = static_cast<int64_t>(w->num_items) * p->kv.num_kv_heads * w->max_partitions;
-  if (units > 4096) a.wave_tokens = 128;
+  const DecodeArgs a = {*p, *w, 0, 0};
   const int G = p->num_heads / p->kv.num_kv_heads;
   const bool fp8 = p->kv.format == RLK_KV_BLOCK_FP8;
   const bool ok = p->kv.head_dim == 128

@@ -155,7 +155,8 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_blocks_kernel(PrefillArgs
   for (int d = 0; d < D / 32; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
-  float m = -FLT_MAX, l = 0.f;
+  // (below every score of fp16 rows, and far above a masked one)
+  float m = -1e30f, l = 0.f;
   const float cs = __builtin_fabsf(p.scale) * kLog2e;
   TileCodes<D> codes;
   int id[kPieces];
@@ -215,8 +216,7 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_blocks_kernel(PrefillArgs
     for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        // a masked score stays 0 while a row has seen no key at all
-        const float e = s[kh][i] == -FLT_MAX ? 0.f : __builtin_amdgcn_exp2f(fmaf(s[kh][i], cs, -mc));
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[kh][i], cs, -mc));
         l += e;
         pb[2 * kh + i / 8][i % 8] = static_cast<_Float16>(e);
       }
