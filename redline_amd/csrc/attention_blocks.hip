@@ -488,8 +488,9 @@ void launch_g(DecodeArgs a, hipStream_t stream) {
   const int64_t units = static_cast<int64_t>(a.w.num_items) * a.p.kv.num_kv_heads * mp;
   const int cus = compute_units();
   bool merge;
-  if (units > static_cast<int64_t>(cus) * 4 && a.w.num_items <= kMaxItemsLds && mp > 1 &&
-      units * (kPart / kStep) < (1 << 30)) {
+  // RLK_TUNE_BLK_DECODE forces a form (0 grid, 1 range; tests and tuning runs)
+  if (tune_knob(kBlkDecode, units > static_cast<int64_t>(cus) * 4) != 0 && a.w.num_items <= kMaxItemsLds &&
+      mp > 1 && units * (kPart / kStep) < (1 << 30)) {
     a.ranges = kWavesPerCu * cus;
     const int64_t most = std::max<int64_t>(a.ranges, (units * (kPart / kStep) + kMaxRange - 1) / kMaxRange);
     decode_blocks_range_kernel<D, G, kFp8>

@@ -313,7 +313,8 @@ __global__ __launch_bounds__(kWriteThreads) void write_kv_blocks_kernel(WriteArg
 
 template <int D, int BS, bool kFp8>
 int launch_write(WriteArgs a, hipStream_t stream) {
-  const int rows = a.num_tokens > 1024 ? 16 : 1;
+  // RLK_TUNE_BLK_WRITE forces the rows of a wave (1 or 16; tests and tuning runs)
+  const int rows = tune_knob(kBlkWrite, a.num_tokens > 1024 ? 16 : 1) == 1 ? 1 : 16;
   const int64_t waves = static_cast<int64_t>((a.num_tokens + rows - 1) / rows) * a.head_groups;
   const int64_t kvg = (waves + kWriteThreads / kWave - 1) / (kWriteThreads / kWave);
   const int64_t qg = (static_cast<int64_t>(a.num_tokens) * a.hq * (D / 16) + kWriteThreads - 1) / kWriteThreads;

@@ -2,25 +2,34 @@
 //
 // Causal attention of a sequence's new tokens over its cached and new keys.
 // Rows are (token, query head) pairs of one kv head, head fastest, so K and V
-// are read and converted once for the G heads of the group; a workgroup of 4
-// waves takes 128 rows, 32 per wave, and walks the keys in tiles of 64.
-//   * Codes go to registers one tile ahead, become fp16 (code * scale, exact) and
-//     are written to one of two LDS images in the operand order of
-//     v_mfma_f32_32x32x16_f16: K as 16-byte chunks [piece][half][key], V as
-//     [16-key tile][lane half][dim], each chunk the 8 keys of a lane's own
-//     scores; both are read as whole contiguous rows (no bank conflicts), and
-//     neither operand is transposed or exchanged anywhere.
+// are read and converted once for the G heads of the group; a wave takes 32
+// rows and walks the keys in tiles of 64.
+//   * Codes go to registers a tile ahead, become fp16 (exactly) and are written
+//     to LDS images in the operand order of v_mfma_f32_32x32x16_f16: K as
+//     16-byte chunks [piece][half][key], V as [16-key tile][lane half][dim], each
+//     chunk the 8 keys of a lane's own scores; both are read as whole contiguous
+//     rows (no bank conflicts), and neither operand is transposed or exchanged
+//     anywhere.
 //   * S^T = K Q^T leaves one query row per lane (its keys split over the two lane
 //     halves), so the running maximum and sum are lane-local, and the scores are
 //     the B operand of O^T = V^T P^T as they stand.
-//   * One barrier per tile: tile t + 1 is converted between the products of
-//     tile t.
-// m, l and the output accumulate in fp32; P is rounded to fp16 (at most 1).
+//   * A tile is two phases, a matrix phase X (P.V of the tile before, K.Q of this
+//     one) and a vector phase Y (softmax, conversion of codes).  A workgroup has
+//     one or two groups of 4 waves; two groups are half a tile apart, so that of
+//     the two waves of a SIMD one has the matrix cores while the other has the
+//     vector ALU.  The groups take
+//       kRows2   256 rows, the same tiles (one image for both): large calls;
+//       kKeys2   the same 128 rows, even and odd tiles (an image each), and join
+//                their partials at the end: calls that do not fill the chip;
+//       kOne     one group, whose CU holds two workgroups: between the two.
+// m, l and the output accumulate in fp32; P is rounded to fp16 (at most 1), and
+// l sums the rounded values, so that numerator and denominator agree.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cfloat>
 #include <cstdint>
+#include <type_traits>
 
 #include "kv_blocks.hpp"
 
@@ -32,8 +41,8 @@ namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kThreads = 256;
-constexpr int kRows = 128;     // (token, head) rows of a workgroup
+constexpr int kGroupThreads = 256;  // a group: 4 waves, one per SIMD
+constexpr int kWaveRows = 32;       // (token, head) rows of a wave
 constexpr int kTileKeys = 64;
 
 struct PrefillArgs {
@@ -42,7 +51,8 @@ struct PrefillArgs {
   int group;  // query heads per kv head
 };
 
-// Four codes times their scale as fp16, exactly.
+// Four codes as fp16: e4m3 times the scale (the conversion takes it, exactly),
+// INT8 V times the scale, INT8 K as it is (its scale multiplies the scores).
 template <bool kFp8>
 __device__ __forceinline__ u32x2 scaled_f16(uint32_t w, float s) {
   f16x4 v;
@@ -56,28 +66,39 @@ __device__ __forceinline__ u32x2 scaled_f16(uint32_t w, float s) {
   return __builtin_bit_cast(u32x2, v);
 }
 
+// Two images of K and of V, used in turn, and the score scale of each 16-key tile
+// of the last 4 key tiles (INT8).
 template <int D>
-struct Image {
-  u32x4 k[D / 16][2][kTileKeys];  // chunk (piece, half, key): 8 dims
-  u32x4 v[4][2][D];               // chunk (16-key tile, lane half, dim index): 8 keys
+struct PrefillLds {
+  u32x4 k[2][D / 16][2][kTileKeys];  // chunk (piece, half, key): 8 dims
+  u32x4 v[2][4][2][D];               // chunk (16-key tile, lane half, dim index): 8 keys
+  f32x4 ks[4];
 };
 
-// A thread's pieces of a key tile: piece i is 16-byte piece (tid + 256 i) of the
-// tile's 4 layout tiles in order.
-template <int D>
-struct TileCodes {
-  static constexpr int kPieces = D / 64;
-  u32x4 k[kPieces], v[kPieces];
-  float ks[kPieces], vs[kPieces];
-};
+enum Split { kOne, kRows2, kKeys2 };
 
-template <int D, bool kFp8>
-__global__ __launch_bounds__(kThreads, 2) void prefill_blocks_kernel(PrefillArgs a) {
-  constexpr int E = D / 16, kPieces = D / 64, kPerTile = D;  // 16-byte pieces of a layout tile
+// Phases, with t the key tile (kKeys2: the group's t-th) and S its scores; group 1
+// is one phase behind.  kRows2:
+//   group 0   X(t) at 2t      Y(t) at 2t + 1, converts its half of K(t + 1), V(t)
+//   group 1   X(t) at 2t + 1  Y(t) at 2t + 2, converts its half of K(t + 2), V(t + 1)
+// X(t) reads K(t) and V(t - 1).  So K(t) is written in the phases 2t - 2 and
+// 2t - 1 and read in 2t and 2t + 1, V(t) is written in 2t and 2t + 1 and read in
+// 2t + 2 and 2t + 3, and neither meets the image of tile t - 2 in the same buffer.
+// Alone or with its own image a group does as group 0, with whole tiles.
+template <int D, bool kFp8, Split kSplit>
+__global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void prefill_blocks_kernel(PrefillArgs a) {
+  constexpr int kGroups = kSplit == kRows2 ? 2 : 1;  // that share a tile's image
+  constexpr bool kKeys = kSplit == kKeys2;
+  constexpr int E = D / 16, kRows = 4 * kWaveRows * kGroups;
+  constexpr int kPerTile = D;                                  // 16-byte pieces of a layout tile
+  constexpr int kItems = 2 * 4 * kPerTile / kGroups / kGroupThreads;  // K and V pieces of a thread and tile
   constexpr float kLog2e = 1.4426950408889634f;
-  __shared__ Image<D> img[2];
+  extern __shared__ u32x4 lds_raw[];
   const rlk_block_attention_params& p = a.p;
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int tid = threadIdx.x % kGroupThreads, grp = wave / 4;
+  const int rgrp = kKeys ? 0 : grp, kgrp = kKeys ? grp : 0;  // the group's part of the rows, of the tiles
+  PrefillLds<D>& lds = reinterpret_cast<PrefillLds<D>*>(lds_raw)[kgrp];
   const int half = lane / 32, col = lane % 32;
   const int kvh = blockIdx.x, G = a.group;
   const int seq = a.w.seq_ids[blockIdx.z];
@@ -87,16 +108,17 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_blocks_kernel(PrefillArgs
   const int row0 = (gridDim.y - 1 - blockIdx.y) * kRows;
   if (row0 >= rows) return;
   const int past = a.w.ctx_len[seq] - q_len, q_start = a.w.q_start[seq];
-  const int bs = p.kv.block_size, tpb = bs / kTileTokens, hkv = p.kv.num_kv_heads;
-  const int most = static_cast<int>(min(static_cast<int64_t>(p.max_blocks_per_seq) * bs, static_cast<int64_t>(1 << 30)));
+  const int tsh = p.kv.block_size == 32 ? 1 : 0, hkv = p.kv.num_kv_heads;  // log2 tiles of a block
+  const int most = static_cast<int>(min(static_cast<int64_t>(p.max_blocks_per_seq) * p.kv.block_size,
+                                        static_cast<int64_t>(1 << 30)));
   // keys of the workgroup's last row; those of each lane's row
-  const int last_tok = min(row0 + kRows, rows) - 1;
-  const int keys = min(past + last_tok / G + 1, most);
-  const int row = min(row0 + wave * 32 + col, rows - 1);  // rows past the end repeat the last one
+  const int last_row = min(row0 + kRows, rows) - 1;
+  const int keys = min(past + last_row / G + 1, most);
+  const int wrow = row0 + (rgrp * 4 + wave % 4) * kWaveRows;  // the wave's first row
+  const int row = min(wrow + col, rows - 1);  // rows past the end repeat the last one
   const int tok = row / G, head = kvh * G + row - tok * G;
   const int row_keys = min(past + tok + 1, most);
-  const int first_row = min(row0 + wave * 32, rows - 1);
-  const int full = min(past + first_row / G + 1, most);  // keys that every row of the wave sees
+  const int full = min(past + min(wrow, rows - 1) / G + 1, most);  // keys that every row of the wave sees
 
   const _Float16* q = reinterpret_cast<const _Float16*>(p.q) + static_cast<int64_t>(q_start + tok) * p.q_stride + head * D;
   f16x8 qb[E];
@@ -106,129 +128,236 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_blocks_kernel(PrefillArgs
     if (p.scale < 0.f) qb[pc] = -qb[pc];  // the maximum is taken before the scale
   }
 
+  // Item j of a thread: 16-byte piece (tid + 256 j') of its group's part of a K or
+  // V tile, the K pieces first.  Tiles past the last repeat its last 16 keys.
+  constexpr int kHalf = kItems * kGroupThreads / 2;  // K pieces of a group's part
+  struct Item {
+    u32x4 codes;
+    float scale;
+  };
+  Item item[kItems];
+  int id[kItems];
   const int32_t* table = p.block_tables + static_cast<int64_t>(seq) * p.max_blocks_per_seq;
-  const int tiles = (keys + kTileKeys - 1) / kTileKeys, last16 = (max(keys, 1) - 1) / kTileTokens;
-  // block of this thread's layout tile i of key tile t (tiles past the last repeat it)
-  auto entry = [&](int t, int i) {
-    const int t16 = min(4 * t + (tid + kThreads * i) / kPerTile, last16);
-    return table[t16 / tpb];
+  // tiles of a group (kKeys2: its last may lie behind the keys; all of it is masked)
+  const int all_tiles = (keys + kTileKeys - 1) / kTileKeys, tiles = kKeys ? (all_tiles + 1) / 2 : all_tiles;
+  auto real = [&](int t) { return kKeys ? 2 * t + kgrp : t; };
+  const int last16 = (max(keys, 1) - 1) / kTileTokens;
+  auto is_v = [&](int j) { return j * kGroupThreads + (kItems == 1 ? tid : 0) >= kHalf; };
+  auto piece = [&](int j) { return (j * kGroupThreads + tid) % kHalf; };  // of the group's part
+  auto part16 = [&](int j) { return rgrp * (4 / kGroups) + piece(j) / kPerTile; };  // 16-key tile of the key tile
+  auto layout_tile = [&](int j, int t) { return min(4 * real(t) + part16(j), last16); };
+  // block of item j for conversion c (K of tile c + 1, V of tile c)
+  auto entry = [&](int j, int c) { return table[layout_tile(j, is_v(j) ? c : c + 1) >> tsh]; };
+  auto request = [&](int j, int c) __attribute__((always_inline)) {
+    const int t16 = layout_tile(j, is_v(j) ? c : c + 1);
+    const int b = static_cast<uint32_t>(id[j]) < static_cast<uint32_t>(p.kv.num_blocks) ? id[j] : 0;
+    const uint32_t cell = static_cast<uint32_t>(b) * hkv + kvh;
+    const uint32_t tile = (cell << tsh) + (t16 & tsh);
+    const uint8_t* base = static_cast<const uint8_t*>(is_v(j) ? p.kv.v : p.kv.k) + (piece(j) % kPerTile) * 16;
+    item[j].codes = load16(base + static_cast<uint64_t>(tile) * (kTileTokens * D));
+    item[j].scale = (is_v(j) ? p.kv.v_scale : p.kv.k_scale)[cell];
   };
-  auto request = [&](TileCodes<D>& c, int t, const int (&id)[kPieces]) {
+  const float cs = __builtin_fabsf(p.scale) * kLog2e;
+  auto convert = [&](int j, int c) __attribute__((always_inline)) {
+    const int t16 = part16(j), pc = piece(j) % kPerTile;
+    if (!is_v(j)) {
+      const int buf = (c + 1) & 1, kp = pc / 16, key = 16 * t16 + pc % 16;
+      const u32x4 w = item[j].codes;
+      u32x2 x[4];
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int t16 = min(4 * t + (tid + kThreads * i) / kPerTile, last16);
-      const int b = static_cast<uint32_t>(id[i]) < static_cast<uint32_t>(p.kv.num_blocks) ? id[i] : 0;
-      const int64_t cell = static_cast<int64_t>(b) * hkv + kvh;
-      const int64_t at = (cell * tpb + t16 % tpb) * (kTileTokens * D) + (tid % kPerTile) * 16;
-      c.k[i] = load16(static_cast<const uint8_t*>(p.kv.k) + at);
-      c.v[i] = load16(static_cast<const uint8_t*>(p.kv.v) + at);
-      c.ks[i] = p.kv.k_scale[cell];
-      c.vs[i] = p.kv.v_scale[cell];
-    }
-  };
-  auto convert = [&](const TileCodes<D>& c, Image<D>& im, int t) {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int t16 = (tid + kThreads * i) / kPerTile, piece = tid % kPerTile;
-      {
-        const int pc = piece / 16, key = 16 * t16 + piece % 16;
-        const u32x2 a0 = scaled_f16<kFp8>(c.k[i][0], c.ks[i]), a1 = scaled_f16<kFp8>(c.k[i][1], c.ks[i]);
-        const u32x2 b0 = scaled_f16<kFp8>(c.k[i][2], c.ks[i]), b1 = scaled_f16<kFp8>(c.k[i][3], c.ks[i]);
-        im.k[pc][0][key] = u32x4{a0[0], a0[1], a1[0], a1[1]};
-        im.k[pc][1][key] = u32x4{b0[0], b0[1], b1[0], b1[1]};
-      }
-      const int g = piece / 64, rho = piece / 16 % 4, m = piece % 16;
-      u32x4 v = c.v[i];
-      if (t * kTileKeys + kTileKeys > keys) {  // uniform: bytes past the keys may be anything
-        const int keep = min(max(keys - t * kTileKeys - 16 * t16 - 4 * rho, 0), 4);
+      for (int e = 0; e < 4; ++e)
+        x[e] = kFp8 ? scaled_f16<kFp8>(w[e], item[j].scale) : __builtin_bit_cast(u32x2, codes_to_f16<kFp8>(w[e]));
+      lds.k[buf][kp][0][key] = u32x4{x[0][0], x[0][1], x[1][0], x[1][1]};
+      lds.k[buf][kp][1][key] = u32x4{x[2][0], x[2][1], x[3][0], x[3][1]};
+      if (!kFp8 && pc == 0) reinterpret_cast<float*>(&lds.ks[(c + 1) & 3])[t16] = item[j].scale * cs;
+    } else {
+      const int g = pc / 64, rho = pc / 16 % 4, m = pc % 16;
+      u32x4 w = item[j].codes;
+      if ((real(c) + 1) * kTileKeys > keys) {  // uniform: bytes past the keys may be anything
+        const int keep = min(max(keys - real(c) * kTileKeys - 16 * t16 - 4 * rho, 0), 4);
         const uint32_t mask = keep == 0 ? 0u : 0xffffffffu >> (32 - 8 * keep);
-        v &= u32x4{mask, mask, mask, mask};
+        w &= u32x4{mask, mask, mask, mask};
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        reinterpret_cast<u32x2*>(&im.v[t16][rho % 2][(4 * g + j) * 16 + m])[rho / 2] = scaled_f16<kFp8>(v[j], c.vs[i]);
+      for (int e = 0; e < 4; ++e)
+        reinterpret_cast<u32x2*>(&lds.v[c & 1][t16][rho % 2][(4 * g + e) * 16 + m])[rho / 2] =
+            scaled_f16<kFp8>(w[e], item[j].scale);
     }
+  };
+  // conversion c of this thread's pieces, and the request of conversion c + 1's
+  auto conversion = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) {
+      convert(j, c);
+      request(j, c + 1);
+    }
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) id[j] = entry(j, c + 2);
   };
 
-  f32x16 o[D / 32];
+  f32x16 o[D / 32], s[2];
 #pragma unroll
   for (int d = 0; d < D / 32; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+  f16x8 pb[4];
   // (below every score of fp16 rows, and far above a masked one)
   float m = -1e30f, l = 0.f;
-  const float cs = __builtin_fabsf(p.scale) * kLog2e;
-  TileCodes<D> codes;
-  int id[kPieces];
-  if (tiles > 0) {
+
+  // Operands come from LDS kAhead fragments before their product; the schedule is
+  // pinned, because the compiler by itself waits for each pair of reads.
+  auto phase_x = [&](int t, auto pv, auto qk) __attribute__((always_inline)) {
+    constexpr int kPv = decltype(pv)::value ? 4 * (D / 32) : 0, kQk = decltype(qk)::value ? 2 * E : 0;
+    constexpr int kAll = kPv + kQk, kAhead = kAll < 8 ? kAll : 8;
+    __builtin_amdgcn_sched_barrier(0);
+    const u32x4* vp = &lds.v[(t + 1) & 1][0][half][col];  // V of tile t - 1
+    const u32x4* kp = &lds.k[t & 1][0][half][col];
+    auto fragment = [&](int i) {
+      return i < kPv ? vp[(i / (D / 32)) * 2 * D + 32 * (i % (D / 32))]
+                     : kp[((i - kPv) / 2) * 2 * kTileKeys + 32 * ((i - kPv) % 2)];
+    };
+    u32x4 f[kAll];
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) id[i] = entry(0, i);
-    request(codes, 0, id);
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) id[i] = entry(1, i);
-    convert(codes, img[0], 0);
-    request(codes, 1, id);
-  }
-  for (int t = 0; t < tiles; ++t) {
-    const Image<D>& im = img[t & 1];
-    __syncthreads();  // tile t is written, tile t - 1 has been read
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) id[i] = entry(t + 2, i);
-    f32x16 s[2];
-#pragma unroll
-    for (int kh = 0; kh < 2; ++kh) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[kh][i] = 0.f;
-#pragma unroll
-      for (int pc = 0; pc < E; ++pc)
-        s[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, im.k[pc][half][32 * kh + col]),
-                                                       qb[pc], s[kh], 0, 0, 0);
-    }
-    if (t + 1 < tiles) {
-      convert(codes, img[(t + 1) & 1], t + 1);
-      request(codes, t + 2, id);
-    }
-    // element i of half kh: key 64 t + 32 kh + 8 (i / 4) + 4 half + i % 4
-    if ((t + 1) * kTileKeys > full) {
+    for (int i = 0; i < kAll; ++i) f[i] = fragment(i);
+    if constexpr (kQk > 0) {
 #pragma unroll
       for (int kh = 0; kh < 2; ++kh)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (t * kTileKeys + 32 * kh + 8 * (i / 4) + 4 * half + i % 4 >= row_keys) s[kh][i] = -FLT_MAX;
+        for (int i = 0; i < 16; ++i) s[kh][i] = 0.f;
     }
-    float mx = s[0][0];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[0][i]);
+    for (int i = 0; i < kAll; ++i) {
+      const f16x8 x = __builtin_bit_cast(f16x8, f[i]);
+      if (i < kPv) {
+        const int d = i % (D / 32);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pb[i / (D / 32)], o[d], 0, 0, 0);
+      } else {
+        const int kh = (i - kPv) % 2;
+        s[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qb[(i - kPv) / 2], s[kh], 0, 0, 0);
+      }
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);  // LDS reads
 #pragma unroll
-    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[1][i]);
+    for (int i = 0; i < kAll - kAhead; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // a product
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, kAhead, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto softmax = [&](int t) __attribute__((always_inline)) {
+    // element i of half kh: key 64 real(t) + 32 kh + 8 (i / 4) + 4 half + i % 4
+    f32x4 c4 = kFp8 ? f32x4{cs, cs, cs, cs} : lds.ks[t & 3];  // score scale of each 16 keys
+    float mx;
+    const int first_key = real(t) * kTileKeys;
+    if (first_key + kTileKeys > full) {  // uniform over the wave: scaled, then masked
+#pragma unroll
+      for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float v = s[kh][i] * c4[2 * kh + i / 8];
+          s[kh][i] = first_key + 32 * kh + 8 * (i / 4) + 4 * half + i % 4 < row_keys ? v : -FLT_MAX;
+        }
+      c4 = f32x4{1.f, 1.f, 1.f, 1.f};
+    }
+    // (the scales are not negative, so the largest score of 16 keys is scaled once)
+    mx = -FLT_MAX;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      float y = s[x / 2][8 * (x % 2)];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) y = fmaxf(y, s[x / 2][8 * (x % 2) + i]);
+      mx = fmaxf(mx, y * c4[x]);
+    }
     mx = rows_max<true>(mx);
     const float mn = fmaxf(m, mx);
     if (__any(mn != m)) {
-      const float f = __builtin_amdgcn_exp2f((m - mn) * cs);
+      const float f = __builtin_amdgcn_exp2f(m - mn);
       l *= f;
 #pragma unroll
       for (int d = 0; d < D / 32; ++d) o[d] *= f;
       m = mn;
     }
-    const float mc = m * cs;
-    f16x8 pb[4];
+    const f16x2 ones = {static_cast<_Float16>(1), static_cast<_Float16>(1)};
 #pragma unroll
-    for (int kh = 0; kh < 2; ++kh)
+    for (int x = 0; x < 4; ++x)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(s[kh][i], cs, -mc));
-        l += e;
-        pb[2 * kh + i / 8][i % 8] = static_cast<_Float16>(e);
+      for (int i = 0; i < 8; i += 2) {
+        const float e0 = __builtin_amdgcn_exp2f(fmaf(s[x / 2][8 * (x % 2) + i], c4[x], -m));
+        const float e1 = __builtin_amdgcn_exp2f(fmaf(s[x / 2][8 * (x % 2) + i + 1], c4[x], -m));
+        const f16x2 e = {static_cast<_Float16>(e0), static_cast<_Float16>(e1)};
+        pb[x][i] = e[0];
+        pb[x][i + 1] = e[1];
+        l = __builtin_amdgcn_fdot2(e, ones, l, false);
       }
+  };
+
+  if (tiles > 0) {
+    // conversion -1 has K(0) only: there is no V tile -1
+#pragma unroll
+    for (int j = 0; j < kItems; ++j)
+      if (!is_v(j)) id[j] = entry(j, -1);
+#pragma unroll
+    for (int j = 0; j < kItems; ++j)
+      if (!is_v(j)) request(j, -1);
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) id[j] = entry(j, 0);
+#pragma unroll
+    for (int j = 0; j < kItems; ++j)
+      if (!is_v(j)) convert(j, -1);  // K(0)
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) request(j, 0);
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) id[j] = entry(j, 1);
+  }
+  __syncthreads();
+  if (grp == 1) {  // one phase behind, kRows2: and one conversion ahead of group 0
+    if (kGroups == 2 && tiles > 0) conversion(0);
+    __syncthreads();
+  }
+  auto phase_y = [&](int t) __attribute__((always_inline)) {
+    __syncthreads();
+    softmax(t);
+    conversion(t + rgrp);
+    __syncthreads();
+  };
+  if (tiles > 0) {
+    phase_x(0, std::false_type{}, std::true_type{});
+    phase_y(0);
+    for (int t = 1; t < tiles; ++t) {
+      phase_x(t, std::true_type{}, std::true_type{});
+      phase_y(t);
+    }
+    phase_x(tiles, std::true_type{}, std::false_type{});
+  }
+  if (kSplit != kOne && grp == 0) __syncthreads();  // as many barriers as group 1
+  l = rows_sum<true>(l);
+  if constexpr (kKeys) {  // group 1's partial joins group 0's through LDS
+    __syncthreads();      // the images have been read
+    struct Partial {
+      float o[D / 2][kGroupThreads], m[kGroupThreads], l[kGroupThreads];
+    };
+    static_assert(sizeof(Partial) <= 2 * sizeof(PrefillLds<D>), "fits where the images were");
+    Partial& part = *reinterpret_cast<Partial*>(lds_raw);
+    if (grp == 1) {
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part.o[16 * d + i][tid] = o[d][i];
+      part.m[tid] = m;
+      part.l[tid] = l;
+    }
+    __syncthreads();
+    if (grp == 1) return;
+    const float m1 = part.m[tid], mn = fmaxf(m, m1);
+    const float f0 = __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(m1 - mn);
+    l = l * f0 + part.l[tid] * f1;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, im.v[kt][half][32 * d + col]),
-                                                      pb[kt], o[d], 0, 0, 0);
+      for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * f0 + part.o[16 * d + i][tid] * f1;
   }
-  l = rows_sum<true>(l);
-  if (row0 + wave * 32 + col >= rows) return;  // no barrier follows
+  if (wrow + col >= rows) return;  // no barrier follows
   const float inv = l > 0.f ? 1.f / l : 0.f;
   _Float16* out = reinterpret_cast<_Float16*>(p.out) + (static_cast<int64_t>(q_start + tok) * p.num_heads + head) * D;
   // element i of tile d: dim index 32 d + 8 (i / 4) + 4 half + i % 4 = 16 dt + mm, i.e. dim E mm + dt
@@ -243,6 +372,33 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_blocks_kernel(PrefillArgs
     } else {
       *reinterpret_cast<u32x2*>(out + 4 * mm) = __builtin_bit_cast(u32x2, f16x4{y[0], y[1], y[2], y[3]});
     }
+  }
+}
+
+template <int D, bool kFp8, Split kSplit>
+hipError_t launch_s(const PrefillArgs& a, int64_t rows, hipStream_t stream) {
+  constexpr int per = kSplit == kRows2 ? 256 : 128;
+  const size_t bytes = sizeof(PrefillLds<D>) * (kSplit == kKeys2 ? 2 : 1);
+  if (bytes > 64 * 1024) {
+    const hipError_t e = grant_dynamic_lds(
+        reinterpret_cast<const void*>(prefill_blocks_kernel<D, kFp8, kSplit>), bytes);
+    if (e != hipSuccess) return e;
+  }
+  const dim3 grid(a.p.kv.num_kv_heads, static_cast<uint32_t>((rows + per - 1) / per), a.w.num_seqs);
+  prefill_blocks_kernel<D, kFp8, kSplit>
+      <<<grid, kGroupThreads * (kSplit == kOne ? 1 : 2), bytes, stream>>>(a);
+  return hipSuccess;
+}
+
+template <int D, bool kFp8>
+hipError_t launch(const PrefillArgs& a, int64_t rows, hipStream_t stream) {
+  const int64_t groups = (rows + 127) / 128 * a.p.kv.num_kv_heads * a.w.num_seqs;
+  const int cus = compute_units();
+  // RLK_TUNE_BLK_PREFILL forces a split (tests and tuning runs)
+  switch (tune_knob(kBlkPrefill, groups <= cus ? kKeys2 : (groups <= 2 * cus ? kOne : kRows2))) {
+    case kKeys2: return launch_s<D, kFp8, kKeys2>(a, rows, stream);
+    case kOne: return launch_s<D, kFp8, kOne>(a, rows, stream);
+    default: return launch_s<D, kFp8, kRows2>(a, rows, stream);
   }
 }
 
@@ -261,19 +417,15 @@ extern "C" int rlk_paged_attention_prefill_blocks(const rlk_block_attention_para
   if (w->seq_ids == nullptr || w->q_start == nullptr || w->q_len == nullptr || w->ctx_len == nullptr)
     return fail(RLK_EINVAL, "%s: null pointer argument", what);
   const int G = p->num_heads / p->kv.num_kv_heads;
-  const int64_t tiles = (static_cast<int64_t>(w->max_q_tiles) * RLK_PREFILL_TILE_Q * G + kRows - 1) / kRows;
-  if (w->num_seqs > 65535 || tiles > 65535)
+  const int64_t rows = static_cast<int64_t>(w->max_q_tiles) * RLK_PREFILL_TILE_Q * G;
+  if (w->num_seqs > 65535 || (rows + 127) / 128 > 65535)
     return fail(RLK_EINVAL, "%s: %d sequences of %d query tiles exceed one launch; split the call",
                 what, w->num_seqs, w->max_q_tiles);
   const PrefillArgs a = {*p, *w, G};
-  const dim3 grid(p->kv.num_kv_heads, static_cast<uint32_t>(tiles), w->num_seqs);
   const bool fp8 = p->kv.format == RLK_KV_BLOCK_FP8;
-  if (p->kv.head_dim == 128) {
-    if (fp8) prefill_blocks_kernel<128, true><<<grid, kThreads, 0, stream>>>(a);
-    else prefill_blocks_kernel<128, false><<<grid, kThreads, 0, stream>>>(a);
-  } else {
-    if (fp8) prefill_blocks_kernel<64, true><<<grid, kThreads, 0, stream>>>(a);
-    else prefill_blocks_kernel<64, false><<<grid, kThreads, 0, stream>>>(a);
-  }
+  const hipError_t e = p->kv.head_dim == 128
+                           ? (fp8 ? launch<128, true>(a, rows, stream) : launch<128, false>(a, rows, stream))
+                           : (fp8 ? launch<64, true>(a, rows, stream) : launch<64, false>(a, rows, stream));
+  if (e != hipSuccess) return fail(static_cast<int>(e), "%s: %s", what, hipGetErrorString(e));
   return launch_status(what);
 }

@@ -18,6 +18,22 @@ def torch():
     return torch
 
 
+@pytest.fixture(params=[None, 0, 1], ids=["rule", "grid", "range"])
+def decode_form(request):
+    """The launcher's two decode forms, forced, and its own choice."""
+    from redline_amd._lib import tune_knob
+    with tune_knob("RLK_TUNE_BLK_DECODE", request.param):
+        yield request.param
+
+
+@pytest.fixture(params=[0, 1, 2], ids=["one", "rows2", "keys2"])
+def prefill_split(request):
+    """The launcher's three prefill kernels, forced."""
+    from redline_amd._lib import tune_knob
+    with tune_knob("RLK_TUNE_BLK_PREFILL", request.param):
+        yield request.param
+
+
 def make(rng, hkv, D, bs, fmt, lens, extra=1, lo=-6, hi=-3):
     """A filled cache and tables over distinct blocks; entries past a sequence's
     blocks are 0, and bytes past its context are e4m3 NaNs or 0x80."""
@@ -73,9 +89,9 @@ DECODE_CASES = [(hq, hkv, D, bs, fmt, lens) for hq, hkv, D, bs, fmt, lens in [
 
 @pytest.mark.parametrize("scale", ["usual", "large", "negative"])
 @pytest.mark.parametrize("hq,hkv,D,bs,fmt,lens", DECODE_CASES)
-def test_decode(torch, hq, hkv, D, bs, fmt, lens, scale):
+def test_decode(torch, hq, hkv, D, bs, fmt, lens, scale, decode_form):
     from redline_amd import kernels as K
-    say(f"decode_blocks hq={hq} hkv={hkv} D={D} bs={bs} fmt={fmt} lens={lens} scale={scale}")
+    say(f"decode_blocks hq={hq} hkv={hkv} D={D} bs={bs} fmt={fmt} lens={lens} scale={scale} form={decode_form}")
     rng = np.random.default_rng(hq * 100 + D + bs)
     c, tab = make(rng, hkv, D, bs, fmt, lens)
     t, view = gpu_cache(torch, K, c)
@@ -92,7 +108,7 @@ def test_decode(torch, hq, hkv, D, bs, fmt, lens, scale):
 
 
 @pytest.mark.parametrize("fmt", [B.INT8, B.FP8])
-def test_decode_scales_far_apart(torch, fmt):
+def test_decode_scales_far_apart(torch, fmt, decode_form):
     """K and V scales from 2^-24 to 2^10 (e4m3: 2^8), and 0, in one context; V so
     small that the whole output is below fp16's normal range, and mixed."""
     from redline_amd import kernels as K
@@ -119,7 +135,7 @@ def test_decode_scales_far_apart(torch, fmt):
 
 
 @pytest.mark.parametrize("fmt", [B.INT8, B.FP8])
-def test_decode_skips_empty_rows_and_bad_ids(torch, fmt):
+def test_decode_skips_empty_rows_and_bad_ids(torch, fmt, decode_form):
     """Items with a negative token write nothing; a negative position gives
     zeros; ids outside the pool are block 0; contexts past the table row or past
     max_partitions end there; several items of one sequence."""
@@ -202,9 +218,9 @@ PREFILL_CASES = [
 
 @pytest.mark.parametrize("scale", ["usual", "large", "negative"])
 @pytest.mark.parametrize("hq,hkv,D,bs,fmt,segs", PREFILL_CASES)
-def test_prefill(torch, hq, hkv, D, bs, fmt, segs, scale):
+def test_prefill(torch, hq, hkv, D, bs, fmt, segs, scale, prefill_split):
     from redline_amd import kernels as K
-    say(f"prefill_blocks hq={hq} hkv={hkv} D={D} bs={bs} fmt={fmt} segs={segs} scale={scale}")
+    say(f"prefill_blocks hq={hq} hkv={hkv} D={D} bs={bs} fmt={fmt} segs={segs} scale={scale} split={prefill_split}")
     rng = np.random.default_rng(hq * 100 + D + bs)
     lens = [p + n for p, n in segs]
     c, tab = make(rng, hkv, D, bs, fmt, lens)
@@ -224,7 +240,7 @@ def test_prefill(torch, hq, hkv, D, bs, fmt, segs, scale):
 
 
 @pytest.mark.parametrize("fmt", [B.INT8, B.FP8])
-def test_prefill_edges(torch, fmt):
+def test_prefill_edges(torch, fmt, prefill_split):
     """Skipped and idle sequences, rows before the context's start (zeros), ids
     outside the pool, a context that ends at its table row."""
     from redline_amd import kernels as K
@@ -248,6 +264,31 @@ def test_prefill_edges(torch, fmt):
         want, bound = B.attention(c, tab[s], q[r], 0.05, [past + i + 1 for i in range(new[s])])
         check(got[r], want, bound, f"sequence {s}")
     assert (got[20:40] == 0).all() and (got[90:] == 9.0).all()
+
+
+@pytest.mark.parametrize("fmt", [B.INT8, B.FP8])
+@pytest.mark.parametrize("gap", [10.5, 14.0])
+def test_many_small_probabilities(torch, fmt, gap, decode_form, prefill_split):
+    """One key ahead of thousands of equal ones by `gap` (natural log): each of
+    those is near or below the smallest normal fp16 number relative to it, all of
+    them together are not small (gap 10.5: 0.14 of the sum)."""
+    from redline_amd import kernels as K
+    say(f"small probabilities fmt={fmt} gap={gap}")
+    rng = np.random.default_rng(13)
+    hq, hkv, D, bs, n = 2, 1, 128, 16, 5200
+    c, tab = make(rng, hkv, D, bs, fmt, [n])
+    c.codes[0][...] = 0
+    c.scale[0][...] = 1.0
+    one = B.bytes_of(np.array([1.0]), fmt)[0]
+    c.codes[0][tab[0, 100], 0, 5, 0] = one  # key 1605 has 1 in dim 0, the others 0
+    q = np.zeros((1, hq, D), np.float16)
+    q[:, :, 0] = gap
+    t, view = gpu_cache(torch, K, c)
+    want, bound = B.attention(c, tab[0], q, 1.0, [n])
+    got = run_decode(torch, K, c, view, tab, q, hq, 1.0, [n - 1], [0], [0], 21)
+    check(got, want, bound, "decode")
+    got = run_prefill(torch, K, c, view, tab, q, hq, 1.0, [0], [0], [1], [n], 1)
+    check(got, want, bound, "prefill")
 
 
 def test_attention_in_graphs_sharing_a_workspace(torch):

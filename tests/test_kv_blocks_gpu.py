@@ -81,12 +81,20 @@ WRITE_CASES = [
 ]
 
 
+@pytest.fixture(params=[None, 1, 16], ids=["rule", "rows1", "rows16"])
+def write_rows(request):
+    """Rows that a wave looks at: the launcher's choice, and each forced."""
+    from redline_amd._lib import tune_knob
+    with tune_knob("RLK_TUNE_BLK_WRITE", request.param):
+        yield request.param
+
+
 @pytest.mark.parametrize("hq,hkv,D,bs,fmt,bias,segs", WRITE_CASES)
-def test_write_matches_definition(torch, hq, hkv, D, bs, fmt, bias, segs):
+def test_write_matches_definition(torch, hq, hkv, D, bs, fmt, bias, segs, write_rows):
     """Two steps, the second continuing blocks with larger and smaller rows, so
     scales grow and stay; bytes outside the runs are untouched."""
     from redline_amd import kernels as K
-    say(f"write_blocks hq={hq} hkv={hkv} D={D} bs={bs} fmt={fmt} bias={bias} seqs={len(segs)}")
+    say(f"write_blocks hq={hq} hkv={hkv} D={D} bs={bs} fmt={fmt} bias={bias} seqs={len(segs)} rows={write_rows}")
     rng = np.random.default_rng(len(segs) * 7 + D + bs)
     nb = 2 + sum((p + n - 1) // bs - p // bs + 2 for p, n in segs)
     c = B.Cache(nb, hkv, bs, D, fmt)
