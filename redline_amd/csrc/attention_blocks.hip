@@ -203,9 +203,10 @@ __device__ __forceinline__ void attend(const DecodeArgs& a, WaveState<D>& w, int
     float mx = fmaxf(fmaxf(fmaxf(e[0][0], e[0][1]), fmaxf(e[0][2], e[0][3])),
                      fmaxf(fmaxf(e[1][0], e[1][1]), fmaxf(e[1][2], e[1][3])));
     mx = rows_max<true>(rows_max<false>(mx));
-    const float mn = fmaxf(w.m, mx);
-    if (__any(mn != w.m)) {  // the output so far moves to the new maximum
-      const float f = __builtin_amdgcn_exp2f(w.m - mn);
+    // m is a reference within 2^8 of the maximum: moving it costs a pass over the
+    // output, and p up to 2^8 fits fp16 as well as p up to 1 does
+    if (__any(mx > w.m + 8.f)) {
+      const float mn = fmaxf(w.m, mx), f = __builtin_amdgcn_exp2f(w.m - mn);
       w.l *= f;
 #pragma unroll
       for (int d = 0; d < E; ++d) w.o[d] *= f;

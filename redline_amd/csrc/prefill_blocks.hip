@@ -22,7 +22,7 @@
 //       kKeys2   the same 128 rows, even and odd tiles (an image each), and join
 //                their partials at the end: calls that do not fill the chip;
 //       kOne     one group, whose CU holds two workgroups: between the two.
-// m, l and the output accumulate in fp32; P is rounded to fp16 (at most 1), and
+// m, l and the output accumulate in fp32; P is rounded to fp16 (at most 2^8), and
 // l sums the rounded values, so that numerator and denominator agree.
 #include <hip/hip_runtime.h>
 
@@ -51,19 +51,28 @@ struct PrefillArgs {
   int group;  // query heads per kv head
 };
 
-// Four codes as fp16: e4m3 times the scale (the conversion takes it, exactly),
+// Four codes as fp16, exactly: e4m3 times the scale (the conversion takes it),
 // INT8 V times the scale, INT8 K as it is (its scale multiplies the scores).
-template <bool kFp8>
-__device__ __forceinline__ u32x2 scaled_f16(uint32_t w, float s) {
-  f16x4 v;
-  if constexpr (kFp8) {
-    const f16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, false);
-    const f16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, true);
-    v = f16x4{lo[0], lo[1], hi[0], hi[1]};
+// INT8 comes as 1152 + code (codes_to_f16); times s, minus 1152 s, is one exact
+// fma while 1152 s is an fp16 number (`fused`, s <= 32).
+__device__ __forceinline__ u32x2 fp8_scaled_f16(uint32_t w, float s) {
+  const f16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, false);
+  const f16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, true);
+  return u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+}
+template <bool kFused>
+__device__ __forceinline__ u32x2 int8_scaled_f16(uint32_t w, _Float16 s) {
+  if constexpr (!kFused) {
+    return __builtin_bit_cast(u32x2, codes_to_f16<false>(w) * s);
   } else {
-    v = codes_to_f16<false>(w) * static_cast<_Float16>(s);
+    const uint32_t u = w ^ 0x80808080u;
+    const f16x2 s2 = {s, s}, c = f16x2{static_cast<_Float16>(-1152), static_cast<_Float16>(-1152)} * s2;
+    const f16x2 lo = __builtin_elementwise_fma(
+        __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)), s2, c);
+    const f16x2 hi = __builtin_elementwise_fma(
+        __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)), s2, c);
+    return u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
   }
-  return __builtin_bit_cast(u32x2, v);
 }
 
 // Two images of K and of V, used in turn, and the score scale of each 16-key tile
@@ -166,7 +175,7 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
       u32x2 x[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        x[e] = kFp8 ? scaled_f16<kFp8>(w[e], item[j].scale) : __builtin_bit_cast(u32x2, codes_to_f16<kFp8>(w[e]));
+        x[e] = kFp8 ? fp8_scaled_f16(w[e], item[j].scale) : __builtin_bit_cast(u32x2, codes_to_f16<kFp8>(w[e]));
       lds.k[buf][kp][0][key] = u32x4{x[0][0], x[0][1], x[1][0], x[1][1]};
       lds.k[buf][kp][1][key] = u32x4{x[2][0], x[2][1], x[3][0], x[3][1]};
       if (!kFp8 && pc == 0) reinterpret_cast<float*>(&lds.ks[(c + 1) & 3])[t16] = item[j].scale * cs;
@@ -178,10 +187,20 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
         const uint32_t mask = keep == 0 ? 0u : 0xffffffffu >> (32 - 8 * keep);
         w &= u32x4{mask, mask, mask, mask};
       }
+      auto put = [&](int e, u32x2 x) {
+        reinterpret_cast<u32x2*>(&lds.v[c & 1][t16][rho % 2][(4 * g + e) * 16 + m])[rho / 2] = x;
+      };
+      const _Float16 sc = static_cast<_Float16>(item[j].scale);
+      if constexpr (kFp8) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        reinterpret_cast<u32x2*>(&lds.v[c & 1][t16][rho % 2][(4 * g + e) * 16 + m])[rho / 2] =
-            scaled_f16<kFp8>(w[e], item[j].scale);
+        for (int e = 0; e < 4; ++e) put(e, fp8_scaled_f16(w[e], item[j].scale));
+      } else if (__any(item[j].scale > 32.f)) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) put(e, int8_scaled_f16<false>(w[e], sc));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) put(e, int8_scaled_f16<true>(w[e], sc));
+      }
     }
   };
   // conversion c of this thread's pieces, and the request of conversion c + 1's
@@ -270,9 +289,10 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
       mx = fmaxf(mx, y * c4[x]);
     }
     mx = rows_max<true>(mx);
-    const float mn = fmaxf(m, mx);
-    if (__any(mn != m)) {
-      const float f = __builtin_amdgcn_exp2f(m - mn);
+    // m is a reference within 2^8 of the maximum: moving it costs a pass over the
+    // output, and p up to 2^8 fits fp16 as well as p up to 1 does
+    if (__any(mx > m + 8.f)) {
+      const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - mn);
       l *= f;
 #pragma unroll
       for (int d = 0; d < D / 32; ++d) o[d] *= f;
@@ -392,10 +412,16 @@ hipError_t launch_s(const PrefillArgs& a, int64_t rows, hipStream_t stream) {
 
 template <int D, bool kFp8>
 hipError_t launch(const PrefillArgs& a, int64_t rows, hipStream_t stream) {
+  // Workgroups of 128 rows (of the grid: ragged prompts leave some of them empty).
+  // Up to two per CU, splitting the keys beats more rows; past that, at D = 128,
+  // 256 rows to an image beat 128, at D = 64 (three workgroups a CU) they do not.
+  // us, kOne / kRows2 / kKeys2: 2 chunks of 512, 8 kv heads of 128, e4m3 60 / 76 / 52;
+  // of 1024 92 / 97 / 81; of 2048 192 / 174 / 209; 4 x 4096 INT8 1600 / 1463 / 1828;
+  // D = 64: 2 chunks of 512 39 / - / 35, 24 ragged prompts 117 / 130 / 176, 4 x 4096
+  // 956 / 958 / 1128.  RLK_TUNE_BLK_PREFILL forces a split (tests and tuning runs).
   const int64_t groups = (rows + 127) / 128 * a.p.kv.num_kv_heads * a.w.num_seqs;
-  const int cus = compute_units();
-  // RLK_TUNE_BLK_PREFILL forces a split (tests and tuning runs)
-  switch (tune_knob(kBlkPrefill, groups <= cus ? kKeys2 : (groups <= 2 * cus ? kOne : kRows2))) {
+  const Split rule = groups <= 2 * compute_units() ? kKeys2 : (D == 64 ? kOne : kRows2);
+  switch (tune_knob(kBlkPrefill, rule)) {
     case kKeys2: return launch_s<D, kFp8, kKeys2>(a, rows, stream);
     case kOne: return launch_s<D, kFp8, kOne>(a, rows, stream);
     default: return launch_s<D, kFp8, kRows2>(a, rows, stream);
