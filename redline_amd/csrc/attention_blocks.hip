@@ -256,25 +256,24 @@ __device__ __forceinline__ void mark_whole(const DecodeArgs& a, int item, int he
   if (a.w.max_partitions > 1) a.w.ws_sum[slot_row(a, item, head)] = -1.f;
 }
 
-// The rows of an item that attends to nothing, for one kv head, by `threads`
-// threads.
+// The rows of an item that attends to nothing, for one kv head.
 template <int D, int G>
 __device__ __forceinline__ void attend_nothing(const DecodeArgs& a, int item, int token, int kvh) {
-  for (int i = threadIdx.x; i < G * D; i += kThreads) {
+  for (int i = threadIdx.x; i < G * D; i += blockDim.x) {
     out_row(a, token, kvh * G, D)[i] = static_cast<_Float16>(0.f);
     if (i % D == 0) mark_whole(a, item, kvh * G + i / D);
   }
 }
 
-// Grid form, for calls of few keys: one workgroup per (group_tokens keys, kv
-// head, item), whose waves split the keys and meet in LDS.
+// Grid form: one workgroup per (group_tokens keys, kv head, item), whose waves
+// split the keys and meet in LDS.
 template <int D, int G, bool kFp8>
 __global__ __launch_bounds__(kThreads, 2) void decode_blocks_grid_kernel(DecodeArgs a) {
   struct Lds {
-    float o[kWaves][G][D];
+    float o[kWaves][G][D + 4];  // padded: heads of one dim in different banks
     float m[kWaves][G], l[kWaves][G];
   };
-  __shared__ Lds s;
+  __shared__ alignas(16) Lds s;
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int slot = blockIdx.x, kvh = blockIdx.y, item = blockIdx.z;
   const int token = a.w.item_token[item];
@@ -292,9 +291,11 @@ __global__ __launch_bounds__(kThreads, 2) void decode_blocks_grid_kernel(DecodeA
   const int c = lane % 16;
   if (c < G) {
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s.o[wave][c][w.dim(d, i)] = w.o[d][i] * w.vref;
+      for (int d = 0; d < D / 16; d += 4)
+        *reinterpret_cast<f32x4*>(&s.o[wave][c][w.dim(d, i)]) =
+            f32x4{w.o[d][i], w.o[d + 1][i], w.o[d + 2][i], w.o[d + 3][i]} * w.vref;
     if (lane < 16) {
       s.m[wave][c] = w.m;
       s.l[wave][c] = w.l;
@@ -441,7 +442,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_blocks_range_kernel(Decode
 // rows' sums.
 template <int D>
 __global__ __launch_bounds__(D) void merge_blocks_kernel(DecodeArgs a) {
-  constexpr int kUnroll = 8;
+  constexpr int kUnroll = 16;
   const int item = blockIdx.x, h = blockIdx.y, d = threadIdx.x, lane = d % kWave;
   const int mp = a.w.max_partitions;
   const int64_t row = slot_row(a, item, h);
@@ -489,16 +490,27 @@ void launch_g(DecodeArgs a, hipStream_t stream) {
   const int64_t units = static_cast<int64_t>(a.w.num_items) * a.p.kv.num_kv_heads * mp;
   const int cus = compute_units();
   bool merge;
-  // RLK_TUNE_BLK_DECODE forces a form (0 grid, 1 range; tests and tuning runs)
-  if (tune_knob(kBlkDecode, units > static_cast<int64_t>(cus) * 4) != 0 && a.w.num_items <= kMaxItemsLds &&
-      mp > 1 && units * (kPart / kStep) < (1 << 30)) {
+  // RLK_TUNE_BLK_DECODE forces a form where it can serve the call (0 grid, 1
+  // range; tests and tuning runs)
+  // Equal ranges pay where contexts are several ranges long and fill the chip;
+  // they cost a longer start, and more where a range holds several short contexts.
+  // us, grid / range (8 kv heads of 128, contexts from 0 to the named one): 8 items
+  // to 8191 20.0 / 19.6, 16 35.4 / 27.2, 32 66 / 48; 32 to 4000 32.9 / 26.5; 32 to
+  // 2000 22.9 / 23.8, 64 31.5 / 29.8; 128 to 1000 29.1 / 35.4; 256 to 500 27.6 / 44.7.
+  const bool range = mp >= 8 && units > static_cast<int64_t>(cus) * 8;
+  if (tune_knob(kBlkDecode, range) != 0 && a.w.num_items <= kMaxItemsLds && mp > 1 &&
+      units * (kPart / kStep) < (1 << 30)) {
     a.ranges = kWavesPerCu * cus;
     const int64_t most = std::max<int64_t>(a.ranges, (units * (kPart / kStep) + kMaxRange - 1) / kMaxRange);
     decode_blocks_range_kernel<D, G, kFp8>
         <<<static_cast<uint32_t>((most + kWaves - 1) / kWaves), kThreads, 0, stream>>>(a);
     merge = true;
   } else {
-    a.group_tokens = units > static_cast<int64_t>(cus) * 16 ? 1024 : 256;
+    // as many slots as fill the chip with 4 workgroups a CU, of at most 4096 keys
+    const int64_t pairs = static_cast<int64_t>(a.w.num_items) * a.p.kv.num_kv_heads;
+    const int want = static_cast<int>(std::min<int64_t>(mp, (cus * 4 + pairs - 1) / pairs));
+    constexpr int kUnit = kWaves * kStep;
+    a.group_tokens = std::min((mp * kPart / want + kUnit - 1) / kUnit * kUnit, 1024 * kWaves);
     const int slots = (mp * kPart + a.group_tokens - 1) / a.group_tokens;
     const dim3 grid(slots, a.p.kv.num_kv_heads, a.w.num_items);
     decode_blocks_grid_kernel<D, G, kFp8><<<grid, kThreads, 0, stream>>>(a);

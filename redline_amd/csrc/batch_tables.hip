@@ -4,12 +4,15 @@
 // One launch.  Every workgroup reads all sequences and forms the running sums
 // (token rows, block needs, blocks given back, work items) for itself -- a few
 // thousand lengths cost less than a second launch or a wait between
-// workgroups would -- then does its share of the sequences, token rows and
-// returned blocks, finding the sequence of a row by binary search of the sums
-// in LDS.  Blocks are taken from the ring's head and returned at its tail, so
-// no workgroup writes an entry that another reads; the ring's state is written
-// by the workgroup that finishes reading it last (a ticket in its third word).
-// Bound: the launch and a chain of two dependent reads (lengths, table or ring).
+// workgroups would -- then does its share of the token rows and returned
+// blocks, finding the sequence of a row by binary search of the sums in LDS; the
+// first workgroup writes what there is one of per sequence.  All sums come from
+// one scan that takes every request for granted; only where the rows or the free
+// blocks do not suffice are they formed again step by step.  Blocks are taken
+// from the ring's head and returned at its tail, so no workgroup writes an entry
+// that another reads; the ring's state is written by the workgroup that is done
+// with it last (a ticket in its third word).
+// Bound: the launch and a chain of dependent reads (lengths, then table or ring).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -24,7 +27,7 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / kWave;
-constexpr int kRowsPerGroup = 2048;
+constexpr int kRowsPerGroup = kThreads;
 constexpr int kSat = 1 << 30;  // running sums of rows saturate here
 
 struct TableArgs {
@@ -37,7 +40,8 @@ __device__ __forceinline__ int sat_add(int a, int b) { return min(a + b, kSat); 
 // Exclusive sums of N values over the workgroup's threads (saturating); the
 // totals come back in `total`.
 template <int N>
-__device__ __forceinline__ void block_scan(int (&v)[N], int (&total)[N], int (*wave_tot)[N]) {
+__device__ __forceinline__ void block_scan(int (&v)[N], int (&total)[N], int (*wave_tot)[5]) {
+  static_assert(N <= 5, "room for 5 sums");
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   int incl[N];
 #pragma unroll
@@ -71,34 +75,30 @@ __device__ __forceinline__ void block_scan(int (&v)[N], int (&total)[N], int (*w
   }
 }
 
-// What one sequence asks for.
-struct Request {
-  int past, len, have, want;
-  bool live, ended;
-};
-
 __device__ __forceinline__ int blocks_of(uint32_t tokens, uint32_t bs) {
   const uint32_t b = tokens / bs;
   return static_cast<int>(b * bs == tokens ? b : b + 1);
 }
 
-__device__ __forceinline__ Request request(const rlk_batch_tables& t, int s) {
+// What one sequence asks for.
+struct Request {
+  int past, len, have, need, back;  // tokens cached, new; blocks held, needed, returned
+  bool live, ended, fits;           // fits: its table row, and past is sound
+};
+
+__device__ __forceinline__ Request request(const rlk_batch_tables& t, int past, int n) {
   Request r;
-  const int n = t.new_len[s];
-  r.past = t.past_len[s];
+  r.past = past;
   r.live = n > 0;
   r.ended = n < 0;
   r.len = min(max(n, 0), kSat);
-  const uint32_t past = max(r.past, 0);
-  r.have = blocks_of(past, t.block_size);
-  r.want = blocks_of(past + r.len, t.block_size);  // below 2^31 + 2^30
+  const uint32_t p = max(past, 0);
+  r.have = blocks_of(p, t.block_size);
+  const int want = blocks_of(p + r.len, t.block_size);  // p + len is below 2^31 + 2^30
+  r.need = want - r.have;
+  r.back = r.ended ? min(r.have, t.max_blocks_per_seq) : 0;
+  r.fits = r.live && past >= 0 && want >= 0 && want <= t.max_blocks_per_seq;
   return r;
-}
-
-// Whether a live sequence fits its table row and the token rows.
-__device__ __forceinline__ bool fits(const rlk_batch_tables& t, const Request& r, int start) {
-  return r.live && r.past >= 0 && r.want >= 0 && r.want <= t.max_blocks_per_seq && r.len <= t.num_rows &&
-         start <= t.num_rows - r.len;
 }
 
 // Last s in [0, n) with at[s] <= x (at[0] == 0 <= x).
@@ -111,10 +111,13 @@ __device__ __forceinline__ int find(const int* at, int n, int x) {
   return lo;
 }
 
+// kPer: sequences of a thread, which hold its requests in registers.
+template <int kPer>
 __global__ __launch_bounds__(kThreads) void build_batch_tables_kernel(TableArgs a) {
   const rlk_batch_tables& t = a.t;
   extern __shared__ int lds[];
-  __shared__ int wave_tot[kWaves][3];
+  __shared__ int wave_tot[kWaves][5];
+  __shared__ int taken_s;
   const int S = t.num_seqs, tid = threadIdx.x, group = blockIdx.x, groups = gridDim.x;
   // per sequence: first row, first taken block (-1: no rows of it), tokens
   // before, first returned block
@@ -122,86 +125,115 @@ __global__ __launch_bounds__(kThreads) void build_batch_tables_kernel(TableArgs 
   int* base_of = start_of + S;
   int* past_of = base_of + S;
   int* back_of = past_of + S;
-  const int cap = a.pool.capacity, mb = t.max_blocks_per_seq, bs = t.block_size;
+  const int cap = a.pool.capacity, mb = t.max_blocks_per_seq, bs = t.block_size, thr = t.decode_query_threshold;
   // (a state outside the ring is brought inside it: no index leaves the ring)
   const int head0 = a.pool.state[0], count = min(max(a.pool.state[1], 0), cap);
   const int head = head0 >= 0 && head0 < cap ? head0 : 0;
 
-  const int per = (S + kThreads - 1) / kThreads;
-  const int s0 = min(tid * per, S), s1 = min(s0 + per, S);
-  int rows[1] = {0}, rows_total[1];
-  for (int s = s0; s < s1; ++s) rows[0] = sat_add(rows[0], request(t, s).len);
-  block_scan(rows, rows_total, reinterpret_cast<int(*)[1]>(wave_tot));
-
-  int blk[2] = {0, 0}, blk_total[2];  // needed, returned
-  int start = rows[0];
-  for (int s = s0; s < s1; ++s) {
-    const Request r = request(t, s);
-    if (fits(t, r, start)) blk[0] = sat_add(blk[0], r.want - r.have);
-    if (r.ended) blk[1] = sat_add(blk[1], min(r.have, mb));
-    start = sat_add(start, r.len);
+  const int per = (S + kThreads - 1) / kThreads;  // at most kPer
+  const int s0 = tid * per, mine = max(min(S - s0, per), 0);
+  Request req[kPer];
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const bool on = k < mine;
+    req[k] = request(t, on ? t.past_len[s0 + k] : 0, on ? t.new_len[s0 + k] : 0);
   }
-  block_scan(blk, blk_total, reinterpret_cast<int(*)[2]>(wave_tot));
-
-  // decode items, prefill sequences, refused sequences; and the blocks taken
-  // (granted needs are a prefix of the needs)
-  int item[3] = {0, 0, 0}, item_total[3];
-  start = rows[0];
-  int need = blk[0];
-  auto granted = [&](const Request& r, int at, int before) {
-    const int n = r.want - r.have;
-    return fits(t, r, at) && (n == 0 || (before <= count && n <= count - before));
+  // rows, blocks needed and returned, decode items, prefill and refused
+  // sequences (16 bits each), as if every request that fits were granted
+  auto items = [&](const Request& r, bool ok, int& dec, int& seqs) {
+    dec = ok && r.len <= thr ? r.len : 0;
+    seqs = (ok && r.len > thr ? 1 : 0) + (r.live && !ok ? 1 << 16 : 0);
   };
-  for (int s = s0; s < s1; ++s) {
-    const Request r = request(t, s);
-    const bool ok = granted(r, start, need);
-    if (ok && r.len <= t.decode_query_threshold) item[0] = sat_add(item[0], r.len);
-    if (ok && r.len > t.decode_query_threshold) item[1] += 1;
-    if (r.live && !ok) item[2] += 1;
-    if (fits(t, r, start)) need = sat_add(need, r.want - r.have);
-    start = sat_add(start, r.len);
+  int sum[5] = {0, 0, 0, 0, 0}, total[5];
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    int dec, seqs;
+    items(req[k], req[k].fits, dec, seqs);
+    sum[0] = sat_add(sum[0], req[k].len);
+    sum[1] = sat_add(sum[1], req[k].fits ? req[k].need : 0);
+    sum[2] = sat_add(sum[2], req[k].back);
+    sum[3] = sat_add(sum[3], dec);
+    sum[4] += seqs;
   }
-  block_scan(item, item_total, wave_tot);
-
-  start = rows[0];
-  need = blk[0];
-  int back = blk[1], dec = item[0], pre = item[1];
-  for (int s = s0; s < s1; ++s) {
-    const Request r = request(t, s);
-    const bool ok = granted(r, start, need);
-    start_of[s] = start;
-    base_of[s] = ok ? need : -1;
-    past_of[s] = r.past;
-    back_of[s] = back;
-    if (group == 0) {
-      t.q_start[s] = start;
-      t.q_len[s] = ok ? r.len : 0;
-      t.ctx_len[s] = ok ? r.past + r.len : (r.ended ? 0 : r.past);
-      if (ok && r.len <= t.decode_query_threshold) {
-        for (int i = 0; i < r.len; ++i) {
-          t.decode_token[dec + i] = start + i;
-          t.decode_seq[dec + i] = s;
-        }
-      }
-      if (ok && r.len > t.decode_query_threshold) t.prefill_seq[pre] = s;
+  block_scan(sum, total, wave_tot);
+  const bool ample = total[0] <= t.num_rows && total[1] <= count;  // uniform
+  if (!ample) {
+    // rows first: who fits them; then the needs in order; then who is granted
+    int at = sum[0], need[1] = {0}, need_total[1];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      req[k].fits = req[k].fits && req[k].len <= t.num_rows && at <= t.num_rows - req[k].len;
+      need[0] = sat_add(need[0], req[k].fits ? req[k].need : 0);
+      at = sat_add(at, req[k].len);
     }
-    if (ok && r.len <= t.decode_query_threshold) dec += r.len;
-    if (ok && r.len > t.decode_query_threshold) pre += 1;
-    if (fits(t, r, start)) need = sat_add(need, r.want - r.have);
-    if (r.ended) back = sat_add(back, min(r.have, mb));
-    start = sat_add(start, r.len);
+    block_scan(need, need_total, wave_tot);
+    sum[1] = need[0];
+    int before = need[0], last[2] = {0, 0}, last_total[2];
+    if (tid == 0) taken_s = 0;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int n = req[k].fits ? req[k].need : 0;
+      const bool ok = req[k].fits && (n == 0 || (before <= count && n <= count - before));
+      int dec, seqs;
+      items(req[k], ok, dec, seqs);
+      last[0] = sat_add(last[0], dec);
+      last[1] += seqs;
+      // granted needs are a prefix of the needs
+      if (ok && n > 0) atomicMax(&taken_s, before + n);
+      before = sat_add(before, n);
+    }
+    block_scan(last, last_total, wave_tot);
+    sum[3] = last[0];
+    sum[4] = last[1];
+    total[1] = taken_s;
+    total[3] = last_total[0];
+    total[4] = last_total[1];
+  }
+  const int taken = total[1], pre_total = total[4] & 0xffff;
+  {
+    int start = sum[0], need = sum[1], back = sum[2], dec = sum[3], pre = sum[4] & 0xffff;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      if (k < mine) {
+        const Request& r = req[k];
+        const int s = s0 + k, n = r.fits ? r.need : 0;
+        const bool ok = r.fits && (n == 0 || (need <= count && n <= count - need));
+        start_of[s] = start;
+        base_of[s] = ok ? need : -1;
+        past_of[s] = r.past;
+        back_of[s] = back;
+        if (group == 0) {
+          t.q_start[s] = start;
+          t.q_len[s] = ok ? r.len : 0;
+          t.ctx_len[s] = ok ? r.past + r.len : (r.ended ? 0 : r.past);
+          if (ok && r.len <= thr) {
+            for (int i = 0; i < r.len; ++i) {
+              t.decode_token[dec + i] = start + i;
+              t.decode_seq[dec + i] = s;
+            }
+          }
+          if (ok && r.len > thr) t.prefill_seq[pre] = s;
+        }
+        if (ok && r.len <= thr) dec += r.len;
+        if (ok && r.len > thr) pre += 1;
+        need = sat_add(need, n);
+        back = sat_add(back, r.back);
+        start = sat_add(start, r.len);
+      }
+    }
   }
   if (group == 0) {
-    for (int i = item_total[0] + tid; i < t.num_rows; i += kThreads) {
+    for (int i = total[3] + tid; i < t.num_rows; i += kThreads) {
       t.decode_token[i] = -1;
       t.decode_seq[i] = 0;
     }
-    for (int i = item_total[1] + tid; i < S; i += kThreads) t.prefill_seq[i] = -1;
+    for (int i = pre_total + tid; i < S; i += kThreads) t.prefill_seq[i] = -1;
     if (tid == 0) {
-      t.counts[0] = rows_total[0];
-      t.counts[1] = item_total[0];
-      t.counts[2] = item_total[1];
-      t.counts[3] = item_total[2];
+      t.counts[0] = total[0];
+      t.counts[1] = total[3];
+      t.counts[2] = pre_total;
+      t.counts[3] = total[4] >> 16;
     }
   }
   __syncthreads();
@@ -210,10 +242,10 @@ __global__ __launch_bounds__(kThreads) void build_batch_tables_kernel(TableArgs 
     const uint32_t x = static_cast<uint32_t>(head) + static_cast<uint32_t>(i);  // i <= cap
     return static_cast<int>(x >= static_cast<uint32_t>(cap) ? x - cap : x);
   };
-  const int r_end = min((group + 1) * kRowsPerGroup, t.num_rows);
-  for (int row = group * kRowsPerGroup + tid; row < r_end; row += kThreads) {
+  const int row = group * kRowsPerGroup + tid;
+  if (row < t.num_rows) {
     int pos = 0, slot = -1;
-    if (row < rows_total[0]) {
+    if (row < total[0]) {
       const int s = find(start_of, S, row);
       if (base_of[s] >= 0) {
         const int past = past_of[s], have = blocks_of(past, bs);
@@ -234,41 +266,37 @@ __global__ __launch_bounds__(kThreads) void build_batch_tables_kernel(TableArgs 
     t.slot_mapping[row] = slot;
   }
   // blocks of ended sequences, behind the free ones
-  const int returned = min(blk_total[1], cap - count);
+  const int returned = min(total[2], cap - count);
   for (int i = group * kThreads + tid; i < returned; i += groups * kThreads) {
     const int s = find(back_of, S, i);
     a.pool.ring[ring_at(count + i)] = t.block_tables[static_cast<int64_t>(s) * mb + (i - back_of[s])];
   }
-
-  // Taken: needs are granted in order until one exceeds the count, so the sum
-  // is the largest prefix of whole requests within it.
-  __shared__ int taken_s;
-  if (tid == 0) taken_s = 0;
-  __syncthreads();
-  if (blk_total[0] <= count) {
-    if (tid == 0) taken_s = blk_total[0];
-  } else {
-    for (int s = s0; s < s1; ++s)
-      if (base_of[s] >= 0) {
-        const Request r = request(t, s);
-        if (r.want > r.have) atomicMax(&taken_s, base_of[s] + r.want - r.have);
-      }
-  }
-  __syncthreads();
   if (tid == 0) {
     int32_t* state = a.pool.state;
     int32_t* out = a.pool.state_out != nullptr ? a.pool.state_out : state;
-    const int taken = taken_s;
-    const int left = count - taken + returned;
-    if (groups == 1) {
+    // with several workgroups the one whose ticket is the last: every other has
+    // read the state
+    const bool last = groups == 1 || atomicAdd(&state[2], 1) == groups - 1;
+    if (last) {
+      if (groups > 1) state[2] = 0;
       out[0] = ring_at(taken);
-      out[1] = left;
-    } else if (atomicAdd(&state[2], 1) == groups - 1) {  // every group has read the state
-      state[2] = 0;
-      out[0] = ring_at(taken);
-      out[1] = left;
+      out[1] = count - taken + returned;
     }
   }
+}
+
+template <int kPer>
+int launch_tables(const TableArgs& a, hipStream_t stream) {
+  const char* what = "build_batch_tables";
+  const size_t lds = static_cast<size_t>(a.t.num_seqs) * 4 * sizeof(int);
+  if (lds > 48 * 1024) {
+    const hipError_t e = grant_dynamic_lds(reinterpret_cast<const void*>(build_batch_tables_kernel<kPer>),
+                                           RLK_BATCH_TABLES_MAX_SEQS * 4 * sizeof(int));
+    if (e != hipSuccess) return fail(static_cast<int>(e), "%s: %s", what, hipGetErrorString(e));
+  }
+  const int groups = std::max(1, (a.t.num_rows + kRowsPerGroup - 1) / kRowsPerGroup);
+  build_batch_tables_kernel<kPer><<<groups, kThreads, lds, stream>>>(a);
+  return launch_status(what);
 }
 
 }  // namespace
@@ -302,15 +330,10 @@ extern "C" int rlk_build_batch_tables(const rlk_block_pool* pool, const rlk_batc
       (t.num_rows > 0 && (t.positions == nullptr || t.slot_mapping == nullptr ||
                           t.decode_token == nullptr || t.decode_seq == nullptr)))
     return fail(RLK_EINVAL, "%s: null pointer argument", what);
-  const size_t lds = static_cast<size_t>(t.num_seqs) * 4 * sizeof(int);
-  if (lds > 48 * 1024) {
-    const hipError_t e = grant_dynamic_lds(reinterpret_cast<const void*>(build_batch_tables_kernel),
-                                           RLK_BATCH_TABLES_MAX_SEQS * 4 * sizeof(int));
-    if (e != hipSuccess)
-      return fail(static_cast<int>(e), "%s: %s", what, hipGetErrorString(e));
-  }
-  const int groups = std::max(1, (t.num_rows + kRowsPerGroup - 1) / kRowsPerGroup);
   const TableArgs a = {*pool, t};
-  build_batch_tables_kernel<<<groups, kThreads, lds, stream>>>(a);
-  return launch_status(what);
+  const int per = (t.num_seqs + kThreads - 1) / kThreads;
+  if (per <= 1) return launch_tables<1>(a, stream);
+  if (per <= 5) return launch_tables<5>(a, stream);
+  static_assert(RLK_BATCH_TABLES_MAX_SEQS <= 16 * kThreads, "16 sequences a thread at most");
+  return launch_tables<16>(a, stream);
 }

@@ -1,13 +1,14 @@
 // The block-scaled 8-bit KV cache, written (RoPE fused) and read back.
 //
 // Work of the write.  Rows that continue one block form a run (consecutive
-// rows, consecutive offsets); one group of 16 lanes does a whole run of one
-// kv head's K or V, so the scale of the (block, head) is decided, the old codes
-// requantised and the new ones stored without any exchange beyond a row of 16
-// lanes.  A wave does 4 heads of the same run, so its control flow is uniform.
-// A wave looks at kRows consecutive token rows and does the runs that start
-// among them; their starts are one ballot over the slots.  The q heads are
-// rotated by other workgroups of the same launch.
+// rows, consecutive offsets); the scale of the (block, head) follows from the
+// whole run, so one group of lanes does a whole run of one kv head's K or V:
+// decides the scale, requantises the old codes and stores the new ones, with no
+// exchange beyond a reduction over its lanes.  A wave does one K or V head for the
+// runs that start among kRows consecutive token rows, found by one ballot over
+// their slots: long runs (prompts) with all 64 lanes, runs of up to 4 rows
+// (decoding sequences) four at a time with 16 lanes each.  The q heads are rotated
+// by other workgroups of the same launch.
 //   K: lane p of a token holds the 8 rotation pairs (8p + e, D/2 + 8p + e),
 //      which are one 16-byte piece of the layout.
 //   V: lane m holds dims E m .. E m + E - 1 of the 4 tokens of a quad, which
@@ -60,24 +61,27 @@ struct WriteArgs {
   rlk_kv_block_view kv;
   int num_tokens, hq;
   int kv_groups;    // workgroups of the kv part, before those of the q part
-  int head_groups;  // waves a chunk of rows takes: ceil(2 * hkv / 4)
 };
 
-// The 8 rotation pairs of (x0, x1) at token position pos, rounded to fp16.
+// cos and sin of a token position for 8 rotation pairs, and their rotation
+// (rounded to fp16).
 template <int D>
-__device__ __forceinline__ void rotate8(const WriteArgs& a, int pos, int p0, f32x8& x0, f32x8& x1) {
+struct Angles {
+  f32x8 c, s;
+  __device__ __forceinline__ Angles(const WriteArgs& a, int pos, int p0) {
+    c = *reinterpret_cast<const f32x8*>(a.cos_t + static_cast<int64_t>(pos) * (D / 2) + p0);
+    s = *reinterpret_cast<const f32x8*>(a.sin_t + static_cast<int64_t>(pos) * (D / 2) + p0);
+  }
+  __device__ __forceinline__ void rotate(f32x8& x0, f32x8& x1) const {
 #pragma clang fp contract(off)
-  const float* cp = a.cos_t + static_cast<int64_t>(pos) * (D / 2) + p0;
-  const float* sp = a.sin_t + static_cast<int64_t>(pos) * (D / 2) + p0;
-  const f32x8 c = *reinterpret_cast<const f32x8*>(cp), s = *reinterpret_cast<const f32x8*>(sp);
-  const f32x8 y0 = x0 * c - x1 * s;
-  const f32x8 y1 = x1 * c + x0 * s;
-  x0 = round_f16(y0);
-  x1 = round_f16(y1);
-}
+    const f32x8 y0 = x0 * c - x1 * s;
+    const f32x8 y1 = x1 * c + x0 * s;
+    x0 = round_f16(y0);
+    x1 = round_f16(y1);
+  }
+};
 
-__device__ __forceinline__ f32x8 load_biased(const _Float16* row, const _Float16* bias, int col) {
-  u32x4 v = load16(row + col);
+__device__ __forceinline__ f32x8 biased(u32x4 v, const _Float16* bias, int col) {
   if (bias != nullptr)
     v = __builtin_bit_cast(u32x4, __builtin_bit_cast(f16x8, v) +
                                       __builtin_bit_cast(f16x8, load16(bias + col)));
@@ -95,6 +99,14 @@ struct Run {
   int row0, n, blk, off;
 };
 
+// Maximum over a group of 16 or 64 lanes.
+template <int kLanes>
+__device__ __forceinline__ float lanes_max(float v) {
+  v = group_max<16>(v);
+  if constexpr (kLanes == 64) v = rows_max<true>(rows_max<false>(v));
+  return v;
+}
+
 // The scale of the run's block and head: old (0 when the run starts the block)
 // joined with what amax asks for.  ratio = old / new for the old codes.
 template <bool kFp8>
@@ -104,38 +116,46 @@ __device__ __forceinline__ float join_scale(float old, float amax, float& ratio)
   return s;
 }
 
-// K of one head: lane p of D / 16 lanes per token; pos: the run's positions.
-template <int D, int BS, bool kFp8>
-__device__ __forceinline__ void write_k(const WriteArgs& a, const Run& r, const int* pos, int kvh,
-                                        int l16) {
-  constexpr int kLanes = D / 16, kTok = 16 / kLanes;  // lanes per token, tokens in flight
-  constexpr int kIts = BS / kTok;
-  const int p = l16 % kLanes, sub = l16 / kLanes;
+template <bool kFp8>
+__device__ __forceinline__ uint32_t requant4(uint32_t w, float ratio) {
+  const f32x4 v = decode4<kFp8>(w);
+  return encode4<kFp8>(v[0], v[1], v[2], v[3], ratio, BlockFormat<kFp8>::kMax);
+}
+
+// K of one head for a run of at most kMax rows, by kGroup lanes of which this is
+// number l; pos: the run's positions.
+template <int D, int BS, bool kFp8, int kGroup, int kMax>
+__device__ __forceinline__ void write_k(const WriteArgs& a, const Run& r, const int* pos, int kvh, int l) {
+  constexpr int kLanes = D / 16, kTok = kGroup / kLanes;  // lanes of a token, tokens in flight
+  constexpr int kIts = (kMax + kTok - 1) / kTok;
+  const int p = l % kLanes, sub = l / kLanes;
   const int heads = a.hq + 2 * a.kv.num_kv_heads, col = (a.hq + kvh) * D;
   const int64_t cell = static_cast<int64_t>(r.blk) * a.kv.num_kv_heads + kvh;
   const float old = r.off > 0 ? a.kv.k_scale[cell] : 0.f;
   uint8_t* dst = static_cast<uint8_t*>(a.kv.k) + cell * (BS * D) + p * 256;
+  // a lane past the run repeats its last row
   u32x4 x[kIts][2];
+#pragma unroll
+  for (int it = 0; it < kIts; ++it) {
+    const _Float16* row = a.qkv + static_cast<int64_t>(r.row0 + min(it * kTok + sub, r.n - 1)) * heads * D + col;
+    x[it][0] = ld16<true>(reinterpret_cast<const u32x4*>(row + 8 * p));
+    x[it][1] = ld16<true>(reinterpret_cast<const u32x4*>(row + D / 2 + 8 * p));
+  }
   float amax = 0.f;
 #pragma unroll
   for (int it = 0; it < kIts; ++it) {
-    if (it * kTok < r.n) {  // uniform
-      const int j = min(it * kTok + sub, r.n - 1);  // a lane past the run repeats its last row
-      const _Float16* row = a.qkv + static_cast<int64_t>(r.row0 + j) * heads * D;
-      f32x8 x0 = load_biased(row, a.bias, col + 8 * p);
-      f32x8 x1 = load_biased(row, a.bias, col + D / 2 + 8 * p);
-      rotate8<D>(a, pos[j], 8 * p, x0, x1);
-      amax = amax8(x1, amax8(x0, amax));
-      x[it][0] = pack8(x0);
-      x[it][1] = pack8(x1);
-    }
+    f32x8 x0 = biased(x[it][0], a.bias, col + 8 * p), x1 = biased(x[it][1], a.bias, col + D / 2 + 8 * p);
+    Angles<D>(a, pos[min(it * kTok + sub, r.n - 1)], 8 * p).rotate(x0, x1);
+    amax = amax8(x1, amax8(x0, amax));
+    x[it][0] = pack8(x0);
+    x[it][1] = pack8(x1);
   }
-  amax = group_max<16>(amax);
+  amax = lanes_max<kGroup>(amax);
   float ratio;
   const float s = join_scale<kFp8>(old, amax, ratio), inv = inv_scale(s), lim = code_limit<kFp8>(s);
 #pragma unroll
   for (int it = 0; it < kIts; ++it) {
-    if (it * kTok < r.n && it * kTok + sub < r.n) {
+    if (it * kTok + sub < r.n) {
       const f32x8 x0 = unpack8(x[it][0]), x1 = unpack8(x[it][1]);
       const int key = r.off + it * kTok + sub;
       const u32x4 w = {encode4<kFp8>(x0[0], x0[1], x0[2], x0[3], inv, lim),
@@ -145,188 +165,220 @@ __device__ __forceinline__ void write_k(const WriteArgs& a, const Run& r, const 
       store16(dst + (key / 16) * (16 * D) + (key % 16) * 16, w);
     }
   }
-  if (ratio != 1.f) {  // the same for the 16 lanes: requantise the earlier offsets
+  if (ratio != 1.f) {  // the same for the group's lanes: requantise the earlier offsets
     for (int key = sub; key < r.off; key += kTok) {
       u32x4* at = reinterpret_cast<u32x4*>(dst + (key / 16) * (16 * D) + (key % 16) * 16);
       u32x4 w = *at;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const f32x4 v = decode4<kFp8>(w[e]);
-        w[e] = encode4<kFp8>(v[0], v[1], v[2], v[3], ratio, BlockFormat<kFp8>::kMax);
-      }
+      for (int e = 0; e < 4; ++e) w[e] = requant4<kFp8>(w[e], ratio);
       *at = w;
     }
   }
-  if (l16 == 0 && (r.off == 0 || ratio != 1.f)) a.kv.k_scale[cell] = s;
+  if (l == 0 && (r.off == 0 || ratio != 1.f)) a.kv.k_scale[cell] = s;
 }
 
-// V of one head: lane m.
-template <int D, int BS, bool kFp8>
-__device__ __forceinline__ void write_v(const WriteArgs& a, const Run& r, int kvh, int m) {
-  constexpr int E = D / 16, kQuads = BS / 4;
+// V of one head likewise: lane m of a row of 16 holds dims E m .. E m + E - 1;
+// the rows of 16 take every kRows16-th quad of the block.
+template <int D, int BS, bool kFp8, int kGroup, int kMax>
+__device__ __forceinline__ void write_v(const WriteArgs& a, const Run& r, int kvh, int l) {
+  constexpr int E = D / 16, kRows16 = kGroup / 16;
+  // quads that a run of kMax rows can touch (it may start inside one)
+  constexpr int kQuads = (kMax + 6) / 4 < BS / 4 ? (kMax + 6) / 4 : BS / 4;
+  constexpr int kIts = (kQuads + kRows16 - 1) / kRows16;
   using Raw = typename std::conditional<E == 8, u32x4, u32x2>::type;  // E halves
   typedef _Float16 f16xE __attribute__((ext_vector_type(E)));
+  const int m = l % 16;
   const int heads = a.hq + 2 * a.kv.num_kv_heads;
   const int col = (a.hq + a.kv.num_kv_heads + kvh) * D + E * m;
   const int64_t cell = static_cast<int64_t>(r.blk) * a.kv.num_kv_heads + kvh;
   const float old = r.off > 0 ? a.kv.v_scale[cell] : 0.f;
   uint8_t* dst = static_cast<uint8_t*>(a.kv.v) + cell * (BS * D) + m * 16;
-  const int q0 = r.off / 4, q1 = (r.off + r.n - 1) / 4;  // quads that the run touches
-  f16xE x[kQuads][4];
+  const int q0 = r.off / 4, q1 = (r.off + r.n - 1) / 4;  // quads of the run
+  f16xE x[kIts][4];
+#pragma unroll
+  for (int it = 0; it < kIts; ++it)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // keys outside the run repeat one inside it
+      const int j = min(max(4 * (q0 + it * kRows16 + l / 16) + i - r.off, 0), r.n - 1);
+      const _Float16* row = a.qkv + static_cast<int64_t>(r.row0 + j) * heads * D;
+      x[it][i] = __builtin_bit_cast(f16xE, __builtin_nontemporal_load(reinterpret_cast<const Raw*>(row + col)));
+    }
   f16xE bias = {};
   if (a.bias != nullptr) bias = *reinterpret_cast<const f16xE*>(a.bias + col);
+  // a quad's bytes of keys inside the run, and of those before it; the pieces of
+  // quads that the run fills in part are read with its rows
+  auto piece = [&](int quad, int g) {
+    return reinterpret_cast<u32x4*>(dst + (quad / 4) * (16 * D) + (quad % 4) * 256 + g * 1024);
+  };
+  uint32_t mine[kIts], below[kIts];
+  u32x4 had[kIts][E / 4];
+#pragma unroll
+  for (int it = 0; it < kIts; ++it) {
+    const int quad = q0 + it * kRows16 + l / 16;
+    const int lo = min(max(r.off - 4 * quad, 0), 4), hi = min(max(r.off + r.n - 4 * quad, 0), 4);
+    below[it] = lo == 0 ? 0u : 0xffffffffu >> (32 - 8 * lo);
+    mine[it] = (hi == 0 ? 0u : 0xffffffffu >> (32 - 8 * hi)) & ~below[it];
+#pragma unroll
+    for (int g = 0; g < E / 4; ++g)
+      had[it][g] = quad <= q1 && mine[it] != 0xffffffffu ? *piece(quad, g) : u32x4{0, 0, 0, 0};
+  }
   float amax = 0.f;
 #pragma unroll
-  for (int q = 0; q < kQuads; ++q) {
-    if (q <= q1 - q0) {  // uniform
+  for (int it = 0; it < kIts; ++it)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // keys outside the run repeat one inside it
-        const int j = min(max(4 * (q0 + q) + i - r.off, 0), r.n - 1);
-        const _Float16* row = a.qkv + static_cast<int64_t>(r.row0 + j) * heads * D;
-        f16xE v = __builtin_bit_cast(f16xE, *reinterpret_cast<const Raw*>(row + col));
-        if (a.bias != nullptr) v += bias;
-        x[q][i] = v;
+    for (int i = 0; i < 4; ++i) {
+      if (a.bias != nullptr) x[it][i] += bias;
 #pragma unroll
-        for (int d = 0; d < E; ++d) amax = fmaxf(amax, __builtin_fabsf(static_cast<float>(v[d])));
-      }
+      for (int d = 0; d < E; ++d) amax = fmaxf(amax, __builtin_fabsf(static_cast<float>(x[it][i][d])));
     }
-  }
-  amax = group_max<16>(amax);
+  amax = lanes_max<kGroup>(amax);
   float ratio;
   const float s = join_scale<kFp8>(old, amax, ratio), inv = inv_scale(s), lim = code_limit<kFp8>(s);
-  auto requant = [&](uint32_t w) {
-    const f32x4 v = decode4<kFp8>(w);
-    return encode4<kFp8>(v[0], v[1], v[2], v[3], ratio, BlockFormat<kFp8>::kMax);
-  };
 #pragma unroll
-  for (int q = 0; q < kQuads; ++q) {
-    if (q <= q1 - q0) {
-      const int quad = q0 + q;
-      uint8_t* at = dst + (quad / 4) * (16 * D) + (quad % 4) * 256;
-      // bytes of the quad's keys inside the run, and of those before it
-      const int lo = max(r.off - 4 * quad, 0), hi = min(r.off + r.n - 4 * quad, 4);
-      const uint32_t below = lo == 0 ? 0u : 0xffffffffu >> (32 - 8 * lo);
-      const uint32_t mine = (hi == 4 ? 0xffffffffu : 0xffffffffu >> (32 - 8 * hi)) & ~below;
+  for (int it = 0; it < kIts; ++it) {
+    const int quad = q0 + it * kRows16 + l / 16;
+    if (quad <= q1) {
 #pragma unroll
       for (int g = 0; g < E / 4; ++g) {
-        u32x4* piece = reinterpret_cast<u32x4*>(at + g * 1024);
         u32x4 w;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int d = 4 * g + j;
-          w[j] = encode4<kFp8>(static_cast<float>(x[q][0][d]), static_cast<float>(x[q][1][d]),
-                               static_cast<float>(x[q][2][d]), static_cast<float>(x[q][3][d]), inv, lim);
-        }
-        if (mine != 0xffffffffu) {  // uniform
-          const u32x4 had = *piece;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t keep = ratio != 1.f ? (requant(had[j]) & below) | (had[j] & ~below) : had[j];
-            w[j] = (w[j] & mine) | (keep & ~mine);
+          w[j] = encode4<kFp8>(static_cast<float>(x[it][0][d]), static_cast<float>(x[it][1][d]),
+                               static_cast<float>(x[it][2][d]), static_cast<float>(x[it][3][d]), inv, lim);
+          if (mine[it] != 0xffffffffu) {
+            const uint32_t h = had[it][g][j];
+            const uint32_t keep = ratio != 1.f ? (requant4<kFp8>(h, ratio) & below[it]) | (h & ~below[it]) : h;
+            w[j] = (w[j] & mine[it]) | (keep & ~mine[it]);
           }
         }
-        *piece = w;
+        *piece(quad, g) = w;
       }
     }
   }
   if (ratio != 1.f) {
-    for (int quad = 0; quad < q0; ++quad) {
-      uint8_t* at = dst + (quad / 4) * (16 * D) + (quad % 4) * 256;
+    for (int quad = l / 16; quad < q0; quad += kRows16) {
 #pragma unroll
       for (int g = 0; g < E / 4; ++g) {
-        u32x4* piece = reinterpret_cast<u32x4*>(at + g * 1024);
-        u32x4 w = *piece;
+        u32x4 w = *piece(quad, g);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = requant(w[j]);
-        *piece = w;
+        for (int j = 0; j < 4; ++j) w[j] = requant4<kFp8>(w[j], ratio);
+        *piece(quad, g) = w;
       }
     }
   }
-  if (m == 0 && (r.off == 0 || ratio != 1.f)) a.kv.v_scale[cell] = s;
+  if (l == 0 && (r.off == 0 || ratio != 1.f)) a.kv.v_scale[cell] = s;
 }
 
 constexpr int kWriteThreads = 256;
+constexpr int kShort = 4;  // rows of a run that 16 lanes do
 
-// The runs that start in rows chunk0 .. chunk0 + kRows - 1, for 4 of the
-// 2 * hkv (K heads, then V heads): head unit 4 * group + lane / 16.
+// The runs that start in rows chunk0 .. chunk0 + kRows - 1, for K head `unit` or
+// V head unit - hkv.
 template <int D, int BS, bool kFp8, int kRows>
-__device__ __forceinline__ void write_chunk(const WriteArgs& a, int chunk0, int group, int lane,
-                                            int* pos) {
+__device__ __forceinline__ void write_chunk(const WriteArgs& a, int chunk0, int unit, int lane, int* pos) {
   static_assert(kRows + BS <= kWave, "a chunk's rows and the last run's rest fit one wave");
   const int hkv = a.kv.num_kv_heads;
   const int row = chunk0 + lane;
   const int slot = row < a.num_tokens ? a.slots[row] : -1;
   int before = __shfl_up(slot, 1, kWave);
   if (lane == 0) before = chunk0 > 0 ? a.slots[chunk0 - 1] : -1;
-  // positions of the rows, in LDS: the lanes of a K head need those of other
-  // rows, and lanes of the wave that do a V head are not there to hand them over
+  // positions of the rows, in LDS: lanes of one run need those of other rows
   pos[lane] = row < a.num_tokens ? a.positions[row] : 0;
   __builtin_amdgcn_wave_barrier();
   const bool valid = slot >= 0 && slot / BS < a.kv.num_blocks;
   // a row starts a run unless it continues the block of the row before
-  const bool start = !valid || slot % BS == 0 || slot != before + 1;
-  const uint64_t starts = __ballot(start);
-  uint64_t todo = __ballot(start && valid) & ((1ull << kRows) - 1);
-  const int unit = 4 * group + lane / 16;
+  const uint64_t starts = __ballot(!valid || slot % BS == 0 || slot != before + 1);
+  uint64_t todo = starts & __ballot(valid) & ((1ull << kRows) - 1);
+  auto run_at = [&](int i) {  // the run that starts at row chunk0 + i
+    const uint64_t after = starts >> (i + 1);
+    const int sl = __shfl(slot, i, kWave);
+    return Run{chunk0 + i, after != 0 ? __builtin_ctzll(after) + 1 : kWave - i, sl / BS, sl % BS};
+  };
   while (todo != 0) {  // uniform over the wave
     const int i = __builtin_ctzll(todo);
-    todo &= todo - 1;
     const uint64_t after = starts >> (i + 1);
-    const int n = after != 0 ? __builtin_ctzll(after) + 1 : kWave - i;
-    const int sl = __builtin_amdgcn_readlane(slot, i);
-    const Run r = {chunk0 + i, n, sl / BS, sl % BS};
-    if (unit < hkv) {
-      write_k<D, BS, kFp8>(a, r, pos + i, unit, lane % 16);
-    } else if (unit < 2 * hkv) {
-      write_v<D, BS, kFp8>(a, r, unit - hkv, lane % 16);
+    if (after == 0 || __builtin_ctzll(after) + 1 > kShort) {  // a long run, by the whole wave
+      todo &= todo - 1;
+      const Run r = run_at(i);
+      if (unit < hkv) write_k<D, BS, kFp8, 64, BS>(a, r, pos + i, unit, lane);
+      else write_v<D, BS, kFp8, 64, BS>(a, r, unit - hkv, lane);
+    } else {  // up to four short ones, one to each 16 lanes
+      int mine = -1;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int k = todo != 0 ? __builtin_ctzll(todo) : -1;
+        const uint64_t rest = k >= 0 ? starts >> (k + 1) : 0;
+        if (rest == 0 || __builtin_ctzll(rest) + 1 > kShort) break;
+        if (lane / 16 == g) mine = k;
+        todo &= todo - 1;
+      }
+      const Run r = run_at(max(mine, 0));
+      if (mine >= 0) {
+        if (unit < hkv) write_k<D, BS, kFp8, 16, kShort>(a, r, pos + mine, unit, lane % 16);
+        else write_v<D, BS, kFp8, 16, kShort>(a, r, unit - hkv, lane % 16);
+      }
     }
   }
 }
 
-template <int D, int BS, bool kFp8, int kRows>
+// kHeads: q heads that a lane rotates with one load of cos and sin.
+template <int D, int BS, bool kFp8, int kRows, int kHeads>
 __global__ __launch_bounds__(kWriteThreads) void write_kv_blocks_kernel(WriteArgs a) {
   __shared__ int pos[kWriteThreads / kWave][kWave];
-  const int tid = threadIdx.x, lane = tid % kWave;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   if (static_cast<int>(blockIdx.x) < a.kv_groups) {
-    const int w = blockIdx.x * (kWriteThreads / kWave) + tid / kWave;
-    const int chunk = w / a.head_groups;
-    if (chunk * kRows >= a.num_tokens) return;
-    write_chunk<D, BS, kFp8, kRows>(a, chunk * kRows, w - chunk * a.head_groups, lane,
-                                       pos[tid / kWave]);
+    const int units = 2 * a.kv.num_kv_heads, w = blockIdx.x * (kWriteThreads / kWave) + wave;
+    const int chunk = w / units;
+    if (chunk >= (a.num_tokens + kRows - 1) / kRows) return;
+    write_chunk<D, BS, kFp8, kRows>(a, chunk * kRows, w - chunk * units, lane, pos[wave]);
     return;
   }
-  // q heads: 8 rotation pairs per lane
+  // q heads: 8 rotation pairs of kHeads heads per lane
   constexpr int kLanes = D / 16;
   const int64_t g = static_cast<int64_t>(blockIdx.x - a.kv_groups) * kWriteThreads + tid;
-  const int per = a.hq * kLanes;
+  const int per = a.hq / kHeads * kLanes;
   const int64_t t = g / per;
   if (t >= a.num_tokens) return;
-  const int h = static_cast<int>(g - t * per) / kLanes, p0 = static_cast<int>(g % kLanes) * 8;
-  const int heads = a.hq + 2 * a.kv.num_kv_heads;
+  const int h = static_cast<int>(g - t * per) / kLanes * kHeads, p0 = static_cast<int>(g % kLanes) * 8;
+  const int heads = a.hq + 2 * a.kv.num_kv_heads, col = h * D + p0;
   _Float16* row = a.qkv + t * heads * D;
-  f32x8 x0 = load_biased(row, a.bias, h * D + p0), x1 = load_biased(row, a.bias, h * D + D / 2 + p0);
-  rotate8<D>(a, a.positions[t], p0, x0, x1);
-  st16<true>(reinterpret_cast<u32x4*>(row + h * D + p0), pack8(x0));
-  st16<true>(reinterpret_cast<u32x4*>(row + h * D + D / 2 + p0), pack8(x1));
+  u32x4 v[kHeads][2];
+#pragma unroll
+  for (int k = 0; k < kHeads; ++k) {
+    v[k][0] = ld16<true>(reinterpret_cast<const u32x4*>(row + col + k * D));
+    v[k][1] = ld16<true>(reinterpret_cast<const u32x4*>(row + col + k * D + D / 2));
+  }
+  const Angles<D> an(a, a.positions[t], p0);
+#pragma unroll
+  for (int k = 0; k < kHeads; ++k) {
+    f32x8 x0 = biased(v[k][0], a.bias, col + k * D), x1 = biased(v[k][1], a.bias, col + k * D + D / 2);
+    an.rotate(x0, x1);
+    st16<true>(reinterpret_cast<u32x4*>(row + col + k * D), pack8(x0));
+    st16<true>(reinterpret_cast<u32x4*>(row + col + k * D + D / 2), pack8(x1));
+  }
 }
 
 template <int D, int BS, bool kFp8>
 int launch_write(WriteArgs a, hipStream_t stream) {
-  // RLK_TUNE_BLK_WRITE forces the rows of a wave (1 or 16; tests and tuning runs)
-  const int rows = tune_knob(kBlkWrite, a.num_tokens > 1024 ? 16 : 1) == 1 ? 1 : 16;
-  const int64_t waves = static_cast<int64_t>((a.num_tokens + rows - 1) / rows) * a.head_groups;
+  // RLK_TUNE_BLK_WRITE forces the rows of a wave (4 or 16; tests and tuning runs)
+  const int rows = tune_knob(kBlkWrite, a.num_tokens > 1024 ? 16 : 4) == 4 ? 4 : 16;
+  const int64_t waves = static_cast<int64_t>((a.num_tokens + rows - 1) / rows) * 2 * a.kv.num_kv_heads;
   const int64_t kvg = (waves + kWriteThreads / kWave - 1) / (kWriteThreads / kWave);
-  const int64_t qg = (static_cast<int64_t>(a.num_tokens) * a.hq * (D / 16) + kWriteThreads - 1) / kWriteThreads;
+  const int per = rows == 16 && a.hq % 4 == 0 ? 4 : 1;
+  const int64_t qg = (static_cast<int64_t>(a.num_tokens) * (a.hq / per) * (D / 16) + kWriteThreads - 1) / kWriteThreads;
   if (kvg + qg > 0x7fffffffll)
     return fail(RLK_EINVAL, "rope_and_write_kv_blocks: %d rows exceed one launch; split the call",
                 a.num_tokens);
   a.kv_groups = static_cast<int>(kvg);
   const uint32_t grid = static_cast<uint32_t>(kvg + qg);
-  if (rows == 1) {
-    write_kv_blocks_kernel<D, BS, kFp8, 1><<<grid, kWriteThreads, 0, stream>>>(a);
+  if (rows == 4) {
+    write_kv_blocks_kernel<D, BS, kFp8, 4, 1><<<grid, kWriteThreads, 0, stream>>>(a);
+  } else if (per == 4) {
+    write_kv_blocks_kernel<D, BS, kFp8, 16, 4><<<grid, kWriteThreads, 0, stream>>>(a);
   } else {
-    write_kv_blocks_kernel<D, BS, kFp8, 16><<<grid, kWriteThreads, 0, stream>>>(a);
+    write_kv_blocks_kernel<D, BS, kFp8, 16, 1><<<grid, kWriteThreads, 0, stream>>>(a);
   }
   return launch_status("rope_and_write_kv_blocks");
 }
@@ -351,7 +403,9 @@ __device__ __forceinline__ u32x2 scaled4(f32x4 v, float s) {
   return __builtin_bit_cast(u32x2, __builtin_convertvector(v * s, f16x4));
 }
 
-// 16 lanes take 4 rows of the list for one head's K or V.
+// 16 lanes take 4 rows of the list for one head's K or V.  Where the 4 rows are a
+// quad of the layout (lists of consecutive slots), each V piece is read once and
+// gives 4 rows; other rows take theirs alone, a byte in four of what they read.
 template <int D, bool kFp8>
 __global__ __launch_bounds__(256) void read_kv_blocks_kernel(ReadArgs a) {
   constexpr int E = D / 16, kLanes = D / 16, kTok = 16 / kLanes;
@@ -359,40 +413,74 @@ __global__ __launch_bounds__(256) void read_kv_blocks_kernel(ReadArgs a) {
   const int64_t g = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int l16 = g % 16;
   const int64_t group = g / 16;
-  const int quad = static_cast<int>(group / (2 * hkv)), unit = static_cast<int>(group % (2 * hkv));
-  if (quad * 4 >= a.n) return;
+  const int i0 = static_cast<int>(group / (2 * hkv)) * 4, unit = static_cast<int>(group % (2 * hkv));
+  if (i0 >= a.n) return;
   const bool is_v = unit >= hkv;
   const int kvh = is_v ? unit - hkv : unit;
   _Float16* out = is_v ? a.v_out : a.k_out;
   if (out == nullptr) return;
-  const uint8_t* base = static_cast<const uint8_t*>(is_v ? a.kv.v : a.kv.k);
-  const float* scales = is_v ? a.kv.v_scale : a.kv.k_scale;
-  for (int u = 0; u < 4; u += is_v ? 1 : kTok) {
-    const int i = quad * 4 + u + (is_v ? 0 : l16 / kLanes);
-    if (i >= a.n) continue;
-    const int slot = a.slots[i];
-    if (slot < 0 || slot / bs >= a.kv.num_blocks) continue;
-    const int blk = slot / bs, off = slot - blk * bs;
-    const int64_t cell = static_cast<int64_t>(blk) * hkv + kvh;
-    const float s = scales[cell];
-    const uint8_t* tile = base + cell * (bs * D) + (off / 16) * (16 * D);
-    _Float16* o = out + (static_cast<int64_t>(i) * hkv + kvh) * D;
-    if (!is_v) {
-      const int p = l16 % kLanes;
-      const u32x4 w = load16(tile + p * 256 + (off % 16) * 16);
-      const u32x2 a0 = scaled4(decode4<kFp8>(w[0]), s), a1 = scaled4(decode4<kFp8>(w[1]), s);
-      const u32x2 b0 = scaled4(decode4<kFp8>(w[2]), s), b1 = scaled4(decode4<kFp8>(w[3]), s);
-      store16(o + 8 * p, u32x4{a0[0], a0[1], a1[0], a1[1]});
-      store16(o + D / 2 + 8 * p, u32x4{b0[0], b0[1], b1[0], b1[1]});
-    } else {
+  int slot[4];
 #pragma unroll
-      for (int gg = 0; gg < E / 4; ++gg) {
-        const u32x4 w = load16(tile + gg * 1024 + (off % 16 / 4) * 256 + l16 * 16);
-        const int sh = 8 * (off % 4);
-        const uint32_t b = ((w[0] >> sh) & 0xff) | (((w[1] >> sh) & 0xff) << 8) |
-                           (((w[2] >> sh) & 0xff) << 16) | (((w[3] >> sh) & 0xff) << 24);
-        *reinterpret_cast<u32x2*>(o + E * l16 + 4 * gg) = scaled4(decode4<kFp8>(b), s);
+  for (int u = 0; u < 4; ++u) slot[u] = i0 + u < a.n ? a.slots[i0 + u] : -1;
+  auto tile_of = [&](const void* base, int blk, int off) {
+    const int64_t cell = static_cast<int64_t>(blk) * hkv + kvh;
+    return static_cast<const uint8_t*>(base) + cell * (bs * D) + (off / 16) * (16 * D);
+  };
+  auto valid = [&](int s) { return s >= 0 && s / bs < a.kv.num_blocks; };
+  if (!is_v) {
+    const int p = l16 % kLanes;
+#pragma unroll
+    for (int u = 0; u < 4; u += kTok) {
+      const int v = u + l16 / kLanes, s = v == 0 ? slot[0] : (v == 1 ? slot[1] : (v == 2 ? slot[2] : slot[3]));
+      if (!valid(s)) continue;
+      const int blk = s / bs, off = s - blk * bs;
+      const float sc = a.kv.k_scale[static_cast<int64_t>(blk) * hkv + kvh];
+      const u32x4 w = load16(tile_of(a.kv.k, blk, off) + p * 256 + (off % 16) * 16);
+      const u32x2 a0 = scaled4(decode4<kFp8>(w[0]), sc), a1 = scaled4(decode4<kFp8>(w[1]), sc);
+      const u32x2 b0 = scaled4(decode4<kFp8>(w[2]), sc), b1 = scaled4(decode4<kFp8>(w[3]), sc);
+      _Float16* o = out + (static_cast<int64_t>(i0 + v) * hkv + kvh) * D;
+      st16<true>(reinterpret_cast<u32x4*>(o + 8 * p), u32x4{a0[0], a0[1], a1[0], a1[1]});
+      st16<true>(reinterpret_cast<u32x4*>(o + D / 2 + 8 * p), u32x4{b0[0], b0[1], b1[0], b1[1]});
+    }
+    return;
+  }
+  auto row = [&](int u) { return out + (static_cast<int64_t>(i0 + u) * hkv + kvh) * D + E * l16; };
+  if (valid(slot[0]) && slot[0] % 4 == 0 && slot[1] == slot[0] + 1 && slot[2] == slot[0] + 2 &&
+      slot[3] == slot[0] + 3) {
+    const int blk = slot[0] / bs, off = slot[0] - blk * bs;
+    const float sc = a.kv.v_scale[static_cast<int64_t>(blk) * hkv + kvh];
+    const uint8_t* at = tile_of(a.kv.v, blk, off) + (off % 16 / 4) * 256 + l16 * 16;
+    f32x4 v[E];  // dim E m + d of the 4 rows
+#pragma unroll
+    for (int gg = 0; gg < E / 4; ++gg) {
+      const u32x4 w = load16(at + gg * 1024);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[4 * gg + j] = decode4<kFp8>(w[j]) * sc;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if constexpr (E == 8) {
+        st16<true>(reinterpret_cast<u32x4*>(row(u)),
+                   pack8(f32x8{v[0][u], v[1][u], v[2][u], v[3][u], v[4][u], v[5][u], v[6][u], v[7][u]}));
+      } else {
+        st8<true>(reinterpret_cast<u32x2*>(row(u)), scaled4(f32x4{v[0][u], v[1][u], v[2][u], v[3][u]}, 1.f));
       }
+    }
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    if (!valid(slot[u])) continue;
+    const int blk = slot[u] / bs, off = slot[u] - blk * bs;
+    const float sc = a.kv.v_scale[static_cast<int64_t>(blk) * hkv + kvh];
+    const uint8_t* at = tile_of(a.kv.v, blk, off) + (off % 16 / 4) * 256 + l16 * 16;
+#pragma unroll
+    for (int gg = 0; gg < E / 4; ++gg) {
+      const u32x4 w = load16(at + gg * 1024);
+      const int sh = 8 * (off % 4);
+      const uint32_t b = ((w[0] >> sh) & 0xff) | (((w[1] >> sh) & 0xff) << 8) |
+                         (((w[2] >> sh) & 0xff) << 16) | (((w[3] >> sh) & 0xff) << 24);
+      *reinterpret_cast<u32x2*>(row(u) + 4 * gg) = scaled4(decode4<kFp8>(b), sc);
     }
   }
 }
@@ -427,7 +515,6 @@ extern "C" int rlk_rope_and_write_kv_blocks(uint16_t* qkv, const int32_t* positi
   a.kv = *kv;
   a.num_tokens = num_tokens;
   a.hq = num_heads;
-  a.head_groups = (2 * kv->num_kv_heads + 3) / 4;
   if (kv->head_dim == 128)
     return kv->block_size == 16 ? launch_write_f<128, 16>(a, stream) : launch_write_f<128, 32>(a, stream);
   return kv->block_size == 16 ? launch_write_f<64, 16>(a, stream) : launch_write_f<64, 32>(a, stream);

@@ -81,7 +81,7 @@ WRITE_CASES = [
 ]
 
 
-@pytest.fixture(params=[None, 1, 16], ids=["rule", "rows1", "rows16"])
+@pytest.fixture(params=[None, 4, 16], ids=["rule", "rows4", "rows16"])
 def write_rows(request):
     """Rows that a wave looks at: the launcher's choice, and each forced."""
     from redline_amd._lib import tune_knob
