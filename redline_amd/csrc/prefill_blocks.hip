@@ -51,6 +51,15 @@ struct PrefillArgs {
   int group;  // query heads per kv head
 };
 
+// What no kernel writes while this one reads it, for scalar loads at uniform
+// addresses.
+template <class T>
+using ScalarPtr = const __attribute__((address_space(4))) T*;
+template <class T>
+__device__ __forceinline__ ScalarPtr<T> scalar(const T* p) {
+  return (ScalarPtr<T>)(p);
+}
+
 // Four codes as fp16, exactly: e4m3 times the scale (the conversion takes it),
 // INT8 V times the scale, INT8 K as it is (its scale multiplies the scores).
 // INT8 comes as 1152 + code (codes_to_f16); times s, minus 1152 s, is one exact
@@ -138,22 +147,28 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
   }
 
   // Item j of a thread: 16-byte piece (tid + 256 j') of its group's part of a K or
-  // V tile, the K pieces first.  Tiles past the last repeat its last 16 keys.
+  // V tile, the K pieces first; all lanes of a wave are in one layout tile, so that
+  // its block, scale and address are scalar.  Tiles past the last repeat its last
+  // 16 keys.
   constexpr int kHalf = kItems * kGroupThreads / 2;  // K pieces of a group's part
+  static_assert(kPerTile % kWave == 0, "a wave's pieces lie in one layout tile");
   struct Item {
     u32x4 codes;
     float scale;
   };
   Item item[kItems];
   int id[kItems];
-  const int32_t* table = p.block_tables + static_cast<int64_t>(seq) * p.max_blocks_per_seq;
+  const int wave0 = wave % 4 * kWave;  // tid of the wave's first lane
+  const ScalarPtr<int32_t> table = scalar(p.block_tables + static_cast<int64_t>(seq) * p.max_blocks_per_seq);
   // tiles of a group (kKeys2: its last may lie behind the keys; all of it is masked)
   const int all_tiles = (keys + kTileKeys - 1) / kTileKeys, tiles = kKeys ? (all_tiles + 1) / 2 : all_tiles;
   auto real = [&](int t) { return kKeys ? 2 * t + kgrp : t; };
   const int last16 = (max(keys, 1) - 1) / kTileTokens;
-  auto is_v = [&](int j) { return j * kGroupThreads + (kItems == 1 ? tid : 0) >= kHalf; };
-  auto piece = [&](int j) { return (j * kGroupThreads + tid) % kHalf; };  // of the group's part
-  auto part16 = [&](int j) { return rgrp * (4 / kGroups) + piece(j) / kPerTile; };  // 16-key tile of the key tile
+  auto is_v = [&](int j) { return j * kGroupThreads + (kItems == 1 ? wave0 : 0) >= kHalf; };
+  // first piece of the wave in the group's part; this lane's in its layout tile
+  auto wave_piece = [&](int j) { return (j * kGroupThreads + wave0) % kHalf; };
+  auto piece = [&](int j) { return wave_piece(j) % kPerTile + lane; };
+  auto part16 = [&](int j) { return rgrp * (4 / kGroups) + wave_piece(j) / kPerTile; };  // 16-key tile of the key tile
   auto layout_tile = [&](int j, int t) { return min(4 * real(t) + part16(j), last16); };
   // block of item j for conversion c (K of tile c + 1, V of tile c)
   auto entry = [&](int j, int c) { return table[layout_tile(j, is_v(j) ? c : c + 1) >> tsh]; };
@@ -162,13 +177,14 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
     const int b = static_cast<uint32_t>(id[j]) < static_cast<uint32_t>(p.kv.num_blocks) ? id[j] : 0;
     const uint32_t cell = static_cast<uint32_t>(b) * hkv + kvh;
     const uint32_t tile = (cell << tsh) + (t16 & tsh);
-    const uint8_t* base = static_cast<const uint8_t*>(is_v(j) ? p.kv.v : p.kv.k) + (piece(j) % kPerTile) * 16;
-    item[j].codes = load16(base + static_cast<uint64_t>(tile) * (kTileTokens * D));
-    item[j].scale = (is_v(j) ? p.kv.v_scale : p.kv.k_scale)[cell];
+    const uint8_t* base = static_cast<const uint8_t*>(is_v(j) ? p.kv.v : p.kv.k) +
+                          static_cast<uint64_t>(tile) * (kTileTokens * D) + wave_piece(j) % kPerTile * 16;
+    item[j].codes = reinterpret_cast<const u32x4*>(base)[lane];
+    item[j].scale = scalar(is_v(j) ? p.kv.v_scale : p.kv.k_scale)[cell];
   };
   const float cs = __builtin_fabsf(p.scale) * kLog2e;
   auto convert = [&](int j, int c) __attribute__((always_inline)) {
-    const int t16 = part16(j), pc = piece(j) % kPerTile;
+    const int t16 = part16(j), pc = piece(j);
     if (!is_v(j)) {
       const int buf = (c + 1) & 1, kp = pc / 16, key = 16 * t16 + pc % 16;
       const u32x4 w = item[j].codes;
@@ -194,7 +210,7 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
       if constexpr (kFp8) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) put(e, fp8_scaled_f16(w[e], item[j].scale));
-      } else if (__any(item[j].scale > 32.f)) {
+      } else if (item[j].scale > 32.f) {  // uniform
 #pragma unroll
         for (int e = 0; e < 4; ++e) put(e, int8_scaled_f16<false>(w[e], sc));
       } else {
