@@ -328,7 +328,7 @@ template <int D, int BS, bool kFp8, int kRows, int kHeads>
 __global__ __launch_bounds__(kWriteThreads) void write_kv_blocks_kernel(WriteArgs a) {
   __shared__ int pos[kWriteThreads / kWave][kWave];
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  if (static_cast<int>(blockIdx.x) < a.kv_groups) {
+  if (static_cast<int>(blockIdx.x) < a.kv_groups) {  // first: their chain of reads is the longer
     const int units = 2 * a.kv.num_kv_heads, w = blockIdx.x * (kWriteThreads / kWave) + wave;
     const int chunk = w / units;
     if (chunk >= (a.num_tokens + kRows - 1) / kRows) return;
@@ -366,7 +366,7 @@ int launch_write(WriteArgs a, hipStream_t stream) {
   const int rows = tune_knob(kBlkWrite, a.num_tokens > 1024 ? 16 : 4) == 4 ? 4 : 16;
   const int64_t waves = static_cast<int64_t>((a.num_tokens + rows - 1) / rows) * 2 * a.kv.num_kv_heads;
   const int64_t kvg = (waves + kWriteThreads / kWave - 1) / (kWriteThreads / kWave);
-  const int per = rows == 16 && a.hq % 4 == 0 ? 4 : 1;
+  const int per = rows == 16 && a.hq % 2 == 0 ? 2 : 1;
   const int64_t qg = (static_cast<int64_t>(a.num_tokens) * (a.hq / per) * (D / 16) + kWriteThreads - 1) / kWriteThreads;
   if (kvg + qg > 0x7fffffffll)
     return fail(RLK_EINVAL, "rope_and_write_kv_blocks: %d rows exceed one launch; split the call",
@@ -375,8 +375,8 @@ int launch_write(WriteArgs a, hipStream_t stream) {
   const uint32_t grid = static_cast<uint32_t>(kvg + qg);
   if (rows == 4) {
     write_kv_blocks_kernel<D, BS, kFp8, 4, 1><<<grid, kWriteThreads, 0, stream>>>(a);
-  } else if (per == 4) {
-    write_kv_blocks_kernel<D, BS, kFp8, 16, 4><<<grid, kWriteThreads, 0, stream>>>(a);
+  } else if (per == 2) {
+    write_kv_blocks_kernel<D, BS, kFp8, 16, 2><<<grid, kWriteThreads, 0, stream>>>(a);
   } else {
     write_kv_blocks_kernel<D, BS, kFp8, 16, 1><<<grid, kWriteThreads, 0, stream>>>(a);
   }
