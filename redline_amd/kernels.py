@@ -327,6 +327,21 @@ class KVCache:
 
 # ------------------------------------------------- block-scaled 8-bit KV cache
 
+def _one_device(dev, *tensors):
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise _lib.Error(_lib.RLK_EINVAL, f"tensors are on different devices (cuda:{dev} and {t.device})")
+
+
+def _launch_device(dev, stream):
+    """A launch goes to the current device: it must be the tensors' (and the stream's)."""
+    if torch.cuda.current_device() != dev:
+        raise _lib.Error(_lib.RLK_EINVAL, f"tensors are on cuda:{dev}, the current device is "
+                                          f"cuda:{torch.cuda.current_device()}")
+    if isinstance(stream, torch.cuda.Stream) and stream.device_index != dev:
+        raise _lib.Error(_lib.RLK_EINVAL, f"tensors are on cuda:{dev}, the stream on cuda:{stream.device_index}")
+
+
 class KVBlockFormat:
     kINT8 = _lib.RLK_KV_BLOCK_INT8
     kFP8 = _lib.RLK_KV_BLOCK_FP8  # e4m3, finite values only
@@ -344,9 +359,12 @@ def kv_block_view(k, v, k_scale, v_scale, block_size, num_kv_heads, head_dim, fm
     _need(v, nb * per, "v")
     for t, w in ((k_scale, "k_scale"), (v_scale, "v_scale")):
         _need(t, nb * num_kv_heads, w)
-    return KVBlockView(_ptr(k, dt, "k"), _ptr(v, dt, "v"), _ptr(k_scale, torch.float32, "k_scale"),
+    view = KVBlockView(_ptr(k, dt, "k"), _ptr(v, dt, "v"), _ptr(k_scale, torch.float32, "k_scale"),
                        _ptr(v_scale, torch.float32, "v_scale"), nb, block_size, num_kv_heads,
                        head_dim, fmt)
+    view.device = k.get_device()
+    _one_device(view.device, v, k_scale, v_scale)
+    return view
 
 
 class KVBlockCache:
@@ -383,6 +401,8 @@ def rope_and_write_kv_blocks(qkv, positions, slot_mapping, num_tokens, num_heads
         _need(positions, num_tokens, "positions"); _need(slot_mapping, num_tokens, "slot_mapping")
         cols = (num_heads + 2 * kv.num_kv_heads) * kv.head_dim
         _need(qkv, num_tokens * cols, "qkv"); _need(qkv_bias, cols, "qkv_bias")
+        _one_device(kv.device, qkv, positions, slot_mapping, cos_table, sin_table, qkv_bias)
+        _launch_device(kv.device, stream)
     check(lib().rlk_rope_and_write_kv_blocks(
         _ptr(qkv, torch.float16, "qkv"), _ptr(positions, torch.int32, "positions"),
         _ptr(slot_mapping, torch.int32, "slot_mapping"), num_tokens, num_heads,
@@ -397,6 +417,8 @@ def read_kv_blocks(kv: KVBlockView, slots, n, k_out=None, v_out=None, stream=Non
         _need(slots, n, "slots")
         for t, w in ((k_out, "k_out"), (v_out, "v_out")):
             _need(t, n * kv.num_kv_heads * kv.head_dim, w)
+        _one_device(kv.device, slots, k_out, v_out)
+        _launch_device(kv.device, stream)
     check(lib().rlk_read_kv_blocks(C.byref(kv), _ptr(slots, torch.int32, "slots"), n,
                                    _ptr(k_out, torch.float16, "k_out", True),
                                    _ptr(v_out, torch.float16, "v_out", True), _stream(stream)))
@@ -406,16 +428,20 @@ def block_attention_params(q, q_stride, out, num_heads, scale, kv: KVBlockView, 
                            max_blocks_per_seq, positions) -> _lib.BlockAttentionParams:
     """Parameters of the attention over a block-scaled cache (q may be a view
     into qkv)."""
-    return _lib.BlockAttentionParams(
+    params = _lib.BlockAttentionParams(
         _ptr(q, torch.float16, "q"), q_stride, _ptr(out, torch.float16, "out"), num_heads,
         float(scale), kv, _ptr(block_tables, torch.int32, "block_tables"), max_blocks_per_seq,
         _ptr(positions, torch.int32, "positions"))
+    params.device = kv.device
+    _one_device(kv.device, q, out, block_tables, positions)
+    return params
 
 
 def paged_attention_decode_blocks(params: _lib.BlockAttentionParams, work: _lib.DecodeAttentionWork,
                                   stream=None):
     """Extension: flash-decoding attention over a block-scaled cache; items with
     a negative token are skipped."""
+    _launch_device(params.device, stream)
     check(lib().rlk_paged_attention_decode_blocks(C.byref(params), C.byref(work), _stream(stream)))
 
 
@@ -423,6 +449,7 @@ def paged_attention_prefill_blocks(params: _lib.BlockAttentionParams, work: _lib
                                    stream=None):
     """Extension: causal prefill attention over a block-scaled cache; negative
     sequence ids are skipped."""
+    _launch_device(params.device, stream)
     check(lib().rlk_paged_attention_prefill_blocks(C.byref(params), C.byref(work), _stream(stream)))
 
 
@@ -440,6 +467,8 @@ class BlockPool:
         self.view = _lib.BlockPoolView(_ptr(ring, torch.int32, "ring"), ring.numel(),
                                        _ptr(state, torch.int32, "state"),
                                        _ptr(state_out, torch.int32, "state_out", True))
+        self.device = ring.get_device()
+        _one_device(self.device, state, state_out)
 
     @classmethod
     def of_blocks(cls, num_blocks, device="cuda"):
@@ -467,6 +496,8 @@ def batch_tables(pool: BlockPool, past_len, new_len, num_seqs, num_rows, block_s
         i(q_start, "q_start"), i(q_len, "q_len"), i(ctx_len, "ctx_len"), i(positions, "positions"),
         i(slot_mapping, "slot_mapping"), i(decode_token, "decode_token"),
         i(decode_seq, "decode_seq"), i(prefill_seq, "prefill_seq"), i(counts, "counts"))
+    _one_device(pool.device, past_len, new_len, block_tables, q_start, q_len, ctx_len, positions,
+                slot_mapping, decode_token, decode_seq, prefill_seq, counts)
     return pool, work
 
 
@@ -474,4 +505,5 @@ def build_batch_tables(tables, stream=None):
     """Extension: positions, slots, work lists and block tables of a step from
     its request lengths, with blocks from the pool; `tables` from batch_tables()."""
     pool, work = tables
+    _launch_device(pool.device, stream)
     check(lib().rlk_build_batch_tables(C.byref(pool.view), C.byref(work), _stream(stream)))

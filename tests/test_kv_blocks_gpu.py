@@ -240,3 +240,25 @@ def test_write_on_another_stream_and_in_a_graph(torch):
         torch.cuda.synchronize()
         for a, b, c in zip((x0, *t0), (x1, *t1), (x2, *t2)):
             assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_launches_refuse_another_device(torch):
+    """A launch goes to the current device: tensors of another are refused (the
+    views carry their device, which this test changes)."""
+    from redline_amd import kernels as K
+    cache = K.KVBlockCache(1, 4, 2, 64)
+    kv = cache.layer(0)
+    i = torch.zeros(4, dtype=torch.int32, device="cuda")
+    x = torch.zeros(4, 8 * 64, dtype=torch.float16, device="cuda")
+    p = K.block_attention_params(x, 512, x.clone(), 4, 0.1, kv, i, 1, i)
+    pool = K.BlockPool.of_blocks(4)
+    tb = K.batch_tables(pool, i, i, 1, 1, 16, 1, i, 1, *[torch.zeros(4, dtype=torch.int32, device="cuda") for _ in range(9)])
+    K.read_kv_blocks(kv, i, 4, x[:, :128].contiguous(), None)
+    kv.device, p.device, pool.device = 1, 1, 1
+    f = torch.zeros(16, 32, device="cuda")
+    for call in (lambda: K.read_kv_blocks(kv, i, 4, x, None), lambda: K.paged_attention_decode_blocks(p, K.decode_work(i, i, 1, 1)),
+                 lambda: K.paged_attention_prefill_blocks(p, K.prefill_work(i, i, i, i, 1, 1)),
+                 lambda: K.build_batch_tables(tb),
+                 lambda: K.rope_and_write_kv_blocks(x, i, i, 4, 4, f, f, kv)):
+        with pytest.raises(ra.Error, match="device"):
+            call()

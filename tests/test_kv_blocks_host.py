@@ -1,6 +1,8 @@
 """Refusals of the block-scaled cache's and the batch tables' entry points,
 before anything is launched (no GPU)."""
 import ctypes as C
+import subprocess
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -9,6 +11,7 @@ import redline_amd as ra
 from redline_amd import _lib
 from tests import _kv_blocks as B
 
+ROOT = Path(__file__).resolve().parents[1]
 D16 = 16  # a non-null, 16-byte aligned stand-in: nothing is launched
 EINVAL, EUNSUP = _lib.RLK_EINVAL, _lib.RLK_EUNSUPPORTED
 
@@ -143,6 +146,17 @@ def test_python_launchers_check_their_tensors():
         K.batch_tables(None, i, i, 2, 20, 16, 1, i, 4, i, i, i, i, i, i, i, i, i)
     with pytest.raises(ra.Error, match="bad KV cache"):
         K.KVBlockCache(1, 1, 2, 64)
+
+
+def test_cpp_header_wraps_the_entry_points(tmp_path):
+    """The C++ launchers compile, throw redline::Error on bad arguments and are
+    no-ops for empty calls."""
+    exe = tmp_path / "blocks"
+    subprocess.run(["/opt/rocm/bin/hipcc", "-std=c++17", f"-I{ROOT / 'include'}",
+                    str(ROOT / "tests" / "cpp" / "blocks_main.cpp"), "-o", str(exe), f"-L{ROOT / 'redline_amd'}",
+                    "-lrlk", f"-Wl,-rpath,{ROOT / 'redline_amd'}"], check=True, capture_output=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout
+    assert "PASS" in out, out
 
 
 def test_restated_layout_and_codes():
