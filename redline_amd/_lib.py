@@ -92,6 +92,7 @@ RLK_BATCH_TABLES_MAX_SEQS = 8192
 class KVBlockView(C.Structure):
     """Mirror of rlk_kv_block_view (block-scaled 8-bit cache, an extension)."""
 
+    device = None  # of the tensors, where kernels.kv_block_view made it
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p),
                 ("v_scale", C.c_void_p), ("num_blocks", C.c_int), ("block_size", C.c_int),
                 ("num_kv_heads", C.c_int), ("head_dim", C.c_int), ("format", C.c_int)]
@@ -100,6 +101,7 @@ class KVBlockView(C.Structure):
 class BlockAttentionParams(C.Structure):
     """Mirror of rlk_block_attention_params."""
 
+    device = None
     _fields_ = [("q", C.c_void_p), ("q_stride", C.c_int), ("out", C.c_void_p),
                 ("num_heads", C.c_int), ("scale", C.c_float), ("kv", KVBlockView),
                 ("block_tables", C.c_void_p), ("max_blocks_per_seq", C.c_int),

@@ -364,7 +364,7 @@ template <int D, int BS, bool kFp8>
 int launch_write(WriteArgs a, hipStream_t stream) {
   // RLK_TUNE_BLK_WRITE forces the rows of a wave (4 or 16; tests and tuning runs)
   const int rows = tune_knob(kBlkWrite, a.num_tokens > 1024 ? 16 : 4) == 4 ? 4 : 16;
-  const int64_t waves = static_cast<int64_t>((a.num_tokens + rows - 1) / rows) * 2 * a.kv.num_kv_heads;
+  const int64_t waves = (static_cast<int64_t>(a.num_tokens) + rows - 1) / rows * 2 * a.kv.num_kv_heads;
   const int64_t kvg = (waves + kWriteThreads / kWave - 1) / (kWriteThreads / kWave);
   const int per = rows == 16 && a.hq % 2 == 0 ? 2 : 1;
   const int64_t qg = (static_cast<int64_t>(a.num_tokens) * (a.hq / per) * (D / 16) + kWriteThreads - 1) / kWriteThreads;

@@ -328,6 +328,8 @@ class KVCache:
 # ------------------------------------------------- block-scaled 8-bit KV cache
 
 def _one_device(dev, *tensors):
+    if dev is None:  # a struct filled in by hand
+        return
     for t in tensors:
         if t is not None and t.get_device() != dev:
             raise _lib.Error(_lib.RLK_EINVAL, f"tensors are on different devices (cuda:{dev} and {t.device})")
@@ -335,6 +337,8 @@ def _one_device(dev, *tensors):
 
 def _launch_device(dev, stream):
     """A launch goes to the current device: it must be the tensors' (and the stream's)."""
+    if dev is None:
+        return
     if torch.cuda.current_device() != dev:
         raise _lib.Error(_lib.RLK_EINVAL, f"tensors are on cuda:{dev}, the current device is "
                                           f"cuda:{torch.cuda.current_device()}")
@@ -362,7 +366,7 @@ def kv_block_view(k, v, k_scale, v_scale, block_size, num_kv_heads, head_dim, fm
     view = KVBlockView(_ptr(k, dt, "k"), _ptr(v, dt, "v"), _ptr(k_scale, torch.float32, "k_scale"),
                        _ptr(v_scale, torch.float32, "v_scale"), nb, block_size, num_kv_heads,
                        head_dim, fmt)
-    view.device = k.get_device()
+    view.device, view.tensors = k.get_device(), (k, v, k_scale, v_scale)  # kept with their pointers
     _one_device(view.device, v, k_scale, v_scale)
     return view
 
@@ -432,7 +436,7 @@ def block_attention_params(q, q_stride, out, num_heads, scale, kv: KVBlockView, 
         _ptr(q, torch.float16, "q"), q_stride, _ptr(out, torch.float16, "out"), num_heads,
         float(scale), kv, _ptr(block_tables, torch.int32, "block_tables"), max_blocks_per_seq,
         _ptr(positions, torch.int32, "positions"))
-    params.device = kv.device
+    params.device, params.tensors = kv.device, (kv, q, out, block_tables, positions)
     _one_device(kv.device, q, out, block_tables, positions)
     return params
 
@@ -496,8 +500,9 @@ def batch_tables(pool: BlockPool, past_len, new_len, num_seqs, num_rows, block_s
         i(q_start, "q_start"), i(q_len, "q_len"), i(ctx_len, "ctx_len"), i(positions, "positions"),
         i(slot_mapping, "slot_mapping"), i(decode_token, "decode_token"),
         i(decode_seq, "decode_seq"), i(prefill_seq, "prefill_seq"), i(counts, "counts"))
-    _one_device(pool.device, past_len, new_len, block_tables, q_start, q_len, ctx_len, positions,
-                slot_mapping, decode_token, decode_seq, prefill_seq, counts)
+    work.tensors = (past_len, new_len, block_tables, q_start, q_len, ctx_len, positions, slot_mapping,
+                    decode_token, decode_seq, prefill_seq, counts)
+    _one_device(pool.device, *work.tensors)
     return pool, work
 
 
