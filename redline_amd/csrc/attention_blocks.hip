@@ -21,6 +21,11 @@
 // scale that the wave has met (a power of two, so the ratio is exact and the
 // fp16 operand keeps its 11 bits however small V is).  m, l and the output stay
 // in fp32.
+// Bound: HBM reads for full batches, which stream at 6.1 TB/s between a start of
+// about 4 us (lengths, table entries, scales: dependent reads) and the merge's 4-5:
+// 32 items to 8191 keys (INT8, 8 kv heads of 128, 257 MB) 52 us in all, 4.9 TB/s;
+// 12 items to 40000 (e4m3, 4 kv heads, 332 MB) 65 us, 5.1 TB/s.  Small calls by two
+// launches and those reads: one item of 2000 keys 5 + 3 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -495,8 +500,9 @@ void launch_g(DecodeArgs a, hipStream_t stream) {
   // Equal ranges pay where contexts are several ranges long and fill the chip;
   // they cost a longer start, and more where a range holds several short contexts.
   // us, grid / range (8 kv heads of 128, contexts from 0 to the named one): 8 items
-  // to 8191 20.0 / 19.6, 16 35.4 / 27.2, 32 66 / 48; 32 to 4000 32.9 / 26.5; 32 to
-  // 2000 22.9 / 23.8, 64 31.5 / 29.8; 128 to 1000 29.1 / 35.4; 256 to 500 27.6 / 44.7.
+  // to 8191 20.1 / 20.0, 16 35.5 / 27.7, 32 59 / 49; 32 to 4000 33.1 / 27.0; 32 to
+  // 2000 19.7 / 24.0, 64 31.6 / 30.5; 128 to 1000 29.7 / 36.2; 256 to 500 27.4 / 44.5
+  // (the merge's 5-7 us, which the grid form does without there, come on top).
   const bool range = mp >= 8 && units > static_cast<int64_t>(cus) * 8;
   if (tune_knob(kBlkDecode, range) != 0 && a.w.num_items <= kMaxItemsLds && mp > 1 &&
       units * (kPart / kStep) < (1 << 30)) {

@@ -14,8 +14,9 @@
 //   V: lane m holds dims E m .. E m + E - 1 of the 4 tokens of a quad, which
 //      are E/4 16-byte pieces, every byte of them: no data leaves its lane.
 //      A quad that the run fills in part is read, merged and written back.
-// Bound: HBM bytes for prefill, the launch and one chain of dependent reads
-// (slots -> positions -> cos/sin) for decode.  Numerics: the rotation as in
+// Bound: HBM bytes for prefill (16384 rows of 28 + 2 x 4 heads of 128 with a bias,
+// 294 MB: 55 us, 5.3 TB/s), the launch and one chain of dependent reads (slots ->
+// positions -> cos/sin) for decode (32 rows 4.2 us).  Numerics: the rotation as in
 // rope_kv.hip (fp32 without contraction, rounded to fp16), then kv_blocks.hpp.
 #include <hip/hip_runtime.h>
 
@@ -362,7 +363,11 @@ __global__ __launch_bounds__(kWriteThreads) void write_kv_blocks_kernel(WriteArg
 
 template <int D, int BS, bool kFp8>
 int launch_write(WriteArgs a, hipStream_t stream) {
-  // RLK_TUNE_BLK_WRITE forces the rows of a wave (4 or 16; tests and tuning runs)
+  // Rows of a wave: with 16 a prompt's blocks are found by fewer waves, with 4 single
+  // rows have more waves.  us, 4 / 16: 32 single rows 4.2 / 9.4, 512 7.7 / 14.8, 2048
+  // 20.3 / 21.9; a prompt of 512 5.3 / 5.5, 1024 8.4 / 6.8, 2048 14.2 / 9.6, 4 of 4096
+  // 76 / 56; 61 single rows beside 9 prompts, 4802 rows, D = 64, 16.5 / 14.3.
+  // RLK_TUNE_BLK_WRITE forces them (4 or 16; tests and tuning runs)
   const int rows = tune_knob(kBlkWrite, a.num_tokens > 1024 ? 16 : 4) == 4 ? 4 : 16;
   const int64_t waves = (static_cast<int64_t>(a.num_tokens) + rows - 1) / rows * 2 * a.kv.num_kv_heads;
   const int64_t kvg = (waves + kWriteThreads / kWave - 1) / (kWriteThreads / kWave);
@@ -406,6 +411,8 @@ __device__ __forceinline__ u32x2 scaled4(f32x4 v, float s) {
 // 16 lanes take 4 rows of the list for one head's K or V.  Where the 4 rows are a
 // quad of the layout (lists of consecutive slots), each V piece is read once and
 // gives 4 rows; other rows take theirs alone, a byte in four of what they read.
+// Bound: HBM bytes for runs (16384 rows of 4 heads of 128, 50 MB: 12.5 us, 4 TB/s),
+// the pieces' whole lines for single rows (2048 of 8 heads: 30 us), the launch below.
 template <int D, bool kFp8>
 __global__ __launch_bounds__(256) void read_kv_blocks_kernel(ReadArgs a) {
   constexpr int E = D / 16, kLanes = D / 16, kTok = 16 / kLanes;

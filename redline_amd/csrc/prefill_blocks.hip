@@ -24,6 +24,11 @@
 //       kOne     one group, whose CU holds two workgroups: between the two.
 // m, l and the output accumulate in fp32; P is rounded to fp16 (at most 2^8), and
 // l sums the rounded values, so that numerator and denominator agree.
+// Bound: long prompts by X and Y in turn at the clock that the chip holds under them
+// (about 1.8 GHz of 2.4): 4 x 4096 tokens at depths to 4096, 32 / 8 heads of 128, take
+// 1380 us INT8 and 1350 e4m3, 967 TFLOP/s or 80% of a large library product; 4 x 4096 at
+// D = 64 712 us.  Short ones by the longest workgroup's chain of tiles: 2 chunks of
+// 512 tokens at depths 0 and 1585 45 us, 24 ragged prompts at D = 64 93 us (558 TFLOP/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -431,10 +436,10 @@ hipError_t launch(const PrefillArgs& a, int64_t rows, hipStream_t stream) {
   // Workgroups of 128 rows (of the grid: ragged prompts leave some of them empty).
   // Up to two per CU, splitting the keys beats more rows; past that, at D = 128,
   // 256 rows to an image beat 128, at D = 64 (three workgroups a CU) they do not.
-  // us, kOne / kRows2 / kKeys2: 2 chunks of 512, 8 kv heads of 128, e4m3 60 / 76 / 52;
-  // of 1024 92 / 97 / 81; of 2048 192 / 174 / 209; 4 x 4096 INT8 1600 / 1463 / 1828;
-  // D = 64: 2 chunks of 512 39 / - / 35, 24 ragged prompts 117 / 130 / 176, 4 x 4096
-  // 956 / 958 / 1128.  RLK_TUNE_BLK_PREFILL forces a split (tests and tuning runs).
+  // us, kOne / kRows2 / kKeys2: 2 chunks of 512, 8 kv heads of 128, e4m3 57 / 68 / 49;
+  // of 1024 86 / 88 / 74; of 2048 177 / 166 / 196; 4 x 4096 INT8 1519 / 1393 / 1785;
+  // D = 64: 2 chunks of 512 43 / 48 / 36, 24 ragged prompts 113 / 133 / 165, 4 x 4096
+  // 712 / 742 / 954.  RLK_TUNE_BLK_PREFILL forces a split (tests and tuning runs).
   const int64_t groups = (rows + 127) / 128 * a.p.kv.num_kv_heads * a.w.num_seqs;
   const Split rule = groups <= 2 * compute_units() ? kKeys2 : (D == 64 ? kOne : kRows2);
   switch (tune_knob(kBlkPrefill, rule)) {
