@@ -67,26 +67,13 @@ __device__ __forceinline__ ScalarPtr<T> scalar(const T* p) {
 
 // Four codes as fp16, exactly: e4m3 times the scale (the conversion takes it),
 // INT8 V times the scale, INT8 K as it is (its scale multiplies the scores).
-// INT8 comes as 1152 + code (codes_to_f16); times s, minus 1152 s, is one exact
-// fma while 1152 s is an fp16 number (`fused`, s <= 32).
 __device__ __forceinline__ u32x2 fp8_scaled_f16(uint32_t w, float s) {
   const f16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, false);
   const f16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, true);
   return u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
 }
-template <bool kFused>
 __device__ __forceinline__ u32x2 int8_scaled_f16(uint32_t w, _Float16 s) {
-  if constexpr (!kFused) {
-    return __builtin_bit_cast(u32x2, codes_to_f16<false>(w) * s);
-  } else {
-    const uint32_t u = w ^ 0x80808080u;
-    const f16x2 s2 = {s, s}, c = f16x2{static_cast<_Float16>(-1152), static_cast<_Float16>(-1152)} * s2;
-    const f16x2 lo = __builtin_elementwise_fma(
-        __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)), s2, c);
-    const f16x2 hi = __builtin_elementwise_fma(
-        __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)), s2, c);
-    return u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
-  }
+  return __builtin_bit_cast(u32x2, codes_to_f16<false>(w) * s);
 }
 
 // Two images of K and of V, used in turn, and the score scale of each 16-key tile
@@ -155,6 +142,7 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
   // V tile, the K pieces first; all lanes of a wave are in one layout tile, so that
   // its block, scale and address are scalar.  Tiles past the last repeat its last
   // 16 keys.
+  static_assert(kItems % 2 == 0, "an item is K or V for the whole group");
   constexpr int kHalf = kItems * kGroupThreads / 2;  // K pieces of a group's part
   static_assert(kPerTile % kWave == 0, "a wave's pieces lie in one layout tile");
   struct Item {
@@ -169,7 +157,7 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
   const int all_tiles = (keys + kTileKeys - 1) / kTileKeys, tiles = kKeys ? (all_tiles + 1) / 2 : all_tiles;
   auto real = [&](int t) { return kKeys ? 2 * t + kgrp : t; };
   const int last16 = (max(keys, 1) - 1) / kTileTokens;
-  auto is_v = [&](int j) { return j * kGroupThreads + (kItems == 1 ? wave0 : 0) >= kHalf; };
+  auto is_v = [&](int j) { return j >= kItems / 2; };
   // first piece of the wave in the group's part; this lane's in its layout tile
   auto wave_piece = [&](int j) { return (j * kGroupThreads + wave0) % kHalf; };
   auto piece = [&](int j) { return wave_piece(j) % kPerTile + lane; };
@@ -177,62 +165,58 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
   auto layout_tile = [&](int j, int t) { return min(4 * real(t) + part16(j), last16); };
   // block of item j for conversion c (K of tile c + 1, V of tile c)
   auto entry = [&](int j, int c) { return table[layout_tile(j, is_v(j) ? c : c + 1) >> tsh]; };
-  auto request = [&](int j, int c) __attribute__((always_inline)) {
-    const int t16 = layout_tile(j, is_v(j) ? c : c + 1);
+  // cell (block, head) of item j for conversion c, from its block id[j]; its codes
+  auto cell_of = [&](int j) __attribute__((always_inline)) {
     const int b = static_cast<uint32_t>(id[j]) < static_cast<uint32_t>(p.kv.num_blocks) ? id[j] : 0;
-    const uint32_t cell = static_cast<uint32_t>(b) * hkv + kvh;
-    const uint32_t tile = (cell << tsh) + (t16 & tsh);
+    return static_cast<uint32_t>(b) * hkv + kvh;
+  };
+  auto fetch = [&](int j, int c, uint32_t cell) __attribute__((always_inline)) {
+    const uint32_t tile = (cell << tsh) + (layout_tile(j, is_v(j) ? c : c + 1) & tsh);
     const uint8_t* base = static_cast<const uint8_t*>(is_v(j) ? p.kv.v : p.kv.k) +
                           static_cast<uint64_t>(tile) * (kTileTokens * D) + wave_piece(j) % kPerTile * 16;
     item[j].codes = reinterpret_cast<const u32x4*>(base)[lane];
-    item[j].scale = scalar(is_v(j) ? p.kv.v_scale : p.kv.k_scale)[cell];
   };
+  auto scale_of = [&](int j, uint32_t cell) { return scalar(is_v(j) ? p.kv.v_scale : p.kv.k_scale)[cell]; };
   const float cs = __builtin_fabsf(p.scale) * kLog2e;
-  auto convert = [&](int j, int c) __attribute__((always_inline)) {
-    const int t16 = part16(j), pc = piece(j);
+  // Conversion c of item j: the codes as fp16, and their way to the image.  `last`:
+  // tile c is the last, whose bytes past the keys may be anything.
+  struct Halves {
+    u32x2 x[4];
+  };
+  auto convert = [&](int j, int c, bool last) __attribute__((always_inline)) {
+    Halves h;
+    u32x4 w = item[j].codes;
     if (!is_v(j)) {
-      const int buf = (c + 1) & 1, kp = pc / 16, key = 16 * t16 + pc % 16;
-      const u32x4 w = item[j].codes;
-      u32x2 x[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        x[e] = kFp8 ? fp8_scaled_f16(w[e], item[j].scale) : __builtin_bit_cast(u32x2, codes_to_f16<kFp8>(w[e]));
-      lds.k[buf][kp][0][key] = u32x4{x[0][0], x[0][1], x[1][0], x[1][1]};
-      lds.k[buf][kp][1][key] = u32x4{x[2][0], x[2][1], x[3][0], x[3][1]};
-      if (!kFp8 && pc == 0) reinterpret_cast<float*>(&lds.ks[(c + 1) & 3])[t16] = item[j].scale * cs;
+        h.x[e] = kFp8 ? fp8_scaled_f16(w[e], item[j].scale) : __builtin_bit_cast(u32x2, codes_to_f16<kFp8>(w[e]));
     } else {
-      const int g = pc / 64, rho = pc / 16 % 4, m = pc % 16;
-      u32x4 w = item[j].codes;
-      if ((real(c) + 1) * kTileKeys > keys) {  // uniform: bytes past the keys may be anything
-        const int keep = min(max(keys - real(c) * kTileKeys - 16 * t16 - 4 * rho, 0), 4);
+      if (last) {
+        const int keep = min(max(keys - real(c) * kTileKeys - 16 * part16(j) - 4 * (piece(j) / 16 % 4), 0), 4);
         const uint32_t mask = keep == 0 ? 0u : 0xffffffffu >> (32 - 8 * keep);
         w &= u32x4{mask, mask, mask, mask};
       }
-      auto put = [&](int e, u32x2 x) {
-        reinterpret_cast<u32x2*>(&lds.v[c & 1][t16][rho % 2][(4 * g + e) * 16 + m])[rho / 2] = x;
-      };
-      const _Float16 sc = static_cast<_Float16>(item[j].scale);
-      if constexpr (kFp8) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) put(e, fp8_scaled_f16(w[e], item[j].scale));
-      } else if (item[j].scale > 32.f) {  // uniform
-#pragma unroll
-        for (int e = 0; e < 4; ++e) put(e, int8_scaled_f16<false>(w[e], sc));
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) put(e, int8_scaled_f16<true>(w[e], sc));
-      }
+      for (int e = 0; e < 4; ++e)
+        h.x[e] = kFp8 ? fp8_scaled_f16(w[e], item[j].scale)
+                      : int8_scaled_f16(w[e], static_cast<_Float16>(item[j].scale));
     }
+    return h;
   };
-  // conversion c of this thread's pieces, and the request of conversion c + 1's
-  auto conversion = [&](int c) __attribute__((always_inline)) {
+  auto store = [&](int j, int c, const Halves& h) __attribute__((always_inline)) {
+    const int t16 = part16(j), pc = piece(j);
+    if (!is_v(j)) {
+      const int buf = (c + 1) & 1, kp = pc / 16, key = 16 * t16 + pc % 16;
+      lds.k[buf][kp][0][key] = u32x4{h.x[0][0], h.x[0][1], h.x[1][0], h.x[1][1]};
+      lds.k[buf][kp][1][key] = u32x4{h.x[2][0], h.x[2][1], h.x[3][0], h.x[3][1]};
+      // (the same word and value from each lane)
+      if (!kFp8) reinterpret_cast<float*>(&lds.ks[(c + 1) & 3])[t16] = item[j].scale * cs;
+    } else {
+      const int g = pc / 64, rho = pc / 16 % 4, m = pc % 16;
 #pragma unroll
-    for (int j = 0; j < kItems; ++j) {
-      convert(j, c);
-      request(j, c + 1);
+      for (int e = 0; e < 4; ++e)
+        reinterpret_cast<u32x2*>(&lds.v[c & 1][t16][rho % 2][(4 * g + e) * 16 + m])[rho / 2] = h.x[e];
     }
-#pragma unroll
-    for (int j = 0; j < kItems; ++j) id[j] = entry(j, c + 2);
   };
 
   f32x16 o[D / 32], s[2];
@@ -246,10 +230,34 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
 
   // Operands come from LDS kAhead fragments before their product; the schedule is
   // pinned, because the compiler by itself waits for each pair of reads.
-  auto phase_x = [&](int t, auto pv, auto qk) __attribute__((always_inline)) {
+  // Beside the products go conversion t (kLast: of V alone; there is no further tile)
+  // and the request of conversion t + 1's codes.
+  uint32_t cell[kItems];
+  auto do_convert = [&](int t, auto on, auto last) __attribute__((always_inline)) {
+    if constexpr (decltype(on)::value) {
+      constexpr bool kLast = decltype(last)::value;
+      Halves h[kItems];
+#pragma unroll
+      for (int j = kLast ? kItems / 2 : 0; j < kItems; ++j) {
+        h[j] = convert(j, t, kLast);
+        if (!kLast) {
+          cell[j] = cell_of(j);
+          fetch(j, t + 1, cell[j]);
+        }
+      }
+#pragma unroll
+      for (int j = kLast ? kItems / 2 : 0; j < kItems; ++j) store(j, t, h[j]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto phase_x = [&](int t, auto pv, auto qk, auto last) __attribute__((always_inline)) {
+    constexpr auto yes_convert = qk;
     constexpr int kPv = decltype(pv)::value ? 4 * (D / 32) : 0, kQk = decltype(qk)::value ? 2 * E : 0;
     constexpr int kAll = kPv + kQk, kAhead = kAll < 8 ? kAll : 8;
     __builtin_amdgcn_sched_barrier(0);
+#ifdef BEFORE
+    do_convert(t, yes_convert, last);
+#endif
     const u32x4* vp = &lds.v[(t + 1) & 1][0][half][col];  // V of tile t - 1
     const u32x4* kp = &lds.k[t & 1][0][half][col];
     auto fragment = [&](int i) {
@@ -284,6 +292,9 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
     }
     __builtin_amdgcn_sched_group_barrier(0x8, kAhead, 0);
     __builtin_amdgcn_sched_barrier(0);
+#ifndef BEFORE
+    do_convert(t, yes_convert, last);
+#endif
   };
   auto softmax = [&](int t) __attribute__((always_inline)) {
     // element i of half kh: key 64 real(t) + 32 kh + 8 (i / 4) + 4 half + i % 4
@@ -304,9 +315,9 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
     mx = -FLT_MAX;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      float y = s[x / 2][8 * (x % 2)];
+      float y = -FLT_MAX;
 #pragma unroll
-      for (int i = 1; i < 8; ++i) y = fmaxf(y, s[x / 2][8 * (x % 2) + i]);
+      for (int i = 0; i < 8; ++i) y = fmaxf(y, s[x / 2][8 * (x % 2) + i]);
       mx = fmaxf(mx, y * c4[x]);
     }
     mx = rows_max<true>(mx);
@@ -319,6 +330,14 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
       for (int d = 0; d < D / 32; ++d) o[d] *= f;
       m = mn;
     }
+    // scalar loads for the next tiles, waited for at the end of the phase
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) {
+      item[j].scale = scale_of(j, cell[j]);
+      id[j] = entry(j, t + 2);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    float ls[4] = {l, 0.f, 0.f, 0.f};
     const f16x2 ones = {static_cast<_Float16>(1), static_cast<_Float16>(1)};
 #pragma unroll
     for (int x = 0; x < 4; ++x)
@@ -329,48 +348,61 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
         const f16x2 e = {static_cast<_Float16>(e0), static_cast<_Float16>(e1)};
         pb[x][i] = e[0];
         pb[x][i + 1] = e[1];
-        l = __builtin_amdgcn_fdot2(e, ones, l, false);
+        ls[x] = __builtin_amdgcn_fdot2(e, ones, ls[x], false);
       }
+    l = (ls[0] + ls[1]) + (ls[2] + ls[3]);
   };
 
   if (tiles > 0) {
     // conversion -1 has K(0) only: there is no V tile -1
+    Halves h[kItems];
 #pragma unroll
-    for (int j = 0; j < kItems; ++j)
-      if (!is_v(j)) id[j] = entry(j, -1);
+    for (int j = 0; j < kItems / 2; ++j) id[j] = entry(j, -1);
 #pragma unroll
-    for (int j = 0; j < kItems; ++j)
-      if (!is_v(j)) request(j, -1);
+    for (int j = 0; j < kItems / 2; ++j) {
+      cell[j] = cell_of(j);
+      fetch(j, -1, cell[j]);
+      item[j].scale = scale_of(j, cell[j]);
+    }
 #pragma unroll
     for (int j = 0; j < kItems; ++j) id[j] = entry(j, 0);
 #pragma unroll
-    for (int j = 0; j < kItems; ++j)
-      if (!is_v(j)) convert(j, -1);  // K(0)
+    for (int j = 0; j < kItems / 2; ++j) {
+      h[j] = convert(j, -1, false);
+      store(j, -1, h[j]);
+    }
 #pragma unroll
-    for (int j = 0; j < kItems; ++j) request(j, 0);
+    for (int j = 0; j < kItems; ++j) {
+      cell[j] = cell_of(j);
+      fetch(j, 0, cell[j]);
+      item[j].scale = scale_of(j, cell[j]);
+    }
 #pragma unroll
     for (int j = 0; j < kItems; ++j) id[j] = entry(j, 1);
   }
   __syncthreads();
-  if (grp == 1) {  // one phase behind, kRows2: and one conversion ahead of group 0
-    if (kGroups == 2 && tiles > 0) conversion(0);
-    __syncthreads();
-  }
+  if (grp == 1) __syncthreads();  // one phase behind
   auto phase_y = [&](int t) __attribute__((always_inline)) {
     __syncthreads();
     softmax(t);
-    conversion(t + rgrp);
     __syncthreads();
   };
-  if (tiles > 0) {
-    phase_x(0, std::false_type{}, std::true_type{});
+  const std::true_type yes;
+  const std::false_type no;
+  if (tiles == 1) {
+    phase_x(0, no, yes, yes);
     phase_y(0);
-    for (int t = 1; t < tiles; ++t) {
-      phase_x(t, std::true_type{}, std::true_type{});
+  } else if (tiles > 1) {
+    phase_x(0, no, yes, no);
+    phase_y(0);
+    for (int t = 1; t < tiles - 1; ++t) {
+      phase_x(t, yes, yes, no);
       phase_y(t);
     }
-    phase_x(tiles, std::true_type{}, std::false_type{});
+    phase_x(tiles - 1, yes, yes, yes);
+    phase_y(tiles - 1);
   }
+  if (tiles > 0) phase_x(tiles, yes, no, no);
   if (kSplit != kOne && grp == 0) __syncthreads();  // as many barriers as group 1
   l = rows_sum<true>(l);
   if constexpr (kKeys) {  // group 1's partial joins group 0's through LDS
@@ -444,8 +476,10 @@ hipError_t launch(const PrefillArgs& a, int64_t rows, hipStream_t stream) {
   const Split rule = groups <= 2 * compute_units() ? kKeys2 : (D == 64 ? kOne : kRows2);
   switch (tune_knob(kBlkPrefill, rule)) {
     case kKeys2: return launch_s<D, kFp8, kKeys2>(a, rows, stream);
-    case kOne: return launch_s<D, kFp8, kOne>(a, rows, stream);
-    default: return launch_s<D, kFp8, kRows2>(a, rows, stream);
+    case kRows2:
+      if constexpr (D == 128) return launch_s<D, kFp8, kRows2>(a, rows, stream);
+      [[fallthrough]];
+    default: return launch_s<D, kFp8, kOne>(a, rows, stream);
   }
 }
 
