@@ -89,8 +89,8 @@ enum Split { kOne, kRows2, kKeys2 };
 
 // Phases, with t the key tile (kKeys2: the group's t-th) and S its scores; group 1
 // is one phase behind.  kRows2:
-//   group 0   X(t) at 2t      Y(t) at 2t + 1, converts its half of K(t + 1), V(t)
-//   group 1   X(t) at 2t + 1  Y(t) at 2t + 2, converts its half of K(t + 2), V(t + 1)
+//   group 0   X(t) at 2t, converts its half of K(t + 1)      Y(t) at 2t + 1, of V(t)
+//   group 1   X(t) at 2t + 1, converts its half of K(t + 1)  Y(t) at 2t + 2, of V(t + 1)
 // X(t) reads K(t) and V(t - 1).  So K(t) is written in the phases 2t - 2 and
 // 2t - 1 and read in 2t and 2t + 1, V(t) is written in 2t and 2t + 1 and read in
 // 2t + 2 and 2t + 3, and neither meets the image of tile t - 2 in the same buffer.
@@ -99,6 +99,8 @@ template <int D, bool kFp8, Split kSplit>
 __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void prefill_blocks_kernel(PrefillArgs a) {
   constexpr int kGroups = kSplit == kRows2 ? 2 : 1;  // that share a tile's image
   constexpr bool kKeys = kSplit == kKeys2;
+  // where V is converted: beside K in X, or (two groups at D = 128) in Y, for phases of one length
+  constexpr bool kVInX = D == 64 || kSplit == kOne;
   constexpr int E = D / 16, kRows = 4 * kWaveRows * kGroups;
   constexpr int kPerTile = D;                                  // 16-byte pieces of a layout tile
   constexpr int kItems = 2 * 4 * kPerTile / kGroups / kGroupThreads;  // K and V pieces of a thread and tile
@@ -178,12 +180,11 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
   };
   auto scale_of = [&](int j, uint32_t cell) { return scalar(is_v(j) ? p.kv.v_scale : p.kv.k_scale)[cell]; };
   const float cs = __builtin_fabsf(p.scale) * kLog2e;
-  // Conversion c of item j: the codes as fp16, and their way to the image.  `last`:
-  // tile c is the last, whose bytes past the keys may be anything.
+  // Conversion c of item j: the codes as fp16, and their way to the image.
   struct Halves {
     u32x2 x[4];
   };
-  auto convert = [&](int j, int c, bool last) __attribute__((always_inline)) {
+  auto convert = [&](int j, int c) __attribute__((always_inline)) {
     Halves h;
     u32x4 w = item[j].codes;
     if (!is_v(j)) {
@@ -191,7 +192,7 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
       for (int e = 0; e < 4; ++e)
         h.x[e] = kFp8 ? fp8_scaled_f16(w[e], item[j].scale) : __builtin_bit_cast(u32x2, codes_to_f16<kFp8>(w[e]));
     } else {
-      if (last) {
+      if ((real(c) + 1) * kTileKeys > keys) {  // uniform: bytes past the keys may be anything
         const int keep = min(max(keys - real(c) * kTileKeys - 16 * part16(j) - 4 * (piece(j) / 16 % 4), 0), 4);
         const uint32_t mask = keep == 0 ? 0u : 0xffffffffu >> (32 - 8 * keep);
         w &= u32x4{mask, mask, mask, mask};
@@ -230,34 +231,37 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
 
   // Operands come from LDS kAhead fragments before their product; the schedule is
   // pinned, because the compiler by itself waits for each pair of reads.
-  // Beside the products go conversion t (kLast: of V alone; there is no further tile)
-  // and the request of conversion t + 1's codes.
+  // After the products come K's part of conversion t, the request of the next codes, and
+  // the cells of the next scales.
   uint32_t cell[kItems];
-  auto do_convert = [&](int t, auto on, auto last) __attribute__((always_inline)) {
-    if constexpr (decltype(on)::value) {
-      constexpr bool kLast = decltype(last)::value;
-      Halves h[kItems];
+  auto convert_x = [&](int t) __attribute__((always_inline)) {
+    constexpr int kEnd = kVInX ? kItems : kItems / 2;
+    Halves h[kEnd];
 #pragma unroll
-      for (int j = kLast ? kItems / 2 : 0; j < kItems; ++j) {
-        h[j] = convert(j, t, kLast);
-        if (!kLast) {
-          cell[j] = cell_of(j);
-          fetch(j, t + 1, cell[j]);
-        }
-      }
-#pragma unroll
-      for (int j = kLast ? kItems / 2 : 0; j < kItems; ++j) store(j, t, h[j]);
+    for (int j = 0; j < kEnd; ++j) {
+      h[j] = convert(j, t);
+      cell[j] = cell_of(j);
+      fetch(j, t + 1, cell[j]);
     }
+#pragma unroll
+    for (int j = 0; j < kEnd; ++j) store(j, t, h[j]);
+#pragma unroll
+    for (int j = kEnd; j < kItems; ++j) cell[j] = cell_of(j);
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto phase_x = [&](int t, auto pv, auto qk, auto last) __attribute__((always_inline)) {
-    constexpr auto yes_convert = qk;
+  // V's part of conversion c
+  auto convert_v = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = kItems / 2; j < kItems; ++j) {
+      const Halves h = convert(j, c);
+      fetch(j, c + 1, cell[j]);
+      store(j, c, h);
+    }
+  };
+  auto phase_x = [&](int t, auto pv, auto qk) __attribute__((always_inline)) {
     constexpr int kPv = decltype(pv)::value ? 4 * (D / 32) : 0, kQk = decltype(qk)::value ? 2 * E : 0;
     constexpr int kAll = kPv + kQk, kAhead = kAll < 8 ? kAll : 8;
     __builtin_amdgcn_sched_barrier(0);
-#ifdef BEFORE
-    do_convert(t, yes_convert, last);
-#endif
     const u32x4* vp = &lds.v[(t + 1) & 1][0][half][col];  // V of tile t - 1
     const u32x4* kp = &lds.k[t & 1][0][half][col];
     auto fragment = [&](int i) {
@@ -292,9 +296,7 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
     }
     __builtin_amdgcn_sched_group_barrier(0x8, kAhead, 0);
     __builtin_amdgcn_sched_barrier(0);
-#ifndef BEFORE
-    do_convert(t, yes_convert, last);
-#endif
+    if constexpr (kQk > 0) convert_x(t);
   };
   auto softmax = [&](int t) __attribute__((always_inline)) {
     // element i of half kh: key 64 real(t) + 32 kh + 8 (i / 4) + 4 half + i % 4
@@ -330,13 +332,17 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
       for (int d = 0; d < D / 32; ++d) o[d] *= f;
       m = mn;
     }
-    // scalar loads for the next tiles, waited for at the end of the phase
+    // scalar loads for the next conversions, waited for at the end of the phase
+    float next_scale[kItems];
 #pragma unroll
     for (int j = 0; j < kItems; ++j) {
-      item[j].scale = scale_of(j, cell[j]);
-      id[j] = entry(j, t + 2);
+      next_scale[j] = scale_of(j, cell[j]);
+      id[j] = entry(j, (is_v(j) ? t + rgrp : t) + 2);
     }
     __builtin_amdgcn_sched_barrier(0);
+    if (!kVInX) convert_v(t + rgrp);
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) item[j].scale = next_scale[j];
     float ls[4] = {l, 0.f, 0.f, 0.f};
     const f16x2 ones = {static_cast<_Float16>(1), static_cast<_Float16>(1)};
 #pragma unroll
@@ -355,30 +361,22 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
 
   if (tiles > 0) {
     // conversion -1 has K(0) only: there is no V tile -1
-    Halves h[kItems];
-#pragma unroll
-    for (int j = 0; j < kItems / 2; ++j) id[j] = entry(j, -1);
-#pragma unroll
-    for (int j = 0; j < kItems / 2; ++j) {
+    auto read = [&](int j, int c) __attribute__((always_inline)) {
+      id[j] = entry(j, c);
       cell[j] = cell_of(j);
-      fetch(j, -1, cell[j]);
+      fetch(j, c, cell[j]);
       item[j].scale = scale_of(j, cell[j]);
-    }
+    };
 #pragma unroll
-    for (int j = 0; j < kItems; ++j) id[j] = entry(j, 0);
+    for (int j = 0; j < kItems; ++j)
+      if (!is_v(j) || rgrp == 1) read(j, is_v(j) ? 0 : -1);
 #pragma unroll
-    for (int j = 0; j < kItems / 2; ++j) {
-      h[j] = convert(j, -1, false);
-      store(j, -1, h[j]);
-    }
+    for (int j = 0; j < kItems; ++j)
+      if (!is_v(j) || rgrp == 1) store(j, is_v(j) ? 0 : -1, convert(j, is_v(j) ? 0 : -1));
 #pragma unroll
-    for (int j = 0; j < kItems; ++j) {
-      cell[j] = cell_of(j);
-      fetch(j, 0, cell[j]);
-      item[j].scale = scale_of(j, cell[j]);
-    }
+    for (int j = 0; j < kItems; ++j) read(j, is_v(j) ? rgrp : 0);
 #pragma unroll
-    for (int j = 0; j < kItems; ++j) id[j] = entry(j, 1);
+    for (int j = 0; j < kItems; ++j) id[j] = entry(j, (is_v(j) ? rgrp : 0) + 1);
   }
   __syncthreads();
   if (grp == 1) __syncthreads();  // one phase behind
@@ -387,22 +385,15 @@ __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void p
     softmax(t);
     __syncthreads();
   };
-  const std::true_type yes;
-  const std::false_type no;
-  if (tiles == 1) {
-    phase_x(0, no, yes, yes);
+  if (tiles > 0) {
+    phase_x(0, std::false_type{}, std::true_type{});
     phase_y(0);
-  } else if (tiles > 1) {
-    phase_x(0, no, yes, no);
-    phase_y(0);
-    for (int t = 1; t < tiles - 1; ++t) {
-      phase_x(t, yes, yes, no);
+    for (int t = 1; t < tiles; ++t) {
+      phase_x(t, std::true_type{}, std::true_type{});
       phase_y(t);
     }
-    phase_x(tiles - 1, yes, yes, yes);
-    phase_y(tiles - 1);
+    phase_x(tiles, std::true_type{}, std::false_type{});
   }
-  if (tiles > 0) phase_x(tiles, yes, no, no);
   if (kSplit != kOne && grp == 0) __syncthreads();  // as many barriers as group 1
   l = rows_sum<true>(l);
   if constexpr (kKeys) {  // group 1's partial joins group 0's through LDS
