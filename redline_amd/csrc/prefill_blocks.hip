@@ -26,9 +26,9 @@
 // l sums the rounded values, so that numerator and denominator agree.
 // Bound: long prompts by X and Y in turn at the clock that the chip holds under them
 // (about 1.8 GHz of 2.4): 4 x 4096 tokens at depths to 4096, 32 / 8 heads of 128, take
-// 1380 us INT8 and 1350 e4m3, 967 TFLOP/s or 80% of a large library product; 4 x 4096 at
-// D = 64 712 us.  Short ones by the longest workgroup's chain of tiles: 2 chunks of
-// 512 tokens at depths 0 and 1585 45 us, 24 ragged prompts at D = 64 93 us (558 TFLOP/s).
+// 1298 us INT8 and 1277 e4m3, 1.03 PFLOP/s or 85% of a large library product; 4 x 4096 at
+// D = 64 699 us.  Short ones by the longest workgroup's chain of tiles: 2 chunks of
+// 512 tokens at depths 0 and 1585 41 us, 24 ragged prompts at D = 64 92 us (560 TFLOP/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -458,11 +458,13 @@ template <int D, bool kFp8>
 hipError_t launch(const PrefillArgs& a, int64_t rows, hipStream_t stream) {
   // Workgroups of 128 rows (of the grid: ragged prompts leave some of them empty).
   // Up to two per CU, splitting the keys beats more rows; past that, at D = 128,
-  // 256 rows to an image beat 128, at D = 64 (three workgroups a CU) they do not.
-  // us, kOne / kRows2 / kKeys2: 2 chunks of 512, 8 kv heads of 128, e4m3 57 / 68 / 49;
-  // of 1024 86 / 88 / 74; of 2048 177 / 166 / 196; 4 x 4096 INT8 1519 / 1393 / 1785;
-  // D = 64: 2 chunks of 512 43 / 48 / 36, 24 ragged prompts 113 / 133 / 165, 4 x 4096
-  // 712 / 742 / 954.  RLK_TUNE_BLK_PREFILL forces a split (tests and tuning runs).
+  // 256 rows to an image beat 128, at D = 64 they would not (nor is it built).
+  // us, kOne / kRows2 / kKeys2: 2 chunks of 512, 8 kv heads of 128, e4m3 60 / 61 / 45;
+  // of 1024 87 / 80 / 69; of 2048 174 / 157 / 188; 4 x 4096 INT8 1525 / 1319 / 1547;
+  // D = 64, kOne / kKeys2: 2 chunks of 512 44 / 31, 24 ragged prompts 111 / 154, 4 x 4096
+  // 699 / 815.  (Between one and two per CU it depends on what the host does not know: even,
+  // deep contexts lose by kKeys2, 1 x 2048 INT8 at 3986 217 / 239, uneven or short ones
+  // gain, 8 x 100-256 62 / 46.)  RLK_TUNE_BLK_PREFILL forces a split (tests and tuning runs).
   const int64_t groups = (rows + 127) / 128 * a.p.kv.num_kv_heads * a.w.num_seqs;
   const Split rule = groups <= 2 * compute_units() ? kKeys2 : (D == 64 ? kOne : kRows2);
   switch (tune_knob(kBlkPrefill, rule)) {

@@ -335,15 +335,18 @@ def _one_device(dev, *tensors):
             raise _lib.Error(_lib.RLK_EINVAL, f"tensors are on different devices (cuda:{dev} and {t.device})")
 
 
-def _launch_device(dev, stream):
-    """A launch goes to the current device: it must be the tensors' (and the stream's)."""
-    if dev is None:
-        return
-    if torch.cuda.current_device() != dev:
-        raise _lib.Error(_lib.RLK_EINVAL, f"tensors are on cuda:{dev}, the current device is "
-                                          f"cuda:{torch.cuda.current_device()}")
-    if isinstance(stream, torch.cuda.Stream) and stream.device_index != dev:
-        raise _lib.Error(_lib.RLK_EINVAL, f"tensors are on cuda:{dev}, the stream on cuda:{stream.device_index}")
+def _stream_on(dev, stream):
+    """_stream, for tensors of device dev: a launch goes to the current device, which must
+    be theirs and the stream's."""
+    if dev is not None:
+        cur = torch._C._cuda_getDevice()
+        if cur != dev:
+            raise _lib.Error(_lib.RLK_EINVAL, f"tensors are on cuda:{dev}, the current device is cuda:{cur}")
+        if stream is None:
+            return torch._C._cuda_getCurrentRawStream(dev)
+        if isinstance(stream, torch.cuda.Stream) and stream.device_index != dev:
+            raise _lib.Error(_lib.RLK_EINVAL, f"tensors are on cuda:{dev}, the stream on cuda:{stream.device_index}")
+    return _stream(stream)
 
 
 class KVBlockFormat:
@@ -406,12 +409,11 @@ def rope_and_write_kv_blocks(qkv, positions, slot_mapping, num_tokens, num_heads
         cols = (num_heads + 2 * kv.num_kv_heads) * kv.head_dim
         _need(qkv, num_tokens * cols, "qkv"); _need(qkv_bias, cols, "qkv_bias")
         _one_device(kv.device, qkv, positions, slot_mapping, cos_table, sin_table, qkv_bias)
-        _launch_device(kv.device, stream)
     check(lib().rlk_rope_and_write_kv_blocks(
         _ptr(qkv, torch.float16, "qkv"), _ptr(positions, torch.int32, "positions"),
         _ptr(slot_mapping, torch.int32, "slot_mapping"), num_tokens, num_heads,
         _ptr(cos_table, torch.float32, "cos_table"), _ptr(sin_table, torch.float32, "sin_table"),
-        C.byref(kv), _ptr(qkv_bias, torch.float16, "qkv_bias", True), _stream(stream)))
+        C.byref(kv), _ptr(qkv_bias, torch.float16, "qkv_bias", True), _stream_on(kv.device, stream)))
 
 
 def read_kv_blocks(kv: KVBlockView, slots, n, k_out=None, v_out=None, stream=None):
@@ -422,10 +424,10 @@ def read_kv_blocks(kv: KVBlockView, slots, n, k_out=None, v_out=None, stream=Non
         for t, w in ((k_out, "k_out"), (v_out, "v_out")):
             _need(t, n * kv.num_kv_heads * kv.head_dim, w)
         _one_device(kv.device, slots, k_out, v_out)
-        _launch_device(kv.device, stream)
     check(lib().rlk_read_kv_blocks(C.byref(kv), _ptr(slots, torch.int32, "slots"), n,
                                    _ptr(k_out, torch.float16, "k_out", True),
-                                   _ptr(v_out, torch.float16, "v_out", True), _stream(stream)))
+                                   _ptr(v_out, torch.float16, "v_out", True),
+                                   _stream_on(kv.device, stream)))
 
 
 def block_attention_params(q, q_stride, out, num_heads, scale, kv: KVBlockView, block_tables,
@@ -445,16 +447,16 @@ def paged_attention_decode_blocks(params: _lib.BlockAttentionParams, work: _lib.
                                   stream=None):
     """Extension: flash-decoding attention over a block-scaled cache; items with
     a negative token are skipped."""
-    _launch_device(params.device, stream)
-    check(lib().rlk_paged_attention_decode_blocks(C.byref(params), C.byref(work), _stream(stream)))
+    check(lib().rlk_paged_attention_decode_blocks(C.byref(params), C.byref(work),
+                                                    _stream_on(params.device, stream)))
 
 
 def paged_attention_prefill_blocks(params: _lib.BlockAttentionParams, work: _lib.PrefillAttentionWork,
                                    stream=None):
     """Extension: causal prefill attention over a block-scaled cache; negative
     sequence ids are skipped."""
-    _launch_device(params.device, stream)
-    check(lib().rlk_paged_attention_prefill_blocks(C.byref(params), C.byref(work), _stream(stream)))
+    check(lib().rlk_paged_attention_prefill_blocks(C.byref(params), C.byref(work),
+                                                     _stream_on(params.device, stream)))
 
 
 # ------------------------------------------------------- block tables on the GPU
@@ -510,5 +512,4 @@ def build_batch_tables(tables, stream=None):
     """Extension: positions, slots, work lists and block tables of a step from
     its request lengths, with blocks from the pool; `tables` from batch_tables()."""
     pool, work = tables
-    _launch_device(pool.device, stream)
-    check(lib().rlk_build_batch_tables(C.byref(pool.view), C.byref(work), _stream(stream)))
+    check(lib().rlk_build_batch_tables(C.byref(pool.view), C.byref(work), _stream_on(pool.device, stream)))
