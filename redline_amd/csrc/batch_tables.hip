@@ -117,12 +117,16 @@ __device__ __forceinline__ int find(const int* at, int n, int x) {
 template <int kPer>
 __global__ __launch_bounds__(kThreads) void build_batch_tables_kernel(TableArgs a) {
   const rlk_batch_tables& t = a.t;
+  // The sequences of a thread are lines of memory apart where it has many: arrays per
+  // sequence are then read and written through LDS, whole lines at a time (8000 sequences
+  // 22 us, without 33; 2094 would take 10.6 instead of 10.0).
+  constexpr bool kLines = kPer > 5;
   extern __shared__ int lds[];
   __shared__ int wave_tot[kWaves][5];
   __shared__ int taken_s;
   const int S = t.num_seqs, tid = threadIdx.x, group = blockIdx.x, groups = gridDim.x;
-  // per sequence: first row, first taken block (-1: no rows of it), tokens
-  // before, first returned block
+  // per sequence: first row, first taken block (-1: no rows of it, -2: it has ended),
+  // tokens before, first returned block
   int* start_of = lds;
   int* base_of = start_of + S;
   int* past_of = base_of + S;
@@ -135,10 +139,18 @@ __global__ __launch_bounds__(kThreads) void build_batch_tables_kernel(TableArgs 
   const int per = (S + kThreads - 1) / kThreads;  // at most kPer
   const int s0 = tid * per, mine = max(min(S - s0, per), 0);
   Request req[kPer];
+  if constexpr (kLines) {
+    for (int s = tid; s < S; s += kThreads) {
+      past_of[s] = t.past_len[s];
+      start_of[s] = t.new_len[s];
+    }
+    __syncthreads();
+  }
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
     const bool on = k < mine;
-    req[k] = request(t, on ? t.past_len[s0 + k] : 0, on ? t.new_len[s0 + k] : 0);
+    req[k] = request(t, on ? (kLines ? past_of : t.past_len)[s0 + k] : 0,
+                     on ? (kLines ? start_of : t.new_len)[s0 + k] : 0);
   }
   // rows, blocks needed and returned, decode items, prefill and refused
   // sequences (16 bits each), as if every request that fits were granted
@@ -202,13 +214,15 @@ __global__ __launch_bounds__(kThreads) void build_batch_tables_kernel(TableArgs 
         const int s = s0 + k, n = r.fits ? r.need : 0;
         const bool ok = r.fits && (n == 0 || (need <= count && n <= count - need));
         start_of[s] = start;
-        base_of[s] = ok ? need : -1;
+        base_of[s] = ok ? need : (r.ended ? -2 : -1);
         past_of[s] = r.past;
         back_of[s] = back;
         if (group == 0) {
-          t.q_start[s] = start;
-          t.q_len[s] = ok ? r.len : 0;
-          t.ctx_len[s] = ok ? r.past + r.len : (r.ended ? 0 : r.past);
+          if constexpr (!kLines) {
+            t.q_start[s] = start;
+            t.q_len[s] = ok ? r.len : 0;
+            t.ctx_len[s] = ok ? r.past + r.len : (r.ended ? 0 : r.past);
+          }
           if (ok && r.len <= thr) {
             for (int i = 0; i < r.len; ++i) {
               t.decode_token[dec + i] = start + i;
@@ -239,6 +253,14 @@ __global__ __launch_bounds__(kThreads) void build_batch_tables_kernel(TableArgs 
     }
   }
   __syncthreads();
+  for (int s = group * kThreads + tid; kLines && s < S; s += groups * kThreads) {
+    // (a granted sequence's sums are not saturated)
+    const int start = start_of[s], len = (s + 1 < S ? start_of[s + 1] : total[0]) - start;
+    const int base = base_of[s];
+    t.q_start[s] = start;
+    t.q_len[s] = base >= 0 ? len : 0;
+    t.ctx_len[s] = base >= 0 ? past_of[s] + len : (base == -2 ? 0 : past_of[s]);
+  }
 
   auto ring_at = [&](int i) {  // entry i from the head
     const uint32_t x = static_cast<uint32_t>(head) + static_cast<uint32_t>(i);  // i <= cap
