@@ -335,6 +335,17 @@ def _one_device(dev, *tensors):
             raise _lib.Error(_lib.RLK_EINVAL, f"tensors are on different devices (cuda:{dev} and {t.device})")
 
 
+def _arg(t, dtype, what, n, dev):
+    """_ptr of a tensor of at least n elements on device dev, with the checks in one call."""
+    if (isinstance(t, torch.Tensor) and t.dtype == dtype and t.is_cuda and t.is_contiguous()
+            and t.numel() >= n and (dev is None or t.get_device() == dev)):
+        return t.data_ptr()
+    p = _ptr(t, dtype, what)  # says which check fails
+    _need(t, n, what)
+    _one_device(dev, t)
+    return p
+
+
 def _stream_on(dev, stream):
     """_stream, for tensors of device dev: a launch goes to the current device, which must
     be theirs and the stream's."""
@@ -404,30 +415,24 @@ def rope_and_write_kv_blocks(qkv, positions, slot_mapping, num_tokens, num_heads
                              kv: KVBlockView, qkv_bias=None, stream=None):
     """Extension: RoPE on q/k heads (q in place) and the write of k/v into a
     block-scaled cache; rows of a block come consecutively, at rising offsets."""
-    if num_tokens > 0:
-        _need(positions, num_tokens, "positions"); _need(slot_mapping, num_tokens, "slot_mapping")
-        cols = (num_heads + 2 * kv.num_kv_heads) * kv.head_dim
-        _need(qkv, num_tokens * cols, "qkv"); _need(qkv_bias, cols, "qkv_bias")
-        _one_device(kv.device, qkv, positions, slot_mapping, cos_table, sin_table, qkv_bias)
+    n, dev = max(num_tokens, 0), kv.device
+    cols = (num_heads + 2 * kv.num_kv_heads) * kv.head_dim if n > 0 else 0
     check(lib().rlk_rope_and_write_kv_blocks(
-        _ptr(qkv, torch.float16, "qkv"), _ptr(positions, torch.int32, "positions"),
-        _ptr(slot_mapping, torch.int32, "slot_mapping"), num_tokens, num_heads,
-        _ptr(cos_table, torch.float32, "cos_table"), _ptr(sin_table, torch.float32, "sin_table"),
-        C.byref(kv), _ptr(qkv_bias, torch.float16, "qkv_bias", True), _stream_on(kv.device, stream)))
+        _arg(qkv, torch.float16, "qkv", n * cols, dev), _arg(positions, torch.int32, "positions", n, dev),
+        _arg(slot_mapping, torch.int32, "slot_mapping", n, dev), num_tokens, num_heads,
+        _arg(cos_table, torch.float32, "cos_table", 0, dev), _arg(sin_table, torch.float32, "sin_table", 0, dev),
+        C.byref(kv), None if qkv_bias is None else _arg(qkv_bias, torch.float16, "qkv_bias", cols, dev),
+        _stream_on(dev, stream)))
 
 
 def read_kv_blocks(kv: KVBlockView, slots, n, k_out=None, v_out=None, stream=None):
     """Extension: the stored rows of `slots` as fp16 [n, Hkv * D] (code * scale);
     a slot outside the pool leaves its rows as they were."""
-    if n > 0:
-        _need(slots, n, "slots")
-        for t, w in ((k_out, "k_out"), (v_out, "v_out")):
-            _need(t, n * kv.num_kv_heads * kv.head_dim, w)
-        _one_device(kv.device, slots, k_out, v_out)
-    check(lib().rlk_read_kv_blocks(C.byref(kv), _ptr(slots, torch.int32, "slots"), n,
-                                   _ptr(k_out, torch.float16, "k_out", True),
-                                   _ptr(v_out, torch.float16, "v_out", True),
-                                   _stream_on(kv.device, stream)))
+    dev, size = kv.device, max(n, 0) * kv.num_kv_heads * kv.head_dim
+    check(lib().rlk_read_kv_blocks(
+        C.byref(kv), _arg(slots, torch.int32, "slots", n, dev), n,
+        None if k_out is None else _arg(k_out, torch.float16, "k_out", size, dev),
+        None if v_out is None else _arg(v_out, torch.float16, "v_out", size, dev), _stream_on(dev, stream)))
 
 
 def block_attention_params(q, q_stride, out, num_heads, scale, kv: KVBlockView, block_tables,
