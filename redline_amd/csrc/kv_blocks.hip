@@ -411,8 +411,9 @@ __device__ __forceinline__ u32x2 scaled4(f32x4 v, float s) {
 // 16 lanes take 4 rows of the list for one head's K or V.  Where the 4 rows are a
 // quad of the layout (lists of consecutive slots), each V piece is read once and
 // gives 4 rows; other rows take theirs alone, a byte in four of what they read.
-// Bound: HBM bytes for runs (16384 rows of 4 heads of 128, 50 MB: 12.5 us, 4 TB/s),
-// the pieces' whole lines for single rows (2048 of 8 heads: 30 us), the launch below.
+// Bound: HBM bytes for runs (16384 rows of 4 heads of 128, 50 MB: 11.3 us, 4.4 TB/s),
+// address translation for single rows far apart (2048 of 8 heads in a 17 GB cache: 28 us),
+// the launch and two dependent reads below (32 rows 3.7 us).
 template <int D, bool kFp8>
 __global__ __launch_bounds__(256) void read_kv_blocks_kernel(ReadArgs a) {
   constexpr int E = D / 16, kLanes = D / 16, kTok = 16 / kLanes;
@@ -436,13 +437,24 @@ __global__ __launch_bounds__(256) void read_kv_blocks_kernel(ReadArgs a) {
   auto valid = [&](int s) { return s >= 0 && s / bs < a.kv.num_blocks; };
   if (!is_v) {
     const int p = l16 % kLanes;
+    // all rows are requested before the first is used; a slot outside the pool reads slot 0
+    int s[4];
+    float scale[4];
+    u32x4 code[4];
 #pragma unroll
     for (int u = 0; u < 4; u += kTok) {
-      const int v = u + l16 / kLanes, s = v == 0 ? slot[0] : (v == 1 ? slot[1] : (v == 2 ? slot[2] : slot[3]));
-      if (!valid(s)) continue;
-      const int blk = s / bs, off = s - blk * bs;
-      const float sc = a.kv.k_scale[static_cast<int64_t>(blk) * hkv + kvh];
-      const u32x4 w = load16(tile_of(a.kv.k, blk, off) + p * 256 + (off % 16) * 16);
+      const int v = u + l16 / kLanes;
+      s[u] = v == 0 ? slot[0] : (v == 1 ? slot[1] : (v == 2 ? slot[2] : slot[3]));
+      const int at = valid(s[u]) ? s[u] : 0, blk = at / bs, off = at - blk * bs;
+      scale[u] = a.kv.k_scale[static_cast<int64_t>(blk) * hkv + kvh];
+      code[u] = load16(tile_of(a.kv.k, blk, off) + p * 256 + (off % 16) * 16);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; u += kTok) {
+      if (!valid(s[u])) continue;
+      const int v = u + l16 / kLanes;
+      const float sc = scale[u];
+      const u32x4 w = code[u];
       const u32x2 a0 = scaled4(decode4<kFp8>(w[0]), sc), a1 = scaled4(decode4<kFp8>(w[1]), sc);
       const u32x2 b0 = scaled4(decode4<kFp8>(w[2]), sc), b1 = scaled4(decode4<kFp8>(w[3]), sc);
       _Float16* o = out + (static_cast<int64_t>(i0 + v) * hkv + kvh) * D;
@@ -475,16 +487,24 @@ __global__ __launch_bounds__(256) void read_kv_blocks_kernel(ReadArgs a) {
     }
     return;
   }
+  float scale[4];
+  u32x4 code[4][E / 4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int s = valid(slot[u]) ? slot[u] : 0, blk = s / bs, off = s - blk * bs;
+    scale[u] = a.kv.v_scale[static_cast<int64_t>(blk) * hkv + kvh];
+    const uint8_t* at = tile_of(a.kv.v, blk, off) + (off % 16 / 4) * 256 + l16 * 16;
+#pragma unroll
+    for (int gg = 0; gg < E / 4; ++gg) code[u][gg] = load16(at + gg * 1024);
+  }
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
     if (!valid(slot[u])) continue;
-    const int blk = slot[u] / bs, off = slot[u] - blk * bs;
-    const float sc = a.kv.v_scale[static_cast<int64_t>(blk) * hkv + kvh];
-    const uint8_t* at = tile_of(a.kv.v, blk, off) + (off % 16 / 4) * 256 + l16 * 16;
+    const float sc = scale[u];
 #pragma unroll
     for (int gg = 0; gg < E / 4; ++gg) {
-      const u32x4 w = load16(at + gg * 1024);
-      const int sh = 8 * (off % 4);
+      const u32x4 w = code[u][gg];
+      const int sh = 8 * (slot[u] % 4);  // (blocks are whole quads)
       const uint32_t b = ((w[0] >> sh) & 0xff) | (((w[1] >> sh) & 0xff) << 8) |
                          (((w[2] >> sh) & 0xff) << 16) | (((w[3] >> sh) & 0xff) << 24);
       *reinterpret_cast<u32x2*>(row(u) + 4 * gg) = scaled4(decode4<kFp8>(b), sc);
