@@ -14,14 +14,16 @@
 //     halves), so the running maximum and sum are lane-local, and the scores are
 //     the B operand of O^T = V^T P^T as they stand.
 //   * A tile is two phases, a matrix phase X (P.V of the tile before, K.Q of this
-//     one) and a vector phase Y (softmax, conversion of codes).  A workgroup has
-//     one or two groups of 4 waves; two groups are half a tile apart, so that of
-//     the two waves of a SIMD one has the matrix cores while the other has the
-//     vector ALU.  The groups take
-//       kRows2   256 rows, the same tiles (one image for both): large calls;
+//     one, then the conversion of K) and a vector phase Y (softmax, conversion of V; at
+//     D = 64 V is converted in X too).  At D = 128 X takes some 1400 + 260 clocks and Y
+//     1800; with all conversion in Y it was 1350 and 2060, 4 x 4096 tokens 1390 us
+//     against 1313.  A workgroup has one or two groups of 4 waves; two groups are half a
+//     tile apart, so that of the two waves of a SIMD one has the matrix cores while the
+//     other has the vector ALU.  The groups take
+//       kRows2   256 rows, the same tiles (one image for both): large calls, D = 128;
+//       kOne     one group, three workgroups to a CU: large calls, D = 64;
 //       kKeys2   the same 128 rows, even and odd tiles (an image each), and join
-//                their partials at the end: calls that do not fill the chip;
-//       kOne     one group, whose CU holds two workgroups: between the two.
+//                their partials at the end: calls that do not fill the chip.
 // m, l and the output accumulate in fp32; P is rounded to fp16 (at most 2^8), and
 // l sums the rounded values, so that numerator and denominator agree.
 // Bound: long prompts by X and Y in turn at the clock that the chip holds under them
@@ -99,8 +101,8 @@ template <int D, bool kFp8, Split kSplit>
 __global__ __launch_bounds__(kGroupThreads * (kSplit == kOne ? 1 : 2), 2) void prefill_blocks_kernel(PrefillArgs a) {
   constexpr int kGroups = kSplit == kRows2 ? 2 : 1;  // that share a tile's image
   constexpr bool kKeys = kSplit == kKeys2;
-  // where V is converted: beside K in X, or (two groups at D = 128) in Y, for phases of one length
-  constexpr bool kVInX = D == 64 || kSplit == kOne;
+  // where V is converted: beside K in X, or (at D = 128) in Y, for phases of one length
+  constexpr bool kVInX = D == 64;
   constexpr int E = D / 16, kRows = 4 * kWaveRows * kGroups;
   constexpr int kPerTile = D;                                  // 16-byte pieces of a layout tile
   constexpr int kItems = 2 * 4 * kPerTile / kGroups / kGroupThreads;  // K and V pieces of a thread and tile
@@ -458,7 +460,7 @@ template <int D, bool kFp8>
 hipError_t launch(const PrefillArgs& a, int64_t rows, hipStream_t stream) {
   // Workgroups of 128 rows (of the grid: ragged prompts leave some of them empty).
   // Up to two per CU, splitting the keys beats more rows; past that, at D = 128,
-  // 256 rows to an image beat 128, at D = 64 they would not (nor is it built).
+  // 256 rows to an image beat 128, at D = 64 they do not (the slower one is not built).
   // us, kOne / kRows2 / kKeys2: 2 chunks of 512, 8 kv heads of 128, e4m3 60 / 61 / 45;
   // of 1024 87 / 80 / 69; of 2048 174 / 157 / 188; 4 x 4096 INT8 1525 / 1319 / 1547;
   // D = 64, kOne / kKeys2: 2 chunks of 512 44 / 31, 24 ragged prompts 111 / 154, 4 x 4096
@@ -466,14 +468,10 @@ hipError_t launch(const PrefillArgs& a, int64_t rows, hipStream_t stream) {
   // deep contexts lose by kKeys2, 1 x 2048 INT8 at 3986 217 / 239, uneven or short ones
   // gain, 8 x 100-256 62 / 46.)  RLK_TUNE_BLK_PREFILL forces a split (tests and tuning runs).
   const int64_t groups = (rows + 127) / 128 * a.p.kv.num_kv_heads * a.w.num_seqs;
-  const Split rule = groups <= 2 * compute_units() ? kKeys2 : (D == 64 ? kOne : kRows2);
-  switch (tune_knob(kBlkPrefill, rule)) {
-    case kKeys2: return launch_s<D, kFp8, kKeys2>(a, rows, stream);
-    case kRows2:
-      if constexpr (D == 128) return launch_s<D, kFp8, kRows2>(a, rows, stream);
-      [[fallthrough]];
-    default: return launch_s<D, kFp8, kOne>(a, rows, stream);
-  }
+  constexpr Split kLarge = D == 64 ? kOne : kRows2;
+  const Split rule = groups <= 2 * compute_units() ? kKeys2 : kLarge;
+  if (tune_knob(kBlkPrefill, rule) == kKeys2) return launch_s<D, kFp8, kKeys2>(a, rows, stream);
+  return launch_s<D, kFp8, kLarge>(a, rows, stream);
 }
 
 }  // namespace
