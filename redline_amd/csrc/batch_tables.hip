@@ -20,6 +20,7 @@
 #include <algorithm>
 #include <cstdint>
 
+#include "batch_sums.hpp"
 #include "device.hpp"
 #include "redline_amd/rlk.h"
 #include "status.hpp"
@@ -30,14 +31,11 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kRowsPerGroup = kThreads;
-constexpr int kSat = 1 << 30;  // running sums of rows saturate here
 
 struct TableArgs {
   rlk_block_pool pool;
   rlk_batch_tables t;
 };
-
-__device__ __forceinline__ int sat_add(int a, int b) { return min(a + b, kSat); }  // a, b <= kSat
 
 // Exclusive sums of N values over the workgroup's threads (saturating); the
 // totals come back in `total`.
@@ -97,7 +95,7 @@ __device__ __forceinline__ Request request(const rlk_batch_tables& t, int past, 
   const uint32_t p = max(past, 0);
   r.have = blocks_of(p, t.block_size);
   const int want = blocks_of(p + r.len, t.block_size);  // p + len is below 2^31 + 2^30
-  r.need = want - r.have;
+  r.need = static_cast<int>(static_cast<uint32_t>(want) - static_cast<uint32_t>(r.have));
   r.back = r.ended ? min(r.have, t.max_blocks_per_seq) : 0;
   r.fits = r.live && past >= 0 && want >= 0 && want <= t.max_blocks_per_seq;
   return r;
