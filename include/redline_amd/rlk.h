@@ -360,7 +360,7 @@ typedef struct rlk_kv_block_view {
  * values of the head; 0 when all are 0.  A run that starts later continues the
  * block: s = max(old scale, that power of two), and when s grew, the codes of
  * the earlier offsets are requantised, code' = rne(code * old / s).  New codes
- * are rne(x / s) of the fp16 value x, saturating at the largest code whose
+ * are rne(x / s) of the fp16 value x.  Both saturate at the largest code whose
  * value is an fp16 number (INT8 127, 63 at s = 2^10; e4m3 448, 240 at 2^8);
  * infinities saturate, NaN is stored as some finite value.  Bytes of offsets
  * past the run are left as they were, and so are slots < 0 or past the pool.

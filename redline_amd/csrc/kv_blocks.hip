@@ -117,10 +117,12 @@ __device__ __forceinline__ float join_scale(float old, float amax, float& ratio)
   return s;
 }
 
+// Codes at the grown scale; lim is that scale's: an INT8 code of 127 at 2^9 would round
+// to 64 at 2^10, which no fp16 number holds.
 template <bool kFp8>
-__device__ __forceinline__ uint32_t requant4(uint32_t w, float ratio) {
+__device__ __forceinline__ uint32_t requant4(uint32_t w, float ratio, float lim) {
   const f32x4 v = decode4<kFp8>(w);
-  return encode4<kFp8>(v[0], v[1], v[2], v[3], ratio, BlockFormat<kFp8>::kMax);
+  return encode4<kFp8>(v[0], v[1], v[2], v[3], ratio, lim);
 }
 
 // K of one head for a run of at most kMax rows, by kGroup lanes of which this is
@@ -171,7 +173,7 @@ __device__ __forceinline__ void write_k(const WriteArgs& a, const Run& r, const 
       u32x4* at = reinterpret_cast<u32x4*>(dst + (key / 16) * (16 * D) + (key % 16) * 16);
       u32x4 w = *at;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = requant4<kFp8>(w[e], ratio);
+      for (int e = 0; e < 4; ++e) w[e] = requant4<kFp8>(w[e], ratio, lim);
       *at = w;
     }
   }
@@ -250,7 +252,7 @@ __device__ __forceinline__ void write_v(const WriteArgs& a, const Run& r, int kv
                                static_cast<float>(x[it][2][d]), static_cast<float>(x[it][3][d]), inv, lim);
           if (mine[it] != 0xffffffffu) {
             const uint32_t h = had[it][g][j];
-            const uint32_t keep = ratio != 1.f ? (requant4<kFp8>(h, ratio) & below[it]) | (h & ~below[it]) : h;
+            const uint32_t keep = ratio != 1.f ? (requant4<kFp8>(h, ratio, lim) & below[it]) | (h & ~below[it]) : h;
             w[j] = (w[j] & mine[it]) | (keep & ~mine[it]);
           }
         }
@@ -264,7 +266,7 @@ __device__ __forceinline__ void write_v(const WriteArgs& a, const Run& r, int kv
       for (int g = 0; g < E / 4; ++g) {
         u32x4 w = *piece(quad, g);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = requant4<kFp8>(w[j], ratio);
+        for (int j = 0; j < 4; ++j) w[j] = requant4<kFp8>(w[j], ratio, lim);
         *piece(quad, g) = w;
       }
     }
