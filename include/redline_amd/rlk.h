@@ -399,13 +399,18 @@ typedef struct rlk_block_attention_params {
  * workspace and max_partitions contract).  An item whose token is negative is
  * skipped (its rows of out are not known); an item whose position is negative
  * attends to nothing and gets zeros.  Keys past the sequence's table row
- * (max_blocks_per_seq * block_size) are not read. */
+ * (max_blocks_per_seq * block_size) are not read.  A key's probability times its
+ * V scale is rounded to fp16 (11 bits; below 2^-14 of the row's largest such
+ * product to 2^-25 of it), all else is held in fp32. */
 int rlk_paged_attention_decode_blocks(const rlk_block_attention_params* params,
                                       const rlk_decode_attention_work* work, hipStream_t stream);
 
 /* rlk_paged_attention_prefill over a block-scaled cache (same work
  * description).  A negative sequence id is skipped; rows with nothing to
- * attend to get zeros; keys past the sequence's table row are not read. */
+ * attend to get zeros; keys past the sequence's table row are not read.  A key's
+ * probability is rounded to fp16 (11 bits; below 2^-14 of the row's largest to
+ * 2^-25 of it, so that a key of less adds nothing, however large its V), all else
+ * is held in fp32. */
 int rlk_paged_attention_prefill_blocks(const rlk_block_attention_params* params,
                                        const rlk_prefill_attention_work* work,
                                        hipStream_t stream);

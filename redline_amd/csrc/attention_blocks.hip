@@ -17,10 +17,12 @@
 //        4 rho .. 4 rho + 3, and the scores of those tokens are what the first
 //        product left in the lane.
 // Codes become fp16 exactly; the K scale multiplies the fp32 scores (with the
-// softmax scale), the V scale the fp32 probabilities, relative to the largest V
-// scale that the wave has met (a power of two, so the ratio is exact and the
-// fp16 operand keeps its 11 bits however small V is).  m, l and the output stay
-// in fp32.
+// softmax scale), the V scale s_k the fp32 probabilities.  The running reference m
+// is the maximum of scale q.k + log s_k, not of scale q.k alone: the fp16 operand
+// p_k s_k then has its 11 bits for the keys that weigh most in the output, however
+// small their V is and whatever V the keys without weight have (scales lie in
+// 2^-24 .. 2^10, so p_k and its sum stay far inside fp32's range).  m, l and the
+// output stay in fp32.
 // Bound: HBM reads for full batches, which stream at 6.1 TB/s between a start of
 // about 4 us (lengths, table entries, scales: dependent reads) and the merge's 4-5:
 // 32 items to 8191 keys (INT8, 8 kv heads of 128, 257 MB) 52 us in all, 4.9 TB/s;
@@ -83,7 +85,7 @@ __device__ __forceinline__ float lane_value(float v, int lane) {
 template <int D>
 struct WaveState {
   f32x4 o[D / 16];
-  float m = -FLT_MAX, l = 0.f, vref = 0.f;  // o is relative to the V scale vref
+  float m = -FLT_MAX, l = 0.f;
 
   __device__ __forceinline__ WaveState() {
 #pragma unroll
@@ -141,8 +143,10 @@ __device__ __forceinline__ void attend(const DecodeArgs& a, WaveState<D>& w, int
         s.v[t][x] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vbase + at[t] + x * 1024) + lane);
     __builtin_amdgcn_sched_barrier(0);
   };
-  // lane t: the scales of tile t
-  float ksl = p.kv.k_scale[cell], vsl = p.kv.v_scale[cell];
+  // lane t: the scales of tile t, and the V scale's logarithm (0 counts as 2^-24)
+  float ksl = p.kv.k_scale[cell];
+  const float vsl = p.kv.v_scale[cell];
+  const float vll = static_cast<float>(max(static_cast<int>(__builtin_bit_cast(uint32_t, vsl) >> 23) - 127, -24));
   // q: column c = head c, zero past the group
   const _Float16* q = reinterpret_cast<const _Float16*>(p.q) + static_cast<int64_t>(token) * p.q_stride +
                       (kvh * G + min(c, G - 1)) * D;
@@ -159,15 +163,6 @@ __device__ __forceinline__ void attend(const DecodeArgs& a, WaveState<D>& w, int
     for (int h = 0; h < 2; ++h)
       if (c >= G) qb[x][h] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
   ksl *= p.scale * kLog2e;
-  float vmax = lane < tiles ? vsl : 0.f;
-  vmax = fmaxf(w.vref, rows_max<true>(rows_max<false>(group_max<16>(vmax))));
-  vsl *= inv_scale(vmax);
-  if (w.vref > 0.f && w.vref != vmax) {  // continued: o moves to the larger reference
-    const float f = w.vref * inv_scale(vmax);
-#pragma unroll
-    for (int d = 0; d < E; ++d) w.o[d] *= f;
-  }
-  w.vref = vmax;
   auto step = [&](StepCodes<D>& s, int st, bool tail) {
     f32x4 acc[2];
 #pragma unroll
@@ -186,6 +181,7 @@ __device__ __forceinline__ void attend(const DecodeArgs& a, WaveState<D>& w, int
     const int t1 = min(2 * st + 1, tiles - 1);
     const float ks[2] = {lane_value(ksl, 2 * st), lane_value(ksl, t1)};
     const float vs[2] = {lane_value(vsl, 2 * st), lane_value(vsl, t1)};
+    const float vl[2] = {lane_value(vll, 2 * st), lane_value(vll, t1)};
     float e[2][4];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -205,11 +201,11 @@ __device__ __forceinline__ void attend(const DecodeArgs& a, WaveState<D>& w, int
         for (int x = 0; x < kX; ++x) s.v[t][x] &= u32x4{mask, mask, mask, mask};
       }
     }
-    float mx = fmaxf(fmaxf(fmaxf(e[0][0], e[0][1]), fmaxf(e[0][2], e[0][3])),
-                     fmaxf(fmaxf(e[1][0], e[1][1]), fmaxf(e[1][2], e[1][3])));
+    float mx = fmaxf(fmaxf(fmaxf(e[0][0], e[0][1]), fmaxf(e[0][2], e[0][3])) + vl[0],
+                     fmaxf(fmaxf(e[1][0], e[1][1]), fmaxf(e[1][2], e[1][3])) + vl[1]);
     mx = rows_max<true>(rows_max<false>(mx));
     // m is a reference within 2^8 of the maximum: moving it costs a pass over the
-    // output, and p up to 2^8 fits fp16 as well as p up to 1 does
+    // output, and p s up to 2^8 fits fp16 as well as p s up to 1 does
     if (__any(mx > w.m + 8.f)) {
       const float mn = fmaxf(w.m, mx), f = __builtin_amdgcn_exp2f(w.m - mn);
       w.l *= f;
@@ -300,7 +296,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_blocks_grid_kernel(DecodeA
 #pragma unroll
       for (int d = 0; d < D / 16; d += 4)
         *reinterpret_cast<f32x4*>(&s.o[wave][c][w.dim(d, i)]) =
-            f32x4{w.o[d][i], w.o[d + 1][i], w.o[d + 2][i], w.o[d + 3][i]} * w.vref;
+            f32x4{w.o[d][i], w.o[d + 1][i], w.o[d + 2][i], w.o[d + 3][i]};
     if (lane < 16) {
       s.m[wave][c] = w.m;
       s.l[wave][c] = w.l;
@@ -412,7 +408,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_blocks_range_kernel(Decode
     if (c < G) {
       const int head = kvh * G + c;
       if (todo == steps) {
-        const float inv = w.vref / w.l;
+        const float inv = 1.f / w.l;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           _Float16* o = out_row(a, token, head, D) + w.dim(0, i);
@@ -428,7 +424,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_blocks_range_kernel(Decode
           float* o = a.w.ws_out + row * D + w.dim(0, i);
 #pragma unroll
           for (int d = 0; d < D / 16; d += 4)
-            *reinterpret_cast<f32x4*>(o + d) = f32x4{w.o[d][i], w.o[d + 1][i], w.o[d + 2][i], w.o[d + 3][i]} * w.vref;
+            *reinterpret_cast<f32x4*>(o + d) = f32x4{w.o[d][i], w.o[d + 1][i], w.o[d + 2][i], w.o[d + 3][i]};
         }
         if (lane < 16) {
           a.w.ws_max[row] = w.m;
