@@ -73,6 +73,7 @@ class AttentionParams(C.Structure):
 class DecodeAttentionWork(C.Structure):
     """Mirror of rlk_decode_attention_work / kernels::DecodeAttentionWork."""
 
+    device = tensors = room = None  # of the lists and the workspace, where kernels.decode_work made it
     _fields_ = [("item_token", C.c_void_p), ("item_seq", C.c_void_p), ("num_items", C.c_int),
                 ("max_partitions", C.c_int), ("ws_out", C.c_void_p), ("ws_max", C.c_void_p),
                 ("ws_sum", C.c_void_p)]
@@ -81,6 +82,7 @@ class DecodeAttentionWork(C.Structure):
 class PrefillAttentionWork(C.Structure):
     """Mirror of rlk_prefill_attention_work / kernels::PrefillAttentionWork."""
 
+    device = tensors = None
     _fields_ = [("seq_ids", C.c_void_p), ("q_start", C.c_void_p), ("q_len", C.c_void_p),
                 ("ctx_len", C.c_void_p), ("num_seqs", C.c_int), ("max_q_tiles", C.c_int)]
 

@@ -222,21 +222,35 @@ def attention_params(q, q_stride, out, num_heads, scale, kv: KVLayerView, block_
 
 def decode_work(item_token, item_seq, num_items, max_partitions, workspace=None):
     """kernels::DecodeAttentionWork; `workspace` is a DecodeWorkspace (needed
-    when max_partitions > 1)."""
+    when max_partitions > 1).  The struct keeps its tensors."""
     ws = workspace
-    return _lib.DecodeAttentionWork(
+    _need(item_token, num_items, "item_token"); _need(item_seq, num_items, "item_seq")
+    work = _lib.DecodeAttentionWork(
         _ptr(item_token, torch.int32, "item_token"), _ptr(item_seq, torch.int32, "item_seq"),
         num_items, max_partitions,
         None if ws is None else ws.out.data_ptr(), None if ws is None else ws.max.data_ptr(),
         None if ws is None else ws.sum.data_ptr())
+    if ws is not None and max_partitions > 1:  # (item, head) rows that the workspace holds, elements of ws.out
+        work.room = min(ws.max.numel(), ws.sum.numel()) // max_partitions, ws.out.numel() // max_partitions
+    return _keep(work, item_token, item_seq, *(() if ws is None else (ws.out, ws.max, ws.sum)))
+
+
+def _keep(work, *tensors):
+    """`work` with the tensors whose pointers it holds, and their device."""
+    work.device, work.tensors = tensors[0].get_device(), tensors
+    _one_device(work.device, *tensors)
+    return work
 
 
 def prefill_work(seq_ids, q_start, q_len, ctx_len, num_seqs, max_q_tiles):
-    """kernels::PrefillAttentionWork (max_q_tiles in 32-row tiles, as BatchBuilder writes it)."""
-    return _lib.PrefillAttentionWork(
+    """kernels::PrefillAttentionWork (max_q_tiles in 32-row tiles, as BatchBuilder writes it).
+    The struct keeps its tensors."""
+    if max_q_tiles > 0:
+        _need(seq_ids, num_seqs, "seq_ids")
+    return _keep(_lib.PrefillAttentionWork(
         _ptr(seq_ids, torch.int32, "seq_ids"), _ptr(q_start, torch.int32, "q_start"),
         _ptr(q_len, torch.int32, "q_len"), _ptr(ctx_len, torch.int32, "ctx_len"), num_seqs,
-        max_q_tiles)
+        max_q_tiles), seq_ids, q_start, q_len, ctx_len)
 
 
 def paged_attention_prefill(params: _lib.AttentionParams, work: _lib.PrefillAttentionWork,
@@ -448,10 +462,24 @@ def block_attention_params(q, q_stride, out, num_heads, scale, kv: KVBlockView, 
     return params
 
 
+def _same_device(params, work):
+    if params.device is not None and work.device is not None and params.device != work.device:
+        raise _lib.Error(_lib.RLK_EINVAL, f"the work lists are on cuda:{work.device}, the tensors on another "
+                                          f"device (cuda:{params.device})")
+
+
 def paged_attention_decode_blocks(params: _lib.BlockAttentionParams, work: _lib.DecodeAttentionWork,
                                   stream=None):
     """Extension: flash-decoding attention over a block-scaled cache; items with
     a negative token are skipped."""
+    if work.device != params.device:
+        _same_device(params, work)
+    if work.room is not None:
+        rows = work.num_items * params.num_heads
+        if rows > work.room[0] or rows * params.kv.head_dim > work.room[1]:
+            raise _lib.Error(_lib.RLK_EINVAL, f"the workspace holds {work.room[0]} (item, head) rows and "
+                                              f"{work.room[1]} elements a partition, needs {rows} of "
+                                              f"{params.kv.head_dim}")
     check(lib().rlk_paged_attention_decode_blocks(C.byref(params), C.byref(work),
                                                     _stream_on(params.device, stream)))
 
@@ -460,6 +488,8 @@ def paged_attention_prefill_blocks(params: _lib.BlockAttentionParams, work: _lib
                                    stream=None):
     """Extension: causal prefill attention over a block-scaled cache; negative
     sequence ids are skipped."""
+    if work.device != params.device:
+        _same_device(params, work)
     check(lib().rlk_paged_attention_prefill_blocks(C.byref(params), C.byref(work),
                                                      _stream_on(params.device, stream)))
 
