@@ -469,6 +469,9 @@ typedef struct rlk_batch_tables {
  * them).  The ceil(past / block_size) blocks of an ended sequence join the
  * ring's tail in order and can be taken from the next call on; its table row
  * is left as it was.  q_start and counts[0] saturate at 2^30.
+ * ctx_len may be past_len itself: the call then leaves the lengths that the next
+ * step starts from, so that a captured step can be replayed as it is.  q_len may be
+ * new_len.  Any other output that overlaps past_len or new_len: RLK_EINVAL.
  * num_seqs > RLK_BATCH_TABLES_MAX_SEQS: RLK_EUNSUPPORTED; num_seqs and
  * num_rows both 0: no-op. */
 #define RLK_BATCH_TABLES_MAX_SEQS 8192

@@ -11,7 +11,8 @@
 // blocks do not suffice are they formed again step by step.  Blocks are taken
 // from the ring's head and returned at its tail, so no workgroup writes an entry
 // that another reads; the ring's state is written by the workgroup that is done
-// with it last (a ticket in its third word).
+// with it last (a ticket in its third word), and so are the lengths where they take
+// the place of the ones that every workgroup reads.
 // Bound: the launch and a chain of dependent reads (lengths, then table or ring): 32
 // decoding sequences 4.2 us, 16k rows of 8 sequences 5.9, 2100 sequences 9.8 (5 of
 // them in each thread; forming the sums twice took 23), 8000 22.
@@ -35,6 +36,7 @@ constexpr int kRowsPerGroup = kThreads;
 struct TableArgs {
   rlk_block_pool pool;
   rlk_batch_tables t;
+  int in_place;  // ctx_len is past_len, or q_len is new_len
 };
 
 // Exclusive sums of N values over the workgroup's threads (saturating); the
@@ -121,7 +123,7 @@ __global__ __launch_bounds__(kThreads) void build_batch_tables_kernel(TableArgs 
   constexpr bool kLines = kPer > 5;
   extern __shared__ int lds[];
   __shared__ int wave_tot[kWaves][5];
-  __shared__ int taken_s;
+  __shared__ int taken_s, last_s;
   const int S = t.num_seqs, tid = threadIdx.x, group = blockIdx.x, groups = gridDim.x;
   // per sequence: first row, first taken block (-1: no rows of it, -2: it has ended),
   // tokens before, first returned block
@@ -216,7 +218,7 @@ __global__ __launch_bounds__(kThreads) void build_batch_tables_kernel(TableArgs 
         past_of[s] = r.past;
         back_of[s] = back;
         if (group == 0) {
-          if constexpr (!kLines) {
+          if (!kLines && !a.in_place) {
             t.q_start[s] = start;
             t.q_len[s] = ok ? r.len : 0;
             t.ctx_len[s] = ok ? r.past + r.len : (r.ended ? 0 : r.past);
@@ -251,14 +253,18 @@ __global__ __launch_bounds__(kThreads) void build_batch_tables_kernel(TableArgs 
     }
   }
   __syncthreads();
-  for (int s = group * kThreads + tid; kLines && s < S; s += groups * kThreads) {
-    // (a granted sequence's sums are not saturated)
-    const int start = start_of[s], len = (s + 1 < S ? start_of[s + 1] : total[0]) - start;
-    const int base = base_of[s];
-    t.q_start[s] = start;
-    t.q_len[s] = base >= 0 ? len : 0;
-    t.ctx_len[s] = base >= 0 ? past_of[s] + len : (base == -2 ? 0 : past_of[s]);
-  }
+  // lengths of the sequences first, first + step, .. from the sums
+  auto write_lengths = [&](int first, int step) {
+    for (int s = first; s < S; s += step) {
+      // (a granted sequence's sums are not saturated)
+      const int start = start_of[s], len = (s + 1 < S ? start_of[s + 1] : total[0]) - start;
+      const int base = base_of[s];
+      t.q_start[s] = start;
+      t.q_len[s] = base >= 0 ? len : 0;
+      t.ctx_len[s] = base >= 0 ? past_of[s] + len : (base == -2 ? 0 : past_of[s]);
+    }
+  };
+  if (kLines && !a.in_place) write_lengths(group * kThreads + tid, groups * kThreads);
 
   auto ring_at = [&](int i) {  // entry i from the head
     const uint32_t x = static_cast<uint32_t>(head) + static_cast<uint32_t>(i);  // i <= cap
@@ -297,13 +303,18 @@ __global__ __launch_bounds__(kThreads) void build_batch_tables_kernel(TableArgs 
     int32_t* state = a.pool.state;
     int32_t* out = a.pool.state_out != nullptr ? a.pool.state_out : state;
     // with several workgroups the one whose ticket is the last: every other has
-    // read the state
+    // read the state, and the lengths
     const bool last = groups == 1 || atomicAdd(&state[2], 1) == groups - 1;
+    last_s = last;
     if (last) {
       if (groups > 1) state[2] = 0;
       out[0] = ring_at(taken);
       out[1] = count - taken + returned;
     }
+  }
+  if (a.in_place) {
+    __syncthreads();
+    if (last_s) write_lengths(tid, kThreads);
   }
 }
 
@@ -352,7 +363,24 @@ extern "C" int rlk_build_batch_tables(const rlk_block_pool* pool, const rlk_batc
       (t.num_rows > 0 && (t.positions == nullptr || t.slot_mapping == nullptr ||
                           t.decode_token == nullptr || t.decode_seq == nullptr)))
     return fail(RLK_EINVAL, "%s: null pointer argument", what);
-  const TableArgs a = {*pool, t};
+  // every workgroup reads past_len and new_len: what is written must not lie there, but
+  // for the lengths themselves (`same`), which are then written last
+  struct Out {
+    const int32_t* at;
+    int64_t n;
+    const int32_t* same;
+  };
+  const int64_t S = t.num_seqs, rows = t.num_rows;
+  for (const int32_t* in : {t.past_len, t.new_len})
+    for (const Out& o : {Out{t.q_len, S, t.new_len}, Out{t.ctx_len, S, t.past_len}, Out{t.q_start, S, nullptr},
+                         Out{t.prefill_seq, S, nullptr}, Out{t.block_tables, S * t.max_blocks_per_seq, nullptr},
+                         Out{t.positions, rows, nullptr}, Out{t.slot_mapping, rows, nullptr},
+                         Out{t.decode_token, rows, nullptr}, Out{t.decode_seq, rows, nullptr},
+                         Out{t.counts, 4, nullptr}})
+      if (S > 0 && o.n > 0 && in < o.at + o.n && o.at < in + S && !(in == o.same && o.at == o.same))
+        return fail(RLK_EINVAL, "%s: past_len and new_len must not overlap what is written (ctx_len may be "
+                                "past_len, q_len new_len)", what);
+  const TableArgs a = {*pool, t, t.num_seqs > 0 && (t.ctx_len == t.past_len || t.q_len == t.new_len)};
   const int per = (t.num_seqs + kThreads - 1) / kThreads;
   if (per <= 1) return launch_tables<1>(a, stream);
   if (per <= 5) return launch_tables<5>(a, stream);
