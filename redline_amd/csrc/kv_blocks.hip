@@ -281,6 +281,8 @@ constexpr int kShort = 4;  // rows of a run that 16 lanes do
 // V head unit - hkv.
 template <int D, int BS, bool kFp8, int kRows>
 __device__ __forceinline__ void write_chunk(const WriteArgs& a, int chunk0, int unit, int lane, int* pos) {
+  // (so a run that starts in the chunk ends, at the block's end at the latest, before a
+  // row that this wave sees)
   static_assert(kRows + BS <= kWave, "a chunk's rows and the last run's rest fit one wave");
   const int hkv = a.kv.num_kv_heads;
   const int row = chunk0 + lane;
@@ -294,15 +296,14 @@ __device__ __forceinline__ void write_chunk(const WriteArgs& a, int chunk0, int 
   // a row starts a run unless it continues the block of the row before
   const uint64_t starts = __ballot(!valid || slot % BS == 0 || slot != before + 1);
   uint64_t todo = starts & __ballot(valid) & ((1ull << kRows) - 1);
+  auto rows_of = [&](int i) { return __builtin_ctzll(starts >> (i + 1)) + 1; };  // of the run from row i on
   auto run_at = [&](int i) {  // the run that starts at row chunk0 + i
-    const uint64_t after = starts >> (i + 1);
     const int sl = __shfl(slot, i, kWave);
-    return Run{chunk0 + i, after != 0 ? __builtin_ctzll(after) + 1 : kWave - i, sl / BS, sl % BS};
+    return Run{chunk0 + i, rows_of(i), sl / BS, sl % BS};
   };
   while (todo != 0) {  // uniform over the wave
     const int i = __builtin_ctzll(todo);
-    const uint64_t after = starts >> (i + 1);
-    if (after == 0 || __builtin_ctzll(after) + 1 > kShort) {  // a long run, by the whole wave
+    if (rows_of(i) > kShort) {  // a long run, by the whole wave
       todo &= todo - 1;
       const Run r = run_at(i);
       if (unit < hkv) write_k<D, BS, kFp8, 64, BS>(a, r, pos + i, unit, lane);
@@ -311,9 +312,9 @@ __device__ __forceinline__ void write_chunk(const WriteArgs& a, int chunk0, int 
       int mine = -1;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int k = todo != 0 ? __builtin_ctzll(todo) : -1;
-        const uint64_t rest = k >= 0 ? starts >> (k + 1) : 0;
-        if (rest == 0 || __builtin_ctzll(rest) + 1 > kShort) break;
+        if (todo == 0) break;
+        const int k = __builtin_ctzll(todo);
+        if (rows_of(k) > kShort) break;
         if (lane / 16 == g) mine = k;
         todo &= todo - 1;
       }
