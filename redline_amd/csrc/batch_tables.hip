@@ -14,8 +14,9 @@
 // with it last (a ticket in its third word), and so are the lengths where they take
 // the place of the ones that every workgroup reads.
 // Bound: the launch and a chain of dependent reads (lengths, then table or ring): 32
-// decoding sequences 4.2 us, 16k rows of 8 sequences 5.9, 2100 sequences 9.8 (5 of
-// them in each thread; forming the sums twice took 23), 8000 22.
+// decoding sequences 4.2 us, 16k rows of 8 sequences 5.8; of thousands of sequences the
+// scan, and what the first workgroup writes alone: 2094 sequences 9.9 us (5 of them in
+// each thread; forming the sums twice took 23), 4000 17, 8000 22.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -381,6 +382,8 @@ extern "C" int rlk_build_batch_tables(const rlk_block_pool* pool, const rlk_batc
         return fail(RLK_EINVAL, "%s: past_len and new_len must not overlap what is written (ctx_len may be "
                                 "past_len, q_len new_len)", what);
   const TableArgs a = {*pool, t, t.num_seqs > 0 && (t.ctx_len == t.past_len || t.q_len == t.new_len)};
+  // (2560 sequences: 5 a thread 10.3 us, the form for up to 16, which spills scalar
+  // registers, 15.1; 2561 take 15.5 by it)
   const int per = (t.num_seqs + kThreads - 1) / kThreads;
   if (per <= 1) return launch_tables<1>(a, stream);
   if (per <= 5) return launch_tables<5>(a, stream);

@@ -28,8 +28,8 @@
 // l sums the rounded values, so that numerator and denominator agree.
 // Bound: long prompts by X and Y in turn at the clock that the chip holds under them
 // (about 1.8 GHz of 2.4): 4 x 4096 tokens at depths to 4096, 32 / 8 heads of 128, take
-// 1298 us INT8 and 1277 e4m3, 1.03 PFLOP/s or 85% of a large library product; 4 x 4096 at
-// D = 64 699 us.  Short ones by the longest workgroup's chain of tiles: 2 chunks of
+// 1275-1330 us INT8 (by run) and 1275 e4m3, 1.0-1.05 PFLOP/s or 83-86% of a large library
+// product; 4 x 4096 at D = 64 699 us.  Short ones by the longest workgroup's chain of tiles: 2 chunks of
 // 512 tokens at depths 0 and 1585 41 us, 24 ragged prompts at D = 64 92 us (560 TFLOP/s).
 #include <hip/hip_runtime.h>
 
