@@ -224,12 +224,12 @@ def decode_work(item_token, item_seq, num_items, max_partitions, workspace=None)
     """kernels::DecodeAttentionWork; `workspace` is a DecodeWorkspace (needed
     when max_partitions > 1).  The struct keeps its tensors."""
     ws = workspace
-    _need(item_token, num_items, "item_token"); _need(item_seq, num_items, "item_seq")
     work = _lib.DecodeAttentionWork(
         _ptr(item_token, torch.int32, "item_token"), _ptr(item_seq, torch.int32, "item_seq"),
         num_items, max_partitions,
         None if ws is None else ws.out.data_ptr(), None if ws is None else ws.max.data_ptr(),
         None if ws is None else ws.sum.data_ptr())
+    _need(item_token, num_items, "item_token"); _need(item_seq, num_items, "item_seq")
     if ws is not None and max_partitions > 1:  # (item, head) rows that the workspace holds, elements of ws.out
         work.room = min(ws.max.numel(), ws.sum.numel()) // max_partitions, ws.out.numel() // max_partitions
     return _keep(work, item_token, item_seq, *(() if ws is None else (ws.out, ws.max, ws.sum)))
@@ -245,12 +245,13 @@ def _keep(work, *tensors):
 def prefill_work(seq_ids, q_start, q_len, ctx_len, num_seqs, max_q_tiles):
     """kernels::PrefillAttentionWork (max_q_tiles in 32-row tiles, as BatchBuilder writes it).
     The struct keeps its tensors."""
-    if max_q_tiles > 0:
-        _need(seq_ids, num_seqs, "seq_ids")
-    return _keep(_lib.PrefillAttentionWork(
+    work = _lib.PrefillAttentionWork(
         _ptr(seq_ids, torch.int32, "seq_ids"), _ptr(q_start, torch.int32, "q_start"),
         _ptr(q_len, torch.int32, "q_len"), _ptr(ctx_len, torch.int32, "ctx_len"), num_seqs,
-        max_q_tiles), seq_ids, q_start, q_len, ctx_len)
+        max_q_tiles)
+    if max_q_tiles > 0:
+        _need(seq_ids, num_seqs, "seq_ids")
+    return _keep(work, seq_ids, q_start, q_len, ctx_len)
 
 
 def paged_attention_prefill(params: _lib.AttentionParams, work: _lib.PrefillAttentionWork,
