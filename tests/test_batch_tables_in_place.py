@@ -39,8 +39,9 @@ def test_overlapping_lengths_are_refused(at):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("both", [False, True])
+@pytest.mark.parametrize("scarce", [False, True])  # blocks for all sequences, or for half of them
 @pytest.mark.parametrize("S,rows,bs", [(5, 40, 16), (600, 700, 16), (3000, 5000, 32), (8192, 8192, 16)])
-def test_lengths_in_place(S, rows, bs, both):
+def test_lengths_in_place(S, rows, bs, scarce, both):
     """Steps of S sequences, captured once and replayed: each starts from the lengths
     that the one before left.  new_len is written anew between the replays where q_len
     takes its place."""
@@ -48,9 +49,9 @@ def test_lengths_in_place(S, rows, bs, both):
     from redline_amd import kernels as K
     from tests.test_kv_blocks_gpu import dev
     assert torch.cuda.is_available()
-    say(f"tables in place S={S} rows={rows} bs={bs} both={both}")
+    say(f"tables in place S={S} rows={rows} bs={bs} scarce={scarce} both={both}")
     rng = np.random.default_rng(S + rows)
-    mb, nb = 6, 3 * S
+    mb, nb = 6, S // 2 + 2 if scarce else 3 * S
     pool = K.BlockPool.of_blocks(nb)
     ring, head, count = np.arange(1, nb, dtype=np.int32), 0, nb - 1
     table = np.zeros((S, mb), np.int32)
@@ -62,7 +63,7 @@ def test_lengths_in_place(S, rows, bs, both):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         K.build_batch_tables(work)
-    h_past = np.zeros(S, np.int64)
+    h_past, refused = np.zeros(S, np.int64), 0
     for step in range(12):
         h_new = np.where(rng.random(S) < 0.5, 1, 0) if step % 3 else rng.integers(-1, 3, S)
         new.copy_(dev(torch, h_new.astype(np.int32)))
@@ -75,4 +76,5 @@ def test_lengths_in_place(S, rows, bs, both):
         assert np.array_equal(d_table.cpu().numpy(), table) and np.array_equal(pool.ring.cpu().numpy(), ring), step
         assert pool.state.tolist() == [head, count, 0]
         h_past = want["ctx_len"].astype(np.int64)
-    assert h_past.max() > 3
+        refused += int(want["counts"][3])
+    assert h_past.max() > 3 and (refused > 0 or not scarce)
