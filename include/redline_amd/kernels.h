@@ -272,5 +272,45 @@ inline void build_batch_tables(const BlockPool& pool, const BatchTables& tables,
   detail::check(rlk_build_batch_tables(&pool, &tables, stream));
 }
 
+// ---- extensions: normed heads and several position axes in the cache write, rows
+// read back, decode attention over shared prefixes, sampling; contracts in rlk.h.
+using NormRopeOptions = rlk_norm_rope_options;
+using SharedPrefixWork = rlk_shared_prefix_work;
+using SamplingWork = rlk_sampling_work;
+
+// rope_and_write_kv with RMS-normed q and k heads and up to four position axes.
+inline void rope_and_write_kv_norm(half* qkv, const int32_t* positions, const int32_t* slot_mapping,
+                                   int num_tokens, int num_heads, const float* cos_table,
+                                   const float* sin_table, const KVLayerView& kv,
+                                   const NormRopeOptions& options, hipStream_t stream) {
+  detail::check(rlk_rope_and_write_kv_norm(detail::bits(qkv), positions, slot_mapping, num_tokens,
+                                           num_heads, cos_table, sin_table,
+                                           reinterpret_cast<const rlk_kv_layer_view*>(&kv), &options,
+                                           stream));
+}
+
+// Stored rows of a cache as fp16 (either output may be null).
+inline void read_kv(const KVLayerView& kv, const int32_t* slots, int n, half* k_out, half* v_out,
+                    int scale_dtype, hipStream_t stream) {
+  detail::check(rlk_read_kv(reinterpret_cast<const rlk_kv_layer_view*>(&kv), slots, n,
+                            detail::bits(k_out), detail::bits(v_out), scale_dtype, stream));
+}
+
+// Decode attention for groups of items that share their first tokens.
+inline void paged_attention_decode_shared(const AttentionParams& p, const SharedPrefixWork& w,
+                                          int scale_dtype, hipStream_t stream) {
+  const rlk_attention_options options = {scale_dtype};
+  detail::check(rlk_paged_attention_decode_shared(reinterpret_cast<const rlk_attention_params*>(&p),
+                                                  &w, &options, stream));
+}
+
+// The next token of each row of logits.
+inline size_t sampling_workspace_bytes(int max_rows, int max_vocab) {
+  return rlk_sampling_workspace_bytes(max_rows, max_vocab);
+}
+inline void sample_tokens(const SamplingWork& work, hipStream_t stream) {
+  detail::check(rlk_sample_tokens(&work, stream));
+}
+
 }  // namespace kernels
 }  // namespace redline

@@ -478,6 +478,132 @@ typedef struct rlk_batch_tables {
 int rlk_build_batch_tables(const rlk_block_pool* pool, const rlk_batch_tables* tables,
                            hipStream_t stream);
 
+/* ------------------------------- normed heads, several axes, rows read back
+ *
+ * Extension, no counterpart in the reference: rlk_rope_and_write_kv_ex with an
+ * RMS norm of each query and key head before the rotation, and a rotation by
+ * several position axes (time, height, width, ...).  Of a head's elements x
+ * (bias added, fp16):
+ *   n_i = x_i / sqrt(mean(x^2) + eps) * w_i,  w = q_norm for query heads, k_norm
+ *         for key heads; NULL: n = x
+ *   rotated by the cos/sin rows of the positions that each pair's axis has
+ * in fp32, rounded to fp16 once.  v heads, the write, INT8 codes and scales are
+ * those of rlk_rope_and_write_kv_ex. */
+#define RLK_ROPE_MAX_AXES 4
+
+typedef struct rlk_norm_rope_options {
+  const uint16_t* q_norm;   /* fp16 [D] or NULL */
+  const uint16_t* k_norm;   /* fp16 [D] or NULL */
+  float eps;                /* of both norms, >= 0 */
+  const uint16_t* qkv_bias; /* as in rlk_rope_kv_options */
+  int scale_dtype;          /* RLK_SCALE_F32 | RLK_SCALE_F16 */
+  int num_axes;             /* 0 or 1: positions [num_tokens]; up to RLK_ROPE_MAX_AXES:
+                               positions [num_axes, num_tokens] */
+  int sections[RLK_ROPE_MAX_AXES]; /* pairs of each axis, D/2 in all (num_axes > 1) */
+  int interleaved;          /* 0: the first sections[0] pairs have axis 0, the next axis 1,
+                               ...; else pair i has axis i % num_axes as long as that axis
+                               has had fewer than its pairs, otherwise axis 0 */
+} rlk_norm_rope_options;
+
+/* NULL options: no norm, one axis; the bits of rlk_rope_and_write_kv_ex.  num_tokens <= 0: no-op.  head_dim not in
+ * {64, 128}: RLK_EUNSUPPORTED.  qkv, tables, bias, norm weights and cache planes
+ * 16-byte aligned, else RLK_EINVAL.  Rows whose slot is negative get their
+ * rotated q and write no cell. */
+int rlk_rope_and_write_kv_norm(uint16_t* qkv, const int32_t* positions, const int32_t* slot_mapping,
+                               int num_tokens, int num_heads, const float* cos_table,
+                               const float* sin_table, const rlk_kv_layer_view* kv,
+                               const rlk_norm_rope_options* options, hipStream_t stream);
+
+/* Extension: the stored rows of `slots` as fp16: k_out[i] / v_out[i]
+ * [n, num_kv_heads * head_dim] (either may be NULL) = the fp16 cells, or
+ * fp16(code * scale).  A negative slot leaves its rows as they were; other slots
+ * must lie in the cache.  scale_dtype as the cache was written.  n <= 0: no-op.
+ * Outputs and cache planes 16-byte aligned, else RLK_EINVAL. */
+int rlk_read_kv(const rlk_kv_layer_view* kv, const int32_t* slots, int n, uint16_t* k_out, uint16_t* v_out,
+                int scale_dtype, hipStream_t stream);
+
+/* ------------------------------------- decode attention over a shared prefix
+ *
+ * Extension, no counterpart in the reference: rlk_paged_attention_decode for
+ * items whose sequences share their first tokens in the cache (continuations of
+ * one prompt, a common system prompt): a group's prefix is read once for all its
+ * items.  Items of a group stand next to each other: group g has the items
+ * group_start[g] .. group_start[g + 1] - 1; an item outside every group, or past
+ * the first max_group_items of its group, attends to its own keys alone.  Item i
+ * attends to positions [0, positions[t]] of its sequence; those below
+ * group_prefix[g] are read through the table row of the group's FIRST item
+ * (item_seq[group_start[g]], whose own token may be negative), the rest through its own.
+ * Where an item ends inside its group's prefix, the values after its last key
+ * must be finite.
+ * A negative token skips its item (its rows of out are not known); an item whose
+ * position is negative gets zeros. */
+typedef struct rlk_shared_prefix_work {
+  const int32_t* item_token;   /* [num_items] query token of each item */
+  const int32_t* item_seq;     /* [num_items] its sequence (row of block_tables) */
+  int num_items;
+  const int32_t* group_start;  /* [num_groups + 1], not falling */
+  const int32_t* group_prefix; /* [num_groups] shared tokens; <= 0: none */
+  int num_groups;              /* 0: no groups */
+  int max_group_items;         /* items of the largest group */
+  int max_prefix_partitions;   /* >= ceil(prefix / 256) of every group; what a prefix has beyond
+                                  them, an item reads for itself */
+  int max_partitions;          /* >= ceil(keys / 256) of the keys that an item reads for itself;
+                                  keys past them are not read */
+  float* ws_out; /* [num_items, num_heads, max_prefix_partitions + max_partitions, head_dim] */
+  float* ws_max; /* [num_items, num_heads, max_prefix_partitions + max_partitions] */
+  float* ws_sum;
+} rlk_shared_prefix_work;
+
+/* options: RLK_SCALE_F32 or RLK_SCALE_F16 of an INT8 cache; NULL: RLK_SCALE_F32.
+ * Keys past the sequence's table row are not read.  INT8 values enter the sums as
+ * fp16(code * scale), as in prefill attention; a key's probability is rounded to
+ * fp16, all else is held in fp32.  num_items <= 0: no-op.  head_dim not in {64, 128}
+ * or more than 8 query heads a kv head: RLK_EUNSUPPORTED.  q and out rows and the
+ * cache planes 16-byte aligned, else RLK_EINVAL. */
+int rlk_paged_attention_decode_shared(const rlk_attention_params* params, const rlk_shared_prefix_work* work,
+                                      const rlk_attention_options* options, hipStream_t stream);
+
+/* ------------------------------------------------------------------- sampling
+ *
+ * Extension: the next token of each row of logits.  With the tokens in order of
+ * falling logit (ties: the lower index first), T the row's temperature and
+ * w_j = exp((l_j - l_max) / T):
+ *   kept   the first top_k tokens (<= 0: all); of those, a token as long as the
+ *          mass before it is below top_p times the mass of the first top_k (>= 1,
+ *          NaN: all); of those, the ones with w_j >= min_p; the first token always
+ *   drawn  the first kept token with w_0 + ... + w_j > u (w_0 + ... + w_last kept)
+ * T <= 0 or NaN: the first token.  min_p is held at 1 at most (NaN: 1).  u is held in [0, 1): below 0 and NaN as 0,
+ * 1 and above as the largest below.  NaN logits count as -infinity; tokens of
+ * -infinity are not drawn, but of a row that holds nothing else token 0 is.  Tokens
+ * of +infinity share the draw.  Weights are held to 2^-35 of themselves, and those
+ * below 2^-48 of the largest count as 0.  The same inputs give the same token,
+ * whatever else the call holds. */
+typedef struct rlk_sampling_work {
+  const void* logits;      /* [num_rows] rows of vocab, row_stride elements apart */
+  int logits_fp32;         /* 0: fp16, else fp32 */
+  int64_t row_stride;
+  int num_rows;
+  int vocab;
+  const int32_t* param_row;   /* [num_rows] row of the four arrays below; NULL: its own */
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;         /* NULL: 0 */
+  const float* uniform;       /* [num_rows] a random number of each row */
+  int32_t* tokens;            /* [num_rows] */
+  float* logprobs;            /* [num_rows] ln of the drawn token's share of the kept mass; or NULL */
+  void* workspace;            /* rlk_sampling_workspace_bytes, 256-byte aligned; what it holds
+                                 between calls does not matter */
+  size_t workspace_bytes;
+} rlk_sampling_work;
+
+/* Workspace of calls of up to max_rows rows of up to max_vocab tokens (0 for bad arguments). */
+size_t rlk_sampling_workspace_bytes(int max_rows, int max_vocab);
+
+/* num_rows <= 0: no-op.  vocab in 1 .. 2^20 (else RLK_EUNSUPPORTED), logits aligned to
+ * their elements; a workspace too small for the call: RLK_EINVAL. */
+int rlk_sample_tokens(const rlk_sampling_work* work, hipStream_t stream);
+
 /* ------------------------------------------------------ host-side helpers */
 
 /* IEEE fp16 <-> fp32 with round-to-nearest-even.

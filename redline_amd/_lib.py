@@ -30,6 +30,7 @@ class Error(RuntimeError):
 class KVLayerView(C.Structure):
     """Mirror of rlk_kv_layer_view / redline::KVLayerView (kernels.h:18-27)."""
 
+    device = tensors = scale_dtype = None  # of its planes, where kernels.kv_layer_view or KVCache made it
     _fields_ = [
         ("k", C.c_void_p),
         ("v", C.c_void_p),
@@ -64,6 +65,7 @@ RLK_GEMV_W4_MAX_M = 32
 class AttentionParams(C.Structure):
     """Mirror of rlk_attention_params / kernels::AttentionParams (kernels.h:91-101)."""
 
+    device = tensors = None  # where kernels.attention_params made it
     _fields_ = [("q", C.c_void_p), ("q_stride", C.c_int), ("out", C.c_void_p),
                 ("num_heads", C.c_int), ("scale", C.c_float), ("kv", KVLayerView),
                 ("block_tables", C.c_void_p), ("max_blocks_per_seq", C.c_int),
@@ -128,6 +130,38 @@ class BatchTables(C.Structure):
                     "decode_seq", "prefill_seq", "counts")]
 
 
+RLK_ROPE_MAX_AXES = 4
+
+
+class NormRopeOptions(C.Structure):
+    """Mirror of rlk_norm_rope_options."""
+
+    _fields_ = [("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("eps", C.c_float),
+                ("qkv_bias", C.c_void_p), ("scale_dtype", C.c_int), ("num_axes", C.c_int),
+                ("sections", C.c_int * RLK_ROPE_MAX_AXES), ("interleaved", C.c_int)]
+
+
+class SharedPrefixWork(C.Structure):
+    """Mirror of rlk_shared_prefix_work."""
+
+    device = tensors = room = None  # as DecodeAttentionWork, where kernels.shared_prefix_work made it
+    _fields_ = [("item_token", C.c_void_p), ("item_seq", C.c_void_p), ("num_items", C.c_int),
+                ("group_start", C.c_void_p), ("group_prefix", C.c_void_p), ("num_groups", C.c_int),
+                ("max_group_items", C.c_int), ("max_prefix_partitions", C.c_int),
+                ("max_partitions", C.c_int), ("ws_out", C.c_void_p), ("ws_max", C.c_void_p),
+                ("ws_sum", C.c_void_p)]
+
+
+class SamplingWork(C.Structure):
+    """Mirror of rlk_sampling_work."""
+
+    device = tensors = None
+    _fields_ = [("logits", C.c_void_p), ("logits_fp32", C.c_int), ("row_stride", C.c_int64),
+                ("num_rows", C.c_int), ("vocab", C.c_int)] + [(n, C.c_void_p) for n in (
+                    "param_row", "temperature", "top_k", "top_p", "min_p", "uniform", "tokens",
+                    "logprobs", "workspace")] + [("workspace_bytes", C.c_size_t)]
+
+
 class BatchShape(C.Structure):
     _fields_ = [(n, C.c_int) for n in (
         "num_tokens", "num_seqs", "num_logit_rows", "num_decode_items",
@@ -181,6 +215,14 @@ _SIGNATURES = {
     "rlk_paged_attention_prefill_blocks": (_I, [C.POINTER(BlockAttentionParams),
                                                 C.POINTER(PrefillAttentionWork), _P]),
     "rlk_build_batch_tables": (_I, [C.POINTER(BlockPoolView), C.POINTER(BatchTables), _P]),
+    "rlk_rope_and_write_kv_norm": (_I, [_P, _P, _P, _I, _I, _P, _P, C.POINTER(KVLayerView),
+                                        C.POINTER(NormRopeOptions), _P]),
+    "rlk_read_kv": (_I, [C.POINTER(KVLayerView), _P, _I, _P, _P, _I, _P]),
+    "rlk_paged_attention_decode_shared": (_I, [C.POINTER(AttentionParams),
+                                               C.POINTER(SharedPrefixWork),
+                                               C.POINTER(AttentionOptions), _P]),
+    "rlk_sampling_workspace_bytes": (C.c_size_t, [_I, _I]),
+    "rlk_sample_tokens": (_I, [C.POINTER(SamplingWork), _P]),
     "rlk_gemv_w8a16": (_I, [_P, _I, _P, _P, _P, _I, _I, _P, _I, _P]),
     "rlk_gemv_w4a16": (_I, [_P, _I, _P, _P, _P, _I, _P, _I, _I, _P, _I, _P]),
     "rlk_gemv_w4a16_swiglu": (_I, [_P, _I, _P, _P, _P, _I, _I, _I, _P, _P]),

@@ -22,6 +22,7 @@ ARCH = "gfx950"
 
 SOURCES = ["elementwise.hip", "rope_kv.hip", "attention.hip", "prefill.hip", "gemv_w4.hip", "gemv_stream.hip",
            "kv_blocks.hip", "attention_blocks.hip", "prefill_blocks.hip", "batch_tables.hip",
+           "rope_norm.hip", "attention_shared.hip", "sampling.hip",
            "host.cpp",
            "status.cpp"]
 

@@ -1,0 +1,464 @@
+// Paged decode attention for groups of items that share a prefix, for gfx950.
+//
+// Flash-decoding: o = sum_k p_k v_k / sum_k p_k, p_k = exp(scale q.k - m), with the
+// keys in two parts that are joined by the rule of the running maximum:
+//   prefix  a unit is (group, kv head, 128 rows, range of keys), a row being one
+//           (item, query head of the kv head) pair: every K and V byte of the range is
+//           read once for all rows;
+//   suffix  a unit is (item, kv head, range of keys) with the item's G rows.
+// Both run the same loop in one launch; a second kernel joins a row's partials
+// (o, m, l in fp32) through the caller's workspace.
+//
+// The loop: tiles of 64 keys go through registers into two LDS stages (INT8 codes
+// become fp16 on the way), the next tile's loads in flight while the current one is
+// used.  A wave owns 32 rows:
+//   S^T = K Q^T    v_mfma_f32_32x32x16_f16, K rows from LDS, q in registers: a lane
+//                  gets one row (its column) and 32 of the tile's 64 keys, so the
+//                  softmax is per lane with one exchange between the lane halves;
+//   O^T = V^T P^T  the probabilities a lane holds are its B operand, the keys taken in
+//                  the order in which S^T hands them over; V^T by transposing LDS reads.
+// LDS chunks of 16 bytes are XOR-ed with the row so that neither read has bank conflicts.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <cstdint>
+
+#include "device.hpp"
+#include "redline_amd/rlk.h"
+#include "status.hpp"
+
+namespace rlk {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256;
+constexpr int kTile = 64;               // keys
+constexpr int kWaveRows = 32;
+constexpr int kRows = kThreads / kWave * kWaveRows;  // of a workgroup
+constexpr int kPart = RLK_DECODE_PARTITION_SIZE;
+constexpr int64_t kMaxBlocks = 1 << 30;
+constexpr float kLog2e = 1.4426950408889634f;
+
+enum Format { kF16, kI8, kI8Half };  // FP16 cells; INT8 with fp32, with fp16 scales
+
+struct SharedArgs {
+  rlk_attention_params p;
+  rlk_shared_prefix_work w;
+  int grp;                 // query heads of a kv head
+  int prefix_keys, suffix_keys;      // keys of a unit, whole tiles
+  int prefix_splits, suffix_splits;  // units of the longest prefix, of the longest rest
+  int row_tiles;
+  int64_t prefix_blocks;
+};
+
+// Keys that an item attends to, those inside its table row.
+__device__ __forceinline__ int keys_of(const SharedArgs& a, int token) {
+  const int64_t most = static_cast<int64_t>(a.p.max_blocks_per_seq) * a.p.kv.block_size;
+  return static_cast<int>(max(min(static_cast<int64_t>(a.p.positions[token]) + 1, most), static_cast<int64_t>(0)));
+}
+// The part of group g's prefix that its units read.
+__device__ __forceinline__ int prefix_of(const SharedArgs& a, int g) {
+  const int64_t most = min(static_cast<int64_t>(a.p.max_blocks_per_seq) * a.p.kv.block_size,
+                           static_cast<int64_t>(a.w.max_prefix_partitions) * kPart);
+  return static_cast<int>(max(min(static_cast<int64_t>(a.w.group_prefix[g]), most), static_cast<int64_t>(0)));
+}
+// The prefix that an item shares, 0 outside the groups; by a whole wave.
+__device__ __forceinline__ int shared_prefix(const SharedArgs& a, int item) {
+  const int lane = threadIdx.x % kWave;
+  int g = -1;  // the last group that starts at or before the item
+  for (int g0 = 0; g0 < a.w.num_groups; g0 += kWave) {
+    const bool before = g0 + lane < a.w.num_groups && a.w.group_start[min(g0 + lane, a.w.num_groups - 1)] <= item;
+    const uint64_t b = __ballot(before);
+    g += __popcll(b);
+    if (b != ~0ull) break;
+  }
+  if (g < 0) return 0;
+  const int first = a.w.group_start[g];
+  if (first < 0 || item >= a.w.group_start[g + 1] || item - first >= a.w.max_group_items) return 0;
+  return prefix_of(a, g);
+}
+
+__device__ __forceinline__ int64_t slot_row(const SharedArgs& a, int item, int head) {
+  return (static_cast<int64_t>(item) * a.p.num_heads + head) * (a.w.max_prefix_partitions + a.w.max_partitions);
+}
+
+// LDS image of a tile row: 16-byte chunk c of row r stands at chunk c ^ swizzle(r).
+template <int D>
+__device__ __forceinline__ int k_swizzle(int r) { return D == 128 ? r & 15 : (r >> 1) & 7; }
+template <int D>
+__device__ __forceinline__ int v_swizzle(int r) { return D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; }
+
+template <int D, int kFmt>
+__global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArgs a) {
+  constexpr bool kInt8 = kFmt != kF16;
+  constexpr int kPitch = 2 * D, kQ = D / 16, kO = D / 32;
+  constexpr int kChunks = D / (kInt8 ? 16 : 8);             // loads of a row
+  constexpr int kItems = kTile * kChunks / kThreads;        // loads of a thread and tile, of K and of V
+  constexpr int kRowStep = kThreads / kChunks;              // rows between them
+  struct Lds {
+    unsigned char k[2][kTile * kPitch], v[2][kTile * kPitch];
+    float ks[2][kTile];
+  };
+  __shared__ alignas(1024) Lds lds;
+  const rlk_attention_params& p = a.p;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int col = lane % 32, half = lane / 32;
+  const int hkv = p.kv.num_kv_heads, bs = p.kv.block_size, G = a.grp;
+
+  // the unit
+  int kvh, first, rows, row0, begin, end, slot, seq;
+  if (blockIdx.x < a.prefix_blocks) {
+    // the row tiles of a range stand 8 blocks apart: on one XCD, whose L2 has the range
+    const int b = blockIdx.x, rt = b / 8 % a.row_tiles, u = b / 8 / a.row_tiles * 8 + b % 8;
+    const int split = u % a.prefix_splits, gk = u / a.prefix_splits, g = gk / hkv;
+    kvh = gk - g * hkv;
+    if (g >= a.w.num_groups) return;
+    first = a.w.group_start[g];
+    const int n = min(min(a.w.group_start[g + 1], a.w.num_items) - first, a.w.max_group_items);
+    rows = n * G;
+    row0 = rt * kRows;
+    if (first < 0 || rows <= row0) return;
+    begin = split * a.prefix_keys;
+    end = min(prefix_of(a, g), begin + a.prefix_keys);
+    slot = split;
+    seq = a.w.item_seq[first];
+  } else {
+    const int u = static_cast<int>(blockIdx.x - a.prefix_blocks);
+    const int split = u % a.suffix_splits, ik = u / a.suffix_splits;
+    first = ik / hkv;
+    kvh = ik - first * hkv;
+    const int token = a.w.item_token[first];
+    if (token < 0) return;
+    rows = G;
+    row0 = 0;
+    const int prefix = shared_prefix(a, first);
+    const int64_t keys = min(static_cast<int64_t>(keys_of(a, token)),
+                             prefix + static_cast<int64_t>(a.w.max_partitions) * kPart);
+    const int64_t at = prefix + static_cast<int64_t>(split) * a.suffix_keys;
+    if (at >= keys) return;
+    begin = static_cast<int>(at);
+    end = static_cast<int>(min(keys, at + a.suffix_keys));
+    slot = a.w.max_prefix_partitions + split;
+    seq = a.w.item_seq[first];
+  }
+  if (begin >= end) return;
+
+  // the lane's row
+  const bool busy = row0 + wave * kWaveRows < rows;  // the wave has rows
+  const int r = row0 + wave * kWaveRows + col, item = first + r / G, head = kvh * G + r % G;
+  const int token = r < rows ? a.w.item_token[item] : -1;
+  int last = end;  // keys of the row, up to this one
+  f16x8 q[kQ];
+#pragma unroll
+  for (int s = 0; s < kQ; ++s) q[s] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+  if (token >= 0) {
+    last = min(end, keys_of(a, token));
+    const _Float16* qp = reinterpret_cast<const _Float16*>(p.q) + static_cast<int64_t>(token) * p.q_stride + head * D + 8 * half;
+#pragma unroll
+    for (int s = 0; s < kQ; ++s) q[s] = __builtin_bit_cast(f16x8, load16(qp + 16 * s));
+  }
+  int whole = last;  // every row of the wave has the keys up to this one
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) whole = min(whole, __shfl_xor(whole, o, kWave));
+
+  // this thread's part of a tile
+  const int ch = tid % kChunks, tr = tid / kChunks;
+  const int32_t* table = p.block_tables + static_cast<int64_t>(seq) * p.max_blocks_per_seq;
+  const int lbs = (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1;
+  u32x4 kraw[kItems], vraw[kItems];
+  float ksc[kItems], vsc[kItems];
+  int id[kItems], off[kItems];
+  auto find = [&](int k0) {
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) {
+      const int pos = min(k0 + tr + u * kRowStep, end - 1);
+      const int b = lbs >= 0 ? pos >> lbs : pos / bs;
+      off[u] = pos - b * bs;
+      id[u] = table[b];
+    }
+  };
+  auto request = [&]() {
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) {
+      const int64_t cell = (static_cast<int64_t>(id[u]) * hkv + kvh) * bs + off[u];
+      const int64_t at = cell * (kInt8 ? D : 2 * D) + ch * 16;
+      kraw[u] = load16(static_cast<const unsigned char*>(p.kv.k) + at);
+      vraw[u] = load16(static_cast<const unsigned char*>(p.kv.v) + at);
+      if constexpr (kFmt == kI8) {
+        ksc[u] = p.kv.k_scale[cell];
+        vsc[u] = p.kv.v_scale[cell];
+      } else if constexpr (kFmt == kI8Half) {
+        ksc[u] = static_cast<float>(reinterpret_cast<const _Float16*>(p.kv.k_scale)[cell]);
+        vsc[u] = static_cast<float>(reinterpret_cast<const _Float16*>(p.kv.v_scale)[cell]);
+      }
+    }
+  };
+  auto put = [&](int k0, int buf) {
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) {
+      const int row = tr + u * kRowStep;
+      // rows past the range hold its last key; their V is cleared, since 0 times an infinity is no 0
+      const bool in = k0 + row < end;
+      unsigned char* kd = lds.k[buf] + row * kPitch;
+      unsigned char* vd = lds.v[buf] + row * kPitch;
+      const u32x4 vr = in ? vraw[u] : u32x4{0, 0, 0, 0};
+      if constexpr (!kInt8) {
+        store16(kd + ((ch ^ k_swizzle<D>(row)) << 4), kraw[u]);
+        store16(vd + ((ch ^ v_swizzle<D>(row)) << 4), vr);
+      } else {
+        const float vs = in ? vsc[u] : 0.f;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const u32x2 kc = {kraw[u][2 * x], kraw[u][2 * x + 1]}, vc = {vr[2 * x], vr[2 * x + 1]};
+          const f32x8 vf = __builtin_convertvector(__builtin_bit_cast(i8x8, vc), f32x8) * vs;
+          store16(kd + (((2 * ch + x) ^ k_swizzle<D>(row)) << 4), __builtin_bit_cast(u32x4, int8x8_to_f16(kc)));
+          store16(vd + (((2 * ch + x) ^ v_swizzle<D>(row)) << 4), pack8(vf));
+        }
+        if (ch == 0) lds.ks[buf][row] = ksc[u];
+      }
+    }
+  };
+
+  const float c = p.scale * kLog2e;
+  f32x16 o[kO];
+#pragma unroll
+  for (int d = 0; d < kO; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+  float m = -FLT_MAX, l = 0.f;
+  // V^T reads: lane (g, tk, tm) of 16 lanes takes 4 dims of key 4 half + tk
+  const int tk = lane % 16 / 4, tm = lane % 4;
+  const int vrow = (4 * half + tk) * kPitch, vsw = v_swizzle<D>(tk);
+  int vat[kO];
+#pragma unroll
+  for (int d = 0; d < kO; ++d)
+    vat[d] = vrow + (((4 * d + 2 * (lane / 16 % 2) + tm / 2) ^ vsw) << 4) + (tm & 1) * 8;
+
+  auto attend = [&](int k0, int buf) {
+    f32x16 s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
+      const unsigned char* kr = lds.k[buf] + (32 * t + col) * kPitch;
+#pragma unroll
+      for (int x = 0; x < kQ; ++x) {
+        const f16x8 kf = *reinterpret_cast<const f16x8*>(kr + (((2 * x + half) ^ k_swizzle<D>(col)) << 4));
+        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[x], s[t], 0, 0, 0);
+      }
+    }
+    // element i of subtile t: key k0 + 32 t + 8 (i / 4) + 4 half + i % 4
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        f32x4 f = {c, c, c, c};
+        if constexpr (kInt8) f *= *reinterpret_cast<const f32x4*>(&lds.ks[buf][32 * t + 8 * b + 4 * half]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[t][4 * b + i] *= f[i];
+      }
+    if (k0 + kTile > whole) {
+      const int left = last - k0 - 4 * half;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (32 * t + 8 * (i / 4) + i % 4 >= left) s[t][i] = -INFINITY;
+    }
+    float mx = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
+    mx = rows_max<true>(mx);
+    // m is a reference within 2^8 of the maximum: moving it costs a pass over the
+    // output, and probabilities up to 2^8 have the same 11 bits in fp16
+    if (__any(mx > m + 8.f)) {
+      const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - mn);
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < kO; ++d) o[d] *= f;
+      m = mn;
+    }
+    f16x8 pb[2][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float e = __builtin_amdgcn_exp2f(s[t][i] - m);
+        l += e;
+        pb[t][i / 8][i % 8] = static_cast<_Float16>(e);
+      }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        unsigned char* vt = lds.v[buf] + (32 * t + 16 * x) * kPitch;
+#pragma unroll
+        for (int d = 0; d < kO; ++d) {
+          typedef __attribute__((address_space(3))) s16x4* LdsPtr;
+          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(vt + vat[d]));
+          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(vt + vat[d] + 8 * kPitch));
+          const f16x8 vf = __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pb[t][x], o[d], 0, 0, 0);
+        }
+      }
+  };
+
+  find(begin);
+  request();
+  find(begin + kTile);
+  int buf = 0;
+  for (int k0 = begin; k0 < end; k0 += kTile) {
+    put(k0, buf);
+    if (k0 + kTile < end) {
+      request();
+      find(k0 + 2 * kTile);
+    }
+    __syncthreads();  // the stage before this one was last read before the barrier of the step before
+    if (busy) attend(k0, buf);
+    buf ^= 1;
+  }
+  if (token < 0) return;
+  l += __shfl_xor(l, 32, kWave);
+  const int64_t at = slot_row(a, item, head) + slot;
+  float* dst = a.w.ws_out + at * D + 4 * half;
+#pragma unroll
+  for (int d = 0; d < kO; ++d)
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      *reinterpret_cast<f32x4*>(dst + 32 * d + 8 * b) = f32x4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]};
+  if (half == 0) {
+    a.w.ws_max[at] = m;
+    a.w.ws_sum[at] = l;
+  }
+}
+
+// Joins the partials of one (item, head): lane d of the workgroup takes dim d; each
+// wave holds the weights of 64 slots, one a lane.
+template <int D>
+__global__ __launch_bounds__(D) void shared_merge_kernel(SharedArgs a) {
+  constexpr int kUnroll = 8;
+  const int item = blockIdx.x, head = blockIdx.y, d = threadIdx.x, lane = d % kWave;
+  const int token = a.w.item_token[item];
+  if (token < 0) return;
+  const int keys = keys_of(a, token), prefix = shared_prefix(a, item);
+  const int np = (prefix + a.prefix_keys - 1) / max(a.prefix_keys, 1);
+  const int rest = min(max(keys - prefix, 0), a.w.max_partitions * kPart);
+  const int slots = np + (rest + a.suffix_keys - 1) / a.suffix_keys;
+  const int64_t row = slot_row(a, item, head);
+  auto slot_of = [&](int j) { return row + (j < np ? j : a.w.max_prefix_partitions + j - np); };
+  float M = -FLT_MAX, L = 0.f, o = 0.f;
+  for (int j0 = 0; j0 < slots; j0 += kWave) {
+    const int here = min(slots - j0, kWave);
+    const int64_t mine = slot_of(min(j0 + lane, slots - 1));
+    const float ms = lane < here ? a.w.ws_max[mine] : -FLT_MAX, ls = lane < here ? a.w.ws_sum[mine] : 0.f;
+    const float mn = fmaxf(M, rows_max<true>(rows_max<false>(group_max<16>(ms))));
+    const float f0 = __builtin_amdgcn_exp2f(M - mn), f = __builtin_amdgcn_exp2f(ms - mn);
+    L = L * f0 + wave_sum(f * ls);
+    o *= f0;
+    M = mn;
+    for (int s = 0; s < here; s += kUnroll) {
+      float v[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) v[u] = a.w.ws_out[slot_of(j0 + min(s + u, here - 1)) * D + d];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (s + u < here) o += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s + u)) * v[u];
+    }
+  }
+  reinterpret_cast<_Float16*>(a.p.out)[(static_cast<int64_t>(token) * a.p.num_heads + head) * D + d] =
+      static_cast<_Float16>(keys > 0 ? o / L : 0.f);
+}
+
+template <int D, int kFmt>
+int launch(SharedArgs a, const char* what, hipStream_t stream) {
+  const int64_t cus = compute_units(), hkv = a.p.kv.num_kv_heads;
+  const int pp = a.w.num_groups > 0 && a.w.max_group_items > 0 ? a.w.max_prefix_partitions : 0;
+  // ranges that give every CU two workgroups, of at least 256 keys (a workspace slot each)
+  auto keys_of_unit = [&](int partitions, int64_t units) {
+    const int64_t keys = static_cast<int64_t>(partitions) * kPart, want = std::max<int64_t>(1, (2 * cus + units - 1) / units);
+    return static_cast<int>(std::max<int64_t>((keys + want - 1) / want + kTile - 1, kPart) / kTile * kTile);
+  };
+  a.row_tiles = (std::min(a.w.max_group_items, a.w.num_items) * a.grp + kRows - 1) / kRows;
+  int64_t blocks = 0;
+  if (pp > 0) {
+    const int64_t tiles = std::min<int64_t>(static_cast<int64_t>(a.w.num_groups) * a.row_tiles,
+                                            static_cast<int64_t>(a.w.num_items) * a.grp / kRows + a.w.num_groups);
+    a.prefix_keys = keys_of_unit(pp, tiles * hkv);
+    a.prefix_splits = (pp * kPart + a.prefix_keys - 1) / a.prefix_keys;
+    const int64_t ranges = a.w.num_groups * hkv * a.prefix_splits;
+    if (ranges > kMaxBlocks) return fail(RLK_EINVAL, "%s: %d groups exceed one launch; split the call", what, a.w.num_groups);
+    blocks = (ranges + 7) / 8 * 8 * a.row_tiles;
+  } else {
+    a.prefix_keys = kPart;
+    a.w.num_groups = 0;
+  }
+  a.prefix_blocks = blocks;
+  a.suffix_keys = keys_of_unit(a.w.max_partitions, a.w.num_items * hkv);
+  a.suffix_splits = (a.w.max_partitions * kPart + a.suffix_keys - 1) / a.suffix_keys;
+  blocks += static_cast<int64_t>(a.w.num_items) * hkv * a.suffix_splits;
+  if (blocks > kMaxBlocks) return fail(RLK_EINVAL, "%s: %d items exceed one launch; split the call", what, a.w.num_items);
+  shared_attention_kernel<D, kFmt><<<static_cast<uint32_t>(blocks), kThreads, 0, stream>>>(a);
+  shared_merge_kernel<D><<<dim3(a.w.num_items, a.p.num_heads), D, 0, stream>>>(a);
+  return launch_status(what);
+}
+
+}  // namespace
+}  // namespace rlk
+
+using namespace rlk;
+
+extern "C" int rlk_paged_attention_decode_shared(const rlk_attention_params* p, const rlk_shared_prefix_work* w,
+                                                 const rlk_attention_options* options, hipStream_t stream) {
+  const char* what = "paged_attention_decode_shared";
+  if (p == nullptr || w == nullptr) return fail(RLK_EINVAL, "%s: null params or work", what);
+  if (w->num_items <= 0) return RLK_OK;
+  const int scale_dtype = options != nullptr ? options->scale_dtype : RLK_SCALE_F32;
+  const rlk_kv_layer_view& kv = p->kv;
+  if (scale_dtype != RLK_SCALE_F32 && scale_dtype != RLK_SCALE_F16)
+    return fail(RLK_EINVAL, "%s: unknown scale dtype %d", what, scale_dtype);
+  if (kv.head_dim != 64 && kv.head_dim != 128)
+    return fail(RLK_EUNSUPPORTED, "%s: unsupported head_dim %d (supported: 64, 128)", what, kv.head_dim);
+  if (kv.dtype != RLK_KV_FP16 && kv.dtype != RLK_KV_INT8)
+    return fail(RLK_EINVAL, "%s: unknown KV dtype %d", what, kv.dtype);
+  if (kv.num_kv_heads <= 0 || kv.block_size <= 0)
+    return fail(RLK_EINVAL, "%s: bad kv head count %d or block size %d", what, kv.num_kv_heads, kv.block_size);
+  if (p->num_heads <= 0 || p->num_heads % kv.num_kv_heads != 0)
+    return fail(RLK_EINVAL, "%s: num_heads must be a multiple of num_kv_heads (%d, %d)", what, p->num_heads, kv.num_kv_heads);
+  const int G = p->num_heads / kv.num_kv_heads;
+  if (G > 8) return fail(RLK_EUNSUPPORTED, "%s: unsupported GQA group size %d", what, G);
+  if (p->max_blocks_per_seq <= 0 || static_cast<int64_t>(p->max_blocks_per_seq) * kv.block_size > (1 << 30))
+    return fail(RLK_EINVAL, "%s: bad table width %d", what, p->max_blocks_per_seq);
+  if (w->num_groups < 0 || w->max_group_items < 0)
+    return fail(RLK_EINVAL, "%s: bad group counts (%d, %d)", what, w->num_groups, w->max_group_items);
+  if (w->max_partitions < 1 || w->max_prefix_partitions < 0 || w->max_partitions > (1 << 20) ||
+      w->max_prefix_partitions > (1 << 20))
+    return fail(RLK_EINVAL, "%s: bad partition counts (%d, %d)", what, w->max_prefix_partitions, w->max_partitions);
+  if (p->num_heads > 65535 || w->num_items > (1 << 20) || w->num_groups > (1 << 20))
+    return fail(RLK_EINVAL, "%s: %d items in %d groups exceed one launch; split the call", what, w->num_items, w->num_groups);
+  if (p->q == nullptr || p->out == nullptr || p->block_tables == nullptr || p->positions == nullptr ||
+      kv.k == nullptr || kv.v == nullptr || (kv.dtype == RLK_KV_INT8 && (kv.k_scale == nullptr || kv.v_scale == nullptr)) ||
+      w->item_token == nullptr || w->item_seq == nullptr ||
+      (w->num_groups > 0 && (w->group_start == nullptr || w->group_prefix == nullptr)))
+    return fail(RLK_EINVAL, "%s: null pointer argument", what);
+  if (w->ws_out == nullptr || w->ws_max == nullptr || w->ws_sum == nullptr)
+    return fail(RLK_EINVAL, "%s: the workspace is required", what);
+  if (p->q_stride % 8 != 0 || ((reinterpret_cast<uintptr_t>(p->q) | reinterpret_cast<uintptr_t>(p->out) |
+                                reinterpret_cast<uintptr_t>(kv.k) | reinterpret_cast<uintptr_t>(kv.v) |
+                                reinterpret_cast<uintptr_t>(w->ws_out)) & 15) != 0)
+    return fail(RLK_EINVAL, "%s: q and out rows, cache planes and workspace must be 16-byte aligned (q_stride %d)", what,
+                p->q_stride);
+  SharedArgs a = {};
+  a.p = *p;
+  a.w = *w;
+  a.grp = G;
+  const int fmt = kv.dtype == RLK_KV_FP16 ? kF16 : (scale_dtype == RLK_SCALE_F16 ? kI8Half : kI8);
+  if (kv.head_dim == 128) {
+    if (fmt == kF16) return launch<128, kF16>(a, what, stream);
+    return fmt == kI8 ? launch<128, kI8>(a, what, stream) : launch<128, kI8Half>(a, what, stream);
+  }
+  if (fmt == kF16) return launch<64, kF16>(a, what, stream);
+  return fmt == kI8 ? launch<64, kI8>(a, what, stream) : launch<64, kI8Half>(a, what, stream);
+}

@@ -26,10 +26,13 @@ __all__ = [
     "kGemvW4MaxM", "KVBlockFormat", "KVBlockCache", "kv_block_view", "rope_and_write_kv_blocks",
     "read_kv_blocks", "block_attention_params", "paged_attention_decode_blocks",
     "paged_attention_prefill_blocks", "BlockPool", "batch_tables", "build_batch_tables",
+    "kRopeMaxAxes", "kv_layer_view", "rope_and_write_kv_norm", "read_kv", "shared_prefix_work",
+    "paged_attention_decode_shared", "SamplingWorkspace", "sampling_work", "sample_tokens",
 ]
 
 kDecodePartitionSize = _lib.RLK_DECODE_PARTITION_SIZE
 kGemvW4MaxM = _lib.RLK_GEMV_W4_MAX_M
+kRopeMaxAxes = _lib.RLK_ROPE_MAX_AXES
 
 SCALE_F32 = _lib.RLK_SCALE_F32
 SCALE_F16 = _lib.RLK_SCALE_F16
@@ -213,11 +216,14 @@ def rope_and_write_kv_ex(qkv, positions, slot_mapping, num_tokens, num_heads, co
 
 def attention_params(q, q_stride, out, num_heads, scale, kv: KVLayerView, block_tables,
                      max_blocks_per_seq, positions) -> _lib.AttentionParams:
-    """kernels::AttentionParams from torch tensors (q may be a view into qkv)."""
-    return _lib.AttentionParams(
+    """kernels::AttentionParams from torch tensors (q may be a view into qkv).
+    The struct keeps its tensors."""
+    params = _lib.AttentionParams(
         _ptr(q, torch.float16, "q"), q_stride, _ptr(out, torch.float16, "out"), num_heads,
         float(scale), kv, _ptr(block_tables, torch.int32, "block_tables"), max_blocks_per_seq,
         _ptr(positions, torch.int32, "positions"))
+    params.device, params.tensors = kv.device, (kv, q, out, block_tables, positions)
+    return params
 
 
 def decode_work(item_token, item_seq, num_items, max_partitions, workspace=None):
@@ -329,6 +335,8 @@ class KVCache:
             view = KVLayerView(k.data_ptr(), v.data_ptr(), ks.data_ptr() if ks is not None else None,
                                vs.data_ptr() if vs is not None else None, block_size, num_kv_heads,
                                head_dim, dtype)
+            view.device, view.tensors = self.storage.get_device(), (k, v, ks, vs)
+            view.scale_dtype = scale_dtype if dtype == KVDType.kINT8 else None
             self._views.append(view)
             self._tensors.append((k, v, ks, vs))
 
@@ -549,3 +557,161 @@ def build_batch_tables(tables, stream=None):
     its request lengths, with blocks from the pool; `tables` from batch_tables()."""
     pool, work = tables
     check(lib().rlk_build_batch_tables(C.byref(pool.view), C.byref(work), _stream_on(pool.device, stream)))
+
+
+# ------------------------- normed heads, several position axes, rows read back
+
+def kv_layer_view(k, v, k_scale=None, v_scale=None) -> KVLayerView:
+    """One layer of a paged cache from tensors of its own: k, v [num_blocks, Hkv,
+    block_size, D] fp16, or int8 with k_scale, v_scale [num_blocks, Hkv, block_size]
+    fp32 or fp16.  The view keeps its tensors."""
+    kp = _ptr(k, torch.int8 if k_scale is not None else torch.float16, "k")
+    vp = _ptr(v, k.dtype, "v")
+    if k.dim() != 4 or v.shape != k.shape:
+        raise _lib.Error(_lib.RLK_EINVAL, "k and v must have one shape [num_blocks, Hkv, block_size, D]")
+    _, hkv, bs, dim = k.shape
+    ksp = vsp = sd = None
+    if k_scale is not None:
+        sdt = torch.float16 if isinstance(k_scale, torch.Tensor) and k_scale.dtype == torch.float16 else torch.float32
+        sd = SCALE_F16 if sdt == torch.float16 else SCALE_F32
+        ksp, vsp = _ptr(k_scale, sdt, "k_scale"), _ptr(v_scale, sdt, "v_scale")
+        _need(k_scale, k.numel() // max(dim, 1), "k_scale"); _need(v_scale, k.numel() // max(dim, 1), "v_scale")
+    elif v_scale is not None:
+        raise _lib.Error(_lib.RLK_EINVAL, "v_scale without k_scale")
+    view = KVLayerView(kp, vp, ksp, vsp, bs, hkv, dim, KVDType.kFP16 if ksp is None else KVDType.kINT8)
+    view.device, view.tensors, view.scale_dtype = k.get_device(), (k, v, k_scale, v_scale), sd
+    _one_device(view.device, v, k_scale, v_scale)
+    return view
+
+
+def _scales(kv: KVLayerView, scale_dtype):
+    if kv.scale_dtype is not None and scale_dtype != kv.scale_dtype:
+        raise _lib.Error(_lib.RLK_EINVAL, f"scale dtype {scale_dtype}, the cache's scales have {kv.scale_dtype}")
+
+
+def rope_and_write_kv_norm(qkv, positions, slot_mapping, num_tokens, num_heads, cos_table, sin_table,
+                           kv: KVLayerView, q_norm=None, k_norm=None, eps=1e-6, qkv_bias=None,
+                           scale_dtype=SCALE_F32, sections=None, interleaved=False, stream=None):
+    """Extension: rope_and_write_kv_ex with an RMS norm of each query and key head
+    (q_norm, k_norm fp16 [D] or None) before the rotation, and a rotation by several
+    position axes: `sections` are the pairs of each (D/2 in all), positions then
+    [len(sections), num_tokens]."""
+    n, dev, sections = max(num_tokens, 0), kv.device, tuple(sections or ())
+    if len(sections) > kRopeMaxAxes:
+        raise _lib.Error(_lib.RLK_EINVAL, f"{len(sections)} position axes (at most {kRopeMaxAxes})")
+    if scale_dtype != kv.scale_dtype:
+        _scales(kv, scale_dtype)
+    dim = kv.head_dim if n > 0 else 0
+    cols = (num_heads + 2 * kv.num_kv_heads) * dim
+    half = lambda t, m, w: None if t is None else _arg(t, torch.float16, w, m, dev)  # noqa: E731
+    opt = _lib.NormRopeOptions(half(q_norm, dim, "q_norm"), half(k_norm, dim, "k_norm"), eps,
+                               half(qkv_bias, cols, "qkv_bias"), scale_dtype, len(sections), sections,
+                               bool(interleaved))
+    check(lib().rlk_rope_and_write_kv_norm(
+        _arg(qkv, torch.float16, "qkv", n * cols, dev),
+        _arg(positions, torch.int32, "positions", n * max(1, len(sections)), dev),
+        _arg(slot_mapping, torch.int32, "slot_mapping", n, dev), num_tokens, num_heads,
+        _arg(cos_table, torch.float32, "cos_table", 0, dev), _arg(sin_table, torch.float32, "sin_table", 0, dev),
+        C.byref(kv), C.byref(opt), _stream_on(dev, stream)))
+
+
+def read_kv(kv: KVLayerView, slots, n, k_out=None, v_out=None, scale_dtype=SCALE_F32, stream=None):
+    """Extension: the stored rows of `slots` as fp16 [n, Hkv * D] (INT8: code * scale);
+    a negative slot leaves its rows as they were."""
+    dev, size = kv.device, max(n, 0) * kv.num_kv_heads * kv.head_dim
+    if scale_dtype != kv.scale_dtype:
+        _scales(kv, scale_dtype)
+    check(lib().rlk_read_kv(
+        C.byref(kv), _arg(slots, torch.int32, "slots", n, dev), n,
+        None if k_out is None else _arg(k_out, torch.float16, "k_out", size, dev),
+        None if v_out is None else _arg(v_out, torch.float16, "v_out", size, dev), scale_dtype,
+        _stream_on(dev, stream)))
+
+
+# ------------------------------------------- decode attention over a shared prefix
+
+def shared_prefix_work(item_token, item_seq, num_items, group_start, group_prefix, num_groups, max_group_items,
+                       max_prefix_partitions, max_partitions, workspace):
+    """What paged_attention_decode_shared works on (rlk_shared_prefix_work); `workspace`
+    is a DecodeWorkspace of max_prefix_partitions + max_partitions partitions.  The
+    struct keeps its tensors."""
+    i = lambda t, n, w: _arg(t, torch.int32, w, n, None)  # noqa: E731
+    ws, groups = workspace, num_groups > 0
+    work = _lib.SharedPrefixWork(
+        i(item_token, num_items, "item_token"), i(item_seq, num_items, "item_seq"), num_items,
+        i(group_start, num_groups + 1, "group_start") if groups else None,
+        i(group_prefix, num_groups, "group_prefix") if groups else None, num_groups, max_group_items,
+        max_prefix_partitions, max_partitions, ws.out.data_ptr(), ws.max.data_ptr(), ws.sum.data_ptr())
+    parts = max(1, max_prefix_partitions + max_partitions)
+    work.room = min(ws.max.numel(), ws.sum.numel()) // parts, ws.out.numel() // parts
+    return _keep(work, item_token, item_seq, *((group_start, group_prefix) if groups else ()), ws.out, ws.max, ws.sum)
+
+
+def paged_attention_decode_shared(params: _lib.AttentionParams, work: _lib.SharedPrefixWork,
+                                  scale_dtype=SCALE_F32, stream=None):
+    """Extension: decode attention for groups of items that share their first tokens in
+    the cache; a group's prefix is read once for all its items.  Items with a negative
+    token are skipped."""
+    if work.device != params.device:
+        _same_device(params, work)
+    if params.tensors is not None:
+        _scales(params.tensors[0], scale_dtype)
+        _one_device(params.device, *params.tensors[1:])
+    if work.room is not None:
+        rows = work.num_items * params.num_heads
+        if rows > work.room[0] or rows * params.kv.head_dim > work.room[1]:
+            raise _lib.Error(_lib.RLK_EINVAL, f"the workspace holds {work.room[0]} (item, head) rows and "
+                                              f"{work.room[1]} elements a partition, needs {rows} of "
+                                              f"{params.kv.head_dim}")
+    opt = _lib.AttentionOptions(scale_dtype)
+    check(lib().rlk_paged_attention_decode_shared(C.byref(params), C.byref(work), C.byref(opt),
+                                                  _stream_on(params.device, stream)))
+
+
+# --------------------------------------------------------------------- sampling
+
+class SamplingWorkspace:
+    """Memory of sample_tokens calls of up to max_rows rows of up to max_vocab tokens;
+    calls that may run at the same time need one each."""
+
+    def __init__(self, max_rows, max_vocab, device="cuda"):
+        size = lib().rlk_sampling_workspace_bytes(max_rows, max_vocab)
+        if size == 0:
+            raise _lib.Error(_lib.RLK_EINVAL, f"no sampling workspace of {max_rows} rows of {max_vocab} tokens")
+        self.memory = torch.empty(size, dtype=torch.uint8, device=device)
+
+
+def sampling_work(logits, num_rows, vocab, temperature, top_k, top_p, uniform, tokens, workspace, min_p=None,
+                  param_row=None, logprobs=None):
+    """What sample_tokens reads and writes (rlk_sampling_work): logits fp16 or fp32
+    [num_rows, >= vocab], rows contiguous; without param_row, row r has the settings
+    temperature[r], ...  Values of param_row must lie in the settings.  The struct keeps
+    its tensors."""
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in (torch.float16, torch.float32):
+        raise _lib.Error(_lib.RLK_EINVAL, "logits must be a tensor of torch.float16 or torch.float32")
+    if not logits.is_cuda:
+        raise _lib.Error(_lib.RLK_EINVAL, "logits must be a GPU tensor")
+    n = max(num_rows, 0)
+    if logits.dim() != 2 or logits.shape[0] < n or (n > 0 and logits.shape[1] < vocab):
+        raise _lib.Error(_lib.RLK_EINVAL, f"logits must hold {n} rows of {vocab}, has {tuple(logits.shape)}")
+    if logits.shape[1] > 1 and logits.stride(1) != 1:
+        raise _lib.Error(_lib.RLK_EINVAL, "rows of logits must be contiguous")
+    dev = logits.get_device()
+    rows = n if param_row is None else min(n, 1)  # settings that are there for certain
+    f, i = torch.float32, torch.int32
+    work = _lib.SamplingWork(
+        logits.data_ptr(), logits.dtype == f, logits.stride(0) if n > 1 else vocab, num_rows, vocab,
+        None if param_row is None else _arg(param_row, i, "param_row", n, dev),
+        _arg(temperature, f, "temperature", rows, dev), _arg(top_k, i, "top_k", rows, dev),
+        _arg(top_p, f, "top_p", rows, dev), None if min_p is None else _arg(min_p, f, "min_p", rows, dev),
+        _arg(uniform, f, "uniform", n, dev), _arg(tokens, i, "tokens", n, dev),
+        None if logprobs is None else _arg(logprobs, f, "logprobs", n, dev),
+        _arg(workspace.memory, torch.uint8, "workspace", 0, dev), workspace.memory.numel())
+    return _keep(work, logits, *(t for t in (param_row, temperature, top_k, top_p, min_p, uniform, tokens, logprobs,
+                                             workspace.memory) if t is not None))
+
+
+def sample_tokens(work: _lib.SamplingWork, stream=None):
+    """Extension: the next token of each row of logits by temperature, top-k, top-p and
+    min-p, from one given random number a row; `work` from sampling_work()."""
+    check(lib().rlk_sample_tokens(C.byref(work), _stream_on(work.device, stream)))
