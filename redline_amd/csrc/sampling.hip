@@ -5,27 +5,31 @@
 // exp((l_j - l_max) / T), what the three limits keep is always the first n of them,
 // and the draw is the first whose running weight passes u times the kept weight.  So
 // nothing is sorted: a histogram over bins of the value, with the count and the weight
-// of each, leads to the one bin that a limit or the draw falls into, and only that
-// bin's tokens are put in order.
+// of each, leads to the one bin that a limit or the draw falls into, and only among
+// that bin's tokens is the place sought.
 //
 //   bins      p = l c, c = 8 log2(e) / T in fp64; bin floor(p): an eighth of an octave of
 //             weight.  A chunk of the row keeps the 384 bins (48 octaves) below its own
 //             largest logit; chunks meet by their bins' whole-number distance.
-//   weights   2^((p - floor(p) - 1/2) / 8) in fp64 by a polynomial of degree 6 (|x| <
-//             0.0434, error 6e-14), then rounded to a whole number of 2^-34: sums of whole
-//             numbers do not depend on their order, so atomics give the same bits at
-//             every call.  Count (15 bits) and weight (49) share one 64-bit LDS atomic.
-//             fp32 exponentials would move a border of the running sum by up to 1e-7 of the
-//             whole, and of rows with 10^5 tokens to draw from some would change theirs.
-//   kernel 1  one chunk a workgroup: the logits are read once.
+//   weights   2^((p - floor(p) - 1/2) / 8) in fp64 by a polynomial of degree 5
+//             (interpolated at the Chebyshev nodes, error 2^-41), as a whole number of
+//             2^-34: sums of whole numbers do not depend on their order, so atomics give
+//             the same bits at every call.  Count (15 bits) and weight (49) share one
+//             64-bit LDS atomic.  fp32 exponentials would move a border of the running sum
+//             by up to 1e-7 of the whole, and of rows with 10^5 tokens to draw from some
+//             would change theirs.
+//   kernel 1  one chunk of 8192 a workgroup: the logits are read once, and the places of
+//             the tokens of its first bins (a quarter at most) go out in the bins' order.
 //   kernel 2  one row a workgroup: chunks' bins summed and scanned, then for each limit
-//             and the draw the bin, its tokens gathered from the chunks that have some,
-//             sorted in LDS (bitonic on value and index) and scanned.  A bin of more
-//             than 2048 tokens is narrowed first, by digits of the value's bits.
+//             and the draw the bin and its tokens, from the chunks' lists or, where a list
+//             ends before the bin, from the logits; narrowed to at most 128 by histograms of
+//             their keys (value, then index); of those every pair is compared.
+//   A row of one chunk of 8192 tokens is done by one workgroup from its registers.
 #include <hip/hip_runtime.h>
 
-#include <algorithm>
+#include <climits>
 #include <cstdint>
+#include <type_traits>
 
 #include "device.hpp"
 #include "redline_amd/rlk.h"
@@ -37,26 +41,30 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int kBins = 384;        // of a chunk and of a row: 48 octaves
-constexpr int kPer = 16;          // logits of a thread of kernel 1
-constexpr int kSmallChunk = 256 * kPer, kLargeChunk = 1024 * kPer;
+constexpr int kPer = 16;          // logits of a thread
+constexpr int kThreads = 512;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kChunk = kThreads * kPer;
+constexpr int kListed = kChunk / 4;  // tokens that a chunk lists at most
 constexpr int kMaxVocab = 1 << 20;
-constexpr int kMaxChunks = kMaxVocab / kSmallChunk;
+constexpr int kMaxChunks = kMaxVocab / kChunk;
 constexpr int kCountShift = 49;   // count above, weight in 2^-34 below
-constexpr u64 kWeightMask = (u64{1} << kCountShift) - 1;
-constexpr double kOne = 17179869184.0;  // 2^34
+constexpr u64 kCountOne = u64{1} << kCountShift, kWeightMask = kCountOne - 1, kWeightOne = u64{1} << 34;
 constexpr double kBinsPerNat = 11.541560327111707;  // 8 log2(e)
 constexpr double kFarBins = 2251799813685248.0;     // 2^51: |l c| from here on is not binned
 
 struct ChunkTop {
   float max;
-  int index;  // the lowest with it
+  int index;  // the lowest with it, where the temperature asks for the largest
 };
 
 struct SampleArgs {
   rlk_sampling_work w;
-  ChunkTop* top;  // [rows, chunks]
-  u64* hist;      // [rows, chunks, kBins]
-  int chunk, chunks;
+  u64* hist;       // [rows, chunks, kBins]
+  ChunkTop* top;   // [rows, chunks]
+  uint16_t* start; // [rows, chunks, kBins] tokens before the bin
+  uint16_t* list;  // [rows, chunks, kListed] places in the chunk of the tokens of its first bins
+  int chunks;
 };
 
 // Order-preserving whole number of a logit; NaN as -infinity, -0 as +0.
@@ -68,6 +76,12 @@ __device__ __forceinline__ uint32_t key_of(float l) {
 __device__ __forceinline__ float value_of(uint32_t k) {
   return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
+// Value and index as one number: larger for a larger value, then for a lower index.
+__device__ __forceinline__ u64 rank_key(float l, int index) {
+  return static_cast<u64>(key_of(clean(l))) << 32 | (0xffffffffu - static_cast<uint32_t>(index));
+}
+__device__ __forceinline__ float key_value(u64 k) { return value_of(static_cast<uint32_t>(k >> 32)); }
+__device__ __forceinline__ int key_index(u64 k) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k)); }
 
 // Where a row's bins are: p = l c; far: |l_max c| is too large to bin (a tiny
 // temperature or an infinite logit), only logits equal to the largest have weight.
@@ -76,20 +90,19 @@ struct Scale {
   __device__ explicit Scale(float temperature) : c(kBinsPerNat / static_cast<double>(temperature)) {}
   __device__ bool far(float l) const { return !(__builtin_fabs(static_cast<double>(l) * c) < kFarBins); }
   __device__ double bin(float l) const { return __builtin_floor(static_cast<double>(l) * c); }
-  // the weight of l over that of its bin's middle, in 2^-34
-  __device__ u64 weight(float l, double bin) const {
-    const double f = __builtin_fma(static_cast<double>(l), c, -(bin + 0.5));
-    constexpr double a = 0.08664339756999316;  // ln(2) / 8
-    double y = a * a * a * a * a * a / 720.0;
-    y = __builtin_fma(y, f, a * a * a * a * a / 120.0);
-    y = __builtin_fma(y, f, a * a * a * a / 24.0);
-    y = __builtin_fma(y, f, a * a * a / 6.0);
-    y = __builtin_fma(y, f, a * a / 2.0);
-    y = __builtin_fma(y, f, a);
-    y = __builtin_fma(y, f, 1.0);
-    // adding 2^52 leaves the rounded whole number in the low bits
-    return __builtin_bit_cast(u64, __builtin_fma(y, kOne, 4503599627370496.0)) - 0x4330000000000000ull;
+  // the weight of l over that of its bin's middle in 2^-34, below 2^52 in the bits of 2^52 + weight;
+  // all weights carry one factor of 1 + 2.6e-11, with which the constant is a whole number
+  __device__ u64 weight_bits(float l, double bin) const {
+    const double f = __builtin_fma(static_cast<double>(l), c, -bin);
+    double y = 699.1093111382294;
+    y = __builtin_fma(y, f, 38597.3698262215);
+    y = __builtin_fma(y, f, 1783466.322640276);
+    y = __builtin_fma(y, f, 61751342.16030201);
+    y = __builtin_fma(y, f, 1425413776.8902755);
+    return __builtin_bit_cast(u64, __builtin_fma(y, f, 4503599627370496.0 + 16451499093.0));
   }
+  static constexpr u64 kBits = 0x4330000000000000ull;  // 2^52
+  __device__ u64 weight(float l, double bin) const { return weight_bits(l, bin) - kBits; }
 };
 
 template <bool kF32>
@@ -98,13 +111,13 @@ __device__ __forceinline__ const void* row_of(const SampleArgs& a, int row) {
 }
 template <bool kF32>
 __device__ __forceinline__ float logit(const void* row, int i) {
-  if constexpr (kF32) return clean(static_cast<const float*>(row)[i]);
-  else return clean(static_cast<float>(static_cast<const _Float16*>(row)[i]));
+  if constexpr (kF32) return static_cast<const float*>(row)[i];
+  else return static_cast<float>(static_cast<const _Float16*>(row)[i]);
 }
 
-// The kPer logits of thread tid of a chunk that starts at `base`: element j of the
-// thread stands at index_of(base, tid, j), tokens past the vocabulary are -infinity.
-template <bool kF32, int kThreads>
+// kPer logits a thread from `base` on: element j of the thread stands at
+// index_of(base, tid, j), those at `stop` and behind are -infinity.
+template <bool kF32>
 struct ChunkLoad {
   static constexpr int kVec = kF32 ? 4 : 8;
   bool vec;
@@ -112,428 +125,506 @@ struct ChunkLoad {
   __device__ int index_of(int base, int tid, int j) const {
     return vec ? base + (j / kVec * kThreads + tid) * kVec + j % kVec : base + j * kThreads + tid;
   }
-  __device__ void load(const void* row, int base, int tid, int vocab, float (&l)[kPer]) const {
+  __device__ void load(const void* row, int base, int tid, int stop, float (&l)[kPer]) const {
     if (vec) {
 #pragma unroll
       for (int b = 0; b < kPer / kVec; ++b) {
         const int i = base + (b * kThreads + tid) * kVec;
-        if (i + kVec <= vocab) {
+        if (i + kVec <= stop) {
           if constexpr (kF32) {
             const f32x4 v = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(static_cast<const float*>(row) + i));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) l[4 * b + j] = clean(v[j]);
+            for (int j = 0; j < 4; ++j) l[4 * b + j] = v[j];
           } else {
-            const f32x8 v = unpack8(__builtin_nontemporal_load(reinterpret_cast<const u32x4*>(static_cast<const _Float16*>(row) + i)));
+            const f32x8 v = unpack8(ld16<true>(reinterpret_cast<const u32x4*>(static_cast<const _Float16*>(row) + i)));
 #pragma unroll
-            for (int j = 0; j < 8; ++j) l[8 * b + j] = clean(v[j]);
+            for (int j = 0; j < 8; ++j) l[8 * b + j] = v[j];
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < kVec; ++j) l[b * kVec + j] = i + j < vocab ? logit<kF32>(row, i + j) : -INFINITY;
+          for (int j = 0; j < kVec; ++j) l[b * kVec + j] = i + j < stop ? logit<kF32>(row, i + j) : -INFINITY;
         }
       }
     } else {
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         const int i = base + j * kThreads + tid;
-        l[j] = i < vocab ? logit<kF32>(row, i) : -INFINITY;
+        l[j] = i < stop ? logit<kF32>(row, i) : -INFINITY;
       }
     }
   }
 };
 
-__device__ __forceinline__ u64 wave_max(u64 v) {
+__device__ __forceinline__ float wave_max(float v) { return rows_max<true>(rows_max<false>(group_max<16>(v))); }
+
+// Sum of v over the lanes before this one.
+template <class T>
+__device__ __forceinline__ T lanes_before(T v) {
+  T incl = v;
 #pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) v = max(v, static_cast<u64>(__shfl_xor(v, o, kWave)));
-  return v;
-}
-// Value and index as one number: larger for a larger value, then for a lower index.
-__device__ __forceinline__ u64 rank_key(float l, int index) {
-  return static_cast<u64>(key_of(l)) << 32 | (0xffffffffu - static_cast<uint32_t>(index));
+  for (int o = 1; o < kWave; o <<= 1) {
+    const T y = __shfl_up(incl, o, kWave);
+    if (static_cast<int>(threadIdx.x % kWave) >= o) incl += y;
+  }
+  return incl - v;
 }
 
-template <bool kF32, int kThreads>
-__global__ __launch_bounds__(kThreads) void sample_chunks_kernel(SampleArgs a) {
-  constexpr int kWaves = kThreads / kWave;
-  __shared__ u64 hist[kBins];
-  __shared__ u64 tops[kWaves];
+struct ChunkLds {
+  u64 hist[kBins];
+  float max[kWaves];
+  int index[kWaves];
+};
+
+// The logits of a chunk in registers, their bins below the chunk's largest (kBins: none)
+// and the chunk's histogram.  False: no bins are asked for.
+template <bool kF32>
+__device__ __forceinline__ bool bin_chunk(const void* src, int base, int vocab, float T, ChunkLds& s,
+                                          float (&l)[kPer], int (&d)[kPer], ChunkTop* top) {
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const int row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks, base = chunk * kThreads * kPer;
-  const void* src = row_of<kF32>(a, row);
-  const ChunkLoad<kF32, kThreads> ld(src);
-  float l[kPer];
-  ld.load(src, base, tid, a.w.vocab, l);
-  const float T = a.w.temperature[a.w.param_row != nullptr ? a.w.param_row[row] : row];
-  for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
-  u64 top = 0;
+  const ChunkLoad<kF32> ld(src);
+  ld.load(src, base, tid, vocab, l);
+  for (int i = tid; i < kBins; i += kThreads) s.hist[i] = 0;
+  float mx = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) top = max(top, rank_key(l[j], ld.index_of(base, tid, j)));
-  top = wave_max(top);
-  if (lane == 0) tops[wave] = top;
+  for (int j = 0; j < kPer; ++j) mx = fmaxf(mx, l[j]);  // (passes NaN by)
+  mx = wave_max(mx);
+  if (lane == 0) s.max[wave] = mx;
   __syncthreads();
 #pragma unroll
-  for (int v = 0; v < kWaves; ++v) top = max(top, tops[v]);
-  const float mx = value_of(static_cast<uint32_t>(top >> 32));
-  const int64_t rec = static_cast<int64_t>(row) * a.chunks + chunk;
-  if (tid == 0) a.top[rec] = {mx, static_cast<int>(0xffffffffu - static_cast<uint32_t>(top))};
-  if (!(T > 0.f) || mx == -INFINITY) return;  // no bins are asked for
+  for (int v = 0; v < kWaves; ++v) mx = fmaxf(mx, s.max[v]);
+  *top = {mx, base};
+  if (mx == -INFINITY) return false;
+  if (!(T > 0.f)) {
+    int at = INT_MAX;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) at = l[j] == mx ? min(at, ld.index_of(base, tid, j)) : at;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) at = min(at, __shfl_xor(at, o, kWave));
+    if (lane == 0) s.index[wave] = at;
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) at = min(at, s.index[v]);
+    top->index = at;
+    return false;
+  }
   const Scale sc(T);
   if (sc.far(mx)) {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      if (l[j] == mx) atomicAdd(&hist[0], (u64{1} << kCountShift) + (u64{1} << 34));
+    for (int j = 0; j < kPer; ++j) {
+      d[j] = l[j] == mx ? 0 : kBins;
+      if (d[j] == 0) atomicAdd(&s.hist[0], kCountOne + kWeightOne);
+    }
   } else {
     const double first = sc.bin(mx);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      const double b = sc.bin(l[j]), d = first - b;
-      if (d < kBins) atomicAdd(&hist[static_cast<int>(d)], sc.weight(l[j], b) + (u64{1} << kCountShift));
+      const double b = sc.bin(l[j]), x = first - b;
+      d[j] = kBins;
+      if (x < kBins) {  // (not for NaN)
+        d[j] = static_cast<int>(x);
+        atomicAdd(&s.hist[d[j]], sc.weight_bits(l[j], b) + (kCountOne - Scale::kBits));
+      }
     }
   }
   __syncthreads();
-  for (int i = tid; i < kBins; i += kThreads) a.hist[rec * kBins + i] = hist[i];
+  return true;
 }
 
-// ---- kernel 2
+__device__ __forceinline__ float temperature_of(const SampleArgs& a, int row) {
+  return a.w.temperature[a.w.param_row != nullptr ? a.w.param_row[row] : row];
+}
 
-constexpr int kRowThreads = 512;
-constexpr int kRowWaves = kRowThreads / kWave;
-constexpr int kSort = 2048;   // tokens that are sorted in LDS
-constexpr int kDigits = 2048;
-constexpr int kSub = 1024;    // tokens of a stretch that one wave counts
+template <bool kF32>
+__global__ __launch_bounds__(kThreads) void sample_chunks_kernel(SampleArgs a) {
+  constexpr int kScan = kBins / 2;  // threads that scan, two bins each
+  __shared__ ChunkLds s;
+  __shared__ alignas(16) uint16_t list[kListed];
+  __shared__ int cursor[kBins];
+  __shared__ int wave_sum[kScan / kWave];
+  __shared__ int listed[2];  // bins and tokens of the list
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks, base = chunk * kChunk;
+  const void* src = row_of<kF32>(a, row);
+  const float T = temperature_of(a, row);
+  const int64_t rec = static_cast<int64_t>(row) * a.chunks + chunk;
+  float l[kPer];
+  int d[kPer];
+  ChunkTop top;
+  if (tid == 0) listed[0] = kBins;
+  const bool binned = bin_chunk<kF32>(src, base, a.w.vocab, T, s, l, d, &top);
+  if (tid == 0) a.top[rec] = top;
+  if (!binned) return;
+  int c0 = 0, c1 = 0, before = 0;
+  if (tid < kScan) {
+    const u64 h0 = s.hist[2 * tid], h1 = s.hist[2 * tid + 1];
+    a.hist[rec * kBins + 2 * tid] = h0;
+    a.hist[rec * kBins + 2 * tid + 1] = h1;
+    c0 = static_cast<int>(h0 >> kCountShift);
+    c1 = static_cast<int>(h1 >> kCountShift);
+    before = lanes_before(c0 + c1);
+    if (lane == kWave - 1) wave_sum[wave] = before + c0 + c1;
+  }
+  __syncthreads();
+  if (tid < kScan) {
+#pragma unroll
+    for (int v = 0; v < kScan / kWave; ++v) before += v < wave ? wave_sum[v] : 0;
+    const int mid = before + c0, end = mid + c1;
+    cursor[2 * tid] = before;
+    cursor[2 * tid + 1] = mid;
+    reinterpret_cast<uint32_t*>(a.start + rec * kBins)[tid] = static_cast<uint32_t>(before) | static_cast<uint32_t>(mid) << 16;
+    if (before <= kListed && end > kListed) {
+      listed[0] = mid > kListed ? 2 * tid : 2 * tid + 1;
+      listed[1] = mid > kListed ? before : mid;
+    } else if (tid == kScan - 1 && end <= kListed) {
+      listed[1] = end;
+    }
+  }
+  __syncthreads();
+  const int nb = listed[0], nt = listed[1];
+  const ChunkLoad<kF32> ld(src);
+#pragma unroll
+  for (int j = 0; j < kPer; ++j)
+    if (d[j] < nb) list[atomicAdd(&cursor[d[j]], 1)] = static_cast<uint16_t>(ld.index_of(0, tid, j));
+  __syncthreads();
+  u32x4* dst = reinterpret_cast<u32x4*>(a.list + rec * kListed);
+  for (int i = tid; 8 * i < nt; i += kThreads) dst[i] = reinterpret_cast<const u32x4*>(list)[i];
+}
+
+// ---- the rows
+
+constexpr int kList = 1024;   // tokens of a bin that are kept in LDS
+constexpr int kDigitBits = 10, kDigits = 1 << kDigitBits;  // classes of a narrowing
+constexpr int kFew = 128;     // tokens of which all pairs are compared
+constexpr int kGroup = 16;    // lanes that read a chunk's list
 
 struct RowLds {
-  union {
-    struct {
-      u64 key[kSort];   // in order once sorted
-      u64 upto[kSort];  // running weight
-    } list;
-    struct {
-      u64 weight[kDigits];
-      uint32_t count[kDigits];
-    } digit;
-    uint32_t ties[kMaxVocab / kSub];
-  };
+  ChunkLds chunk;              // kOne: of the row
+  uint16_t place[kChunk];      // kOne: the row's tokens in the order of their bins; else of a chunk without a list
+  u64 key[kList + kFew], weight[kList + kFew];  // the tokens of one bin; from kList on what is left of a bin
+  u64 few_upto[kFew];
+  int few_place[kFew];
+  u64 digit_weight[kDigits];
+  int digit_count[kDigits];
   double mass[kBins + 1];      // weight before bin j
   int count[kBins + 1];        // tokens before bin j
   double bin_scale[kBins];     // of whole-number weights
   int shift[kMaxChunks];       // of a chunk's bins; kBins: none
-  int use[kMaxChunks];         // chunks that have tokens of the bin
-  int n_use, n, at;
-  u64 top[kRowWaves];
-  u64 wave_u64[kRowWaves];
-  double wave_f64[kRowWaves];
-  int wave_int[kRowWaves];
-  int found;
-  double found_mass;
-  uint32_t found_key;
-  u64 found_base;
-  int found_count;
+  int raw[kMaxChunks];         // chunks whose lists end before the bin
+  int raws, n, m;
+  u64 top[kWaves];
+  u64 wave_u64[kWaves];
+  double wave_f64[kWaves];
+  int wave_int[kWaves];
+  int wave_bin[2][kWaves];
+  u64 found_key, found_weight;
+  int found, found_count;
 };
 
-// What a selection inside a bin looks for.
-enum Seek { kRank, kReach, kPass };  // the r-th token; the first whose running mass >= / > the target
+// What is looked for: the first token whose place (from 1) is `most` or whose running mass
+// passes the target (reaches it, if not strict); or, with least > 0, all tokens whose weight
+// is at least that of the largest.
+struct Goal {
+  int most;
+  double target;
+  bool strict;
+  double least;
+  __device__ bool met(int place, double mass) const {
+    return place >= most || (strict ? mass > target : mass >= target);
+  }
+};
 
-template <bool kF32>
+template <bool kF32, bool kOne>
 struct RowSampler {
   RowLds& s;
   const SampleArgs& a;
   const void* src;
   int row, tid, lane, wave;
   Scale sc;
+  double per_bin;    // 1 / sc.c
   bool far;
   float mx;
-  double first;       // bin of mx
-  int sorted_bin = -1, sorted_n = 0;
+  double first;      // bin of mx
+  int cached = -1;   // the bin in s.key
+  int turn = 0;      // of find_bin
 
-  __device__ u64 weight(float l) const { return far ? u64{1} << 34 : sc.weight(l, sc.bin(l)); }
-  __device__ bool in_bin(float l, int bin) const { return far ? l == mx : first - sc.bin(l) == bin; }
+  __device__ u64 weight(float v) const { return far ? kWeightOne : sc.weight(v, sc.bin(v)); }
 
-  // Every token of the bin, chunk by chunk, to f(logit, index); by all threads.
+  // Every token of the bin to f(key); by all threads.
   template <class F>
   __device__ void each(int bin, F f) {
-    const int nu = s.n_use;
-    for (int x = 0; x < nu; ++x) {
-      const int base = s.use[x] * a.chunk, stop = min(base + a.chunk, a.w.vocab);
-      constexpr int kUnroll = 8;
-      for (int i0 = base + tid; i0 < stop; i0 += kUnroll * kRowThreads) {
-        float l[kUnroll];
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) l[u] = logit<kF32>(src, min(i0 + u * kRowThreads, stop - 1));
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-          if (i0 + u * kRowThreads < stop && in_bin(l[u], bin)) f(l[u], i0 + u * kRowThreads);
-      }
-    }
-  }
-  // The chunks that have tokens of the bin.
-  __device__ void find_chunks(int bin) {
-    __syncthreads();
-    if (tid == 0) s.n_use = 0;
-    __syncthreads();
-    for (int c = tid; c < a.chunks; c += kRowThreads) {
-      const int b = bin - s.shift[c];
-      if (s.shift[c] < kBins && b >= 0 && b < kBins &&
-          a.hist[(static_cast<int64_t>(row) * a.chunks + c) * kBins + b] >> kCountShift != 0)
-        s.use[atomicAdd(&s.n_use, 1)] = c;
-    }
-    __syncthreads();
-  }
-  // Sum of v before this thread's, over the workgroup; total in *all.
-  __device__ u64 scan(u64 v, u64* all) {
-    u64 incl = v;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-      const u64 y = __shfl_up(incl, o, kWave);
-      if (lane >= o) incl += y;
-    }
-    __syncthreads();
-    if (lane == kWave - 1) s.wave_u64[wave] = incl;
-    __syncthreads();
-    u64 before = 0, sum = 0;
-#pragma unroll
-    for (int w = 0; w < kRowWaves; ++w) {
-      if (w < wave) before += s.wave_u64[w];
-      sum += s.wave_u64[w];
-    }
-    *all = sum;
-    return before + incl - v;
-  }
-
-  // The tokens of the bin whose key has the high bits of `prefix` (all bits above
-  // `bits`), sorted, with their running weight, in s.list; n of them, n <= kSort.
-  __device__ void sort_list(int bin, uint32_t prefix, int bits, int n) {
-    __syncthreads();
-    if (tid == 0) s.n = 0;
-    __syncthreads();
-    each(bin, [&](float l, int i) {
-      if (bits < 32 && key_of(l) >> bits != prefix) return;
-      const int at = atomicAdd(&s.n, 1);
-      if (at < kSort) s.list.key[at] = rank_key(l, i);
-    });
-    int size = kWave;
-    while (size < n) size *= 2;
-    for (int i = n + tid; i < size; i += kRowThreads) s.list.key[i] = 0;
-    __syncthreads();
-    for (int k = 2; k <= size; k *= 2)
-      for (int j = k / 2; j > 0; j /= 2) {
-        for (int x = tid; x < size / 2; x += kRowThreads) {
-          const int i = 2 * x - (x & (j - 1)), o = i + j;
-          const u64 p = s.list.key[i], q = s.list.key[o];
-          if ((p < q) == ((i & k) == 0)) {  // falling
-            s.list.key[i] = q;
-            s.list.key[o] = p;
-          }
+    auto give = [&](int at) { f(rank_key(logit<kF32>(src, at), at)); };
+    if constexpr (kOne) {
+      for (int i = s.count[bin] + tid; i < s.count[bin + 1]; i += kThreads) give(s.place[i]);
+    } else {
+      __syncthreads();
+      if (tid == 0) s.raws = 0;
+      __syncthreads();
+      for (int c = tid / kGroup; c < a.chunks; c += kThreads / kGroup) {
+        const int b = bin - s.shift[c];
+        if (b < 0) continue;  // (no bins: shift kBins)
+        const int64_t rec = static_cast<int64_t>(row) * a.chunks + c;
+        const int n = static_cast<int>(a.hist[rec * kBins + b] >> kCountShift), at = a.start[rec * kBins + b];
+        if (at + n <= kListed) {
+          for (int i = at + tid % kGroup; i < at + n; i += kGroup) give(c * kChunk + a.list[rec * kListed + i]);
+        } else if (n != 0 && tid % kGroup == 0) {
+          s.raw[atomicAdd(&s.raws, 1)] = c;
         }
+      }
+      __syncthreads();
+      const int nr = s.raws;
+      const ChunkLoad<kF32> ld(src);
+#pragma unroll 1
+      for (int x = 0; x < nr; ++x) {
+        const int base = s.raw[x] * kChunk;
+        float v[kPer];
+        ld.load(src, base, tid, a.w.vocab, v);
+        if (tid == 0) s.m = 0;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+          if (far ? v[j] == mx : first - sc.bin(v[j]) == bin)
+            s.place[atomicAdd(&s.m, 1)] = static_cast<uint16_t>(ld.index_of(0, tid, j));
+        __syncthreads();
+        const int n = s.m;
+        for (int i = tid; i < n; i += kThreads) give(base + s.place[i]);
         __syncthreads();
       }
-    constexpr int kEach = kSort / kRowThreads;
-    u64 v[kEach], sum = 0, all;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const int i = tid * kEach + e;
-      v[e] = i < n ? weight(value_of(static_cast<uint32_t>(s.list.key[i] >> 32))) : 0;
-      sum += v[e];
     }
-    u64 before = scan(sum, &all);
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      before += v[e];
-      s.list.upto[tid * kEach + e] = before;
-    }
-    __syncthreads();
   }
 
-  // Of the first `most` tokens of the bin, the one that `seek` looks for: its place
-  // (from 1) in *place, the bin's mass up to and with it in *upto; its key and index
-  // by return.  The last of them if none fits.
-  __device__ u64 select(int bin, Seek seek, int rank, double target, int most, int* place, double* upto) {
+  // Sums of v and c before this thread's, over the workgroup.
+  __device__ void scan(u64& v, int& c) {
+    const u64 vb = lanes_before(v);
+    const int cb = lanes_before(c);
+    __syncthreads();
+    if (lane == kWave - 1) {
+      s.wave_u64[wave] = vb + v;
+      s.wave_int[wave] = cb + c;
+    }
+    __syncthreads();
+    v = vb;
+    c = cb;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      v += w < wave ? s.wave_u64[w] : 0;
+      c += w < wave ? s.wave_int[w] : 0;
+    }
+  }
+
+  // The token of the bin that the goal (of places in the bin) is met by, the last if by none:
+  // its place in *place, the mass up to and with it in *upto; its key by return.
+  __device__ u64 select(int bin, const Goal& goal, int* place, double* upto) {
+    enum { kCount, kSum, kKeep };
     const double scale = s.bin_scale[bin], before_bin = s.mass[bin];
-    int n = s.count[bin + 1] - s.count[bin], skipped = 0;
+    auto met = [&](int c, u64 w) { return goal.met(c, before_bin + static_cast<double>(w) * scale); };
+    const int all = s.count[bin + 1] - s.count[bin];
+    int n = all, skipped = 0;  // tokens that are left, those before them
     u64 skipped_w = 0;
-    uint32_t prefix = 0;
-    int bits = 32;
-    auto fits = [&](int c, u64 w) {  // the token with this place and running weight, or one before it
-      if (c >= most) return true;
-      const double mass = before_bin + static_cast<double>(w) * scale;
-      return seek == kRank ? c >= rank : (seek == kReach ? mass >= target : mass > target);
-    };
-    const bool cached = sorted_bin == bin;
-    if (!cached) {
-      find_chunks(bin);
-      while (n > kSort && bits > 0) {
-        const int width = bits == 32 ? 11 : (bits == 21 ? 11 : 10), low = bits - width;
-        __syncthreads();
-        for (int i = tid; i < kDigits; i += kRowThreads) {
-          s.digit.weight[i] = 0;
-          s.digit.count[i] = 0;
+    bool listed = cached == bin;  // they are in s.key
+    int held = all, at0 = 0;      // tokens in s.key, the first that is left
+    // keys of the values whose product with c lies in the bin, with a rounding's room
+    u64 lo = 0, hi = ~u64{0};
+    if (far) {
+      lo = static_cast<u64>(key_of(mx)) << 32;
+      hi = lo | 0xffffffffu;
+    } else if (sc.c > 0.0) {  // (T infinite: all keys)
+      const double v0 = (first - bin) * per_bin, v1 = (first - bin + 1.0) * per_bin;
+      lo = static_cast<u64>(key_of(clean(static_cast<float>(v0 - __builtin_fabs(v0) * 0x1p-22 - 0x1p-140)))) << 32;
+      hi = static_cast<u64>(key_of(clean(static_cast<float>(v1 + __builtin_fabs(v1) * 0x1p-22 + 0x1p-140)))) << 32 | 0xffffffffu;
+    }
+#pragma unroll 1
+    for (int pass = 0; pass < 10; ++pass) {  // (64 bits, 10 a narrowing)
+      const bool sums = goal.least > 0.0;
+      if (listed && n == held && n <= kFew && !sums) break;
+      const int mode = sums ? kSum : (n > (listed ? kFew : kList) ? kCount : kKeep);
+      const int bits = 64 - __builtin_clzll((hi - lo) | 1), low = max(bits - kDigitBits, 0);
+      const int keep = listed ? kList : 0, room = listed ? kFew : kList;
+      __syncthreads();
+      if (mode == kCount) {
+        for (int i = tid; i < kDigits; i += kThreads) {
+          s.digit_weight[i] = 0;
+          s.digit_count[i] = 0;
         }
-        __syncthreads();
-        each(bin, [&](float l, int) {
-          const uint32_t k = key_of(l);
-          if (bits < 32 && k >> bits != prefix) return;
-          const uint32_t d = (1u << width) - 1 - ((k >> low) & ((1u << width) - 1));  // falling
-          atomicAdd(&s.digit.weight[d], weight(l));
-          atomicAdd(&s.digit.count[d], 1u);
-        });
-        __syncthreads();
-        constexpr int kEach = kDigits / kRowThreads;
-        u64 wsum = 0, wall;
-        int csum = 0;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-          wsum += s.digit.weight[tid * kEach + e];
-          csum += s.digit.count[tid * kEach + e];
-        }
-        u64 wbefore = skipped_w + scan(wsum, &wall), call;
-        int cbefore = skipped + static_cast<int>(scan(csum, &call));
-        if (tid == 0) s.found = -1;
-        __syncthreads();
-        for (int e = 0; e < kEach; ++e) {
-          const int d = tid * kEach + e, cn = s.digit.count[d];
-          const u64 wn = s.digit.weight[d];
-          if (cn != 0 && !(cbefore > 0 && fits(cbefore, wbefore)) &&
-              (fits(cbefore + cn, wbefore + wn) || cbefore + cn == skipped + n)) {
-            s.found = d;
-            s.found_base = wbefore;
-            s.found_count = cbefore;
-            s.n = cn;
-          }
-          cbefore += cn;
-          wbefore += wn;
-        }
-        __syncthreads();
-        prefix = (bits == 32 ? 0u : prefix << width) | ((1u << width) - 1 - static_cast<uint32_t>(s.found));
-        skipped = s.found_count;
-        skipped_w = s.found_base;
-        n = s.n;
-        bits = low;
       }
-      if (n > kSort) return select_tie(bin, prefix, n, skipped, skipped_w, seek, rank, target, most, place, upto);
-      sort_list(bin, prefix, bits, n);
-      if (bits == 32) {
-        sorted_bin = bin;
-        sorted_n = n;
+      if (tid == 0) {
+        s.n = 0;
+        s.found_weight = 0;
+        s.found_count = 0;
+      }
+      __syncthreads();
+      u64 wsum = 0;
+      int csum = 0;
+      auto take = [&](u64 k, u64 w) {
+        if (k < lo || k > hi) return;
+        if (mode == kCount) {
+          const int x = static_cast<int>((hi - k) >> low);  // falling keys
+          atomicAdd(&s.digit_weight[x], w);
+          atomicAdd(&s.digit_count[x], 1);
+        } else if (mode == kKeep) {
+          const int at = atomicAdd(&s.n, 1);
+          if (at < room) {
+            s.key[keep + at] = k;
+            s.weight[keep + at] = w;
+          }
+        } else if (exp2((static_cast<double>(key_value(k)) - mx) * sc.c * 0.125) >= goal.least) {
+          wsum += w;
+          ++csum;
+        }
+      };
+      if (listed) {
+        for (int i = tid; i < held; i += kThreads) take(s.key[i], s.weight[i]);
       } else {
-        sorted_bin = -1;
+        each(bin, [&](u64 k) { take(k, weight(key_value(k))); });
+      }
+      if (mode == kSum) {
+        if (csum != 0) {
+          atomicAdd(&s.found_weight, wsum);
+          atomicAdd(&s.found_count, csum);
+        }
+        __syncthreads();
+        *place = s.found_count;
+        *upto = before_bin + static_cast<double>(s.found_weight) * scale;
+        return 0;
+      }
+      __syncthreads();
+      if (mode == kKeep) {
+        if (listed) {
+          at0 = kList;
+          break;
+        }
+        listed = true;
+        held = n;
+        cached = n == all ? bin : -1;
+        continue;
+      }
+      constexpr int kEach = kDigits / kThreads;
+      int cb = 0;
+      u64 wb = 0;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        wb += s.digit_weight[tid * kEach + e];
+        cb += s.digit_count[tid * kEach + e];
+      }
+      scan(wb, cb);
+      wb += skipped_w;
+      cb += skipped;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int x = tid * kEach + e, cn = s.digit_count[x];
+        const u64 wn = s.digit_weight[x];
+        if (cn != 0 && !(cb > 0 && met(cb, wb)) && (met(cb + cn, wb + wn) || cb + cn == skipped + n)) {
+          s.found = x;
+          s.found_weight = wb;
+          s.found_count = cb;
+          s.n = cn;
+        }
+        cb += cn;
+        wb += wn;
+      }
+      __syncthreads();
+      hi -= static_cast<u64>(s.found) << low;
+      if (const u64 end = hi - ((u64{1} << low) - 1); end > lo && end <= hi) lo = end;
+      skipped = s.found_count;
+      skipped_w = s.found_weight;
+      n = s.n;
+    }
+    n = min(n, kFew);
+    __syncthreads();
+    if (tid < kFew) {
+      s.few_upto[tid] = 0;
+      s.few_place[tid] = 0;
+    }
+    __syncthreads();
+    // running weight and place of each: the threads share a token's comparisons
+    const int span = n <= kWave ? kWave : kFew, i = tid % span;
+    const int parts = kThreads / span, per = (n + parts - 1) / parts;
+    if (i < n) {
+      const int j0 = tid / span * per, j1 = min(j0 + per, n);
+      const u64 mine = s.key[at0 + i];
+      u64 w = 0;
+      int c = 0;
+      for (int j = j0; j < j1; ++j) {
+        const bool in = s.key[at0 + j] >= mine;
+        w += in ? s.weight[at0 + j] : 0;
+        c += in;
+      }
+      if (c != 0) {
+        atomicAdd(&s.few_upto[i], w);
+        atomicAdd(&s.few_place[i], c);
       }
     }
     __syncthreads();
-    for (int i = tid; i < n; i += kRowThreads) {
-      const u64 w = skipped_w + s.list.upto[i], w0 = skipped_w + (i > 0 ? s.list.upto[i - 1] : 0);
-      const int at = skipped + i + 1;
-      if ((fits(at, w) || i == n - 1) && !(i > 0 && fits(at - 1, w0))) {
+    if (tid < n) {
+      const int at = skipped + s.few_place[tid];
+      const u64 w = skipped_w + s.few_upto[tid];
+      if ((met(at, w) || at == skipped + n) && !(at > 1 && met(at - 1, w - s.weight[at0 + tid]))) {
         s.found = at;
-        s.found_base = w;
-        s.at = i;
+        s.found_weight = w;
+        s.found_key = s.key[at0 + tid];
       }
     }
     __syncthreads();
     *place = s.found;
-    *upto = before_bin + static_cast<double>(s.found_base) * scale;
-    const u64 key = s.list.key[s.at];
-    __syncthreads();
-    return key;
+    *upto = before_bin + static_cast<double>(s.found_weight) * scale;
+    return s.found_key;
   }
 
-  // More than kSort tokens of one value: the place by arithmetic, the token by counting
-  // through the row.
-  __device__ u64 select_tie(int bin, uint32_t key, int n, int skipped, u64 skipped_w, Seek seek, int rank, double target,
-                            int most, int* place, double* upto) {
-    const double scale = s.bin_scale[bin], before_bin = s.mass[bin];
-    const float l = value_of(key);
-    const u64 w = weight(l);
-    auto fits = [&](int c) {
-      if (c >= most) return true;
-      const double mass = before_bin + static_cast<double>(skipped_w + static_cast<u64>(c - skipped) * w) * scale;
-      return seek == kRank ? c >= rank : (seek == kReach ? mass >= target : mass > target);
-    };
-    int lo = skipped + 1, hi = skipped + n;
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (fits(mid)) hi = mid; else lo = mid + 1;
-    }
-    *place = lo;
-    *upto = before_bin + static_cast<double>(skipped_w + static_cast<u64>(lo - skipped) * w) * scale;
-    const int want = lo - skipped;  // the want-th of them, by index
-    const int V = a.w.vocab, subs = (V + kSub - 1) / kSub;
-    auto is_tie = [&](int i) { return i < V && logit<kF32>(src, min(i, V - 1)) == l; };
-    __syncthreads();
-    for (int x = wave; x < subs; x += kRowWaves) {
-      int c = 0;
-#pragma unroll 4
-      for (int b = 0; b < kSub; b += kWave) c += __popcll(__ballot(is_tie(x * kSub + b + lane)));
-      if (lane == 0) s.ties[x] = c;
-    }
-    __syncthreads();
-    if (tid == 0) {
-      int c = 0, x = 0;
-      while (x < subs - 1 && c + static_cast<int>(s.ties[x]) < want) c += s.ties[x++];
-      s.at = x;
-      s.found_count = c;
-    }
-    __syncthreads();
-    if (wave == 0) {
-      int c = s.found_count;
-      const int x = s.at;
-      int hit = -1;
-      for (int b = 0; b < kSub && hit < 0; b += kWave) {
-        const uint64_t t = __ballot(is_tie(x * kSub + b + lane));
-        const int here = __popcll(t);
-        if (c + here >= want) {
-          const uint64_t below = t & ((2ull << lane) - 1);
-          const uint64_t b1 = __ballot((t >> lane & 1) != 0 && c + static_cast<int>(__popcll(below)) == want);
-          hit = x * kSub + b + (b1 != 0 ? __builtin_ctzll(b1) : 0);
-        }
-        c += here;
-      }
-      if (lane == 0) s.found = max(hit, 0);
-    }
-    __syncthreads();
-    const int index = s.found;
-    sorted_bin = -1;
-    __syncthreads();
-    return rank_key(l, index);
-  }
-
-  // The first bin of 0 .. kBins - 1 that has tokens and ends at or past the target.
-  template <class F>
-  __device__ int find_bin(F past) {
-    __syncthreads();
-    if (tid == 0) s.found = kBins - 1;
-    __syncthreads();
+  // The first bin that has tokens and meets the goal (of places in the row), the last if none.
+  __device__ int find_bin(const Goal& goal) {
+    uint64_t hit = 0;
     if (tid < kBins) {
       const int c0 = s.count[tid], c1 = s.count[tid + 1];
-      if (c1 > c0 && (past(c1, s.mass[tid + 1]) || c1 == s.count[kBins])) atomicMin(&s.found, tid);
+      hit = __ballot(c1 > c0 && (goal.met(c1, s.mass[tid + 1]) || c1 == s.count[kBins]));
     }
+    int* out = s.wave_bin[turn];  // (the call before the last has been read by all)
+    turn ^= 1;
+    if (lane == 0) out[wave] = hit != 0 ? wave * kWave + __builtin_ctzll(hit) : kBins - 1;
     __syncthreads();
-    const int b = s.found;
-    __syncthreads();
+    int b = kBins - 1;
+#pragma unroll
+    for (int w = 0; w < kBins / kWave; ++w) b = min(b, out[w]);
     return b;
   }
 };
 
-template <bool kF32>
-__global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(SampleArgs a) {
+template <bool kF32, bool kOne>
+__global__ __launch_bounds__(kThreads) void sample_rows_kernel(SampleArgs a) {
   __shared__ RowLds s;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, row = blockIdx.x;
   const int pr = a.w.param_row != nullptr ? a.w.param_row[row] : row;
   const float T = a.w.temperature[pr];
-  const ChunkTop* tops = a.top + static_cast<int64_t>(row) * a.chunks;
-  u64 top = 0;
-  for (int c = tid; c < a.chunks; c += kRowThreads) {
-    const ChunkTop t = tops[c];
-    top = max(top, rank_key(t.max, t.index));
-  }
-  top = wave_max(top);
-  if (lane == 0) s.top[wave] = top;
-  __syncthreads();
+  const int k = a.w.top_k[pr];
+  const float top_p = a.w.top_p[pr], least = a.w.min_p != nullptr ? fminf(a.w.min_p[pr], 1.f) : 0.f;
+  float u = a.w.uniform[row];
+  u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;  // (NaN: 0)
+  float l[kPer];
+  int d[kPer];
+  float mx;
+  int top_index;
+  if constexpr (kOne) {
+    ChunkTop t;
+    bin_chunk<kF32>(row_of<kF32>(a, row), 0, a.w.vocab, T, s.chunk, l, d, &t);
+    mx = t.max;
+    top_index = t.index;
+  } else {
+    u64 top = 0;
+    if (tid < a.chunks) {
+      const ChunkTop t = a.top[static_cast<int64_t>(row) * a.chunks + tid];
+      top = rank_key(t.max, t.index);
+      s.shift[tid] = __builtin_bit_cast(int, t.max);
+    }
 #pragma unroll
-  for (int v = 0; v < kRowWaves; ++v) top = max(top, s.top[v]);
-  const float mx = value_of(static_cast<uint32_t>(top >> 32));
+    for (int o = 1; o < kWave; o <<= 1) top = max(top, static_cast<u64>(__shfl_xor(top, o, kWave)));
+    if (lane == 0) s.top[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) top = max(top, s.top[v]);
+    mx = key_value(top);
+    top_index = key_index(top);
+  }
   if (!(T > 0.f) || mx == -INFINITY) {
     if (tid == 0) {
-      a.w.tokens[row] = static_cast<int>(0xffffffffu - static_cast<uint32_t>(top));
+      a.w.tokens[row] = top_index;
       if (a.w.logprobs != nullptr) a.w.logprobs[row] = 0.f;
     }
     return;
@@ -541,33 +632,55 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(SampleArgs a) 
   const Scale sc(T);
   const bool far = sc.far(mx);
   const double first = far ? 0.0 : sc.bin(mx);
-  for (int c = tid; c < a.chunks; c += kRowThreads) {
-    const float m = tops[c].max;
-    int shift = kBins;
-    if (far) {
-      shift = m == mx ? 0 : kBins;
-    } else if (!sc.far(m)) {  // (a chunk too low to bin is far below the row's largest)
-      const double d = first - sc.bin(m);
-      shift = d < kBins ? static_cast<int>(d) : kBins;
-    }
-    s.shift[c] = m == -INFINITY ? kBins : shift;
-  }
-  __syncthreads();
   u64 w = 0;
   int n = 0;
-  double scale = 0.0;
-  if (tid < kBins) {
-    const u64* h = a.hist + static_cast<int64_t>(row) * a.chunks * kBins;
-    for (int c = 0; c < a.chunks; ++c) {
-      const int b = tid - s.shift[c];
-      const u64 v = b >= 0 && s.shift[c] < kBins ? h[static_cast<int64_t>(c) * kBins + b] : 0;
-      w += v & kWeightMask;
-      n += static_cast<int>(v >> kCountShift);
+  if constexpr (kOne) {
+    if (tid < kBins) {
+      w = s.chunk.hist[tid] & kWeightMask;
+      n = static_cast<int>(s.chunk.hist[tid] >> kCountShift);
     }
-    scale = exp2(tid * -0.125) / kOne;
-    s.bin_scale[tid] = scale;
+  } else {
+    if (tid < a.chunks) {
+      const float m = __builtin_bit_cast(float, s.shift[tid]);
+      int shift = kBins;
+      if (far) {
+        shift = m == mx ? 0 : kBins;
+      } else if (m != -INFINITY && !sc.far(m)) {  // (a chunk too low to bin is far below the row's largest)
+        const double x = first - sc.bin(m);
+        shift = x < kBins ? static_cast<int>(x) : kBins;
+      }
+      s.shift[tid] = shift;
+    }
+    __syncthreads();
+    if (tid < kBins) {
+      const u64* h = a.hist + static_cast<int64_t>(row) * a.chunks * kBins;
+      constexpr int kUnroll = 16;
+      for (int c0 = 0; c0 < a.chunks; c0 += kUnroll) {
+        u64 v[kUnroll];
+#pragma unroll
+        for (int x = 0; x < kUnroll; ++x) {
+          // (a chunk without bins has no histogram; its place in the workspace is read all the same)
+          const int c = min(c0 + x, a.chunks - 1);
+          v[x] = h[c * kBins + max(tid - s.shift[c], 0)];
+        }
+#pragma unroll
+        for (int x = 0; x < kUnroll; ++x) {
+          const int c = min(c0 + x, a.chunks - 1);
+          if (c0 + x < a.chunks && tid >= s.shift[c]) {
+            w += v[x] & kWeightMask;
+            n += static_cast<int>(v[x] >> kCountShift);
+          }
+        }
+      }
+    }
   }
   // running counts and masses; the order of the sums is fixed
+  double scale = 0.0;
+  if (tid < kBins) {
+    scale = ((tid & 1 ? 0.91700404320467123 : 1.0) * (tid & 2 ? 0.84089641525371454 : 1.0)) * (tid & 4 ? 0.70710678118654752 : 1.0);
+    scale = ldexp(scale, -(tid >> 3) - 34);
+    s.bin_scale[tid] = scale;
+  }
   double mass = static_cast<double>(w) * scale;
   int count = n;
 #pragma unroll
@@ -599,84 +712,95 @@ __global__ __launch_bounds__(kRowThreads) void sample_rows_kernel(SampleArgs a) 
     s.count[0] = 0;
   }
   __syncthreads();
+  if constexpr (kOne) {  // all places in the order of the bins
+    int* cursor = s.digit_count;
+    if (tid < kBins) cursor[tid] = s.count[tid];
+    __syncthreads();
+    const ChunkLoad<kF32> ld(row_of<kF32>(a, row));
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      if (d[j] < kBins) s.place[atomicAdd(&cursor[d[j]], 1)] = static_cast<uint16_t>(ld.index_of(0, tid, j));
+    __syncthreads();
+  }
 
-  RowSampler<kF32> rs{s, a, row_of<kF32>(a, row), row, tid, lane, wave, sc, far, mx, first};
-  int kept = s.count[kBins];
+  RowSampler<kF32, kOne> rs{s, a, row_of<kF32>(a, row), row, tid, lane, wave, sc, T / kBinsPerNat, far, mx, first};
+  int kept = s.count[kBins], bin = 0;
   double Z = s.mass[kBins];
-  const int k = a.w.top_k[pr];
-  if (k > 0 && k < kept) {
-    const int bin = rs.find_bin([&](int c, double) { return c >= k; });
-    if (s.count[bin + 1] == k) {
-      Z = s.mass[bin + 1];
-      kept = k;
+  u64 key = 0;
+  // the limits in turn, then the draw: one loop, since the code is fetched for every row anew
+#pragma unroll 1
+  for (int step = 0; step < 4; ++step) {
+    Goal goal = {INT_MAX, 0.0, true, 0.0};
+    if (step == 0) {
+      if (k <= 0 || k >= kept) continue;
+      goal.most = k;
+      goal.target = __builtin_inf();
+    } else if (step == 1) {
+      if (!(top_p < 1.f)) continue;
+      goal = {kept, static_cast<double>(top_p) * Z, false, 0.0};
+    } else if (step == 2) {
+      if (!(least > 0.f) || far) continue;
+      // the bin that the least weight falls into
+      const double x = first - __builtin_floor(__builtin_fma(static_cast<double>(mx), sc.c, 8.0 * log2(static_cast<double>(least))));
+      if (!(x < kBins) || s.count[static_cast<int>(x)] >= kept) continue;
+      bin = static_cast<int>(x);
+      goal.least = least;
     } else {
-      rs.select(bin, kRank, k - s.count[bin], 0.0, k - s.count[bin], &n, &Z);
-      kept = k;
+      goal = {kept, static_cast<double>(u) * Z, true, 0.0};
     }
-  }
-  const float top_p = a.w.top_p[pr];
-  if (top_p < 1.f) {
-    const double target = static_cast<double>(top_p) * Z;
-    const int bin = rs.find_bin([&](int c, double m) { return c >= kept || m >= target; });
+    if (step != 2) bin = rs.find_bin(goal);
     const int base = s.count[bin];
-    rs.select(bin, kReach, 0, target, min(kept - base, s.count[bin + 1] - base), &n, &Z);
-    kept = base + n;
-  }
-  const float min_p = a.w.min_p != nullptr ? fminf(a.w.min_p[pr], 1.f) : 0.f;
-  if (min_p > 0.f && !far) {
-    // the bin that the least weight falls into
-    const double d = first - __builtin_floor(__builtin_fma(static_cast<double>(mx), sc.c, 8.0 * log2(static_cast<double>(min_p))));
-    if (d < kBins && s.count[static_cast<int>(d)] < kept) {
-      const int bin = static_cast<int>(d), base = s.count[bin];
-      u64 wsum = 0, all;
-      int csum = 0;
-      rs.find_chunks(bin);
-      rs.each(bin, [&](float l, int) {
-        if (exp2((static_cast<double>(l) - mx) * sc.c * 0.125) >= static_cast<double>(min_p)) {
-          wsum += rs.weight(l);
-          ++csum;
-        }
-      });
-      rs.scan(csum, &all);
-      csum = static_cast<int>(all);
-      rs.scan(wsum, &all);
-      if (base + csum < kept) {
-        kept = base + csum;
-        Z = s.mass[bin] + static_cast<double>(all) * s.bin_scale[bin];
-      }
+    if (step == 0 && s.count[bin + 1] == k) {
+      kept = k;
+      Z = s.mass[bin + 1];
+      continue;
+    }
+    goal.most = min(goal.most, s.count[bin + 1]) - base;
+    int place;
+    double upto;
+    key = rs.select(bin, goal, &place, &upto);
+    if (step < 3 && base + place <= kept) {
+      kept = base + place;
+      Z = upto;
     }
   }
-  float u = a.w.uniform[row];
-  u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;  // (NaN: 0)
-  const double target = static_cast<double>(u) * Z;
-  const int bin = rs.find_bin([&](int c, double m) { return c >= kept || m > target; });
-  const int base = s.count[bin];
-  double upto;
-  const u64 key = rs.select(bin, kPass, 0, target, min(kept - base, s.count[bin + 1] - base), &n, &upto);
   if (tid == 0) {
-    a.w.tokens[row] = static_cast<int>(0xffffffffu - static_cast<uint32_t>(key));
+    a.w.tokens[row] = key_index(key);
     if (a.w.logprobs != nullptr) {
-      const float l = value_of(static_cast<uint32_t>(key >> 32));
-      // Z is in weights of the first bin's middle
-      const double top_w = far ? 0.0 : __builtin_fma(static_cast<double>(mx), sc.c, -(first + 0.5)) * 0.08664339756999316;
-      const double own = far ? 0.0 : (static_cast<double>(l) - mx) * sc.c * 0.08664339756999316;
-      a.w.logprobs[row] = static_cast<float>(own + top_w - log(Z));
+      // ln(own / Z) by the rest, which is exact where one token is left
+      const double own = static_cast<double>(rs.weight(key_value(key))) * s.bin_scale[bin];
+      a.w.logprobs[row] = static_cast<float>(-log1p(fmax(Z - own, 0.0) / own));
     }
   }
 }
 
-int chunks_of(int vocab, int chunk) { return (vocab + chunk - 1) / chunk; }
+int chunks_of(int vocab) { return (vocab + kChunk - 1) / kChunk; }
 
-size_t workspace_bytes(int64_t rows, int vocab) {
-  return static_cast<size_t>(rows) * chunks_of(vocab, kSmallChunk) * (sizeof(ChunkTop) + kBins * sizeof(u64)) + 256;
+// Where a call's records stand in its workspace; its size.
+size_t layout(int64_t rows, int vocab, SampleArgs* a) {
+  const size_t recs = static_cast<size_t>(rows) * chunks_of(vocab);
+  size_t n = 0;
+  auto take = [&](auto*& p, size_t count) {
+    if (a != nullptr) p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(static_cast<char*>(a->w.workspace) + n);
+    n += (count * sizeof(*p) + 255) / 256 * 256;
+  };
+  SampleArgs none;
+  SampleArgs& to = a != nullptr ? *a : none;
+  take(to.hist, recs * kBins);
+  take(to.top, recs);
+  take(to.start, recs * kBins);
+  take(to.list, recs * kListed);
+  return n;
 }
 
 template <bool kF32>
 void launch(const SampleArgs& a, hipStream_t stream) {
-  const uint32_t grid = static_cast<uint32_t>(a.w.num_rows) * a.chunks;
-  if (a.chunk == kSmallChunk) sample_chunks_kernel<kF32, 256><<<grid, 256, 0, stream>>>(a);
-  else sample_chunks_kernel<kF32, 1024><<<grid, 1024, 0, stream>>>(a);
-  sample_rows_kernel<kF32><<<a.w.num_rows, kRowThreads, 0, stream>>>(a);
+  if (a.chunks == 1) {
+    sample_rows_kernel<kF32, true><<<a.w.num_rows, kThreads, 0, stream>>>(a);
+    return;
+  }
+  sample_chunks_kernel<kF32><<<static_cast<uint32_t>(a.w.num_rows) * a.chunks, kThreads, 0, stream>>>(a);
+  sample_rows_kernel<kF32, false><<<a.w.num_rows, kThreads, 0, stream>>>(a);
 }
 
 }  // namespace
@@ -686,7 +810,7 @@ using namespace rlk;
 
 extern "C" size_t rlk_sampling_workspace_bytes(int max_rows, int max_vocab) {
   if (max_rows <= 0 || max_vocab <= 0 || max_vocab > kMaxVocab) return 0;
-  return workspace_bytes(max_rows, max_vocab);
+  return layout(max_rows, max_vocab, nullptr);
 }
 
 extern "C" int rlk_sample_tokens(const rlk_sampling_work* w, hipStream_t stream) {
@@ -704,18 +828,15 @@ extern "C" int rlk_sample_tokens(const rlk_sampling_work* w, hipStream_t stream)
     return fail(RLK_EINVAL, "%s: logits must be aligned to their elements", what);
   if ((reinterpret_cast<uintptr_t>(w->workspace) & 255) != 0)
     return fail(RLK_EINVAL, "%s: the workspace must be 256-byte aligned", what);
-  const size_t need = workspace_bytes(w->num_rows, w->vocab);
+  const size_t need = layout(w->num_rows, w->vocab, nullptr);
   if (w->workspace_bytes < need)
     return fail(RLK_EINVAL, "%s: a workspace of %zu bytes, needs %zu", what, w->workspace_bytes, need);
   SampleArgs a;
   a.w = *w;
-  // few rows: small chunks, so that more CUs share a row
-  a.chunk = static_cast<int64_t>(w->num_rows) * chunks_of(w->vocab, kLargeChunk) >= 2 * compute_units() ? kLargeChunk : kSmallChunk;
-  a.chunks = chunks_of(w->vocab, a.chunk);
+  a.chunks = chunks_of(w->vocab);
   if (static_cast<int64_t>(w->num_rows) * a.chunks > (1 << 30))
     return fail(RLK_EINVAL, "%s: %d rows exceed one launch; split the call", what, w->num_rows);
-  a.hist = static_cast<u64*>(w->workspace);
-  a.top = reinterpret_cast<ChunkTop*>(a.hist + static_cast<int64_t>(w->num_rows) * a.chunks * kBins);
+  layout(w->num_rows, w->vocab, &a);
   w->logits_fp32 ? launch<true>(a, stream) : launch<false>(a, stream);
   return launch_status(what);
 }
