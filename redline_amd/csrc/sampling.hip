@@ -94,12 +94,15 @@ struct Scale {
   // all weights carry one factor of 1 + 2.6e-11, with which the constant is a whole number
   __device__ u64 weight_bits(float l, double bin) const {
     const double f = __builtin_fma(static_cast<double>(l), c, -bin);
-    double y = 699.1093111382294;
-    y = __builtin_fma(y, f, 38597.3698262215);
-    y = __builtin_fma(y, f, 1783466.322640276);
-    y = __builtin_fma(y, f, 61751342.16030201);
-    y = __builtin_fma(y, f, 1425413776.8902755);
-    return __builtin_bit_cast(u64, __builtin_fma(y, f, 4503599627370496.0 + 16451499093.0));
+    // (kept in scalar registers: as literals each would be moved into a vector register per use)
+    double c5 = 699.1093111382294, c4 = 38597.3698262215, c3 = 1783466.322640276, c2 = 61751342.16030201;
+    double c1 = 1425413776.8902755, c0 = 4503599627370496.0 + 16451499093.0;
+    asm("" : "+s"(c5), "+s"(c4), "+s"(c3), "+s"(c2), "+s"(c1), "+s"(c0));
+    double y = __builtin_fma(f, c5, c4);
+    y = __builtin_fma(y, f, c3);
+    y = __builtin_fma(y, f, c2);
+    y = __builtin_fma(y, f, c1);
+    return __builtin_bit_cast(u64, __builtin_fma(y, f, c0));
   }
   static constexpr u64 kBits = 0x4330000000000000ull;  // 2^52
   __device__ u64 weight(float l, double bin) const { return weight_bits(l, bin) - kBits; }
@@ -125,6 +128,8 @@ struct ChunkLoad {
   __device__ int index_of(int base, int tid, int j) const {
     return vec ? base + (j / kVec * kThreads + tid) * kVec + j % kVec : base + j * kThreads + tid;
   }
+  // index_of from element and thread as one number, element * kThreads + thread
+  __device__ int index_of(int base, int place) const { return index_of(base, place % kThreads, place / kThreads); }
   __device__ void load(const void* row, int base, int tid, int stop, float (&l)[kPer]) const {
     if (vec) {
 #pragma unroll
@@ -216,14 +221,19 @@ __device__ __forceinline__ bool bin_chunk(const void* src, int base, int vocab, 
     }
   } else {
     const double first = sc.bin(mx);
+    constexpr int kAtOnce = 4;  // weights outside the branches, so that their chains overlap
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const double b = sc.bin(l[j]), x = first - b;
-      d[j] = kBins;
-      if (x < kBins) {  // (not for NaN)
-        d[j] = static_cast<int>(x);
-        atomicAdd(&s.hist[d[j]], sc.weight_bits(l[j], b) + (kCountOne - Scale::kBits));
+    for (int j0 = 0; j0 < kPer; j0 += kAtOnce) {
+      u64 w[kAtOnce];
+#pragma unroll
+      for (int x = 0; x < kAtOnce; ++x) {
+        const double b = sc.bin(l[j0 + x]), below = first - b;
+        d[j0 + x] = below < kBins ? static_cast<int>(below) : kBins;  // (kBins for NaN)
+        w[x] = sc.weight_bits(l[j0 + x], b) + (kCountOne - Scale::kBits);
       }
+#pragma unroll
+      for (int x = 0; x < kAtOnce; ++x)
+        if (d[j0 + x] < kBins) atomicAdd(&s.hist[d[j0 + x]], w[x]);
     }
   }
   __syncthreads();
@@ -281,10 +291,9 @@ __global__ __launch_bounds__(kThreads) void sample_chunks_kernel(SampleArgs a) {
   }
   __syncthreads();
   const int nb = listed[0], nt = listed[1];
-  const ChunkLoad<kF32> ld(src);
 #pragma unroll
   for (int j = 0; j < kPer; ++j)
-    if (d[j] < nb) list[atomicAdd(&cursor[d[j]], 1)] = static_cast<uint16_t>(ld.index_of(0, tid, j));
+    if (d[j] < nb) list[atomicAdd(&cursor[d[j]], 1)] = static_cast<uint16_t>(j * kThreads + tid);
   __syncthreads();
   u32x4* dst = reinterpret_cast<u32x4*>(a.list + rec * kListed);
   for (int i = tid; 8 * i < nt; i += kThreads) dst[i] = reinterpret_cast<const u32x4*>(list)[i];
@@ -302,7 +311,7 @@ struct RowLds {
   uint16_t place[kChunk];      // kOne: the row's tokens in the order of their bins; else of a chunk without a list
   u64 key[kList + kFew], weight[kList + kFew];  // the tokens of one bin; from kList on what is left of a bin
   u64 few_upto[kFew];
-  int few_place[kFew];
+  int few_place[kFew], few_bin[kFew];
   u64 digit_weight[kDigits];
   int digit_count[kDigits];
   double mass[kBins + 1];      // weight before bin j
@@ -349,30 +358,36 @@ struct RowSampler {
 
   __device__ u64 weight(float v) const { return far ? kWeightOne : sc.weight(v, sc.bin(v)); }
 
-  // Every token of the bin to f(key); by all threads.
-  template <class F>
+  // Every token of the bin (kAll: of at most kFew in all bins up to it) to f(key); by all threads.
+  template <bool kAll = false, class F>
   __device__ void each(int bin, F f) {
-    auto give = [&](int at) { f(rank_key(logit<kF32>(src, at), at)); };
+    const ChunkLoad<kF32> ld(src);
+    auto give = [&](int base, int place) {
+      const int at = ld.index_of(base, place);
+      f(rank_key(logit<kF32>(src, at), at));
+    };
     if constexpr (kOne) {
-      for (int i = s.count[bin] + tid; i < s.count[bin + 1]; i += kThreads) give(s.place[i]);
+      for (int i = (kAll ? 0 : s.count[bin]) + tid; i < s.count[bin + 1]; i += kThreads) give(0, s.place[i]);
     } else {
-      __syncthreads();
-      if (tid == 0) s.raws = 0;
-      __syncthreads();
+      if constexpr (!kAll) {
+        __syncthreads();
+        if (tid == 0) s.raws = 0;
+        __syncthreads();
+      }
       for (int c = tid / kGroup; c < a.chunks; c += kThreads / kGroup) {
         const int b = bin - s.shift[c];
         if (b < 0) continue;  // (no bins: shift kBins)
         const int64_t rec = static_cast<int64_t>(row) * a.chunks + c;
         const int n = static_cast<int>(a.hist[rec * kBins + b] >> kCountShift), at = a.start[rec * kBins + b];
         if (at + n <= kListed) {
-          for (int i = at + tid % kGroup; i < at + n; i += kGroup) give(c * kChunk + a.list[rec * kListed + i]);
+          for (int i = (kAll ? 0 : at) + tid % kGroup; i < at + n; i += kGroup) give(c * kChunk, a.list[rec * kListed + i]);
         } else if (n != 0 && tid % kGroup == 0) {
           s.raw[atomicAdd(&s.raws, 1)] = c;
         }
       }
+      if constexpr (kAll) return;  // so few are always listed
       __syncthreads();
       const int nr = s.raws;
-      const ChunkLoad<kF32> ld(src);
 #pragma unroll 1
       for (int x = 0; x < nr; ++x) {
         const int base = s.raw[x] * kChunk;
@@ -383,10 +398,10 @@ struct RowSampler {
 #pragma unroll
         for (int j = 0; j < kPer; ++j)
           if (far ? v[j] == mx : first - sc.bin(v[j]) == bin)
-            s.place[atomicAdd(&s.m, 1)] = static_cast<uint16_t>(ld.index_of(0, tid, j));
+            s.place[atomicAdd(&s.m, 1)] = static_cast<uint16_t>(j * kThreads + tid);
         __syncthreads();
         const int n = s.m;
-        for (int i = tid; i < n; i += kThreads) give(base + s.place[i]);
+        for (int i = tid; i < n; i += kThreads) give(base, s.place[i]);
         __syncthreads();
       }
     }
@@ -408,6 +423,117 @@ struct RowSampler {
     for (int w = 0; w < kWaves; ++w) {
       v += w < wave ? s.wave_u64[w] : 0;
       c += w < wave ? s.wave_int[w] : 0;
+    }
+  }
+
+  // Of each of n <= kFew tokens in s.key from at0 on its place among them and the weight up to and
+  // with it (kBinned: of its bin's), in s.few_place and s.few_upto; the threads share a token's pairs.
+  template <bool kBinned>
+  __device__ void compare(int at0, int n) {
+    __syncthreads();
+    if (tid < kFew) {
+      s.few_upto[tid] = 0;
+      s.few_place[tid] = 0;
+    }
+    __syncthreads();
+    const int span = n <= kWave ? kWave : kFew, i = tid % span;
+    const int parts = kThreads / span, per = (n + parts - 1) / parts;
+    if (i < n) {
+      const int j0 = tid / span * per, j1 = min(j0 + per, n), bin = kBinned ? s.few_bin[i] : 0;
+      const u64 mine = s.key[at0 + i];
+      u64 w = 0;
+      int c = 0;
+      for (int j = j0; j < j1; ++j) {
+        const bool in = s.key[at0 + j] >= mine;
+        w += in && (!kBinned || s.few_bin[j] == bin) ? s.weight[at0 + j] : 0;
+        c += in;
+      }
+      if (c != 0) {
+        atomicAdd(&s.few_upto[i], w);
+        atomicAdd(&s.few_place[i], c);
+      }
+    }
+    __syncthreads();
+  }
+
+  // The limits from `step` on and the draw, of `kept` tokens of weight Z, where the tokens up to the bin are
+  // few: by one wave, two tokens a lane.
+  __device__ void finish_few(int step, int bin, int k, float top_p, float least, float u, int kept, double Z) {
+    __syncthreads();
+    if (tid == 0) s.n = 0;
+    __syncthreads();
+    each<true>(bin, [&](u64 key) {
+      const int at = atomicAdd(&s.n, 1);
+      if (at < kFew) {
+        const float v = key_value(key);
+        s.key[at] = key;
+        s.weight[at] = weight(v);
+        s.few_bin[at] = far ? 0 : static_cast<int>(first - sc.bin(v));
+      }
+    });
+    const int n = s.count[bin + 1];
+    compare<true>(0, n);
+    if (wave != 0) return;
+    int place[2];
+    double upto[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int t = min(lane + e * kWave, n - 1), b = s.few_bin[t];
+      place[e] = lane + e * kWave < n ? s.few_place[t] : INT_MAX;
+      upto[e] = s.mass[b] + static_cast<double>(s.few_upto[t]) * s.bin_scale[b];
+    }
+    auto lane_of = [&](int c, int* e) {  // of the token with this place
+      const uint64_t b0 = __ballot(place[0] == c), b1 = __ballot(place[1] == c);
+      *e = b0 == 0;
+      return b0 != 0 ? __builtin_ctzll(b0) : (b1 != 0 ? __builtin_ctzll(b1) : 0);
+    };
+    auto mass_to = [&](int c) {
+      int e;
+      const int at = lane_of(c, &e);
+      return __shfl(e == 0 ? upto[0] : upto[1], at, kWave);
+    };
+    auto first_that = [&](auto f) {  // the least place of which f holds
+      int c = min(f(place[0], upto[0]) ? place[0] : INT_MAX, f(place[1], upto[1]) ? place[1] : INT_MAX);
+#pragma unroll
+      for (int o = 1; o < kWave; o <<= 1) c = min(c, __shfl_xor(c, o, kWave));
+      return c;
+    };
+    if (step == 0) {
+      kept = k;
+      Z = mass_to(kept);
+    }
+    if (step <= 1 && top_p < 1.f) {
+      const double target = static_cast<double>(top_p) * Z;
+      kept = first_that([&](int c, double m) { return c >= kept || m >= target; });
+      Z = mass_to(kept);
+    }
+    if (least > 0.f && !far) {
+      int c = 0;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float v = key_value(s.key[min(lane + e * kWave, n - 1)]);
+        c += __popcll(__ballot(place[e] <= kept && place[e] != INT_MAX &&
+                               exp2((static_cast<double>(v) - mx) * sc.c * 0.125) >= static_cast<double>(least)));
+      }
+      if (c < kept) {
+        kept = c;
+        Z = mass_to(kept);
+      }
+    }
+    const double target = static_cast<double>(u) * Z;
+    int e;
+    const int at = lane_of(first_that([&](int c, double m) { return c >= kept || m > target; }), &e);
+    write(s.key[at + e * kWave], s.few_bin[at + e * kWave], Z);
+  }
+
+  // The row's results: the token drawn of `bin`, of tokens of weight Z.
+  __device__ void write(u64 key, int bin, double Z) {
+    if (tid != 0) return;
+    a.w.tokens[row] = key_index(key);
+    if (a.w.logprobs != nullptr) {
+      // ln(own / Z) by the rest, which is exact where one token is left
+      const double own = static_cast<double>(weight(key_value(key))) * s.bin_scale[bin];
+      a.w.logprobs[row] = static_cast<float>(-log1p(fmax(Z - own, 0.0) / own));
     }
   }
 
@@ -529,31 +655,7 @@ struct RowSampler {
       n = s.n;
     }
     n = min(n, kFew);
-    __syncthreads();
-    if (tid < kFew) {
-      s.few_upto[tid] = 0;
-      s.few_place[tid] = 0;
-    }
-    __syncthreads();
-    // running weight and place of each: the threads share a token's comparisons
-    const int span = n <= kWave ? kWave : kFew, i = tid % span;
-    const int parts = kThreads / span, per = (n + parts - 1) / parts;
-    if (i < n) {
-      const int j0 = tid / span * per, j1 = min(j0 + per, n);
-      const u64 mine = s.key[at0 + i];
-      u64 w = 0;
-      int c = 0;
-      for (int j = j0; j < j1; ++j) {
-        const bool in = s.key[at0 + j] >= mine;
-        w += in ? s.weight[at0 + j] : 0;
-        c += in;
-      }
-      if (c != 0) {
-        atomicAdd(&s.few_upto[i], w);
-        atomicAdd(&s.few_place[i], c);
-      }
-    }
-    __syncthreads();
+    compare<false>(at0, n);
     if (tid < n) {
       const int at = skipped + s.few_place[tid];
       const u64 w = skipped_w + s.few_upto[tid];
@@ -716,10 +818,9 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(SampleArgs a) {
     int* cursor = s.digit_count;
     if (tid < kBins) cursor[tid] = s.count[tid];
     __syncthreads();
-    const ChunkLoad<kF32> ld(row_of<kF32>(a, row));
 #pragma unroll
     for (int j = 0; j < kPer; ++j)
-      if (d[j] < kBins) s.place[atomicAdd(&cursor[d[j]], 1)] = static_cast<uint16_t>(ld.index_of(0, tid, j));
+      if (d[j] < kBins) s.place[atomicAdd(&cursor[d[j]], 1)] = static_cast<uint16_t>(j * kThreads + tid);
     __syncthreads();
   }
 
@@ -749,6 +850,10 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(SampleArgs a) {
       goal = {kept, static_cast<double>(u) * Z, true, 0.0};
     }
     if (step != 2) bin = rs.find_bin(goal);
+    if (step < 3 && s.count[bin + 1] <= kFew) {
+      rs.finish_few(step, bin, k, top_p, least, u, kept, Z);
+      return;
+    }
     const int base = s.count[bin];
     if (step == 0 && s.count[bin + 1] == k) {
       kept = k;
@@ -764,14 +869,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(SampleArgs a) {
       Z = upto;
     }
   }
-  if (tid == 0) {
-    a.w.tokens[row] = key_index(key);
-    if (a.w.logprobs != nullptr) {
-      // ln(own / Z) by the rest, which is exact where one token is left
-      const double own = static_cast<double>(rs.weight(key_value(key))) * s.bin_scale[bin];
-      a.w.logprobs[row] = static_cast<float>(-log1p(fmax(Z - own, 0.0) / own));
-    }
-  }
+  rs.write(key, bin, Z);
 }
 
 int chunks_of(int vocab) { return (vocab + kChunk - 1) / kChunk; }
