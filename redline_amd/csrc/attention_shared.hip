@@ -6,10 +6,10 @@
 //           (item, query head of the kv head) pair: every K and V byte of the range is
 //           read once for all rows;
 //   suffix  a unit is (item, kv head, range of keys) with the item's G rows.
-// Both run the same loop in one launch; a second kernel joins a row's partials
-// (o, m, l in fp32) through the caller's workspace.
+// Both run in one launch; a second kernel joins a row's partials (o, m, l in fp32)
+// through the caller's workspace.
 //
-// The loop: tiles of 64 keys go through registers into two LDS stages (INT8 codes
+// Prefix: tiles of 64 keys go through registers into two LDS stages (INT8 codes
 // become fp16 on the way), the next tile's loads in flight while the current one is
 // used.  A wave owns 32 rows:
 //   S^T = K Q^T    v_mfma_f32_32x32x16_f16, K rows from LDS, q in registers: a lane
@@ -18,6 +18,17 @@
 //   O^T = V^T P^T  the probabilities a lane holds are its B operand, the keys taken in
 //                  the order in which S^T hands them over; V^T by transposing LDS reads.
 // LDS chunks of 16 bytes are XOR-ed with the row so that neither read has bank conflicts.
+//
+// Suffix: a wave owns a range of keys, without LDS or barriers until the four waves of a
+// unit are joined.  Tiles of 32 keys as v_mfma_f32_16x16x32_f16, K as A from rows as they
+// are loaded (16 keys x 32 dims), the G rows as B.  The lanes of key group g get the scores
+// of keys 4 g + i of both halves of the tile, which is their share of the B operand of
+// O^T = V^T P^T; as A a lane loads those 8 keys' dims E m .. E m + E - 1 (E = D / 16,
+// m = lane % 16), and tile dt of the output takes dim E m + dt: 8 x E values to be
+// transposed inside the lane, a byte permute per register.
+//
+// INT8: K scales multiply the scores, V scales the probabilities before they are rounded,
+// so that codes stay exact and a value is rounded once, as in an FP16 cache.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -91,6 +102,180 @@ __device__ __forceinline__ int k_swizzle(int r) { return D == 128 ? r & 15 : (r 
 template <int D>
 __device__ __forceinline__ int v_swizzle(int r) { return D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; }
 
+// log2 of the largest V scale of kKeys keys, one a lane (from 2^-31 on: no fp16 number
+// but 0 gives less).
+template <int kKeys>
+__device__ __forceinline__ float largest_scale(float vs) {
+  vs = rows_max<false>(group_max<16>(vs));
+  if constexpr (kKeys == 64) vs = rows_max<true>(vs);
+  return __builtin_amdgcn_logf(fmaxf(vs, 0x1p-31f));
+}
+
+// The rows of one key that a lane of the suffix loads: E = D / 16 dims of V, 8 of K.
+template <int kBytes> struct RawOf;
+template <> struct RawOf<16> { using Type = u32x4; };
+template <> struct RawOf<8> { using Type = u32x2; };
+template <> struct RawOf<4> { using Type = uint32_t; };
+
+// One wave's part of a suffix unit: keys [begin, end) of the table row, the kv head's G rows.
+// In: q as B operands.  Out: m, l and o[dt][i] = dim E (4 (lane / 16) + i) + dt of row lane % 16.
+template <int D, int kFmt>
+__device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t* table, int kvh, int begin, int end,
+                                             const f16x8 (&q)[D / 32], float& m, float& l, f32x4 (&o)[D / 16]) {
+  constexpr bool kInt8 = kFmt != kF16;
+  constexpr int E = D / 16, kElem = kInt8 ? 1 : 2, kKeys = 32;
+  using KRaw = typename RawOf<8 * kElem>::Type;
+  using VRaw = typename RawOf<E * kElem>::Type;
+  const rlk_kv_layer_view& kv = a.p.kv;
+  const int lane = threadIdx.x % kWave, col = lane % 16, kg = lane / 16, hkv = kv.num_kv_heads, bs = kv.block_size;
+  const int lbs = (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1;
+  const float c = a.p.scale * kLog2e;
+  m = -FLT_MAX;
+  l = 0.f;
+#pragma unroll
+  for (int d = 0; d < E; ++d) o[d] = f32x4{0, 0, 0, 0};
+  if (begin >= end) return;
+
+  int id, off;  // of key lane % 32 of a tile
+  auto find = [&](int k0) {
+    const int pos = min(k0 + lane % kKeys, end - 1), b = lbs >= 0 ? pos >> lbs : pos / bs;
+    off = pos - b * bs;
+    id = table[b];
+  };
+  uint32_t cell;
+  KRaw kr[2][D / 32];
+  VRaw vr[8];
+  float ks = 0.f, vs = 0.f;
+  auto request_k = [&]() {
+    cell = (static_cast<uint32_t>(id) * hkv + kvh) * bs + off;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint32_t at = __shfl(cell, 16 * t + col, kWave);
+      const unsigned char* row = static_cast<const unsigned char*>(kv.k) + static_cast<int64_t>(at) * (D * kElem) + kg * (8 * kElem);
+#pragma unroll
+      for (int x = 0; x < D / 32; ++x) kr[t][x] = *reinterpret_cast<const KRaw*>(row + x * (32 * kElem));
+    }
+    if constexpr (kFmt == kI8) {
+      ks = kv.k_scale[cell];
+      vs = kv.v_scale[cell];
+    } else if constexpr (kFmt == kI8Half) {
+      ks = static_cast<float>(reinterpret_cast<const _Float16*>(kv.k_scale)[cell]);
+      vs = static_cast<float>(reinterpret_cast<const _Float16*>(kv.v_scale)[cell]);
+    }
+  };
+  auto request_v = [&]() {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t at = __shfl(cell, 16 * (j / 4) + 4 * kg + j % 4, kWave);
+      vr[j] = __builtin_nontemporal_load(reinterpret_cast<const VRaw*>(
+          static_cast<const unsigned char*>(kv.v) + static_cast<int64_t>(at) * (D * kElem) + col * (E * kElem)));
+    }
+  };
+  find(begin);
+  request_k();
+  request_v();
+  find(begin + kKeys);
+#pragma unroll 1
+  for (int k0 = begin; k0 < end; k0 += kKeys) {
+    f32x4 s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int x = 0; x < D / 32; ++x) {
+        f16x8 kf;
+        if constexpr (kInt8) kf = int8x8_to_f16(kr[t][x]);
+        else kf = __builtin_bit_cast(f16x8, kr[t][x]);
+        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[x], s[t], 0, 0, 0);
+      }
+    }
+    // s[t][i]: key k0 + 16 t + 4 kg + i
+    f32x4 vscale[2];
+    float ref = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = 16 * t + 4 * kg + i;
+        float f = c;
+        if constexpr (kInt8) {
+          f *= __shfl(ks, key, kWave);
+          vscale[t][i] = __shfl(vs, key, kWave);
+        }
+        s[t][i] *= f;
+      }
+    if constexpr (kInt8) ref = largest_scale<kKeys>(vs);
+    request_k();  // of the next tile; past the last one its last key again
+    const bool tail = k0 + kKeys > end;
+    if (tail) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (k0 + 16 * t + 4 * kg + i >= end) s[t][i] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i / 4][i % 4]);
+    mx = rows_max<true>(rows_max<false>(mx)) + ref;
+    if (__any(mx > m + 8.f)) {  // as in the prefix
+      const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - mn);
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < E; ++d) o[d] *= f;
+      m = mn;
+    }
+    f16x8 p;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float e = __builtin_amdgcn_exp2f(s[i / 4][i % 4] - m);
+      l += e;
+      if constexpr (kInt8) e *= vscale[i / 4][i % 4];
+      p[i] = static_cast<_Float16>(e);
+    }
+    if (tail) {  // 0 times an infinity is no 0
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (k0 + 16 * (j / 4) + 4 * kg + j % 4 >= end) vr[j] = VRaw{};
+    }
+    // operands: element dt of the 8 rows
+    u32x4 vt[E];
+    if constexpr (kInt8) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (E == 8) {
+          f16x2 pair[8];
+          int8x8_pairs_to_f16x2(vr[2 * j], vr[2 * j + 1], pair);
+#pragma unroll
+          for (int d = 0; d < 8; ++d) vt[d][j] = __builtin_bit_cast(uint32_t, pair[d]);
+        } else {
+          const uint32_t x = vr[2 * j] ^ 0x80808080u, y = vr[2 * j + 1] ^ 0x80808080u;
+          const uint32_t lo = __builtin_amdgcn_perm(y, x, 0x05010400u), hi = __builtin_amdgcn_perm(y, x, 0x07030602u);
+          const uint32_t w[4] = {__builtin_amdgcn_perm(0x64646464u, lo, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, lo, 0x04030402u),
+                                 __builtin_amdgcn_perm(0x64646464u, hi, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, hi, 0x04030402u)};
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+            vt[d][j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, w[d]) - static_cast<_Float16>(1152));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int d = 0; d < E; d += 2) {
+          vt[d][j] = __builtin_amdgcn_perm(vr[2 * j + 1][d / 2], vr[2 * j][d / 2], 0x05040100u);
+          vt[d + 1][j] = __builtin_amdgcn_perm(vr[2 * j + 1][d / 2], vr[2 * j][d / 2], 0x07060302u);
+        }
+    }
+    request_v();
+    find(k0 + 2 * kKeys);
+#pragma unroll
+    for (int d = 0; d < E; ++d)
+      o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, vt[d]), p, o[d], 0, 0, 0);
+  }
+  l = rows_sum<true>(rows_sum<false>(l));
+}
+
 template <int D, int kFmt>
 __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArgs a) {
   constexpr bool kInt8 = kFmt != kF16;
@@ -100,7 +285,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
   constexpr int kRowStep = kThreads / kChunks;              // rows between them
   struct Lds {
     unsigned char k[2][kTile * kPitch], v[2][kTile * kPitch];
-    float ks[2][kTile];
+    float ks[2][kTile], vs[2][kTile];
   };
   __shared__ alignas(1024) Lds lds;
   const rlk_attention_params& p = a.p;
@@ -132,8 +317,6 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
     kvh = ik - first * hkv;
     const int token = a.w.item_token[first];
     if (token < 0) return;
-    rows = G;
-    row0 = 0;
     const int prefix = shared_prefix(a, first);
     const int64_t keys = min(static_cast<int64_t>(keys_of(a, token)),
                              prefix + static_cast<int64_t>(a.w.max_partitions) * kPart);
@@ -141,8 +324,58 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
     if (at >= keys) return;
     begin = static_cast<int>(at);
     end = static_cast<int>(min(keys, at + a.suffix_keys));
+    const int32_t* table = p.block_tables + static_cast<int64_t>(a.w.item_seq[first]) * p.max_blocks_per_seq;
+    // a wave's keys: whole tiles but for the last
+    constexpr int kWaves = kThreads / kWave, kLdsRow = D + 4;
+    const int per = ((end - begin + kWaves - 1) / kWaves + 31) / 32 * 32;
+    const int b0 = min(begin + wave * per, end), b1 = min(b0 + per, end);
+    f16x8 q[D / 32];
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x) {
+      q[x] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+      if (lane % 16 < G)
+        q[x] = __builtin_bit_cast(f16x8, load16(reinterpret_cast<const _Float16*>(p.q) + static_cast<int64_t>(token) * p.q_stride +
+                                                (kvh * G + lane % 16) * D + 32 * x + 8 * (lane / 16)));
+    }
+    float m, l;
+    f32x4 o[D / 16];
+    attend_alone<D, kFmt>(a, table, kvh, b0, b1, q, m, l, o);
+    // the waves joined
+    float* po = reinterpret_cast<float*>(lds.k);  // [kWaves, G, kLdsRow]
+    float *pm = reinterpret_cast<float*>(lds.v), *pl = pm + kWaves * 16;
+    if (lane < 16) {
+      pm[wave * 16 + lane] = m;
+      pl[wave * 16 + lane] = l;
+    }
+    if (lane % 16 < G) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int d = 0; d < D / 16; d += 4)
+          *reinterpret_cast<f32x4*>(po + (wave * G + lane % 16) * kLdsRow + D / 16 * (4 * (lane / 16) + i) + d) =
+              f32x4{o[d][i], o[d + 1][i], o[d + 2][i], o[d + 3][i]};
+    }
+    __syncthreads();
     slot = a.w.max_prefix_partitions + split;
-    seq = a.w.item_seq[first];
+    for (int e = tid; e < G * D; e += kThreads) {
+      const int r = e / D, d = e % D;
+      float M = pm[r], L = 0.f, sum = 0.f;
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) M = fmaxf(M, pm[w * 16 + r]);
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float f = __builtin_amdgcn_exp2f(pm[w * 16 + r] - M);
+        L += f * pl[w * 16 + r];
+        sum += f * po[(w * G + r) * kLdsRow + d];
+      }
+      const int64_t to = slot_row(a, first, kvh * G + r) + slot;
+      a.w.ws_out[to * D + d] = sum;
+      if (d == 0) {
+        a.w.ws_max[to] = M;
+        a.w.ws_sum[to] = L;
+      }
+    }
+    return;
   }
   if (begin >= end) return;
 
@@ -209,15 +442,16 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
         store16(kd + ((ch ^ k_swizzle<D>(row)) << 4), kraw[u]);
         store16(vd + ((ch ^ v_swizzle<D>(row)) << 4), vr);
       } else {
-        const float vs = in ? vsc[u] : 0.f;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const u32x2 kc = {kraw[u][2 * x], kraw[u][2 * x + 1]}, vc = {vr[2 * x], vr[2 * x + 1]};
-          const f32x8 vf = __builtin_convertvector(__builtin_bit_cast(i8x8, vc), f32x8) * vs;
           store16(kd + (((2 * ch + x) ^ k_swizzle<D>(row)) << 4), __builtin_bit_cast(u32x4, int8x8_to_f16(kc)));
-          store16(vd + (((2 * ch + x) ^ v_swizzle<D>(row)) << 4), pack8(vf));
+          store16(vd + (((2 * ch + x) ^ v_swizzle<D>(row)) << 4), __builtin_bit_cast(u32x4, int8x8_to_f16(vc)));
         }
-        if (ch == 0) lds.ks[buf][row] = ksc[u];
+        if (ch == 0) {
+          lds.ks[buf][row] = ksc[u];
+          lds.vs[buf][row] = in ? vsc[u] : 0.f;
+        }
       }
     }
   };
@@ -272,8 +506,9 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
 #pragma unroll
     for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
     mx = rows_max<true>(mx);
+    if constexpr (kInt8) mx += largest_scale<kTile>(lds.vs[buf][lane]);
     // m is a reference within 2^8 of the maximum: moving it costs a pass over the
-    // output, and probabilities up to 2^8 have the same 11 bits in fp16
+    // output, and probabilities (INT8: with their V scale) up to 2^8 have the same 11 bits in fp16
     if (__any(mx > m + 8.f)) {
       const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - mn);
       l *= f;
@@ -285,10 +520,16 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float e = __builtin_amdgcn_exp2f(s[t][i] - m);
-        l += e;
-        pb[t][i / 8][i % 8] = static_cast<_Float16>(e);
+      for (int b = 0; b < 4; ++b) {
+        f32x4 f;
+        if constexpr (kInt8) f = *reinterpret_cast<const f32x4*>(&lds.vs[buf][32 * t + 8 * b + 4 * half]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float e = __builtin_amdgcn_exp2f(s[t][4 * b + i] - m);
+          l += e;
+          if constexpr (kInt8) e *= f[i];
+          pb[t][b / 2][b % 2 * 4 + i] = static_cast<_Float16>(e);
+        }
       }
 #pragma unroll
     for (int t = 0; t < 2; ++t)
