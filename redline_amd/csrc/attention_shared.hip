@@ -9,11 +9,10 @@
 // Both run in one launch; a second kernel joins a row's partials (o, m, l in fp32)
 // through the caller's workspace.
 //
-// Prefix: tiles of 64 keys go through registers into two LDS stages (INT8 codes
-// become fp16 on the way), the next tile's loads in flight while the current one is
-// used.  A wave owns 32 rows:
+// Prefix: tiles of 32 keys go through registers into LDS stages (INT8 codes become
+// fp16 on the way), the loads of the next three or four in flight while one is used.  A wave owns 32 rows:
 //   S^T = K Q^T    v_mfma_f32_32x32x16_f16, K rows from LDS, q in registers: a lane
-//                  gets one row (its column) and 32 of the tile's 64 keys, so the
+//                  gets one row (its column) and 16 of the tile's 32 keys, so the
 //                  softmax is per lane with one exchange between the lane halves;
 //   O^T = V^T P^T  the probabilities a lane holds are its B operand, the keys taken in
 //                  the order in which S^T hands them over; V^T by transposing LDS reads.
@@ -46,10 +45,11 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
-constexpr int kTile = 64;               // keys
+constexpr int kTile = 32;               // keys
 constexpr int kWaveRows = 32;
 constexpr int kRows = kThreads / kWave * kWaveRows;  // of a workgroup
 constexpr int kPart = RLK_DECODE_PARTITION_SIZE;
+constexpr int kMaxGroup = 8;            // query heads of a kv head
 constexpr int64_t kMaxBlocks = 1 << 30;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -62,7 +62,7 @@ struct SharedArgs {
   int prefix_keys, suffix_keys;      // keys of a unit, whole tiles
   int prefix_splits, suffix_splits;  // units of the longest prefix, of the longest rest
   int row_tiles;
-  int64_t prefix_blocks;
+  uint32_t prefix_blocks;
 };
 
 // Keys that an item attends to, those inside its table row.
@@ -95,6 +95,17 @@ __device__ __forceinline__ int shared_prefix(const SharedArgs& a, int item) {
 __device__ __forceinline__ int64_t slot_row(const SharedArgs& a, int item, int head) {
   return (static_cast<int64_t>(item) * a.p.num_heads + head) * (a.w.max_prefix_partitions + a.w.max_partitions);
 }
+
+// Scores enter the exponential as q.k c - m: c > 0, the sign of the scale in q, so that the
+// largest product is the largest score (and not 0, which a masked score must not meet).
+__device__ __forceinline__ float score_factor(float scale) {
+  return fmaxf(__builtin_fabsf(scale) * kLog2e, 0x1p-126f);
+}
+__device__ __forceinline__ f16x8 signed_by(float scale, u32x4 q) {
+  return __builtin_bit_cast(f16x8, q ^ (scale < 0.f ? 0x80008000u : 0u));
+}
+// (fmaxf would first pass each operand through an instruction of its own; NaN stays)
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 // LDS image of a tile row: 16-byte chunk c of row r stands at chunk c ^ swizzle(r).
 template <int D>
@@ -129,29 +140,28 @@ __device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t*
   const rlk_kv_layer_view& kv = a.p.kv;
   const int lane = threadIdx.x % kWave, col = lane % 16, kg = lane / 16, hkv = kv.num_kv_heads, bs = kv.block_size;
   const int lbs = (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1;
-  const float c = a.p.scale * kLog2e;
+  const float c = score_factor(a.p.scale);
   m = -FLT_MAX;
   l = 0.f;
 #pragma unroll
   for (int d = 0; d < E; ++d) o[d] = f32x4{0, 0, 0, 0};
   if (begin >= end) return;
 
-  int id, off;  // of key lane % 32 of a tile
-  auto find = [&](int k0) {
+  struct Cell { int id, off; };
+  auto find = [&](int k0) -> Cell {  // of key lane % 32 of a tile
     const int pos = min(k0 + lane % kKeys, end - 1), b = lbs >= 0 ? pos >> lbs : pos / bs;
-    off = pos - b * bs;
-    id = table[b];
+    return {table[b], pos - b * bs};
   };
   uint32_t cell;
   KRaw kr[2][D / 32];
   VRaw vr[8];
   float ks = 0.f, vs = 0.f;
-  auto request_k = [&]() {
-    cell = (static_cast<uint32_t>(id) * hkv + kvh) * bs + off;
+  auto request_k = [&](Cell at) {
+    cell = (static_cast<uint32_t>(at.id) * hkv + kvh) * bs + at.off;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const uint32_t at = __shfl(cell, 16 * t + col, kWave);
-      const unsigned char* row = static_cast<const unsigned char*>(kv.k) + static_cast<int64_t>(at) * (D * kElem) + kg * (8 * kElem);
+      const uint32_t from = __shfl(cell, 16 * t + col, kWave);
+      const unsigned char* row = static_cast<const unsigned char*>(kv.k) + static_cast<int64_t>(from) * (D * kElem) + kg * (8 * kElem);
 #pragma unroll
       for (int x = 0; x < D / 32; ++x) kr[t][x] = *reinterpret_cast<const KRaw*>(row + x * (32 * kElem));
     }
@@ -171,10 +181,10 @@ __device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t*
           static_cast<const unsigned char*>(kv.v) + static_cast<int64_t>(at) * (D * kElem) + col * (E * kElem)));
     }
   };
-  find(begin);
-  request_k();
+  Cell next = find(begin);
+  request_k(next);
+  next = find(begin + kKeys);
   request_v();
-  find(begin + kKeys);
 #pragma unroll 1
   for (int k0 = begin; k0 < end; k0 += kKeys) {
     f32x4 s[2];
@@ -192,20 +202,20 @@ __device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t*
     // s[t][i]: key k0 + 16 t + 4 kg + i
     f32x4 vscale[2];
     float ref = 0.f;
+    if constexpr (kInt8) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = 16 * t + 4 * kg + i;
-        float f = c;
-        if constexpr (kInt8) {
-          f *= __shfl(ks, key, kWave);
+        for (int i = 0; i < 4; ++i) {
+          const int key = 16 * t + 4 * kg + i;
+          s[t][i] *= __shfl(ks, key, kWave);
           vscale[t][i] = __shfl(vs, key, kWave);
         }
-        s[t][i] *= f;
-      }
-    if constexpr (kInt8) ref = largest_scale<kKeys>(vs);
-    request_k();  // of the next tile; past the last one its last key again
+      ref = largest_scale<kKeys>(vs);
+    }
+    request_k(next);  // of the next tile; past the last one its last key again
+    next = find(k0 + 2 * kKeys);  // before the V rows: loads complete in order, and this one is waited for first
+    __builtin_amdgcn_sched_barrier(0);
     const bool tail = k0 + kKeys > end;
     if (tail) {
 #pragma unroll
@@ -216,8 +226,8 @@ __device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t*
     }
     float mx = s[0][0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i / 4][i % 4]);
-    mx = rows_max<true>(rows_max<false>(mx)) + ref;
+    for (int i = 1; i < 8; ++i) mx = larger(mx, s[i / 4][i % 4]);
+    mx = rows_max<true>(rows_max<false>(mx)) * c + ref;
     if (__any(mx > m + 8.f)) {  // as in the prefix
       const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - mn);
       l *= f;
@@ -228,7 +238,7 @@ __device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t*
     f16x8 p;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float e = __builtin_amdgcn_exp2f(s[i / 4][i % 4] - m);
+      float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], c, -m));
       l += e;
       if constexpr (kInt8) e *= vscale[i / 4][i % 4];
       p[i] = static_cast<_Float16>(e);
@@ -268,7 +278,6 @@ __device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t*
         }
     }
     request_v();
-    find(k0 + 2 * kKeys);
 #pragma unroll
     for (int d = 0; d < E; ++d)
       o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, vt[d]), p, o[d], 0, 0, 0);
@@ -281,13 +290,18 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
   constexpr bool kInt8 = kFmt != kF16;
   constexpr int kPitch = 2 * D, kQ = D / 16, kO = D / 32;
   constexpr int kChunks = D / (kInt8 ? 16 : 8);             // loads of a row
-  constexpr int kItems = kTile * kChunks / kThreads;        // loads of a thread and tile, of K and of V
-  constexpr int kRowStep = kThreads / kChunks;              // rows between them
-  struct Lds {
-    unsigned char k[2][kTile * kPitch], v[2][kTile * kPitch];
-    float ks[2][kTile], vs[2][kTile];
+  constexpr int kRowStep = kThreads / kChunks;              // rows between a thread's loads
+  constexpr int kItems = (kTile + kRowStep - 1) / kRowStep; // loads of a thread and tile, of K and of V
+  constexpr int kAhead = kItems > 1 ? 3 : 4;                // tiles in flight, LDS stages
+  struct Stages {
+    unsigned char k[kAhead][kTile * kPitch], v[kAhead][kTile * kPitch];
+    float ks[kAhead][kTile], vs[kAhead][kTile];
   };
-  __shared__ alignas(1024) Lds lds;
+  struct Join {  // of the waves of a suffix unit
+    float o[kThreads / kWave][kMaxGroup][D + 4], m[kThreads / kWave][16], l[kThreads / kWave][16];
+  };
+  __shared__ alignas(1024) union { Stages st; Join join; } shared;
+  Stages& lds = shared.st;
   const rlk_attention_params& p = a.p;
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int col = lane % 32, half = lane / 32;
@@ -297,7 +311,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
   int kvh, first, rows, row0, begin, end, slot, seq;
   if (blockIdx.x < a.prefix_blocks) {
     // the row tiles of a range stand 8 blocks apart: on one XCD, whose L2 has the range
-    const int b = blockIdx.x, rt = b / 8 % a.row_tiles, u = b / 8 / a.row_tiles * 8 + b % 8;
+    const int b = blockIdx.x / 8, rt = b % a.row_tiles, u = b / a.row_tiles * 8 + blockIdx.x % 8;
     const int split = u % a.prefix_splits, gk = u / a.prefix_splits, g = gk / hkv;
     kvh = gk - g * hkv;
     if (g >= a.w.num_groups) return;
@@ -326,7 +340,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
     end = static_cast<int>(min(keys, at + a.suffix_keys));
     const int32_t* table = p.block_tables + static_cast<int64_t>(a.w.item_seq[first]) * p.max_blocks_per_seq;
     // a wave's keys: whole tiles but for the last
-    constexpr int kWaves = kThreads / kWave, kLdsRow = D + 4;
+    constexpr int kWaves = kThreads / kWave;
     const int per = ((end - begin + kWaves - 1) / kWaves + 31) / 32 * 32;
     const int b0 = min(begin + wave * per, end), b1 = min(b0 + per, end);
     f16x8 q[D / 32];
@@ -334,39 +348,38 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
     for (int x = 0; x < D / 32; ++x) {
       q[x] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
       if (lane % 16 < G)
-        q[x] = __builtin_bit_cast(f16x8, load16(reinterpret_cast<const _Float16*>(p.q) + static_cast<int64_t>(token) * p.q_stride +
-                                                (kvh * G + lane % 16) * D + 32 * x + 8 * (lane / 16)));
+        q[x] = signed_by(p.scale, load16(reinterpret_cast<const _Float16*>(p.q) + static_cast<int64_t>(token) * p.q_stride +
+                                         (kvh * G + lane % 16) * D + 32 * x + 8 * (lane / 16)));
     }
     float m, l;
     f32x4 o[D / 16];
     attend_alone<D, kFmt>(a, table, kvh, b0, b1, q, m, l, o);
     // the waves joined
-    float* po = reinterpret_cast<float*>(lds.k);  // [kWaves, G, kLdsRow]
-    float *pm = reinterpret_cast<float*>(lds.v), *pl = pm + kWaves * 16;
+    Join& j = shared.join;
     if (lane < 16) {
-      pm[wave * 16 + lane] = m;
-      pl[wave * 16 + lane] = l;
+      j.m[wave][lane] = m;
+      j.l[wave][lane] = l;
     }
     if (lane % 16 < G) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int d = 0; d < D / 16; d += 4)
-          *reinterpret_cast<f32x4*>(po + (wave * G + lane % 16) * kLdsRow + D / 16 * (4 * (lane / 16) + i) + d) =
+          *reinterpret_cast<f32x4*>(&j.o[wave][lane % 16][D / 16 * (4 * (lane / 16) + i) + d]) =
               f32x4{o[d][i], o[d + 1][i], o[d + 2][i], o[d + 3][i]};
     }
     __syncthreads();
     slot = a.w.max_prefix_partitions + split;
     for (int e = tid; e < G * D; e += kThreads) {
       const int r = e / D, d = e % D;
-      float M = pm[r], L = 0.f, sum = 0.f;
+      float M = j.m[0][r], L = 0.f, sum = 0.f;
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) M = fmaxf(M, pm[w * 16 + r]);
+      for (int w = 1; w < kWaves; ++w) M = fmaxf(M, j.m[w][r]);
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
-        const float f = __builtin_amdgcn_exp2f(pm[w * 16 + r] - M);
-        L += f * pl[w * 16 + r];
-        sum += f * po[(w * G + r) * kLdsRow + d];
+        const float f = __builtin_amdgcn_exp2f(j.m[w][r] - M);
+        L += f * j.l[w][r];
+        sum += f * j.o[w][r][d];
       }
       const int64_t to = slot_row(a, first, kvh * G + r) + slot;
       a.w.ws_out[to * D + d] = sum;
@@ -391,72 +404,68 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
     last = min(end, keys_of(a, token));
     const _Float16* qp = reinterpret_cast<const _Float16*>(p.q) + static_cast<int64_t>(token) * p.q_stride + head * D + 8 * half;
 #pragma unroll
-    for (int s = 0; s < kQ; ++s) q[s] = __builtin_bit_cast(f16x8, load16(qp + 16 * s));
+    for (int s = 0; s < kQ; ++s) q[s] = signed_by(p.scale, load16(qp + 16 * s));
   }
   int whole = last;  // every row of the wave has the keys up to this one
 #pragma unroll
   for (int o = 1; o < kWave; o <<= 1) whole = min(whole, __shfl_xor(whole, o, kWave));
+  whole = __builtin_amdgcn_readfirstlane(whole);
 
-  // this thread's part of a tile
+  // this thread's part of a tile; lane k finds the cell of key k % 32
   const int ch = tid % kChunks, tr = tid / kChunks;
   const int32_t* table = p.block_tables + static_cast<int64_t>(seq) * p.max_blocks_per_seq;
   const int lbs = (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1;
-  u32x4 kraw[kItems], vraw[kItems];
-  float ksc[kItems], vsc[kItems];
-  int id[kItems], off[kItems];
-  auto find = [&](int k0) {
-#pragma unroll
-    for (int u = 0; u < kItems; ++u) {
-      const int pos = min(k0 + tr + u * kRowStep, end - 1);
-      const int b = lbs >= 0 ? pos >> lbs : pos / bs;
-      off[u] = pos - b * bs;
-      id[u] = table[b];
-    }
+  u32x4 kraw[kAhead][kItems], vraw[kAhead][kItems];
+  float sc[kAhead];  // INT8: wave 0 has the K scales, wave 1 the V scales
+  struct Cell { int id, off; };
+  auto find = [&](int k0) -> Cell {
+    const int pos = min(k0 + lane % kTile, end - 1), b = lbs >= 0 ? pos >> lbs : pos / bs;
+    return {table[b], pos - b * bs};
   };
-  auto request = [&]() {
+  auto request = [&](int u, Cell at) {
+    const uint32_t cell = (static_cast<uint32_t>(at.id) * hkv + kvh) * bs + at.off;
 #pragma unroll
-    for (int u = 0; u < kItems; ++u) {
-      const int64_t cell = (static_cast<int64_t>(id[u]) * hkv + kvh) * bs + off[u];
-      const int64_t at = cell * (kInt8 ? D : 2 * D) + ch * 16;
-      kraw[u] = load16(static_cast<const unsigned char*>(p.kv.k) + at);
-      vraw[u] = load16(static_cast<const unsigned char*>(p.kv.v) + at);
-      if constexpr (kFmt == kI8) {
-        ksc[u] = p.kv.k_scale[cell];
-        vsc[u] = p.kv.v_scale[cell];
-      } else if constexpr (kFmt == kI8Half) {
-        ksc[u] = static_cast<float>(reinterpret_cast<const _Float16*>(p.kv.k_scale)[cell]);
-        vsc[u] = static_cast<float>(reinterpret_cast<const _Float16*>(p.kv.v_scale)[cell]);
+    for (int i = 0; i < kItems; ++i) {
+      const uint32_t row = __shfl(cell, (tr + i * kRowStep) % kTile, kWave);
+      const uint64_t from = static_cast<uint64_t>(row) * (kInt8 ? D : 2 * D) + ch * 16;
+      kraw[u][i] = load16(static_cast<const unsigned char*>(p.kv.k) + from);
+      vraw[u][i] = load16(static_cast<const unsigned char*>(p.kv.v) + from);
+    }
+    if constexpr (kInt8) {
+      if (wave < 2) {
+        const float* scale = wave == 0 ? p.kv.k_scale : p.kv.v_scale;
+        sc[u] = kFmt == kI8 ? scale[cell] : static_cast<float>(reinterpret_cast<const _Float16*>(scale)[cell]);
       }
     }
   };
-  auto put = [&](int k0, int buf) {
+  auto put = [&](int k0, int u) {
 #pragma unroll
-    for (int u = 0; u < kItems; ++u) {
-      const int row = tr + u * kRowStep;
+    for (int i = 0; i < kItems; ++i) {
+      const int row = tr + i * kRowStep;
+      if (kRowStep * kItems > kTile && row >= kTile) break;
       // rows past the range hold its last key; their V is cleared, since 0 times an infinity is no 0
-      const bool in = k0 + row < end;
-      unsigned char* kd = lds.k[buf] + row * kPitch;
-      unsigned char* vd = lds.v[buf] + row * kPitch;
-      const u32x4 vr = in ? vraw[u] : u32x4{0, 0, 0, 0};
+      unsigned char* kd = lds.k[u] + row * kPitch;
+      unsigned char* vd = lds.v[u] + row * kPitch;
+      const u32x4 kr = kraw[u][i], vr = k0 + row < end ? vraw[u][i] : u32x4{0, 0, 0, 0};
       if constexpr (!kInt8) {
-        store16(kd + ((ch ^ k_swizzle<D>(row)) << 4), kraw[u]);
+        store16(kd + ((ch ^ k_swizzle<D>(row)) << 4), kr);
         store16(vd + ((ch ^ v_swizzle<D>(row)) << 4), vr);
       } else {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const u32x2 kc = {kraw[u][2 * x], kraw[u][2 * x + 1]}, vc = {vr[2 * x], vr[2 * x + 1]};
+          const u32x2 kc = {kr[2 * x], kr[2 * x + 1]}, vc = {vr[2 * x], vr[2 * x + 1]};
           store16(kd + (((2 * ch + x) ^ k_swizzle<D>(row)) << 4), __builtin_bit_cast(u32x4, int8x8_to_f16(kc)));
           store16(vd + (((2 * ch + x) ^ v_swizzle<D>(row)) << 4), __builtin_bit_cast(u32x4, int8x8_to_f16(vc)));
         }
-        if (ch == 0) {
-          lds.ks[buf][row] = ksc[u];
-          lds.vs[buf][row] = in ? vsc[u] : 0.f;
-        }
       }
+    }
+    if constexpr (kInt8) {
+      if (wave == 0 && lane < kTile) lds.ks[u][lane] = sc[u];
+      if (wave == 1 && lane < kTile) lds.vs[u][lane] = k0 + lane < end ? sc[u] : 0.f;
     }
   };
 
-  const float c = p.scale * kLog2e;
+  const float c = score_factor(p.scale);
   f32x16 o[kO];
 #pragma unroll
   for (int d = 0; d < kO; ++d)
@@ -471,42 +480,40 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
   for (int d = 0; d < kO; ++d)
     vat[d] = vrow + (((4 * d + 2 * (lane / 16 % 2) + tm / 2) ^ vsw) << 4) + (tm & 1) * 8;
 
-  auto attend = [&](int k0, int buf) {
-    f32x16 s[2];
+  // element i of a tile's scores: key k0 + 8 (i / 4) + 4 half + i % 4
+  auto scores = [&](int u) {
+    f32x16 s;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int i = 0; i < 16; ++i) s[i] = 0.f;
+    const unsigned char* kr = lds.k[u] + col * kPitch;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
-      const unsigned char* kr = lds.k[buf] + (32 * t + col) * kPitch;
-#pragma unroll
-      for (int x = 0; x < kQ; ++x) {
-        const f16x8 kf = *reinterpret_cast<const f16x8*>(kr + (((2 * x + half) ^ k_swizzle<D>(col)) << 4));
-        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[x], s[t], 0, 0, 0);
-      }
+    for (int x = 0; x < kQ; ++x) {
+      const f16x8 kf = *reinterpret_cast<const f16x8*>(kr + (((2 * x + half) ^ k_swizzle<D>(col)) << 4));
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[x], s, 0, 0, 0);
     }
-    // element i of subtile t: key k0 + 32 t + 8 (i / 4) + 4 half + i % 4
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
+    return s;
+  };
+  // The tile at k0 from stage u, whose scores are there; returns those of stage v.
+  auto attend = [&](f32x16 s, int k0, int u, int v) {
+    if constexpr (kInt8) {
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        f32x4 f = {c, c, c, c};
-        if constexpr (kInt8) f *= *reinterpret_cast<const f32x4*>(&lds.ks[buf][32 * t + 8 * b + 4 * half]);
+        const f32x4 f = *reinterpret_cast<const f32x4*>(&lds.ks[u][8 * b + 4 * half]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[t][4 * b + i] *= f[i];
+        for (int i = 0; i < 4; ++i) s[4 * b + i] *= f[i];
       }
+    }
     if (k0 + kTile > whole) {
       const int left = last - k0 - 4 * half;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (32 * t + 8 * (i / 4) + i % 4 >= left) s[t][i] = -INFINITY;
+      for (int i = 0; i < 16; ++i)
+        if (8 * (i / 4) + i % 4 >= left) s[i] = -INFINITY;
     }
-    float mx = fmaxf(s[0][0], s[1][0]);
+    float mx = s[0];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
-    mx = rows_max<true>(mx);
-    if constexpr (kInt8) mx += largest_scale<kTile>(lds.vs[buf][lane]);
+    for (int i = 1; i < 16; ++i) mx = larger(mx, s[i]);
+    mx = rows_max<true>(mx) * c;
+    if constexpr (kInt8) mx += largest_scale<kTile>(lds.vs[u][lane % kTile]);
     // m is a reference within 2^8 of the maximum: moving it costs a pass over the
     // output, and probabilities (INT8: with their V scale) up to 2^8 have the same 11 bits in fp16
     if (__any(mx > m + 8.f)) {
@@ -516,50 +523,65 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
       for (int d = 0; d < kO; ++d) o[d] *= f;
       m = mn;
     }
-    f16x8 pb[2][2];
+    // the next tile's scores run on the matrix cores beside this one's exponentials
+    const f32x16 next = scores(v);
+    f16x8 pb[2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int b = 0; b < 4; ++b) {
+      f32x4 f;
+      if constexpr (kInt8) f = *reinterpret_cast<const f32x4*>(&lds.vs[u][8 * b + 4 * half]);
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        f32x4 f;
-        if constexpr (kInt8) f = *reinterpret_cast<const f32x4*>(&lds.vs[buf][32 * t + 8 * b + 4 * half]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float e = __builtin_amdgcn_exp2f(s[t][4 * b + i] - m);
-          l += e;
-          if constexpr (kInt8) e *= f[i];
-          pb[t][b / 2][b % 2 * 4 + i] = static_cast<_Float16>(e);
-        }
+      for (int i = 0; i < 4; ++i) {
+        float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * b + i], c, -m));
+        l += e;
+        if constexpr (kInt8) e *= f[i];
+        pb[b / 2][b % 2 * 4 + i] = static_cast<_Float16>(e);
       }
+    }
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int x = 0; x < 2; ++x) {
+      unsigned char* vt = lds.v[u] + 16 * x * kPitch;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        unsigned char* vt = lds.v[buf] + (32 * t + 16 * x) * kPitch;
-#pragma unroll
-        for (int d = 0; d < kO; ++d) {
-          typedef __attribute__((address_space(3))) s16x4* LdsPtr;
-          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(vt + vat[d]));
-          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(vt + vat[d] + 8 * kPitch));
-          const f16x8 vf = __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pb[t][x], o[d], 0, 0, 0);
-        }
+      for (int d = 0; d < kO; ++d) {
+        typedef __attribute__((address_space(3))) s16x4* LdsPtr;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(vt + vat[d]));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(vt + vat[d] + 8 * kPitch));
+        const f16x8 vf = __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pb[x], o[d], 0, 0, 0);
       }
+    }
+    return next;
   };
 
-  find(begin);
-  request();
-  find(begin + kTile);
-  int buf = 0;
-  for (int k0 = begin; k0 < end; k0 += kTile) {
-    put(k0, buf);
-    if (k0 + kTile < end) {
-      request();
-      find(k0 + 2 * kTile);
+  Cell cells[kAhead];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) cells[u] = find(begin + u * kTile);
+  // Loads complete in order: a table entry that is waited for takes everything before it along.  So
+  // entries are requested as far ahead of their use as tiles are.
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) {
+    request(u, cells[u]);
+    cells[u] = find(begin + (kAhead + u) * kTile);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  auto stage = [&](int k0, int u) {  // the tile at k0 into stage u, its registers to the one kAhead tiles on
+    put(k0, u);
+    request(u, cells[u]);  // past the range its last key again
+    cells[u] = find(k0 + 2 * kAhead * kTile);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  stage(begin, 0);
+  __syncthreads();
+  f32x16 s = scores(0);
+#pragma unroll 1
+  for (int k0 = begin; k0 < end; k0 += kAhead * kTile) {  // (no exit inside: the loads in flight are then known)
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int at = k0 + u * kTile, v = (u + 1) % kAhead;
+      stage(at + kTile, v);
+      __syncthreads();  // stage v was last read before the barrier of the step before
+      if (busy && at < end) s = attend(s, at, u, v);
     }
-    __syncthreads();  // the stage before this one was last read before the barrier of the step before
-    if (busy) attend(k0, buf);
-    buf ^= 1;
   }
   if (token < 0) return;
   l += __shfl_xor(l, 32, kWave);
@@ -617,9 +639,12 @@ template <int D, int kFmt>
 int launch(SharedArgs a, const char* what, hipStream_t stream) {
   const int64_t cus = compute_units(), hkv = a.p.kv.num_kv_heads;
   const int pp = a.w.num_groups > 0 && a.w.max_group_items > 0 ? a.w.max_prefix_partitions : 0;
-  // ranges that give every CU two workgroups, of at least 256 keys (a workspace slot each)
+  // Ranges of at least 256 keys (a workspace slot each) that give `want` units in all.  With a prefix
+  // its units come first, one a CU, and leave room for one of the suffix beside each: the ones compute
+  // where the others load.
+  const int64_t want_each = pp > 0 ? cus : 2 * cus;
   auto keys_of_unit = [&](int partitions, int64_t units) {
-    const int64_t keys = static_cast<int64_t>(partitions) * kPart, want = std::max<int64_t>(1, (2 * cus + units - 1) / units);
+    const int64_t keys = static_cast<int64_t>(partitions) * kPart, want = std::max<int64_t>(1, (want_each + units - 1) / units);
     return static_cast<int>(std::max<int64_t>((keys + want - 1) / want + kTile - 1, kPart) / kTile * kTile);
   };
   a.row_tiles = (std::min(a.w.max_group_items, a.w.num_items) * a.grp + kRows - 1) / kRows;
@@ -636,10 +661,10 @@ int launch(SharedArgs a, const char* what, hipStream_t stream) {
     a.prefix_keys = kPart;
     a.w.num_groups = 0;
   }
-  a.prefix_blocks = blocks;
   a.suffix_keys = keys_of_unit(a.w.max_partitions, a.w.num_items * hkv);
   a.suffix_splits = (a.w.max_partitions * kPart + a.suffix_keys - 1) / a.suffix_keys;
-  blocks += static_cast<int64_t>(a.w.num_items) * hkv * a.suffix_splits;
+  a.prefix_blocks = static_cast<uint32_t>(blocks <= kMaxBlocks ? blocks : 0);
+  blocks += a.w.num_items * hkv * a.suffix_splits;
   if (blocks > kMaxBlocks) return fail(RLK_EINVAL, "%s: %d items exceed one launch; split the call", what, a.w.num_items);
   shared_attention_kernel<D, kFmt><<<static_cast<uint32_t>(blocks), kThreads, 0, stream>>>(a);
   shared_merge_kernel<D><<<dim3(a.w.num_items, a.p.num_heads), D, 0, stream>>>(a);
@@ -669,7 +694,7 @@ extern "C" int rlk_paged_attention_decode_shared(const rlk_attention_params* p, 
   if (p->num_heads <= 0 || p->num_heads % kv.num_kv_heads != 0)
     return fail(RLK_EINVAL, "%s: num_heads must be a multiple of num_kv_heads (%d, %d)", what, p->num_heads, kv.num_kv_heads);
   const int G = p->num_heads / kv.num_kv_heads;
-  if (G > 8) return fail(RLK_EUNSUPPORTED, "%s: unsupported GQA group size %d", what, G);
+  if (G > kMaxGroup) return fail(RLK_EUNSUPPORTED, "%s: unsupported GQA group size %d", what, G);
   if (p->max_blocks_per_seq <= 0 || static_cast<int64_t>(p->max_blocks_per_seq) * kv.block_size > (1 << 30))
     return fail(RLK_EINVAL, "%s: bad table width %d", what, p->max_blocks_per_seq);
   if (w->num_groups < 0 || w->max_group_items < 0)
@@ -679,6 +704,7 @@ extern "C" int rlk_paged_attention_decode_shared(const rlk_attention_params* p, 
     return fail(RLK_EINVAL, "%s: bad partition counts (%d, %d)", what, w->max_prefix_partitions, w->max_partitions);
   if (p->num_heads > 65535 || w->num_items > (1 << 20) || w->num_groups > (1 << 20))
     return fail(RLK_EINVAL, "%s: %d items in %d groups exceed one launch; split the call", what, w->num_items, w->num_groups);
+  if (!(p->scale - p->scale == 0.f)) return fail(RLK_EINVAL, "%s: the scale is no finite number", what);
   if (p->q == nullptr || p->out == nullptr || p->block_tables == nullptr || p->positions == nullptr ||
       kv.k == nullptr || kv.v == nullptr || (kv.dtype == RLK_KV_INT8 && (kv.k_scale == nullptr || kv.v_scale == nullptr)) ||
       w->item_token == nullptr || w->item_seq == nullptr ||
