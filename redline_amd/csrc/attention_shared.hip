@@ -19,7 +19,7 @@
 // LDS chunks of 16 bytes are XOR-ed with the row so that neither read has bank conflicts.
 //
 // Suffix: a wave owns a range of keys, without LDS or barriers until the four waves of a
-// unit are joined.  Tiles of 32 keys as v_mfma_f32_16x16x32_f16, K as A from rows as they
+// unit are joined.  Tiles of 32 keys, the rows of two in flight, as v_mfma_f32_16x16x32_f16, K as A from rows as they
 // are loaded (16 keys x 32 dims), the G rows as B.  The lanes of key group g get the scores
 // of keys 4 g + i of both halves of the tile, which is their share of the B operand of
 // O^T = V^T P^T; as A a lane loads those 8 keys' dims E m .. E m + E - 1 (E = D / 16,
@@ -63,7 +63,16 @@ struct SharedArgs {
   int prefix_splits, suffix_splits;  // units of the longest prefix, of the longest rest
   int row_tiles;
   uint32_t prefix_blocks;
+  // key / block_size = key >> lbs where magic is 0, else umulhi(key, magic) >> lbs
+  uint32_t magic;
+  int lbs;
 };
+
+// The table's block that a key is in.
+__device__ __forceinline__ int block_of(const SharedArgs& a, int key) {
+  const uint32_t q = a.magic != 0 ? __umulhi(static_cast<uint32_t>(key), a.magic) : static_cast<uint32_t>(key);
+  return static_cast<int>(q >> a.lbs);
+}
 
 // Keys that an item attends to, those inside its table row.
 __device__ __forceinline__ int keys_of(const SharedArgs& a, int token) {
@@ -79,17 +88,16 @@ __device__ __forceinline__ int prefix_of(const SharedArgs& a, int g) {
 // The prefix that an item shares, 0 outside the groups; by a whole wave.
 __device__ __forceinline__ int shared_prefix(const SharedArgs& a, int item) {
   const int lane = threadIdx.x % kWave;
-  int g = -1;  // the last group that starts at or before the item
+  int found = 0;  // of the last group that starts at or before the item
   for (int g0 = 0; g0 < a.w.num_groups; g0 += kWave) {
-    const bool before = g0 + lane < a.w.num_groups && a.w.group_start[min(g0 + lane, a.w.num_groups - 1)] <= item;
-    const uint64_t b = __ballot(before);
-    g += __popcll(b);
-    if (b != ~0ull) break;
+    const int g = min(g0 + lane, a.w.num_groups - 1), first = a.w.group_start[g], last = a.w.group_start[g + 1];
+    const int prefix = prefix_of(a, g);
+    const bool in = first >= 0 && item < last && item - first < a.w.max_group_items;
+    const uint64_t before = __ballot(g0 + lane < a.w.num_groups && first <= item);
+    if (before != 0) found = __builtin_amdgcn_readlane(in ? prefix : 0, 63 - __builtin_clzll(before));
+    if (before != ~0ull) break;
   }
-  if (g < 0) return 0;
-  const int first = a.w.group_start[g];
-  if (first < 0 || item >= a.w.group_start[g + 1] || item - first >= a.w.max_group_items) return 0;
-  return prefix_of(a, g);
+  return found;
 }
 
 __device__ __forceinline__ int64_t slot_row(const SharedArgs& a, int item, int head) {
@@ -129,17 +137,19 @@ template <> struct RawOf<8> { using Type = u32x2; };
 template <> struct RawOf<4> { using Type = uint32_t; };
 
 // One wave's part of a suffix unit: keys [begin, end) of the table row, the kv head's G rows.
-// In: q as B operands.  Out: m, l and o[dt][i] = dim E (4 (lane / 16) + i) + dt of row lane % 16.
+// In: q as B operands; kbuf: 32 rows of K in LDS, this wave's own.  Out: m, l and o[dt][i] = dim E (4 (lane / 16) + i) + dt of row lane % 16.
 template <int D, int kFmt>
 __device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t* table, int kvh, int begin, int end,
-                                             const f16x8 (&q)[D / 32], float& m, float& l, f32x4 (&o)[D / 16]) {
+                                             const f16x8 (&q)[D / 32], unsigned char* kbuf, float& m, float& l, f32x4 (&o)[D / 16]) {
   constexpr bool kInt8 = kFmt != kF16;
-  constexpr int E = D / 16, kElem = kInt8 ? 1 : 2, kKeys = 32;
-  using KRaw = typename RawOf<8 * kElem>::Type;
+  constexpr int E = D / 16, kElem = kInt8 ? 1 : 2, kAhead = 2, kKeys = 32;
+  constexpr int kAheadV = kInt8 ? 2 : 1;  // (FP16: with two tiles the registers do not suffice)
+  // K: whole rows by consecutive lanes.  Loaded as the operands want them, a row a lane, the address
+  // unit took the lanes of an instruction one by one (35 ns a key and wave against 1X).
+  constexpr int kRow = D * kElem, kChunks = kRow / 16, kRowsAtOnce = kWave / kChunks, kLoads = kKeys / kRowsAtOnce;
   using VRaw = typename RawOf<E * kElem>::Type;
   const rlk_kv_layer_view& kv = a.p.kv;
   const int lane = threadIdx.x % kWave, col = lane % 16, kg = lane / 16, hkv = kv.num_kv_heads, bs = kv.block_size;
-  const int lbs = (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1;
   const float c = score_factor(a.p.scale);
   m = -FLT_MAX;
   l = 0.f;
@@ -149,53 +159,59 @@ __device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t*
 
   struct Cell { int id, off; };
   auto find = [&](int k0) -> Cell {  // of key lane % 32 of a tile
-    const int pos = min(k0 + lane % kKeys, end - 1), b = lbs >= 0 ? pos >> lbs : pos / bs;
+    const int pos = min(k0 + lane % kKeys, end - 1), b = block_of(a, pos);
     return {table[b], pos - b * bs};
   };
-  uint32_t cell;
-  KRaw kr[2][D / 32];
-  VRaw vr[8];
-  float ks = 0.f, vs = 0.f;
-  auto request_k = [&](Cell at) {
-    cell = (static_cast<uint32_t>(at.id) * hkv + kvh) * bs + at.off;
+  u32x4 kr[kAhead][kLoads];
+  VRaw vr[kAheadV][8];
+  uint32_t cell[kAhead];
+  float ks[kAhead], vs[kAhead];
+  auto request_k = [&](int u, Cell at) {
+    cell[u] = (static_cast<uint32_t>(at.id) * hkv + kvh) * bs + at.off;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint32_t from = __shfl(cell, 16 * t + col, kWave);
-      const unsigned char* row = static_cast<const unsigned char*>(kv.k) + static_cast<int64_t>(from) * (D * kElem) + kg * (8 * kElem);
-#pragma unroll
-      for (int x = 0; x < D / 32; ++x) kr[t][x] = *reinterpret_cast<const KRaw*>(row + x * (32 * kElem));
+    for (int j = 0; j < kLoads; ++j) {
+      const uint32_t from = __shfl(cell[u], j * kRowsAtOnce + lane / kChunks, kWave);
+      kr[u][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(
+          static_cast<const unsigned char*>(kv.k) + static_cast<int64_t>(from) * kRow + lane % kChunks * 16));
     }
     if constexpr (kFmt == kI8) {
-      ks = kv.k_scale[cell];
-      vs = kv.v_scale[cell];
+      ks[u] = kv.k_scale[cell[u]];
+      vs[u] = kv.v_scale[cell[u]];
     } else if constexpr (kFmt == kI8Half) {
-      ks = static_cast<float>(reinterpret_cast<const _Float16*>(kv.k_scale)[cell]);
-      vs = static_cast<float>(reinterpret_cast<const _Float16*>(kv.v_scale)[cell]);
+      ks[u] = static_cast<float>(reinterpret_cast<const _Float16*>(kv.k_scale)[cell[u]]);
+      vs[u] = static_cast<float>(reinterpret_cast<const _Float16*>(kv.v_scale)[cell[u]]);
     }
   };
-  auto request_v = [&]() {
+  auto request_v = [&](int u) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint32_t at = __shfl(cell, 16 * (j / 4) + 4 * kg + j % 4, kWave);
-      vr[j] = __builtin_nontemporal_load(reinterpret_cast<const VRaw*>(
+      const uint32_t at = __shfl(cell[u], 16 * (j / 4) + 4 * kg + j % 4, kWave);
+      vr[u % kAheadV][j] = __builtin_nontemporal_load(reinterpret_cast<const VRaw*>(
           static_cast<const unsigned char*>(kv.v) + static_cast<int64_t>(at) * (D * kElem) + col * (E * kElem)));
     }
+    asm volatile("" ::: "memory");  // else the compiler moves these loads to where they are used
   };
-  Cell next = find(begin);
-  request_k(next);
-  next = find(begin + kKeys);
-  request_v();
-#pragma unroll 1
-  for (int k0 = begin; k0 < end; k0 += kKeys) {
+  // One tile from slot u; the slot's rows are requested for the tile kAhead on, past the range its last
+  // key again.  Loads complete in order: a table entry is requested before the rows beside it.
+  Cell cells[kAhead];
+  // 16-byte chunk c of row r of kbuf stands at chunk c ^ swizzle(r): no bank conflicts either way
+  auto swizzle = [](int r) { return kChunks == 16 ? r & 15 : (kChunks == 8 ? (r >> 1) & 7 : (r >> 2) & 3); };
+  auto step = [&](int k0, int u) {
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {  // (a wave's LDS accesses complete in order)
+      const int r = j * kRowsAtOnce + lane / kChunks;
+      store16(kbuf + r * kRow + ((lane % kChunks ^ swizzle(r)) << 4), kr[u][j]);
+    }
     f32x4 s[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       s[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int x = 0; x < D / 32; ++x) {
+        const unsigned char* row = kbuf + (16 * t + col) * kRow;
         f16x8 kf;
-        if constexpr (kInt8) kf = int8x8_to_f16(kr[t][x]);
-        else kf = __builtin_bit_cast(f16x8, kr[t][x]);
+        if constexpr (kInt8) kf = int8x8_to_f16(*reinterpret_cast<const u32x2*>(row + ((2 * x + kg / 2) ^ swizzle(col)) * 16 + kg % 2 * 8));
+        else kf = *reinterpret_cast<const f16x8*>(row + (((4 * x + kg) ^ swizzle(col)) << 4));
         s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[x], s[t], 0, 0, 0);
       }
     }
@@ -208,13 +224,14 @@ __device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t*
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int key = 16 * t + 4 * kg + i;
-          s[t][i] *= __shfl(ks, key, kWave);
-          vscale[t][i] = __shfl(vs, key, kWave);
+          s[t][i] *= __shfl(ks[u], key, kWave);
+          vscale[t][i] = __shfl(vs[u], key, kWave);
         }
-      ref = largest_scale<kKeys>(vs);
+      ref = largest_scale<kKeys>(vs[u]);
     }
-    request_k(next);  // of the next tile; past the last one its last key again
-    next = find(k0 + 2 * kKeys);  // before the V rows: loads complete in order, and this one is waited for first
+    const Cell next = find(k0 + 2 * kAhead * kKeys);
+    request_k(u, cells[u]);
+    cells[u] = next;
     __builtin_amdgcn_sched_barrier(0);
     const bool tail = k0 + kKeys > end;
     if (tail) {
@@ -243,23 +260,27 @@ __device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t*
       if constexpr (kInt8) e *= vscale[i / 4][i % 4];
       p[i] = static_cast<_Float16>(e);
     }
-    if (tail) {  // 0 times an infinity is no 0
+    // operands: element dt of the 8 rows; those past the range are cleared, since 0 times an
+    // infinity is no 0
+    VRaw row[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) row[j] = vr[u % kAheadV][j];
+    if (tail) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (k0 + 16 * (j / 4) + 4 * kg + j % 4 >= end) vr[j] = VRaw{};
+        if (k0 + 16 * (j / 4) + 4 * kg + j % 4 >= end) row[j] = VRaw{};
     }
-    // operands: element dt of the 8 rows
     u32x4 vt[E];
     if constexpr (kInt8) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if constexpr (E == 8) {
           f16x2 pair[8];
-          int8x8_pairs_to_f16x2(vr[2 * j], vr[2 * j + 1], pair);
+          int8x8_pairs_to_f16x2(row[2 * j], row[2 * j + 1], pair);
 #pragma unroll
           for (int d = 0; d < 8; ++d) vt[d][j] = __builtin_bit_cast(uint32_t, pair[d]);
         } else {
-          const uint32_t x = vr[2 * j] ^ 0x80808080u, y = vr[2 * j + 1] ^ 0x80808080u;
+          const uint32_t x = row[2 * j] ^ 0x80808080u, y = row[2 * j + 1] ^ 0x80808080u;
           const uint32_t lo = __builtin_amdgcn_perm(y, x, 0x05010400u), hi = __builtin_amdgcn_perm(y, x, 0x07030602u);
           const uint32_t w[4] = {__builtin_amdgcn_perm(0x64646464u, lo, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, lo, 0x04030402u),
                                  __builtin_amdgcn_perm(0x64646464u, hi, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, hi, 0x04030402u)};
@@ -273,15 +294,29 @@ __device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t*
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int d = 0; d < E; d += 2) {
-          vt[d][j] = __builtin_amdgcn_perm(vr[2 * j + 1][d / 2], vr[2 * j][d / 2], 0x05040100u);
-          vt[d + 1][j] = __builtin_amdgcn_perm(vr[2 * j + 1][d / 2], vr[2 * j][d / 2], 0x07060302u);
+          vt[d][j] = __builtin_amdgcn_perm(row[2 * j + 1][d / 2], row[2 * j][d / 2], 0x05040100u);
+          vt[d + 1][j] = __builtin_amdgcn_perm(row[2 * j + 1][d / 2], row[2 * j][d / 2], 0x07060302u);
         }
     }
-    request_v();
+    request_v((u + kAheadV) % kAhead);
 #pragma unroll
     for (int d = 0; d < E; ++d)
       o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, vt[d]), p, o[d], 0, 0, 0);
+  };
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) cells[u] = find(begin + u * kKeys);
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) {
+    const Cell next = find(begin + (kAhead + u) * kKeys);
+    request_k(u, cells[u]);
+    cells[u] = next;
+    __builtin_amdgcn_sched_barrier(0);
+    if (u < kAheadV) request_v(u);
   }
+#pragma unroll 1
+  for (int k0 = begin; k0 < end; k0 += kAhead * kKeys)
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) step(k0 + u * kKeys, u);  // (a tile past the range has no part in the sums)
   l = rows_sum<true>(rows_sum<false>(l));
 }
 
@@ -297,10 +332,12 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
     unsigned char k[kAhead][kTile * kPitch], v[kAhead][kTile * kPitch];
     float ks[kAhead][kTile], vs[kAhead][kTile];
   };
-  struct Join {  // of the waves of a suffix unit
+  struct Suffix {
+    unsigned char k[kThreads / kWave][32 * D * (kInt8 ? 1 : 2)];
+    // of each wave, to be joined
     float o[kThreads / kWave][kMaxGroup][D + 4], m[kThreads / kWave][16], l[kThreads / kWave][16];
   };
-  __shared__ alignas(1024) union { Stages st; Join join; } shared;
+  __shared__ alignas(1024) union { Stages st; Suffix suffix; } shared;
   Stages& lds = shared.st;
   const rlk_attention_params& p = a.p;
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -353,9 +390,9 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
     }
     float m, l;
     f32x4 o[D / 16];
-    attend_alone<D, kFmt>(a, table, kvh, b0, b1, q, m, l, o);
+    attend_alone<D, kFmt>(a, table, kvh, b0, b1, q, shared.suffix.k[wave], m, l, o);
     // the waves joined
-    Join& j = shared.join;
+    Suffix& j = shared.suffix;
     if (lane < 16) {
       j.m[wave][lane] = m;
       j.l[wave][lane] = l;
@@ -414,12 +451,11 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
   // this thread's part of a tile; lane k finds the cell of key k % 32
   const int ch = tid % kChunks, tr = tid / kChunks;
   const int32_t* table = p.block_tables + static_cast<int64_t>(seq) * p.max_blocks_per_seq;
-  const int lbs = (bs & (bs - 1)) == 0 ? __builtin_ctz(bs) : -1;
   u32x4 kraw[kAhead][kItems], vraw[kAhead][kItems];
   float sc[kAhead];  // INT8: wave 0 has the K scales, wave 1 the V scales
   struct Cell { int id, off; };
   auto find = [&](int k0) -> Cell {
-    const int pos = min(k0 + lane % kTile, end - 1), b = lbs >= 0 ? pos >> lbs : pos / bs;
+    const int pos = min(k0 + lane % kTile, end - 1), b = block_of(a, pos);
     return {table[b], pos - b * bs};
   };
   auto request = [&](int u, Cell at) {
@@ -720,6 +756,11 @@ extern "C" int rlk_paged_attention_decode_shared(const rlk_attention_params* p, 
   SharedArgs a = {};
   a.p = *p;
   a.w = *w;
+  while ((int64_t{1} << a.lbs) < kv.block_size) ++a.lbs;
+  if ((int64_t{1} << a.lbs) != kv.block_size) {  // exact for keys below 2^31
+    a.magic = static_cast<uint32_t>((int64_t{1} << (31 + a.lbs)) / kv.block_size + 1);
+    --a.lbs;
+  }
   a.grp = G;
   const int fmt = kv.dtype == RLK_KV_FP16 ? kF16 : (scale_dtype == RLK_SCALE_F16 ? kI8Half : kI8);
   if (kv.head_dim == 128) {
