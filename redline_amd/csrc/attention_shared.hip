@@ -145,7 +145,7 @@ __device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t*
   constexpr int E = D / 16, kElem = kInt8 ? 1 : 2, kAhead = 2, kKeys = 32;
   constexpr int kAheadV = kInt8 ? 2 : 1;  // (FP16: with two tiles the registers do not suffice)
   // K: whole rows by consecutive lanes.  Loaded as the operands want them, a row a lane, the address
-  // unit took the lanes of an instruction one by one (35 ns a key and wave against 1X).
+  // unit took the lanes of an instruction one by one (64 items over 32 k: 87 us against 73).
   constexpr int kRow = D * kElem, kChunks = kRow / 16, kRowsAtOnce = kWave / kChunks, kLoads = kKeys / kRowsAtOnce;
   using VRaw = typename RawOf<E * kElem>::Type;
   const rlk_kv_layer_view& kv = a.p.kv;

@@ -10,10 +10,11 @@
 //
 // The mapping is that of the plain RoPE kernel: a lane owns 8 pairs, a head is
 // D/16 lanes, so the sum of squares is 16 products in the lane and 2 or 3 DPP
-// steps; one token per workgroup, its heads spread over the waves.  An axis of a
-// pair is two bits of the launch arguments.  Where every lane's 8 pairs share an
-// axis (sections of whole eights) a lane loads its own axis' position and then
-// cos/sin as vectors; otherwise it gathers a cos and a sin per pair.
+// steps; one token per workgroup, its heads spread over the waves.  With one axis a
+// lane loads its 8 cos and sin as vectors.  With several, an axis of a pair is two bits
+// of the launch arguments, and the first D/2 threads gather a cos and a sin each into
+// LDS for all heads (every lane for itself, 16 gathers: 19.4 us against 15.2 for 5024
+// tokens of 40 heads of 64).
 // Bound: HBM, as the plain kernel; at a decode step's size the launch.
 #include <hip/hip_runtime.h>
 
@@ -27,7 +28,7 @@
 namespace rlk {
 namespace {
 
-// How a lane finds its pairs' positions.
+// How the pairs' axes lie: one for all, one for every lane's 8 pairs, or in any order.
 enum Axes { kOne, kPerLane, kPerPair };
 
 struct NormRopeArgs {
@@ -46,7 +47,7 @@ struct NormRopeArgs {
 };
 
 template <int D, bool kInt8, int kAxes>
-__global__ __launch_bounds__(512) void norm_rope_kv_kernel(NormRopeArgs a) {
+__global__ __launch_bounds__(512, kInt8 ? 1 : 8) void norm_rope_kv_kernel(NormRopeArgs a) {
 #pragma clang fp contract(off)  // without norms the bits of the plain kernel
   constexpr bool NT = true;
   constexpr int kHalf = D / 2, kLPH = kHalf / 8, kHeadsPerWave = kWave / kLPH;
@@ -55,38 +56,45 @@ __global__ __launch_bounds__(512) void norm_rope_kv_kernel(NormRopeArgs a) {
   const int hg = wave * kHeadsPerWave + lane / kLPH, part = lane % kLPH, p0 = part * 8;
   const int heads = a.hq + 2 * a.hkv;
   const int64_t t = blockIdx.x;
-  if (hg >= heads) return;  // whole heads leave together
   _Float16* row = a.qkv + t * heads * D;
-  u32x4 v0 = ld16<NT>(reinterpret_cast<const u32x4*>(row + hg * D + p0));
-  u32x4 v1 = ld16<NT>(reinterpret_cast<const u32x4*>(row + hg * D + kHalf + p0));
+  u32x4 v0, v1;
+  if (hg < heads) {
+    v0 = ld16<NT>(reinterpret_cast<const u32x4*>(row + hg * D + p0));
+    v1 = ld16<NT>(reinterpret_cast<const u32x4*>(row + hg * D + kHalf + p0));
+  }
   const int slot = a.slots[t];
   f32x8 c, s;
-  if constexpr (kAxes == kPerPair) {
-    int pos[4];
+  // the token's positions are uniform: scalar loads, selected by axis
+  int pos[kAxes == kOne ? 1 : RLK_ROPE_MAX_AXES];
+  pos[0] = a.positions[t];
+  if constexpr (kAxes != kOne) {
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-      pos[x] = a.positions[static_cast<int64_t>(x < a.num_axes ? x : 0) * a.num_tokens + t];
-    uint32_t bits = 0;
+    for (int x = 1; x < RLK_ROPE_MAX_AXES; ++x)
+      pos[x] = a.positions[static_cast<int64_t>(min(x, a.num_axes - 1)) * a.num_tokens + t];
+  }
+  auto position_of = [&](int pair) -> int64_t {
+    if constexpr (kAxes == kOne) return pos[0];
+    else {
+      uint32_t bits = a.axis[0];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) bits = part / 2 == w ? a.axis[w] : bits;
-    bits >>= 16 * (part % 2);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t x = (bits >> (2 * j)) & 3;
+      for (int w = 1; w < D / 32; ++w) bits = pair / 16 == w ? a.axis[w] : bits;
+      const uint32_t x = bits >> (2 * (pair % 16)) & 3;
       const int lo = x & 1 ? pos[1] : pos[0], hi = x & 1 ? pos[3] : pos[2];
-      const int64_t at = static_cast<int64_t>(x & 2 ? hi : lo) * kHalf + p0 + j;
-      c[j] = a.cos_t[at];
-      s[j] = a.sin_t[at];
+      return x & 2 ? hi : lo;
     }
+  };
+  if constexpr (kAxes == kPerPair) {
+    __shared__ f32x4 turn[2][kHalf / 4];
+    for (int i = threadIdx.x; i < kHalf; i += blockDim.x) {
+      const int64_t at = position_of(i) * kHalf + i;
+      reinterpret_cast<float*>(turn[0])[i] = a.cos_t[at];
+      reinterpret_cast<float*>(turn[1])[i] = a.sin_t[at];
+    }
+    __syncthreads();
+    c = __builtin_shufflevector(turn[0][2 * part], turn[0][2 * part + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+    s = __builtin_shufflevector(turn[1][2 * part], turn[1][2 * part + 1], 0, 1, 2, 3, 4, 5, 6, 7);
   } else {
-    int64_t axis = 0;
-    if constexpr (kAxes == kPerLane) {
-      uint32_t bits = 0;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) bits = part / 2 == w ? a.axis[w] : bits;
-      axis = (bits >> (16 * (part % 2))) & 3;
-    }
-    const int64_t at = static_cast<int64_t>(a.positions[axis * a.num_tokens + t]) * kHalf + p0;
+    const int64_t at = position_of(p0) * kHalf + p0;
     const f32x4* cp = reinterpret_cast<const f32x4*>(a.cos_t + at);
     const f32x4* sp = reinterpret_cast<const f32x4*>(a.sin_t + at);
     c = __builtin_shufflevector(cp[0], cp[1], 0, 1, 2, 3, 4, 5, 6, 7);
@@ -142,7 +150,7 @@ void launch_axes(const NormRopeArgs& a, Axes axes, int waves, hipStream_t stream
   }
 }
 
-// The axis of each of the `half` pairs into `axis`, two bits a pair; RLK_OK or a
+// The axis of each of the `half` pairs into `bits`, two bits a pair; RLK_OK or a
 // failure status.
 int axes_of_pairs(const rlk_norm_rope_options& o, int half, uint32_t (&bits)[4], Axes* axes, const char* what) {
   for (uint32_t& b : bits) b = 0;

@@ -360,9 +360,11 @@ def _one_device(dev, *tensors):
 
 def _arg(t, dtype, what, n, dev):
     """_ptr of a tensor of at least n elements on device dev, with the checks in one call."""
-    if (isinstance(t, torch.Tensor) and t.dtype == dtype and t.is_cuda and t.is_contiguous()
-            and t.numel() >= n and (dev is None or t.get_device() == dev)):
-        return t.data_ptr()
+    try:  # (dev -1, of a cache on the CPU, ends at _stream_on)
+        if t.dtype is dtype and t.get_device() == dev and t.is_contiguous() and t.numel() >= n:
+            return t.data_ptr()
+    except AttributeError:
+        pass
     p = _ptr(t, dtype, what)  # says which check fails
     _need(t, n, what)
     _one_device(dev, t)
@@ -596,22 +598,23 @@ def rope_and_write_kv_norm(qkv, positions, slot_mapping, num_tokens, num_heads, 
     (q_norm, k_norm fp16 [D] or None) before the rotation, and a rotation by several
     position axes: `sections` are the pairs of each (D/2 in all), positions then
     [len(sections), num_tokens]."""
-    n, dev, sections = max(num_tokens, 0), kv.device, tuple(sections or ())
-    if len(sections) > kRopeMaxAxes:
-        raise _lib.Error(_lib.RLK_EINVAL, f"{len(sections)} position axes (at most {kRopeMaxAxes})")
+    n, dev, f16, i32, f32 = max(num_tokens, 0), kv.device, torch.float16, torch.int32, torch.float32
     if scale_dtype != kv.scale_dtype:
         _scales(kv, scale_dtype)
     dim = kv.head_dim if n > 0 else 0
     cols = (num_heads + 2 * kv.num_kv_heads) * dim
-    half = lambda t, m, w: None if t is None else _arg(t, torch.float16, w, m, dev)  # noqa: E731
-    opt = _lib.NormRopeOptions(half(q_norm, dim, "q_norm"), half(k_norm, dim, "k_norm"), eps,
-                               half(qkv_bias, cols, "qkv_bias"), scale_dtype, len(sections), sections,
-                               bool(interleaved))
+    opt = _lib.NormRopeOptions(None if q_norm is None else _arg(q_norm, f16, "q_norm", dim, dev),
+                               None if k_norm is None else _arg(k_norm, f16, "k_norm", dim, dev), eps,
+                               None if qkv_bias is None else _arg(qkv_bias, f16, "qkv_bias", cols, dev), scale_dtype)
+    axes = len(sections) if sections else 0
+    if axes:
+        if axes > kRopeMaxAxes:
+            raise _lib.Error(_lib.RLK_EINVAL, f"{axes} position axes (at most {kRopeMaxAxes})")
+        opt.num_axes, opt.sections, opt.interleaved = axes, tuple(sections), bool(interleaved)
     check(lib().rlk_rope_and_write_kv_norm(
-        _arg(qkv, torch.float16, "qkv", n * cols, dev),
-        _arg(positions, torch.int32, "positions", n * max(1, len(sections)), dev),
-        _arg(slot_mapping, torch.int32, "slot_mapping", n, dev), num_tokens, num_heads,
-        _arg(cos_table, torch.float32, "cos_table", 0, dev), _arg(sin_table, torch.float32, "sin_table", 0, dev),
+        _arg(qkv, f16, "qkv", n * cols, dev), _arg(positions, i32, "positions", n * max(1, axes), dev),
+        _arg(slot_mapping, i32, "slot_mapping", n, dev), num_tokens, num_heads,
+        _arg(cos_table, f32, "cos_table", 0, dev), _arg(sin_table, f32, "sin_table", 0, dev),
         C.byref(kv), C.byref(opt), _stream_on(dev, stream)))
 
 
