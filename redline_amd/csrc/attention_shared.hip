@@ -50,6 +50,7 @@ constexpr int kWaveRows = 32;
 constexpr int kRows = kThreads / kWave * kWaveRows;  // of a workgroup
 constexpr int kPart = RLK_DECODE_PARTITION_SIZE;
 constexpr int kMaxGroup = 8;            // query heads of a kv head
+constexpr int kFewRows = 16;            // of units without shared tiles
 constexpr int64_t kMaxBlocks = 1 << 30;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -62,6 +63,7 @@ struct SharedArgs {
   int prefix_keys, suffix_keys;      // keys of a unit, whole tiles
   int prefix_splits, suffix_splits;  // units of the longest prefix, of the longest rest
   int row_tiles;
+  int few_rows;  // units of at most so many rows go by tiles of 16
   uint32_t prefix_blocks;
   // key / block_size = key >> lbs where magic is 0, else umulhi(key, magic) >> lbs
   uint32_t magic;
@@ -136,10 +138,10 @@ template <> struct RawOf<16> { using Type = u32x4; };
 template <> struct RawOf<8> { using Type = u32x2; };
 template <> struct RawOf<4> { using Type = uint32_t; };
 
-// One wave's part of a suffix unit: keys [begin, end) of the table row, the kv head's G rows.
-// In: q as B operands; kbuf: 32 rows of K in LDS, this wave's own.  Out: m, l and o[dt][i] = dim E (4 (lane / 16) + i) + dt of row lane % 16.
+// One wave's part of a unit of up to 16 rows: keys [begin, end) of the table row, for row lane % 16
+// those below `last`.  In: q as B operands; kbuf: 32 rows of K in LDS, this wave's own.  Out: m, l and o[dt][i] = dim E (4 (lane / 16) + i) + dt of row lane % 16.
 template <int D, int kFmt>
-__device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t* table, int kvh, int begin, int end,
+__device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t* table, int kvh, int begin, int end, int last,
                                              const f16x8 (&q)[D / 32], unsigned char* kbuf, float& m, float& l, f32x4 (&o)[D / 16]) {
   constexpr bool kInt8 = kFmt != kF16;
   constexpr int E = D / 16, kElem = kInt8 ? 1 : 2, kAhead = 2, kKeys = 32;
@@ -156,6 +158,10 @@ __device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t*
 #pragma unroll
   for (int d = 0; d < E; ++d) o[d] = f32x4{0, 0, 0, 0};
   if (begin >= end) return;
+  int whole = last;  // every row has the keys up to this one
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) whole = min(whole, __shfl_xor(whole, o, kWave));
+  whole = __builtin_amdgcn_readfirstlane(min(whole, end));
 
   struct Cell { int id, off; };
   auto find = [&](int k0) -> Cell {  // of key lane % 32 of a tile
@@ -233,13 +239,13 @@ __device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t*
     request_k(u, cells[u]);
     cells[u] = next;
     __builtin_amdgcn_sched_barrier(0);
-    const bool tail = k0 + kKeys > end;
-    if (tail) {
+    if (k0 + kKeys > whole) {
+      const int left = min(last, end) - k0 - 4 * kg;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (k0 + 16 * t + 4 * kg + i >= end) s[t][i] = -INFINITY;
+          if (16 * t + i >= left) s[t][i] = -INFINITY;
     }
     float mx = s[0][0];
 #pragma unroll
@@ -265,7 +271,7 @@ __device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t*
     VRaw row[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) row[j] = vr[u % kAheadV][j];
-    if (tail) {
+    if (k0 + kKeys > end) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (k0 + 16 * (j / 4) + 4 * kg + j % 4 >= end) row[j] = VRaw{};
@@ -335,7 +341,8 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
   struct Suffix {
     unsigned char k[kThreads / kWave][32 * D * (kInt8 ? 1 : 2)];
     // of each wave, to be joined
-    float o[kThreads / kWave][kMaxGroup][D + 4], m[kThreads / kWave][16], l[kThreads / kWave][16];
+    float o[kThreads / kWave][kFewRows][D + 4], m[kThreads / kWave][16], l[kThreads / kWave][16];
+    int token[16];
   };
   __shared__ alignas(1024) union { Stages st; Suffix suffix; } shared;
   Stages& lds = shared.st;
@@ -345,7 +352,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
   const int hkv = p.kv.num_kv_heads, bs = p.kv.block_size, G = a.grp;
 
   // the unit
-  int kvh, first, rows, row0, begin, end, slot, seq;
+  int kvh, first, rows, row0 = 0, begin, end, slot;
   if (blockIdx.x < a.prefix_blocks) {
     // the row tiles of a range stand 8 blocks apart: on one XCD, whose L2 has the range
     const int b = blockIdx.x / 8, rt = b % a.row_tiles, u = b / a.row_tiles * 8 + blockIdx.x % 8;
@@ -355,12 +362,11 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
     first = a.w.group_start[g];
     const int n = min(min(a.w.group_start[g + 1], a.w.num_items) - first, a.w.max_group_items);
     rows = n * G;
-    row0 = rt * kRows;
+    row0 = rt * (rows <= a.few_rows ? kFewRows : kRows);
     if (first < 0 || rows <= row0) return;
     begin = split * a.prefix_keys;
     end = min(prefix_of(a, g), begin + a.prefix_keys);
     slot = split;
-    seq = a.w.item_seq[first];
   } else {
     const int u = static_cast<int>(blockIdx.x - a.prefix_blocks);
     const int split = u % a.suffix_splits, ik = u / a.suffix_splits;
@@ -368,6 +374,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
     kvh = ik - first * hkv;
     const int token = a.w.item_token[first];
     if (token < 0) return;
+    rows = G;
     const int prefix = shared_prefix(a, first);
     const int64_t keys = min(static_cast<int64_t>(keys_of(a, token)),
                              prefix + static_cast<int64_t>(a.w.max_partitions) * kPart);
@@ -375,50 +382,60 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
     if (at >= keys) return;
     begin = static_cast<int>(at);
     end = static_cast<int>(min(keys, at + a.suffix_keys));
-    const int32_t* table = p.block_tables + static_cast<int64_t>(a.w.item_seq[first]) * p.max_blocks_per_seq;
-    // a wave's keys: whole tiles but for the last
+    slot = a.w.max_prefix_partitions + split;
+  }
+  if (begin >= end) return;
+  const int32_t* table = p.block_tables + static_cast<int64_t>(a.w.item_seq[first]) * p.max_blocks_per_seq;
+
+  if (rows <= a.few_rows) {
+    // the tile's rows; a wave's keys, whole tiles but for the last
+    const int here = min(rows - row0, kFewRows);
     constexpr int kWaves = kThreads / kWave;
     const int per = ((end - begin + kWaves - 1) / kWaves + 31) / 32 * 32;
     const int b0 = min(begin + wave * per, end), b1 = min(b0 + per, end);
+    const int r = lane % 16, item = first + (row0 + r) / G, token = r < here ? a.w.item_token[item] : -1;
+    int last = end;
     f16x8 q[D / 32];
 #pragma unroll
-    for (int x = 0; x < D / 32; ++x) {
-      q[x] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
-      if (lane % 16 < G)
-        q[x] = signed_by(p.scale, load16(reinterpret_cast<const _Float16*>(p.q) + static_cast<int64_t>(token) * p.q_stride +
-                                         (kvh * G + lane % 16) * D + 32 * x + 8 * (lane / 16)));
+    for (int x = 0; x < D / 32; ++x) q[x] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    if (token >= 0) {
+      last = keys_of(a, token);
+      const _Float16* qp = reinterpret_cast<const _Float16*>(p.q) + static_cast<int64_t>(token) * p.q_stride + (kvh * G + (row0 + r) % G) * D + 8 * (lane / 16);
+#pragma unroll
+      for (int x = 0; x < D / 32; ++x) q[x] = signed_by(p.scale, load16(qp + 32 * x));
     }
     float m, l;
     f32x4 o[D / 16];
-    attend_alone<D, kFmt>(a, table, kvh, b0, b1, q, shared.suffix.k[wave], m, l, o);
+    attend_alone<D, kFmt>(a, table, kvh, b0, b1, last, q, shared.suffix.k[wave], m, l, o);
     // the waves joined
     Suffix& j = shared.suffix;
     if (lane < 16) {
       j.m[wave][lane] = m;
       j.l[wave][lane] = l;
+      j.token[lane] = token;
     }
-    if (lane % 16 < G) {
+    if (r < here) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int d = 0; d < D / 16; d += 4)
-          *reinterpret_cast<f32x4*>(&j.o[wave][lane % 16][D / 16 * (4 * (lane / 16) + i) + d]) =
+          *reinterpret_cast<f32x4*>(&j.o[wave][r][D / 16 * (4 * (lane / 16) + i) + d]) =
               f32x4{o[d][i], o[d + 1][i], o[d + 2][i], o[d + 3][i]};
     }
     __syncthreads();
-    slot = a.w.max_prefix_partitions + split;
-    for (int e = tid; e < G * D; e += kThreads) {
-      const int r = e / D, d = e % D;
-      float M = j.m[0][r], L = 0.f, sum = 0.f;
+    for (int e = tid; e < here * D; e += kThreads) {
+      const int x = e / D, d = e % D;
+      if (j.token[x] < 0) continue;
+      float M = j.m[0][x], L = 0.f, sum = 0.f;
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) M = fmaxf(M, j.m[w][r]);
+      for (int w = 1; w < kWaves; ++w) M = fmaxf(M, j.m[w][x]);
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
-        const float f = __builtin_amdgcn_exp2f(j.m[w][r] - M);
-        L += f * j.l[w][r];
-        sum += f * j.o[w][r][d];
+        const float f = __builtin_amdgcn_exp2f(j.m[w][x] - M);
+        L += f * j.l[w][x];
+        sum += f * j.o[w][x][d];
       }
-      const int64_t to = slot_row(a, first, kvh * G + r) + slot;
+      const int64_t to = slot_row(a, first + (row0 + x) / G, kvh * G + (row0 + x) % G) + slot;
       a.w.ws_out[to * D + d] = sum;
       if (d == 0) {
         a.w.ws_max[to] = M;
@@ -427,7 +444,6 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
     }
     return;
   }
-  if (begin >= end) return;
 
   // the lane's row
   const bool busy = row0 + wave * kWaveRows < rows;  // the wave has rows
@@ -450,7 +466,6 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
 
   // this thread's part of a tile; lane k finds the cell of key k % 32
   const int ch = tid % kChunks, tr = tid / kChunks;
-  const int32_t* table = p.block_tables + static_cast<int64_t>(seq) * p.max_blocks_per_seq;
   u32x4 kraw[kAhead][kItems], vraw[kAhead][kItems];
   float sc[kAhead];  // INT8: wave 0 has the K scales, wave 1 the V scales
   struct Cell { int id, off; };
@@ -683,11 +698,17 @@ int launch(SharedArgs a, const char* what, hipStream_t stream) {
     const int64_t keys = static_cast<int64_t>(partitions) * kPart, want = std::max<int64_t>(1, (want_each + units - 1) / units);
     return static_cast<int>(std::max<int64_t>((keys + want - 1) / want + kTile - 1, kPart) / kTile * kTile);
   };
-  a.row_tiles = (std::min(a.w.max_group_items, a.w.num_items) * a.grp + kRows - 1) / kRows;
+  // Up to 48 rows a group: tiles of 16 rows whose waves split the keys; four waves of keys outweigh
+  // reading a range up to three times, from L2 (24 rows over 24 k, D = 64, INT8: 25.7 us against 35.3).  In a call
+  // with larger groups too only groups of one such tile.
+  const int most_rows = std::min(a.w.max_group_items, a.w.num_items) * a.grp;
+  a.few_rows = most_rows <= 3 * kFewRows ? 3 * kFewRows : kFewRows;
+  const int tile_rows = most_rows <= a.few_rows ? kFewRows : kRows;
+  a.row_tiles = (most_rows + tile_rows - 1) / tile_rows;
   int64_t blocks = 0;
   if (pp > 0) {
     const int64_t tiles = std::min<int64_t>(static_cast<int64_t>(a.w.num_groups) * a.row_tiles,
-                                            static_cast<int64_t>(a.w.num_items) * a.grp / kRows + a.w.num_groups);
+                                            static_cast<int64_t>(a.w.num_items) * a.grp / tile_rows + a.w.num_groups);
     a.prefix_keys = keys_of_unit(pp, tiles * hkv);
     a.prefix_splits = (pp * kPart + a.prefix_keys - 1) / a.prefix_keys;
     const int64_t ranges = a.w.num_groups * hkv * a.prefix_splits;
