@@ -650,36 +650,51 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
 }
 
 // Joins the partials of one (item, head): lane d of the workgroup takes dim d; each
-// wave holds the weights of 64 slots, one a lane.
+// wave holds the weights of 64 slots, one a lane.  The statistics of the first 64 are
+// requested before it is known which of them were written.
 template <int D>
 __global__ __launch_bounds__(D) void shared_merge_kernel(SharedArgs a) {
   constexpr int kUnroll = 8;
   const int item = blockIdx.x, head = blockIdx.y, d = threadIdx.x, lane = d % kWave;
-  const int token = a.w.item_token[item];
+  const int total = a.w.max_prefix_partitions + a.w.max_partitions;
+  const int64_t row = slot_row(a, item, head);
+  float ms = a.w.ws_max[row + min(lane, total - 1)], ls = a.w.ws_sum[row + min(lane, total - 1)];
+  const int token = a.w.item_token[item], prefix = shared_prefix(a, item);
   if (token < 0) return;
-  const int keys = keys_of(a, token), prefix = shared_prefix(a, item);
+  const int keys = keys_of(a, token);
   const int np = (prefix + a.prefix_keys - 1) / max(a.prefix_keys, 1);
   const int rest = min(max(keys - prefix, 0), a.w.max_partitions * kPart);
-  const int slots = np + (rest + a.suffix_keys - 1) / a.suffix_keys;
-  const int64_t row = slot_row(a, item, head);
-  auto slot_of = [&](int j) { return row + (j < np ? j : a.w.max_prefix_partitions + j - np); };
+  const int ns = (rest + a.suffix_keys - 1) / a.suffix_keys;
   float M = -FLT_MAX, L = 0.f, o = 0.f;
-  for (int j0 = 0; j0 < slots; j0 += kWave) {
-    const int here = min(slots - j0, kWave);
-    const int64_t mine = slot_of(min(j0 + lane, slots - 1));
-    const float ms = lane < here ? a.w.ws_max[mine] : -FLT_MAX, ls = lane < here ? a.w.ws_sum[mine] : 0.f;
-    const float mn = fmaxf(M, rows_max<true>(rows_max<false>(group_max<16>(ms))));
-    const float f0 = __builtin_amdgcn_exp2f(M - mn), f = __builtin_amdgcn_exp2f(ms - mn);
-    L = L * f0 + wave_sum(f * ls);
+  for (int j0 = 0; j0 < total; j0 += kWave) {
+    const int j = j0 + lane;
+    const bool there = j < np || (j >= a.w.max_prefix_partitions && j - a.w.max_prefix_partitions < ns);
+    uint64_t left = __ballot(there);
+    if (left == 0) continue;
+    if (j0 > 0) {
+      ms = a.w.ws_max[row + min(j, total - 1)];
+      ls = a.w.ws_sum[row + min(j, total - 1)];
+    }
+    const float mine = there ? ms : -FLT_MAX;
+    const float mn = fmaxf(M, rows_max<true>(rows_max<false>(group_max<16>(mine))));
+    const float f0 = __builtin_amdgcn_exp2f(M - mn), f = there ? __builtin_amdgcn_exp2f(mine - mn) : 0.f;
+    L = L * f0 + wave_sum(there ? f * ls : 0.f);
     o *= f0;
     M = mn;
-    for (int s = 0; s < here; s += kUnroll) {
-      float v[kUnroll];
+    while (left != 0) {
+      float v[kUnroll], w[kUnroll];
+      int at = 0;
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) v[u] = a.w.ws_out[slot_of(j0 + min(s + u, here - 1)) * D + d];
+      for (int u = 0; u < kUnroll; ++u) {  // past the last one its row again, with no weight
+        const bool more = left != 0;
+        at = more ? __builtin_ctzll(left) : at;
+        left &= left - 1;
+        const float x = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), at));
+        w[u] = more ? x : 0.f;
+        v[u] = a.w.ws_out[(row + j0 + at) * D + d];
+      }
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (s + u < here) o += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s + u)) * v[u];
+      for (int u = 0; u < kUnroll; ++u) o += w[u] != 0.f ? w[u] * v[u] : 0.f;
     }
   }
   reinterpret_cast<_Float16*>(a.p.out)[(static_cast<int64_t>(token) * a.p.num_heads + head) * D + d] =
