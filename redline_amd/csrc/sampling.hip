@@ -19,12 +19,13 @@
 //             by up to 1e-7 of the whole, and of rows with 10^5 tokens to draw from some
 //             would change theirs.
 //   kernel 1  one chunk of 8192 a workgroup: the logits are read once, and the places of
-//             the tokens of its first bins (a quarter at most) go out in the bins' order.
+//             its tokens go out in the order of their bins, without those that top-k, or
+//             min-p as the only limit, leaves out for certain.
 //   kernel 2  one row a workgroup: chunks' bins summed and scanned, then for each limit
-//             and the draw the bin and its tokens, from the chunks' lists or, where a list
-//             ends before the bin, from the logits; narrowed to at most 128 by histograms of
-//             their keys (value, then index); of those every pair is compared.
-//   A row of one chunk of 8192 tokens is done by one workgroup from its registers.
+//             and the draw the bin and its tokens from the chunks' lists; narrowed to at most
+//             128 by histograms of their keys (value, then index); of those every pair is
+//             compared.
+//   A row of at most one chunk is done by one workgroup, its list in LDS.
 #include <hip/hip_runtime.h>
 
 #include <climits>
@@ -45,7 +46,6 @@ constexpr int kPer = 16;          // logits of a thread
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kChunk = kThreads * kPer;
-constexpr int kListed = kChunk / 4;  // tokens that a chunk lists at most
 constexpr int kMaxVocab = 1 << 20;
 constexpr int kMaxChunks = kMaxVocab / kChunk;
 constexpr int kCountShift = 49;   // count above, weight in 2^-34 below
@@ -63,7 +63,7 @@ struct SampleArgs {
   u64* hist;       // [rows, chunks, kBins]
   ChunkTop* top;   // [rows, chunks]
   uint16_t* start; // [rows, chunks, kBins] tokens before the bin
-  uint16_t* list;  // [rows, chunks, kListed] places in the chunk of the tokens of its first bins
+  uint16_t* list;  // [rows, chunks, kChunk] places in the chunk of its tokens, by bins
   int chunks;
 };
 
@@ -240,27 +240,30 @@ __device__ __forceinline__ bool bin_chunk(const void* src, int base, int vocab, 
   return true;
 }
 
-__device__ __forceinline__ float temperature_of(const SampleArgs& a, int row) {
-  return a.w.temperature[a.w.param_row != nullptr ? a.w.param_row[row] : row];
-}
-
 template <bool kF32>
 __global__ __launch_bounds__(kThreads) void sample_chunks_kernel(SampleArgs a) {
   constexpr int kScan = kBins / 2;  // threads that scan, two bins each
   __shared__ ChunkLds s;
-  __shared__ alignas(16) uint16_t list[kListed];
+  __shared__ alignas(16) uint16_t list[kChunk];
   __shared__ int cursor[kBins];
   __shared__ int wave_sum[kScan / kWave];
   __shared__ int listed[2];  // bins and tokens of the list
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const int row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks, base = chunk * kChunk;
   const void* src = row_of<kF32>(a, row);
-  const float T = temperature_of(a, row);
+  const int pr = a.w.param_row != nullptr ? a.w.param_row[row] : row;
+  const float T = a.w.temperature[pr], least = a.w.min_p != nullptr ? fminf(a.w.min_p[pr], 1.f) : 0.f;
+  // Bins behind top_k of the chunk's tokens are not listed; nor, where min_p is the only limit,
+  // those of less than min_p of the chunk's largest (two more: one for the largest's place in its
+  // own bin, one for the logarithm's error).
+  const int k = a.w.top_k[pr], most = k > 0 ? k : kChunk;
+  const bool cut = least > 0.f && k <= 0 && !(a.w.top_p[pr] < 1.f);
+  const int bins = cut ? static_cast<int>(fminf(-8.f * __log2f(least), 1e4f)) + 3 : kBins;
   const int64_t rec = static_cast<int64_t>(row) * a.chunks + chunk;
   float l[kPer];
   int d[kPer];
   ChunkTop top;
-  if (tid == 0) listed[0] = kBins;
+  if (tid == 0) listed[0] = min(bins, kBins);
   const bool binned = bin_chunk<kF32>(src, base, a.w.vocab, T, s, l, d, &top);
   if (tid == 0) a.top[rec] = top;
   if (!binned) return;
@@ -282,20 +285,18 @@ __global__ __launch_bounds__(kThreads) void sample_chunks_kernel(SampleArgs a) {
     cursor[2 * tid] = before;
     cursor[2 * tid + 1] = mid;
     reinterpret_cast<uint32_t*>(a.start + rec * kBins)[tid] = static_cast<uint32_t>(before) | static_cast<uint32_t>(mid) << 16;
-    if (before <= kListed && end > kListed) {
-      listed[0] = mid > kListed ? 2 * tid : 2 * tid + 1;
-      listed[1] = mid > kListed ? before : mid;
-    } else if (tid == kScan - 1 && end <= kListed) {
-      listed[1] = end;
-    }
+    // the first bin that is not listed: `most` tokens stand before it
+    if (before < most && end >= most) atomicMin(&listed[0], mid >= most ? 2 * tid + 1 : 2 * tid + 2);
   }
   __syncthreads();
-  const int nb = listed[0], nt = listed[1];
+  const int nb = listed[0];
+  if (tid == (nb - 1) / 2) listed[1] = before + c0 + ((nb & 1) != 0 ? 0 : c1);
 #pragma unroll
   for (int j = 0; j < kPer; ++j)
     if (d[j] < nb) list[atomicAdd(&cursor[d[j]], 1)] = static_cast<uint16_t>(j * kThreads + tid);
   __syncthreads();
-  u32x4* dst = reinterpret_cast<u32x4*>(a.list + rec * kListed);
+  const int nt = listed[1];
+  u32x4* dst = reinterpret_cast<u32x4*>(a.list + rec * kChunk);
   for (int i = tid; 8 * i < nt; i += kThreads) dst[i] = reinterpret_cast<const u32x4*>(list)[i];
 }
 
@@ -308,7 +309,7 @@ constexpr int kGroup = 16;    // lanes that read a chunk's list
 
 struct RowLds {
   ChunkLds chunk;              // kOne: of the row
-  uint16_t place[kChunk];      // kOne: the row's tokens in the order of their bins; else of a chunk without a list
+  uint16_t place[kChunk];      // kOne: the row's tokens in the order of their bins
   u64 key[kList + kFew], weight[kList + kFew];  // the tokens of one bin; from kList on what is left of a bin
   u64 few_upto[kFew];
   int few_place[kFew], few_bin[kFew];
@@ -318,8 +319,7 @@ struct RowLds {
   int count[kBins + 1];        // tokens before bin j
   double bin_scale[kBins];     // of whole-number weights
   int shift[kMaxChunks];       // of a chunk's bins; kBins: none
-  int raw[kMaxChunks];         // chunks whose lists end before the bin
-  int raws, n, m;
+  int n;
   u64 top[kWaves];
   u64 wave_u64[kWaves];
   double wave_f64[kWaves];
@@ -358,51 +358,34 @@ struct RowSampler {
 
   __device__ u64 weight(float v) const { return far ? kWeightOne : sc.weight(v, sc.bin(v)); }
 
-  // Every token of the bin (kAll: of at most kFew in all bins up to it) to f(key); by all threads.
+  // Every token of the bin (kAll: of all bins up to it) to f(key); by all threads.
   template <bool kAll = false, class F>
   __device__ void each(int bin, F f) {
     const ChunkLoad<kF32> ld(src);
-    auto give = [&](int base, int place) {
-      const int at = ld.index_of(base, place);
-      f(rank_key(logit<kF32>(src, at), at));
-    };
     if constexpr (kOne) {
-      for (int i = (kAll ? 0 : s.count[bin]) + tid; i < s.count[bin + 1]; i += kThreads) give(0, s.place[i]);
-    } else {
-      if constexpr (!kAll) {
-        __syncthreads();
-        if (tid == 0) s.raws = 0;
-        __syncthreads();
+      for (int i = (kAll ? 0 : s.count[bin]) + tid; i < s.count[bin + 1]; i += kThreads) {
+        const int at = ld.index_of(0, s.place[i]);
+        f(rank_key(logit<kF32>(src, at), at));
       }
+    } else {
       for (int c = tid / kGroup; c < a.chunks; c += kThreads / kGroup) {
         const int b = bin - s.shift[c];
         if (b < 0) continue;  // (no bins: shift kBins)
         const int64_t rec = static_cast<int64_t>(row) * a.chunks + c;
         const int n = static_cast<int>(a.hist[rec * kBins + b] >> kCountShift), at = a.start[rec * kBins + b];
-        if (at + n <= kListed) {
-          for (int i = (kAll ? 0 : at) + tid % kGroup; i < at + n; i += kGroup) give(c * kChunk, a.list[rec * kListed + i]);
-        } else if (n != 0 && tid % kGroup == 0) {
-          s.raw[atomicAdd(&s.raws, 1)] = c;
-        }
-      }
-      if constexpr (kAll) return;  // so few are always listed
-      __syncthreads();
-      const int nr = s.raws;
-#pragma unroll 1
-      for (int x = 0; x < nr; ++x) {
-        const int base = s.raw[x] * kChunk;
-        float v[kPer];
-        ld.load(src, base, tid, a.w.vocab, v);
-        if (tid == 0) s.m = 0;
-        __syncthreads();
+        const uint16_t* list = a.list + rec * kChunk;
+        constexpr int kUnroll = 4;
+        for (int i0 = (kAll ? 0 : at) + tid % kGroup; i0 < at + n; i0 += kUnroll * kGroup) {
+          int index[kUnroll];
+          float v[kUnroll];
 #pragma unroll
-        for (int j = 0; j < kPer; ++j)
-          if (far ? v[j] == mx : first - sc.bin(v[j]) == bin)
-            s.place[atomicAdd(&s.m, 1)] = static_cast<uint16_t>(j * kThreads + tid);
-        __syncthreads();
-        const int n = s.m;
-        for (int i = tid; i < n; i += kThreads) give(base, s.place[i]);
-        __syncthreads();
+          for (int x = 0; x < kUnroll; ++x) index[x] = ld.index_of(c * kChunk, list[min(i0 + x * kGroup, at + n - 1)]);
+#pragma unroll
+          for (int x = 0; x < kUnroll; ++x) v[x] = logit<kF32>(src, index[x]);
+#pragma unroll
+          for (int x = 0; x < kUnroll; ++x)
+            if (i0 + x * kGroup < at + n) f(rank_key(v[x], index[x]));
+        }
       }
     }
   }
@@ -887,7 +870,7 @@ size_t layout(int64_t rows, int vocab, SampleArgs* a) {
   take(to.hist, recs * kBins);
   take(to.top, recs);
   take(to.start, recs * kBins);
-  take(to.list, recs * kListed);
+  take(to.list, recs * kChunk);
   return n;
 }
 
