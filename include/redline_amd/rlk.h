@@ -505,10 +505,10 @@ typedef struct rlk_norm_rope_options {
                                has had fewer than its pairs, otherwise axis 0 */
 } rlk_norm_rope_options;
 
-/* NULL options: no norm, one axis; the bits of rlk_rope_and_write_kv_ex.  num_tokens <= 0: no-op.  head_dim not in
- * {64, 128}: RLK_EUNSUPPORTED.  qkv, tables, bias, norm weights and cache planes
- * 16-byte aligned, else RLK_EINVAL.  Rows whose slot is negative get their
- * rotated q and write no cell. */
+/* NULL options: no norm, one axis; the bits of rlk_rope_and_write_kv_ex.
+ * num_tokens <= 0: no-op.  head_dim not in {64, 128}: RLK_EUNSUPPORTED.  qkv, tables,
+ * bias, norm weights and cache planes 16-byte aligned, else RLK_EINVAL.  Rows whose
+ * slot is negative get their rotated q and write no cell. */
 int rlk_rope_and_write_kv_norm(uint16_t* qkv, const int32_t* positions, const int32_t* slot_mapping,
                                int num_tokens, int num_heads, const float* cos_table,
                                const float* sin_table, const rlk_kv_layer_view* kv,
@@ -555,11 +555,12 @@ typedef struct rlk_shared_prefix_work {
 } rlk_shared_prefix_work;
 
 /* options: RLK_SCALE_F32 or RLK_SCALE_F16 of an INT8 cache; NULL: RLK_SCALE_F32.
- * Keys past the sequence's table row are not read.  INT8 values enter the sums as
- * fp16(code * scale), as in prefill attention; a key's probability is rounded to
- * fp16, all else is held in fp32.  num_items <= 0: no-op.  head_dim not in {64, 128}
- * or more than 8 query heads a kv head: RLK_EUNSUPPORTED.  q and out rows and the
- * cache planes 16-byte aligned, else RLK_EINVAL. */
+ * Keys past the sequence's table row are not read.  A key's probability is rounded
+ * to fp16, of an INT8 cache after it has been multiplied by the key's V scale; K
+ * scales multiply the scores, codes are exact, all else is held in fp32.
+ * num_items <= 0: no-op.  head_dim not in {64, 128} or more than 8 query heads a kv
+ * head: RLK_EUNSUPPORTED.  A scale that is no finite number, more than 2^20 items or
+ * groups, or q and out rows and cache planes that are not 16-byte aligned: RLK_EINVAL. */
 int rlk_paged_attention_decode_shared(const rlk_attention_params* params, const rlk_shared_prefix_work* work,
                                       const rlk_attention_options* options, hipStream_t stream);
 
@@ -572,8 +573,9 @@ int rlk_paged_attention_decode_shared(const rlk_attention_params* params, const 
  *          mass before it is below top_p times the mass of the first top_k (>= 1,
  *          NaN: all); of those, the ones with w_j >= min_p; the first token always
  *   drawn  the first kept token with w_0 + ... + w_j > u (w_0 + ... + w_last kept)
- * T <= 0 or NaN: the first token.  min_p is held at 1 at most (NaN: 1).  u is held in [0, 1): below 0 and NaN as 0,
- * 1 and above as the largest below.  NaN logits count as -infinity; tokens of
+ * T <= 0 or NaN: the first token.  min_p is held at 1 at most (NaN: 1).  u is held in
+ * [0, 1): below 0 and NaN as 0, 1 and above as the largest below.  NaN logits count
+ * as -infinity; tokens of
  * -infinity are not drawn, but of a row that holds nothing else token 0 is.  Tokens
  * of +infinity share the draw.  Weights are held to 2^-35 of themselves, and those
  * below 2^-48 of the largest count as 0.  The same inputs give the same token,

@@ -73,7 +73,8 @@ def build_library(verbose: bool = True, only_changed: bool = False) -> Path:
     return LIB
 
 
-TEST_PROGRAMS = {"kernels_gpu": ROOT / "tests" / "cpp" / "kernels_gpu_main.cpp"}
+TEST_PROGRAMS = {"kernels_gpu": ROOT / "tests" / "cpp" / "kernels_gpu_main.cpp",
+                 "continuations_gpu": ROOT / "tests" / "cpp" / "continuations_gpu_main.cpp"}
 TEST_BIN = ROOT / "tests" / "cpp" / "bin"
 
 

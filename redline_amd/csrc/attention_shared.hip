@@ -10,7 +10,8 @@
 // through the caller's workspace.
 //
 // Prefix: tiles of 32 keys go through registers into LDS stages (INT8 codes become
-// fp16 on the way), the loads of the next three or four in flight while one is used.  A wave owns 32 rows:
+// fp16 on the way), the loads of the next three or four in flight while one is used, the
+// scores computed one tile ahead of the softmax.  A wave owns 32 rows:
 //   S^T = K Q^T    v_mfma_f32_32x32x16_f16, K rows from LDS, q in registers: a lane
 //                  gets one row (its column) and 16 of the tile's 32 keys, so the
 //                  softmax is per lane with one exchange between the lane halves;
@@ -18,13 +19,15 @@
 //                  the order in which S^T hands them over; V^T by transposing LDS reads.
 // LDS chunks of 16 bytes are XOR-ed with the row so that neither read has bank conflicts.
 //
-// Suffix: a wave owns a range of keys, without LDS or barriers until the four waves of a
-// unit are joined.  Tiles of 32 keys, the rows of two in flight, as v_mfma_f32_16x16x32_f16, K as A from rows as they
-// are loaded (16 keys x 32 dims), the G rows as B.  The lanes of key group g get the scores
-// of keys 4 g + i of both halves of the tile, which is their share of the B operand of
-// O^T = V^T P^T; as A a lane loads those 8 keys' dims E m .. E m + E - 1 (E = D / 16,
-// m = lane % 16), and tile dt of the output takes dim E m + dt: 8 x E values to be
-// transposed inside the lane, a byte permute per register.
+// Suffix, and prefixes of groups of few rows, by tiles of 16 rows: each of the four waves
+// owns a range of keys, without barriers until they are joined.  Tiles of 32 keys, the rows
+// of two in flight, as v_mfma_f32_16x16x32_f16: K as A (16 keys x 32 dims), loaded as
+// whole rows and laid out through a part of LDS that the wave alone uses, up to 16 rows
+// as B.  The lanes of key group g get the scores of keys 4 g + i of both halves of the
+// tile, which is their share of the B operand of O^T = V^T P^T; as A a lane loads those 8
+// keys' dims E m .. E m + E - 1 (E = D / 16, m = lane % 16), and tile dt of the output
+// takes dim E m + dt: 8 x E values to be transposed inside the lane, a byte permute per
+// register.
 //
 // INT8: K scales multiply the scores, V scales the probabilities before they are rounded,
 // so that codes stay exact and a value is rounded once, as in an FP16 cache.

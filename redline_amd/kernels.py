@@ -638,6 +638,8 @@ def shared_prefix_work(item_token, item_seq, num_items, group_start, group_prefi
     """What paged_attention_decode_shared works on (rlk_shared_prefix_work); `workspace`
     is a DecodeWorkspace of max_prefix_partitions + max_partitions partitions.  The
     struct keeps its tensors."""
+    if not isinstance(workspace, DecodeWorkspace):
+        raise _lib.Error(_lib.RLK_EINVAL, "workspace must be a DecodeWorkspace")
     i = lambda t, n, w: _arg(t, torch.int32, w, n, None)  # noqa: E731
     ws, groups = workspace, num_groups > 0
     work = _lib.SharedPrefixWork(
@@ -690,6 +692,8 @@ def sampling_work(logits, num_rows, vocab, temperature, top_k, top_p, uniform, t
     [num_rows, >= vocab], rows contiguous; without param_row, row r has the settings
     temperature[r], ...  Values of param_row must lie in the settings.  The struct keeps
     its tensors."""
+    if not isinstance(workspace, SamplingWorkspace):
+        raise _lib.Error(_lib.RLK_EINVAL, "workspace must be a SamplingWorkspace")
     if not isinstance(logits, torch.Tensor) or logits.dtype not in (torch.float16, torch.float32):
         raise _lib.Error(_lib.RLK_EINVAL, "logits must be a tensor of torch.float16 or torch.float32")
     if not logits.is_cuda:

@@ -316,3 +316,28 @@ def test_launchers_refuse(torch):
         with pytest.raises(ra.Error, match="no sampling workspace"):
             K.SamplingWorkspace(*args)
     K.sample_tokens(K.sampling_work(**(good | dict(num_rows=0))))  # nothing to do
+
+
+@pytest.mark.parametrize("V", [8191, 8192, 8193, 16384, 16385, 24575])
+def test_whole_chunks(torch, V):
+    """Vocabularies at the borders of the 8192 tokens that one workgroup takes."""
+    say("sample chunks", V)
+    rng = np.random.default_rng(V)
+    x = torch.randn(21, V, generator=torch.Generator(device="cuda").manual_seed(V), device="cuda") * 3
+    Call(torch, x, u=rng.random(21), **settings(rng, 21))().check()
+    Call(torch, x.half(), u=rng.random(21), **settings(rng, 21))().check()
+
+
+@pytest.mark.parametrize("T", [0.4, 1.0, 50.0])
+def test_limits_far_down_the_order(torch, T):
+    """Each limit, alone and with the others, whose border has thousands of tokens before it in
+    every chunk, and one chunk that holds the largest tokens."""
+    say("sample far limits", T)
+    grid = [dict(k=k, p=p, m=m, u=u) for k in (0, 127, 128, 129, 8191, 8192, 20000) for p in (1.0, 0.9999, 0.6)
+            for m in (0.0, 1e-7, 1e-3, 0.5) for u in (0.37, 0.9999)]
+    pick = {n: np.array([c[n] for c in grid]) for n in ("k", "p", "m", "u")}
+    x = torch.randn(1, 41000, generator=torch.Generator(device="cuda").manual_seed(6), device="cuda") * 2
+    x[:, 8192:16384] += 3
+    x = x.repeat(len(grid), 1)
+    Call(torch, x, T=T, **pick)().check()
+    Call(torch, x.half(), T=T, **pick)().check()

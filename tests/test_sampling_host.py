@@ -36,3 +36,10 @@ def test_workspace_and_nothing_to_do():
     n = size(3, 1000)
     assert call(bytes=n - 1) == EINVAL and call(rows=0) == 0 and call(rows=-1, logits=None) == 0
     assert ra.lib().rlk_sample_tokens(None, None) == EINVAL
+
+
+def test_the_workspace_is_one():
+    from redline_amd import kernels as K
+    for bad in (None, 5, "x"):
+        with pytest.raises(ra.Error, match="SamplingWorkspace"):
+            K.sampling_work(None, 1, 10, None, None, None, None, None, bad)

@@ -370,3 +370,17 @@ def test_launchers_refuse(torch):
         a = list(args)
         a[2] = n
         K.paged_attention_decode_shared(p, K.shared_prefix_work(*a, ws))  # nothing to do
+
+
+@pytest.mark.parametrize("heads", [(4, 4, 64, 16), (8, 4, 128, 16), (3, 1, 64, 24)], ids=lambda h: "x".join(map(str, h)))
+@pytest.mark.parametrize("cache", ["fp16", "int8"])
+def test_group_sizes_at_every_border(torch, heads, cache):
+    """Groups of 15 to 17, 47 to 49 and 127 to 129 rows, of one kind and all in one call."""
+    say("shared borders", heads, cache)
+    per = heads[0] // heads[1]
+    sizes = sorted({max(1, r // per + e) for r in (16, 48, 128) for e in (-1, 0, 1)})
+    for n in sizes:
+        c = Case(torch, [(600, [1 + i % 3 for i in range(n)]), (300, [70])], *heads, cache, n)
+        c.check(c.run())
+    c = Case(torch, [(97 + 61 * j, [2] * n) for j, n in enumerate(sizes)], *heads, cache, 31)
+    c.check(c.run())

@@ -44,3 +44,15 @@ def test_refusals(kw, status, text):
 def test_nothing_to_do():
     assert call(w=dict(items=0)) == 0 and call(w=dict(items=-1, token=None)) == 0
     assert ra.lib().rlk_paged_attention_decode_shared(None, None, None, None) == EINVAL
+
+
+def test_scales_that_are_no_number():
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        assert call(p=dict(scale=bad)) == EINVAL and b"finite" in ra.lib().rlk_last_error()
+
+
+def test_the_workspace_is_one():
+    from redline_amd import kernels as K
+    for bad in (None, 5, "x"):
+        with pytest.raises(ra.Error, match="DecodeWorkspace"):
+            K.shared_prefix_work(None, None, 1, None, None, 0, 0, 0, 1, bad)
