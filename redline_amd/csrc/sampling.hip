@@ -175,16 +175,25 @@ __device__ __forceinline__ T lanes_before(T v) {
 }
 
 struct ChunkLds {
-  u64 hist[kBins];
+  u64 hist[kBins + kWave];  // (one a lane for what has no bin, so that no lane branches)
   float max[kWaves];
   int index[kWaves];
 };
 
-// The logits of a chunk in registers, their bins below the chunk's largest (kBins: none)
-// and the chunk's histogram.  False: no bins are asked for.
+// A token's bin below the chunk's largest (kBins and above: none) and its place among those
+// of the bin, in any order: the count that its atomic found.
+struct Place {
+  uint32_t bits;
+  __device__ void set(int bin, u64 found) { bits = static_cast<uint32_t>(found >> kCountShift) << 16 | static_cast<uint32_t>(bin); }
+  __device__ int bin() const { return static_cast<int>(bits & 0xffffu); }
+  __device__ int place() const { return static_cast<int>(bits >> 16); }
+};
+
+// The logits of a chunk in registers, their places and the chunk's histogram.  False: no bins
+// are asked for.
 template <bool kF32>
 __device__ __forceinline__ bool bin_chunk(const void* src, int base, int vocab, float T, ChunkLds& s,
-                                          float (&l)[kPer], int (&d)[kPer], ChunkTop* top) {
+                                          float (&l)[kPer], Place (&d)[kPer], ChunkTop* top) {
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const ChunkLoad<kF32> ld(src);
   ld.load(src, base, tid, vocab, l);
@@ -216,24 +225,26 @@ __device__ __forceinline__ bool bin_chunk(const void* src, int base, int vocab, 
   if (sc.far(mx)) {
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      d[j] = l[j] == mx ? 0 : kBins;
-      if (d[j] == 0) atomicAdd(&s.hist[0], kCountOne + kWeightOne);
+      const int bin = l[j] == mx ? 0 : kBins + lane;
+      d[j].set(bin, atomicAdd(&s.hist[bin], kCountOne + kWeightOne));
     }
   } else {
     const double first = sc.bin(mx);
     constexpr int kAtOnce = 4;  // weights outside the branches, so that their chains overlap
 #pragma unroll
     for (int j0 = 0; j0 < kPer; j0 += kAtOnce) {
-      u64 w[kAtOnce];
+      u64 w[kAtOnce], found[kAtOnce];
+      int bin[kAtOnce];
 #pragma unroll
       for (int x = 0; x < kAtOnce; ++x) {
         const double b = sc.bin(l[j0 + x]), below = first - b;
-        d[j0 + x] = below < kBins ? static_cast<int>(below) : kBins;  // (kBins for NaN)
+        bin[x] = below < kBins ? static_cast<int>(below) : kBins + lane;  // (none for NaN)
         w[x] = sc.weight_bits(l[j0 + x], b) + (kCountOne - Scale::kBits);
       }
 #pragma unroll
-      for (int x = 0; x < kAtOnce; ++x)
-        if (d[j0 + x] < kBins) atomicAdd(&s.hist[d[j0 + x]], w[x]);
+      for (int x = 0; x < kAtOnce; ++x) found[x] = atomicAdd(&s.hist[bin[x]], w[x]);
+#pragma unroll
+      for (int x = 0; x < kAtOnce; ++x) d[j0 + x].set(bin[x], found[x]);
     }
   }
   __syncthreads();
@@ -245,7 +256,7 @@ __global__ __launch_bounds__(kThreads) void sample_chunks_kernel(SampleArgs a) {
   constexpr int kScan = kBins / 2;  // threads that scan, two bins each
   __shared__ ChunkLds s;
   __shared__ alignas(16) uint16_t list[kChunk];
-  __shared__ int cursor[kBins];
+  __shared__ int first[kBins];  // tokens before the bin
   __shared__ int wave_sum[kScan / kWave];
   __shared__ int listed[2];  // bins and tokens of the list
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
@@ -261,7 +272,7 @@ __global__ __launch_bounds__(kThreads) void sample_chunks_kernel(SampleArgs a) {
   const int bins = cut ? static_cast<int>(fminf(-8.f * __log2f(least), 1e4f)) + 3 : kBins;
   const int64_t rec = static_cast<int64_t>(row) * a.chunks + chunk;
   float l[kPer];
-  int d[kPer];
+  Place d[kPer];
   ChunkTop top;
   if (tid == 0) listed[0] = min(bins, kBins);
   const bool binned = bin_chunk<kF32>(src, base, a.w.vocab, T, s, l, d, &top);
@@ -282,8 +293,8 @@ __global__ __launch_bounds__(kThreads) void sample_chunks_kernel(SampleArgs a) {
 #pragma unroll
     for (int v = 0; v < kScan / kWave; ++v) before += v < wave ? wave_sum[v] : 0;
     const int mid = before + c0, end = mid + c1;
-    cursor[2 * tid] = before;
-    cursor[2 * tid + 1] = mid;
+    first[2 * tid] = before;
+    first[2 * tid + 1] = mid;
     reinterpret_cast<uint32_t*>(a.start + rec * kBins)[tid] = static_cast<uint32_t>(before) | static_cast<uint32_t>(mid) << 16;
     // the first bin that is not listed: `most` tokens stand before it
     if (before < most && end >= most) atomicMin(&listed[0], mid >= most ? 2 * tid + 1 : 2 * tid + 2);
@@ -293,7 +304,7 @@ __global__ __launch_bounds__(kThreads) void sample_chunks_kernel(SampleArgs a) {
   if (tid == (nb - 1) / 2) listed[1] = before + c0 + ((nb & 1) != 0 ? 0 : c1);
 #pragma unroll
   for (int j = 0; j < kPer; ++j)
-    if (d[j] < nb) list[atomicAdd(&cursor[d[j]], 1)] = static_cast<uint16_t>(j * kThreads + tid);
+    if (d[j].bin() < nb) list[first[d[j].bin()] + d[j].place()] = static_cast<uint16_t>(j * kThreads + tid);
   __syncthreads();
   const int nt = listed[1];
   u32x4* dst = reinterpret_cast<u32x4*>(a.list + rec * kChunk);
@@ -683,7 +694,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(SampleArgs a) {
   float u = a.w.uniform[row];
   u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;  // (NaN: 0)
   float l[kPer];
-  int d[kPer];
+  Place d[kPer];
   float mx;
   int top_index;
   if constexpr (kOne) {
@@ -798,12 +809,9 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(SampleArgs a) {
   }
   __syncthreads();
   if constexpr (kOne) {  // all places in the order of the bins
-    int* cursor = s.digit_count;
-    if (tid < kBins) cursor[tid] = s.count[tid];
-    __syncthreads();
 #pragma unroll
     for (int j = 0; j < kPer; ++j)
-      if (d[j] < kBins) s.place[atomicAdd(&cursor[d[j]], 1)] = static_cast<uint16_t>(j * kThreads + tid);
+      if (d[j].bin() < kBins) s.place[s.count[d[j].bin()] + d[j].place()] = static_cast<uint16_t>(j * kThreads + tid);
     __syncthreads();
   }
 
