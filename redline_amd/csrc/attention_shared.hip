@@ -59,7 +59,7 @@ constexpr int kRows = kThreads / kWave * kWaveRows;  // of a workgroup
 constexpr int kPart = RLK_DECODE_PARTITION_SIZE;
 constexpr int kMaxGroup = 8;            // query heads of a kv head
 constexpr int kFewRows = 16;            // of units without shared tiles
-constexpr int64_t kMaxBlocks = 1 << 30;
+constexpr int64_t kMaxBlocks = (int64_t{1} << 32) / kThreads - 1;  // (a grid has 32 bits of threads)
 constexpr float kLog2e = 1.4426950408889634f;
 
 enum Format { kF16, kI8, kI8Half };  // FP16 cells; INT8 with fp32, with fp16 scales

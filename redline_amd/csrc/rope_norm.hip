@@ -292,6 +292,8 @@ extern "C" int rlk_rope_and_write_kv_norm(uint16_t* qkv, const int32_t* position
   const int per_wave = kWave / (kv->head_dim / 16);
   const int waves = static_cast<int>(heads + per_wave - 1) / per_wave;
   const int w = waves > 8 ? 8 : waves;
+  if (static_cast<int64_t>(num_tokens) * w * kWave > UINT32_MAX)
+    return fail(RLK_EINVAL, "%s: %d tokens exceed one launch; split the call", what, num_tokens);
   const bool int8 = kv->dtype == RLK_KV_INT8;
   if (kv->head_dim == 128)
     int8 ? launch_axes<128, true>(a, axes, w, stream) : launch_axes<128, false>(a, axes, w, stream);

@@ -929,7 +929,7 @@ extern "C" int rlk_sample_tokens(const rlk_sampling_work* w, hipStream_t stream)
   SampleArgs a;
   a.w = *w;
   a.chunks = chunks_of(w->vocab);
-  if (static_cast<int64_t>(w->num_rows) * a.chunks > (1 << 30))
+  if (static_cast<int64_t>(w->num_rows) * a.chunks * kThreads > UINT32_MAX)
     return fail(RLK_EINVAL, "%s: %d rows exceed one launch; split the call", what, w->num_rows);
   layout(w->num_rows, w->vocab, &a);
   w->logits_fp32 ? launch<true>(a, stream) : launch<false>(a, stream);

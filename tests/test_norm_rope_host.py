@@ -65,3 +65,7 @@ def test_bad_arguments():
 def test_nothing_to_do():
     assert write(n=0) == 0 and write(n=-1, qkv=None) == 0 and read(n=0, slots=None) == 0
     assert read(k=None, v=None) == 0
+
+
+def test_more_tokens_than_a_launch_takes():
+    assert write(n=2 ** 31 - 1, heads=40) == EINVAL and b"split the call" in ra.lib().rlk_last_error()

@@ -43,3 +43,9 @@ def test_the_workspace_is_one():
     for bad in (None, 5, "x"):
         with pytest.raises(ra.Error, match="SamplingWorkspace"):
             K.sampling_work(None, 1, 10, None, None, None, None, None, bad)
+
+
+def test_more_rows_than_a_launch_takes():
+    for rows, vocab in ((1 << 23, 1000), (1 << 17, 1 << 20)):
+        assert call(rows=rows, vocab=vocab, stride=vocab, bytes=1 << 62) == EINVAL
+        assert b"split the call" in ra.lib().rlk_last_error()

@@ -56,3 +56,9 @@ def test_the_workspace_is_one():
     for bad in (None, 5, "x"):
         with pytest.raises(ra.Error, match="DecodeWorkspace"):
             K.shared_prefix_work(None, None, 1, None, None, 0, 0, 0, 1, bad)
+
+
+def test_more_units_than_a_launch_takes():
+    for w in (dict(), dict(groups=0)):
+        assert call(kv=dict(num_kv_heads=32), p=dict(num_heads=32), w=dict(items=1 << 20) | w) == EINVAL
+        assert b"split the call" in ra.lib().rlk_last_error()
