@@ -556,8 +556,10 @@ typedef struct rlk_shared_prefix_work {
 
 /* options: RLK_SCALE_F32 or RLK_SCALE_F16 of an INT8 cache; NULL: RLK_SCALE_F32.
  * Keys past the sequence's table row are not read.  A key's probability is rounded
- * to fp16, of an INT8 cache after it has been multiplied by the key's V scale; K
- * scales multiply the scores, codes are exact, all else is held in fp32.
+ * to fp16, of an INT8 cache after it has been multiplied by the key's V scale, to
+ * half a step or 2^-25 of the largest such product that the item has (rows of zeros
+ * aside, whatever their scale); K scales multiply the scores, codes are exact, all else
+ * is held in fp32.
  * num_items <= 0: no-op.  head_dim not in {64, 128} or more than 8 query heads a kv
  * head: RLK_EUNSUPPORTED.  A scale that is no finite number, more than 2^20 items or
  * groups, or q and out rows and cache planes that are not 16-byte aligned: RLK_EINVAL. */

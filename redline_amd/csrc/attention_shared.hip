@@ -30,7 +30,8 @@
 // register.
 //
 // INT8: K scales multiply the scores, V scales the probabilities before they are rounded,
-// so that codes stay exact and a value is rounded once, as in an FP16 cache.
+// so that codes stay exact and a value is rounded once, as in an FP16 cache; the reference of
+// the exponentials is that of the products (kNoValue).
 //
 // Bound: the prefix by a wave's chain LDS -> product -> exponential -> product, some 1950
 // clocks a tile with two waves a SIMD (64 items x 7 heads a kv head over 32 k and up to 2 k of
@@ -131,13 +132,27 @@ __device__ __forceinline__ int k_swizzle(int r) { return D == 128 ? r & 15 : (r 
 template <int D>
 __device__ __forceinline__ int v_swizzle(int r) { return D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; }
 
-// log2 of the largest V scale of kKeys keys, one a lane (from 2^-31 on: no fp16 number
-// but 0 gives less).
-template <int kKeys>
-__device__ __forceinline__ float largest_scale(float vs) {
-  vs = rows_max<false>(group_max<16>(vs));
-  if constexpr (kKeys == 64) vs = rows_max<true>(vs);
-  return __builtin_amdgcn_logf(fmaxf(vs, 0x1p-31f));
+// INT8: the reference m of the exponentials is the maximum of score + log2(V scale) of the same
+// key, since p vs is what is rounded: keys of a large V scale that have no weight, or that are
+// masked, take no bits from the others.  A row of zeros (whose scale is 1) gives nothing and is
+// not to set it either; its scale counts as 0, whose logarithm is held at kNoValue: where the
+// scores of such keys lie further above all others, the output is below fp16, and their
+// exponentials stay in fp32.
+constexpr float kNoValue = -64.f;
+__device__ __forceinline__ float log2_scale(float vs) {
+  return __builtin_amdgcn_logf(fmaxf(vs, 0x1p-64f));
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t or_dpp(uint32_t v) {
+  return v | static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), CTRL, 0xF, 0xF, true));
+}
+// Bits of v of aligned groups of 4 or 8 lanes.
+template <int N>
+__device__ __forceinline__ uint32_t group_or(uint32_t v) {
+  static_assert(N == 4 || N == 8);
+  v = or_dpp<0x4E>(or_dpp<0xB1>(v));
+  if constexpr (N == 8) v = or_dpp<0x141>(v);
+  return v;
 }
 
 // The rows of one key that a lane of the suffix loads: E = D / 16 dims of V, 8 of K.
@@ -147,10 +162,12 @@ template <> struct RawOf<8> { using Type = u32x2; };
 template <> struct RawOf<4> { using Type = uint32_t; };
 
 // One wave's part of a unit of up to 16 rows: keys [begin, end) of the table row, for row lane % 16
-// those below `last`.  In: q as B operands; kbuf: 32 rows of K in LDS, this wave's own.  Out: m, l and o[dt][i] = dim E (4 (lane / 16) + i) + dt of row lane % 16.
+// those below `last`.  In: q as B operands; kbuf: 32 rows of K in LDS, scales: of 32 keys, this wave's
+// own.  Out: m, l and o[dt][i] = dim E (4 (lane / 16) + i) + dt of row lane % 16.
 template <int D, int kFmt>
 __device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t* table, int kvh, int begin, int end, int last,
-                                             const f16x8 (&q)[D / 32], unsigned char* kbuf, float& m, float& l, f32x4 (&o)[D / 16]) {
+                                             const f16x8 (&q)[D / 32], unsigned char* kbuf, float (*scales)[32], float& m, float& l,
+                                             f32x4 (&o)[D / 16]) {
   constexpr bool kInt8 = kFmt != kF16;
   constexpr int E = D / 16, kElem = kInt8 ? 1 : 2, kAhead = 2, kKeys = 32;
   constexpr int kAheadV = kInt8 ? 2 : 1;  // (FP16: with two tiles the registers do not suffice)
@@ -216,6 +233,11 @@ __device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t*
       const int r = j * kRowsAtOnce + lane / kChunks;
       store16(kbuf + r * kRow + ((lane % kChunks ^ swizzle(r)) << 4), kr[u][j]);
     }
+    if constexpr (kInt8) {
+      scales[0][lane % kKeys] = ks[u];
+      scales[1][lane % kKeys] = vs[u];
+      scales[2][lane % kKeys] = log2_scale(vs[u]);
+    }
     f32x4 s[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -230,18 +252,17 @@ __device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t*
       }
     }
     // s[t][i]: key k0 + 16 t + 4 kg + i
-    f32x4 vscale[2];
-    float ref = 0.f;
+    f32x4 vscale[2], vlog[2];
     if constexpr (kInt8) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t) {
+        const int key = 16 * t + 4 * kg;
+        const f32x4 f = *reinterpret_cast<const f32x4*>(&scales[0][key]);
+        vscale[t] = *reinterpret_cast<const f32x4*>(&scales[1][key]);
+        vlog[t] = *reinterpret_cast<const f32x4*>(&scales[2][key]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = 16 * t + 4 * kg + i;
-          s[t][i] *= __shfl(ks[u], key, kWave);
-          vscale[t][i] = __shfl(vs[u], key, kWave);
-        }
-      ref = largest_scale<kKeys>(vs[u]);
+        for (int i = 0; i < 4; ++i) s[t][i] *= f[i];
+      }
     }
     const Cell next = find(k0 + 2 * kAhead * kKeys);
     request_k(u, cells[u]);
@@ -255,11 +276,32 @@ __device__ __forceinline__ void attend_alone(const SharedArgs& a, const int32_t*
         for (int i = 0; i < 4; ++i)
           if (16 * t + i >= left) s[t][i] = -INFINITY;
     }
-    float mx = s[0][0];
+    auto largest = [&] {
+      float mx = -INFINITY;
 #pragma unroll
-    for (int i = 1; i < 8; ++i) mx = larger(mx, s[i / 4][i % 4]);
-    mx = rows_max<true>(rows_max<false>(mx)) * c + ref;
+      for (int i = 0; i < 8; ++i) {
+        float x = s[i / 4][i % 4];
+        if constexpr (kInt8) x = __builtin_fmaf(x, c, vlog[i / 4][i % 4]);
+        mx = larger(mx, x);
+      }
+      mx = rows_max<true>(rows_max<false>(mx));
+      return kInt8 ? mx : mx * c;
+    };
+    float mx = largest();
     if (__any(mx > m + 8.f)) {  // as in the prefix
+      if constexpr (kInt8) {  // rows of zeros are looked for only where m would move
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint32_t any = 0;
+          if constexpr (E == 8) any = vr[u][j][0] | vr[u][j][1];
+          else any = vr[u][j];
+          const uint64_t rows = __ballot(any != 0) >> (16 * kg);  // (the 16 lanes of a group hold a row)
+          const bool value = (rows & 0xffff) != 0;
+          vscale[j / 4][j % 4] = value ? vscale[j / 4][j % 4] : 0.f;
+          vlog[j / 4][j % 4] = value ? vlog[j / 4][j % 4] : kNoValue;
+        }
+        mx = largest();
+      }
       const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - mn);
       l *= f;
 #pragma unroll
@@ -344,10 +386,11 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
   constexpr int kAhead = kItems > 1 ? 3 : 4;                // tiles in flight, LDS stages
   struct Stages {
     unsigned char k[kAhead][kTile * kPitch], v[kAhead][kTile * kPitch];
-    float ks[kAhead][kTile], vs[kAhead][kTile];
+    float ks[kAhead][kTile], vs[kAhead][kTile], vlog[kAhead][kTile];
   };
   struct Suffix {
     unsigned char k[kThreads / kWave][32 * D * (kInt8 ? 1 : 2)];
+    float scales[kThreads / kWave][3][32];  // of K, of V and their logarithms
     // of each wave, to be joined
     float o[kThreads / kWave][kFewRows][D + 4], m[kThreads / kWave][16], l[kThreads / kWave][16];
     int token[16];
@@ -414,7 +457,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
     }
     float m, l;
     f32x4 o[D / 16];
-    attend_alone<D, kFmt>(a, table, kvh, b0, b1, last, q, shared.suffix.k[wave], m, l, o);
+    attend_alone<D, kFmt>(a, table, kvh, b0, b1, last, q, shared.suffix.k[wave], shared.suffix.scales[wave], m, l, o);
     // the waves joined
     Suffix& j = shared.suffix;
     if (lane < 16) {
@@ -475,7 +518,8 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
   // this thread's part of a tile; lane k finds the cell of key k % 32
   const int ch = tid % kChunks, tr = tid / kChunks;
   u32x4 kraw[kAhead][kItems], vraw[kAhead][kItems];
-  float sc[kAhead];  // INT8: wave 0 has the K scales, wave 1 the V scales
+  float ksc[kAhead], vsc[kAhead];  // INT8: wave 0 has the K scales, every thread that of its V row
+  static_assert(!kInt8 || kItems == 1);
   struct Cell { int id, off; };
   auto find = [&](int k0) -> Cell {
     const int pos = min(k0 + lane % kTile, end - 1), b = block_of(a, pos);
@@ -483,18 +527,20 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
   };
   auto request = [&](int u, Cell at) {
     const uint32_t cell = (static_cast<uint32_t>(at.id) * hkv + kvh) * bs + at.off;
+    uint32_t row;
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
-      const uint32_t row = __shfl(cell, (tr + i * kRowStep) % kTile, kWave);
+      row = __shfl(cell, (tr + i * kRowStep) % kTile, kWave);
       const uint64_t from = static_cast<uint64_t>(row) * (kInt8 ? D : 2 * D) + ch * 16;
       kraw[u][i] = load16(static_cast<const unsigned char*>(p.kv.k) + from);
       vraw[u][i] = load16(static_cast<const unsigned char*>(p.kv.v) + from);
     }
     if constexpr (kInt8) {
-      if (wave < 2) {
-        const float* scale = wave == 0 ? p.kv.k_scale : p.kv.v_scale;
-        sc[u] = kFmt == kI8 ? scale[cell] : static_cast<float>(reinterpret_cast<const _Float16*>(scale)[cell]);
-      }
+      auto scale = [](const float* of, uint32_t at) {
+        return kFmt == kI8 ? of[at] : static_cast<float>(reinterpret_cast<const _Float16*>(of)[at]);
+      };
+      vsc[u] = scale(p.kv.v_scale, row);
+      if (wave == 0) ksc[u] = scale(p.kv.k_scale, cell);
     }
   };
   auto put = [&](int k0, int u) {
@@ -506,6 +552,13 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
       unsigned char* kd = lds.k[u] + row * kPitch;
       unsigned char* vd = lds.v[u] + row * kPitch;
       const u32x4 kr = kraw[u][i], vr = k0 + row < end ? vraw[u][i] : u32x4{0, 0, 0, 0};
+      if constexpr (kInt8) {
+        const float f = group_or<kChunks>(vr[0] | vr[1] | vr[2] | vr[3]) != 0 ? vsc[u] : 0.f;
+        if (ch == 0) {
+          lds.vs[u][row] = f;
+          lds.vlog[u][row] = log2_scale(f);
+        }
+      }
       if constexpr (!kInt8) {
         store16(kd + ((ch ^ k_swizzle<D>(row)) << 4), kr);
         store16(vd + ((ch ^ v_swizzle<D>(row)) << 4), vr);
@@ -519,8 +572,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
       }
     }
     if constexpr (kInt8) {
-      if (wave == 0 && lane < kTile) lds.ks[u][lane] = sc[u];
-      if (wave == 1 && lane < kTile) lds.vs[u][lane] = k0 + lane < end ? sc[u] : 0.f;
+      if (wave == 0 && lane < kTile) lds.ks[u][lane] = ksc[u];
     }
   };
 
@@ -568,11 +620,16 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
       for (int i = 0; i < 16; ++i)
         if (8 * (i / 4) + i % 4 >= left) s[i] = -INFINITY;
     }
-    float mx = s[0];
+    float mx = -INFINITY;
 #pragma unroll
-    for (int i = 1; i < 16; ++i) mx = larger(mx, s[i]);
-    mx = rows_max<true>(mx) * c;
-    if constexpr (kInt8) mx += largest_scale<kTile>(lds.vs[u][lane % kTile]);
+    for (int b = 0; b < 4; ++b) {
+      f32x4 f;
+      if constexpr (kInt8) f = *reinterpret_cast<const f32x4*>(&lds.vlog[u][8 * b + 4 * half]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = larger(mx, kInt8 ? __builtin_fmaf(s[4 * b + i], c, f[i]) : s[4 * b + i]);
+    }
+    mx = rows_max<true>(mx);
+    if constexpr (!kInt8) mx *= c;
     // m is a reference within 2^8 of the maximum: moving it costs a pass over the
     // output, and probabilities (INT8: with their V scale) up to 2^8 have the same 11 bits in fp16
     if (__any(mx > m + 8.f)) {
