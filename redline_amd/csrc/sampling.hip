@@ -492,11 +492,13 @@ struct RowSampler {
       const int at = lane_of(c, &e);
       return __shfl(e == 0 ? upto[0] : upto[1], at, kWave);
     };
-    auto first_that = [&](auto f) {  // the least place of which f holds
+    // The least place of which f holds, the last if of none, as in select: find_bin went by the scan's
+    // mass up to the bin's end, which may lie a rounding above what its tokens add up to here.
+    auto first_that = [&](auto f) {
       int c = min(f(place[0], upto[0]) ? place[0] : INT_MAX, f(place[1], upto[1]) ? place[1] : INT_MAX);
 #pragma unroll
       for (int o = 1; o < kWave; o <<= 1) c = min(c, __shfl_xor(c, o, kWave));
-      return c;
+      return min(c, n);
     };
     if (step == 0) {
       kept = k;
