@@ -375,6 +375,8 @@ def _stream_on(dev, stream):
     """_stream, for tensors of device dev: a launch goes to the current device, which must
     be theirs and the stream's."""
     if dev is not None:
+        if dev < 0:  # before the driver is asked, which a machine without a GPU answers with an error of its own
+            raise _lib.Error(_lib.RLK_EINVAL, "the cache and the tensors beside it must be GPU tensors")
         cur = torch._C._cuda_getDevice()
         if cur != dev:
             raise _lib.Error(_lib.RLK_EINVAL, f"tensors are on cuda:{dev}, the current device is cuda:{cur}")
