@@ -28,6 +28,7 @@ class Scales(Case):
         self.q[:, :self.hq * D].view(self.rows, self.hq, D)[..., 0] = Q0
 
     def cell(self, item, pos):
+        """(block, row) of a key that the item attends to."""
         first = self.firsts[item]
         if first is not None and pos < self.prefix[np.searchsorted(self.starts, item, "right") - 1]:
             item = first
@@ -58,7 +59,7 @@ class Scales(Case):
         torch, D, bs = self.torch, self.D, self.bs  # noqa: F811
         for i in range(self.S) if items is None else items:
             n = int(self.pos[self.tokens[i]]) + 1
-            at = [self.cell(i, t) for t in range(n)]
+            at = [Scales.cell(self, i, t) for t in range(n)]
             b, off = (torch.tensor(x, device="cuda") for x in zip(*at))
             k, v, ks, vs = (t[b, :, off].double().transpose(0, 1) for t in self.planes)
             q = self.q[int(self.tokens[i]), :self.hq * D].double().view(self.hkv, -1, D)
@@ -158,3 +159,21 @@ def test_zero_scales(torch, form, D, cache):  # noqa: F811
     c.put(0, 400, 0.0, 0.0)
     c.put(len(c.own) - 1, 3, 12.0, 0.0)
     c.close(c.run())
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cache", ["fp16", "int8", "int8_f16"])
+@pytest.mark.parametrize("factor", [-1.0, 0.0, -0.0, -3.0, 1e-30, -1e-42])
+def test_signs_of_the_softmax_scale(torch, factor, cache, D, form):  # noqa: F811
+    """The scale may have either sign (the smallest score then has the weight) or none (all keys
+    weigh the same)."""
+    say("shared scale signs", factor, cache, D, form)
+    per, own = FORMS[form]
+    groups = [(260, own), (None, [300])]
+    c = Case(torch, groups, 2 * per, 2, D, 16, cache, 7, amp=1.0)
+    c.scale *= factor
+    out = c.run()
+    c.check(out)
+    if cache != "fp16":
+        Scales.close(c, out)
