@@ -579,7 +579,7 @@ int rlk_paged_attention_decode_shared(const rlk_attention_params* params, const 
  * [0, 1): below 0 and NaN as 0, 1 and above as the largest below.  NaN logits count
  * as -infinity; tokens of
  * -infinity are not drawn, but of a row that holds nothing else token 0 is.  Tokens
- * of +infinity share the draw.  Weights are held to 2^-35 of themselves, and those
+ * of +infinity share the draw.  Weights are held to 1.1 * 2^-35 of themselves, and those
  * below 2^-48 of the largest count as 0.  The same inputs give the same token,
  * whatever else the call holds. */
 typedef struct rlk_sampling_work {

@@ -33,10 +33,21 @@
 // so that codes stay exact and a value is rounded once, as in an FP16 cache; the reference of
 // the exponentials is that of the products (kNoValue).
 //
-// Bound: the prefix by a wave's chain LDS -> product -> exponential -> product, some 1950
-// clocks a tile with two waves a SIMD (64 items x 7 heads a kv head over 32 k and up to 2 k of
-// their own, D = 128: 72.7 us, 426 TFLOP/s; 32 items x 4 over 8 k: 30.2); the suffix by
-// a chain of 1 us for 32 keys and wave (118 items of 7 groups, INT8: 70.8 us, 3.3 TB/s).
+// A probability (INT8: with its V scale) goes to fp16 for the second product: 2.5-2.7e-4 from 64
+// bits in the 2-norm, where outputs that are rounded alone are off by 2.1e-4; a second term
+// would double that product's instructions.
+//
+// Bound (D = 128; clock stamps, caches warm - cold):
+//   64 items x 7 heads a kv head over 32 k and up to 2 k of their own: 72.6 us, 425 TFLOP/s.  A
+//   prefix unit's 64 tiles at 0.88 - 0.99 us each (a wave's chain LDS -> product -> exponential ->
+//   product; one prefix wave a SIMD, whose products take 512 of some 2000 clocks),
+//   3 us to the merge, which takes 6.
+//   32 items x 4 over 8 k: 30.3 us.  Units end at 22 - 30: 2.3 - 3.3 until the first loads, 8
+//   prefix tiles at 1.4 - 2.1 beside the suffix's loads; 3.4 to the merge and 5.6 in it, of 17 MB
+//   of partials.
+//   118 items of 7 groups, INT8: 70.5 us, 3.3 TB/s.  512 of 1160 units are resident; prefix units
+//   (26 tiles at 1.2 us) hold their places to 37 - 54 us, the last of the long suffix units, of 15 -
+//   18 us, start at 40 - 46.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -16,8 +16,8 @@
 // LDS for all heads (every lane for itself, 16 gathers: 19.4 us against 15.2 for 5024
 // tokens of 40 heads of 64).
 // Bound: HBM, as the plain kernel (11470 tokens of 48 heads of 128, FP16, write and read
-// back: 66.9 us, 5.7 TB/s; 16384 tokens of 36 heads, INT8: 70.1 us, 4.9 TB/s); at a decode step's
-// size the launch (4.8 us).
+// back: 67.2 us, 5.7 TB/s; 16384 tokens of 36 heads, INT8: 70.3 us, 4.9 TB/s); at a decode step's
+// size the launch (5.0 us).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
