@@ -361,7 +361,8 @@ def _one_device(dev, *tensors):
 def _arg(t, dtype, what, n, dev):
     """_ptr of a tensor of at least n elements on device dev, with the checks in one call."""
     try:  # (dev -1, of a cache on the CPU, ends at _stream_on)
-        if t.dtype is dtype and t.get_device() == dev and t.is_contiguous() and t.numel() >= n:
+        if (t.dtype is dtype and (t.get_device() == dev or dev is None and t.is_cuda) and t.is_contiguous()
+                and t.numel() >= n):
             return t.data_ptr()
     except AttributeError:
         pass
