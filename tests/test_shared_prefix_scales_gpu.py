@@ -96,6 +96,20 @@ def test_large_scale_without_weight(torch, ratio, form, D, cache):  # noqa: F811
     c.close(c.run())
 
 
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("D", [64, 128])
+def test_largest_ratio_of_scales(torch, form, D):  # noqa: F811
+    """Values of 2^-14 at most beside V rows of 65024 without weight: scales 2^30 apart (fp32
+    scales alone hold so small ones)."""
+    say("shared largest ratio", form, D)
+    c = Scales(torch, form, D, "int8", 2.0 ** -21, seed=8)
+    for item, pos in ((0, 0), (0, 37), (0, 705), (len(c.own) - 1, 250)):
+        c.put(item, pos, -40.0, 2.0 ** 9)
+    out = c.run()
+    c.close(out)
+    assert (out[torch.from_numpy(c.tokens).cuda()] != 0).any(1).all()
+
+
 @variants
 def test_large_scales_past_an_items_last_key(torch, form, D, cache):  # noqa: F811
     """Items that end inside their group's prefix, before a key that has both a large V scale and
